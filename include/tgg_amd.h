@@ -36,6 +36,21 @@ extern "C" {
 int tgg_m_grouped_gemm(const void* A, const void* B, void* C, const void* sizes, int sizes_i64, int G, int64_t M,
                        int N, int K, int trans_b, int dtype, int num_cu, void* stream);
 
+/* Gated feed-forward block: H[r,:] = A[r,:] . B[g(r)]^T (trans_b=1, B is [G,2F,K]) or A[r,:] . B[g(r)] (trans_b=0, B is
+ * [G,K,2F]), whose first F columns are the gate and last F the up projection, and C[r,:] = act(gate) * up, [M,F], with
+ * everything between the products and the one rounding to `dtype` in fp32.  H [M,2F] may be NULL; otherwise it receives both
+ * projections, rounded to `dtype`: what tgg_gated_backward takes.  Rows past sum(sizes) are not written.  F and K are
+ * multiples of 8.  The reference has no counterpart: its layers run the grouped product and the activation as separate operators. */
+#define TGG_SILU 0      /* x sigma(x) */
+#define TGG_GELU_TANH 1 /* x sigma(2 sqrt(2/pi) (x + 0.044715 x^3)) */
+int tgg_m_grouped_gated_gemm(const void* A, const void* B, void* C, void* H, const void* sizes, int sizes_i64, int G, int64_t M,
+                             int F, int K, int trans_b, int activation, int dtype, int num_cu, void* stream);
+
+/* Gradient of C = act(gate) * up with respect to H: dh[r,:] = [dout up act'(gate) | dout act(gate)] for all M rows, dout [M,F],
+ * h and dh [M,2F].  The gradients of A and B are the grouped products of dh (tgg_m_grouped_gemm with trans_b flipped,
+ * tgg_k_grouped_gemm_sizes). */
+int tgg_gated_backward(const void* dout, const void* h, void* dh, int64_t M, int F, int activation, int dtype, void* stream);
+
 /* Same contraction with A/C physically padded: group g starts at sum_{h<g} round_up(sizes[h], align).
  * Replaces deep_gemm.m_grouped_bf16_gemm_nt_contiguous as called from m_grouped_bf16_nt_contiguous
  * (gemm/deep_gemm_ops.py:24-57).  Pad rows of C are not written. */
@@ -225,6 +240,19 @@ int tgg_moe_unpermute(const void* input, void* output, const int32_t* row_id_map
 int tgg_moe_unpermute_bwd(const void* grad_output, const void* fwd_input, const int32_t* row_id_map, const float* probs,
                           void* act_grad, float* prob_grad, int64_t num_tokens, int topk, int hidden, int dtype,
                           void* stream);
+
+/* Top-k router: of each token's num_experts logits (num_tokens rows, row_stride elements apart; dtype TGG_BF16, TGG_F16 or 2 = fp32) the topk
+ * largest, equal ones by index and NaN above all, to indices [num_tokens, topk], with their probabilities in fp32 to probs
+ * [num_tokens, topk]: softmax over all experts or sigmoid, and with renormalize divided by their sum.  A logit of -inf is never
+ * chosen; entries without an expert get index -1, which the token movement drops, and probability 0.  num_experts <= 1024, topk <= 64.
+ * _bwd: the gradient of the logits, dlogits [num_tokens, num_experts] in their type, from that of probs; probs and indices
+ * are the forward call's.  The reference leaves routing to its callers. */
+#define TGG_SOFTMAX 0
+#define TGG_SIGMOID 1
+int tgg_moe_router(const void* logits, int64_t row_stride, int64_t num_tokens, int num_experts, int topk, int scoring, int renormalize, int dtype, float* probs,
+                   int32_t* indices, void* stream);
+int tgg_moe_router_bwd(const void* logits, int64_t row_stride, const float* probs, const int32_t* indices, const float* grad, int64_t num_tokens, int num_experts,
+                       int topk, int scoring, int renormalize, int dtype, void* dlogits, void* stream);
 
 /* Test hook, runs entirely on the host (no GPU needed): the order in which `grid` persistent workgroups walk
  * the output tiles of a launch, computed by the same scheduler functions the kernels execute.  It restates

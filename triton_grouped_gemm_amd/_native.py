@@ -24,6 +24,8 @@ _P, _I, _L = c_void_p, c_int, c_int64
 # name -> argument types; every function returns int unless noted
 SIGNATURES = {
     "tgg_m_grouped_gemm": [_P, _P, _P, _P, _I, _I, _L, _I, _I, _I, _I, _I, _P],
+    "tgg_m_grouped_gated_gemm": [_P, _P, _P, _P, _P, _I, _I, _L, _I, _I, _I, _I, _I, _I, _P],
+    "tgg_gated_backward": [_P, _P, _P, _L, _I, _I, _I, _P],
     "tgg_m_grouped_gemm_padded": [_P, _P, _P, _P, _I, _I, _L, _I, _I, _I, _I, _I, _P],
     "tgg_m_grouped_gemm_placed": [_P, _P, _P, _P, _I, _P, _I, _L, _I, _I, _I, _I, _P],
     "tgg_m_grouped_gemm_masked": [_P, _P, _P, _P, _I, _I, _L, _L, _I, _I, _I, _I, _I, _P],
@@ -53,6 +55,8 @@ SIGNATURES = {
     "tgg_moe_permute_rows": [_P, _P, _P, _L, _I, _I, _I, _P],
     "tgg_moe_unpermute": [_P, _P, _P, _P, _L, _I, _I, _I, _P],
     "tgg_moe_unpermute_bwd": [_P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _P],
+    "tgg_moe_router": [_P, _L, _L, _I, _I, _I, _I, _I, _P, _P, _P],
+    "tgg_moe_router_bwd": [_P, _L, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P, _P],
     "tgg_debug_tile_order": [_P, _I, _I, _L, _L, _I, _I, _I, _I, _P, _L, _P],
     "tgg_debug_row_tiles": [_P, _I, _I, _L, _L, _I, _I, _P, _L, _P],
     "tgg_debug_queue_order": [_I, _I, _P],
@@ -173,4 +177,5 @@ def require_gpu(*tensors: torch.Tensor) -> None:
 
 
 DTYPE_CODE = {torch.bfloat16: BF16, torch.float16: F16}
+ACTIVATION_CODE = {"silu": 0, "gelu_tanh": 1}  # TGG_SILU, TGG_GELU_TANH
 FP8_CODE = {torch.float8_e4m3fn: E4M3, torch.float8_e5m2: E5M2}

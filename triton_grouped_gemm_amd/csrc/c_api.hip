@@ -81,6 +81,10 @@ bool fast_quant_supported(const GemmParams& p, int dt, int layout);
 int launch_fast_16bit_quant(const GemmParams& p, int dt, int layout, hipStream_t s);
 void set_fast_variant(int v);
 void set_fp8_variant(int v);
+bool fast_gated_supported(const GemmParams& p, int dt, int layout);
+int launch_fast_gated(const GemmParams& p, int dt, int layout, hipStream_t s);
+int launch_generic_gated(const GemmParams& p, int dt, int layout, hipStream_t s);
+int launch_gated_bwd(const void* dout, const void* h, void* dh, int64_t rows, int F, int act, int dt, hipStream_t s);
 
 static bool aligned16(const void* p) { return (((uintptr_t)p) & 15) == 0; }
 
@@ -236,6 +240,12 @@ static int dispatch_16bit(const GemmParams& p, int dt, int layout, hipStream_t s
   }
 }
 
+// The gated block (GemmParams::H)
+static int dispatch_gated(const GemmParams& p, int dt, int layout, hipStream_t s) {
+  if (!g_force_generic.load() && fast_gated_supported(p, dt, layout)) return launch_fast_gated(p, dt, layout, s);
+  return launch_generic_gated(p, dt, layout, s);
+}
+
 }  // namespace tgg
 
 using namespace tgg;
@@ -334,6 +344,32 @@ int tgg_m_grouped_gemm(const void* A, const void* B, void* C, const void* sizes,
   if (M == 0) return 0;
   const GemmParams p = params_m_grouped(A, B, C, sizes, sizes_i64, G, M, N, K, trans_b, num_cu);
   return dispatch_16bit(p, dtype, trans_b ? 0 : 1, (hipStream_t)stream);
+}
+
+int tgg_m_grouped_gated_gemm(const void* A, const void* B, void* C, void* H, const void* sizes, int sizes_i64, int G, int64_t M,
+                             int F, int K, int trans_b, int activation, int dtype, int num_cu, void* stream) {
+  if (int e = check_common(A, B, C, sizes, G, F, TGG_MAX_GROUPS)) return e;
+  if (M < 0 || K < 0) return set_error("negative M or K");
+  if (dtype != TGG_BF16 && dtype != TGG_F16) return set_error("data type code %d not supported", dtype);
+  if (activation != TGG_SILU && activation != TGG_GELU_TANH) return set_error("activation code %d not supported", activation);
+  if ((K & 7) || (F & 7)) return set_error("F and K must be multiples of 8 (16-byte rows), got F=%d K=%d", F, K);
+  if (F >= (1 << 30)) return set_error("F=%d is too large", F);
+  if (H && !aligned16(H)) return set_error("operand pointers must be 16-byte aligned");
+  if (M == 0) return 0;
+  GemmParams p = params_m_grouped(A, B, C, sizes, sizes_i64, G, M, 2 * F, K, trans_b, num_cu);
+  p.H = H;
+  p.act = activation;
+  return dispatch_gated(p, dtype, trans_b ? 0 : 1, (hipStream_t)stream);
+}
+
+int tgg_gated_backward(const void* dout, const void* h, void* dh, int64_t M, int F, int activation, int dtype, void* stream) {
+  if (!dout || !h || !dh) return set_error("null operand pointer");
+  if (!aligned16(dout) || !aligned16(h) || !aligned16(dh)) return set_error("operand pointers must be 16-byte aligned");
+  if (M < 0 || F < 8 || (F & 7) || F >= (1 << 30)) return set_error("F must be a multiple of 8 (16-byte rows) and M not negative, got F=%d M=%lld", F, (long long)M);
+  if (dtype != TGG_BF16 && dtype != TGG_F16) return set_error("data type code %d not supported", dtype);
+  if (activation != TGG_SILU && activation != TGG_GELU_TANH) return set_error("activation code %d not supported", activation);
+  if (M == 0) return 0;
+  return launch_gated_bwd(dout, h, dh, M, F, activation, dtype, (hipStream_t)stream);
 }
 
 int tgg_m_grouped_gemm_fp8_out(const void* A, const void* B, void* codes, float* scales, const void* sizes,
@@ -694,6 +730,34 @@ int tgg_moe_unpermute_bwd(const void* grad_output, const void* fwd_input, const 
     return set_error("activation pointers must be 16-byte aligned");
   return launch_moe_unpermute_bwd(grad_output, fwd_input, row_id_map, probs, act_grad, prob_grad, num_tokens, topk, rb,
                                   dtype, (hipStream_t)stream);
+}
+
+static int router_check(const void* logits, int64_t row_stride, int64_t num_tokens, int num_experts, int topk, int scoring, int dtype) {
+  if (dtype != TGG_BF16 && dtype != TGG_F16 && dtype != 2) return set_error("logits of type code %d not supported", dtype);
+  if (num_experts < 1 || num_experts > TGG_MAX_GROUPS) return set_error("num_experts=%d outside [1, %d]", num_experts, TGG_MAX_GROUPS);
+  if (topk < 1 || topk > 64 || topk > num_experts) return set_error("topk=%d outside [1, min(64, %d experts)]", topk, num_experts);
+  if (scoring != TGG_SOFTMAX && scoring != TGG_SIGMOID) return set_error("scoring code %d not supported", scoring);
+  if (num_tokens < 0 || row_stride < 0) return set_error("negative num_tokens or row stride");
+  if (num_tokens > 0 && !logits) return set_error("null pointer");
+  if ((uintptr_t)logits & (dtype == 2 ? 3 : 1)) return set_error("logits must be aligned to their type");
+  return 0;
+}
+
+int tgg_moe_router(const void* logits, int64_t row_stride, int64_t num_tokens, int num_experts, int topk, int scoring, int renormalize, int dtype, float* probs,
+                   int32_t* indices, void* stream) {
+  if (int e = router_check(logits, row_stride, num_tokens, num_experts, topk, scoring, dtype)) return e;
+  if (num_tokens == 0) return 0;
+  if (!probs || !indices) return set_error("null pointer");
+  return launch_moe_router(logits, row_stride * (dtype == 2 ? 4 : 2), num_tokens, num_experts, topk, scoring, renormalize != 0, dtype, probs, indices, (hipStream_t)stream);
+}
+
+int tgg_moe_router_bwd(const void* logits, int64_t row_stride, const float* probs, const int32_t* indices, const float* grad, int64_t num_tokens, int num_experts,
+                       int topk, int scoring, int renormalize, int dtype, void* dlogits, void* stream) {
+  if (int e = router_check(logits, row_stride, num_tokens, num_experts, topk, scoring, dtype)) return e;
+  if (num_tokens == 0) return 0;
+  if (!probs || !indices || !grad || !dlogits) return set_error("null pointer");
+  return launch_moe_router_bwd(logits, row_stride * (dtype == 2 ? 4 : 2), probs, indices, grad, num_tokens, num_experts, topk, scoring, renormalize != 0, dtype, dlogits,
+                               (hipStream_t)stream);
 }
 
 int tgg_debug_tile_order(const int64_t* sizes, int G, int mode, int64_t m_total, int64_t aux, int N, int tile,

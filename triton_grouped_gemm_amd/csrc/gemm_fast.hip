@@ -31,6 +31,7 @@
 //     small per-wave LDS staging area (separate from the slab buffers, so the copy stream keeps running) and
 //     leave as 16-byte stores that cover whole row segments of the wave's columns.
 #include "fast_common.hpp"
+#include "gate.hpp"
 #include "launch.hpp"
 #include <atomic>
 #include <type_traits>
@@ -93,7 +94,9 @@ struct FastCfg {
 
 // The whole kernel but for the group table, which the caller has built at byte SCHED_AT of the workgroup's LDS
 // (C::SCHED_OFF unless two tile configurations share one kernel, see gemm_fast_auto_kernel).
-template <class C, int DT, int LAYOUT, bool QUANT, int SCHED_AT>
+// GATED: the gated feed-forward block (GemmParams::H).  A wave's columns are half gate, half up projection: of its TN column blocks the first
+// TN / 2 are the gate's, so both sums of an output are in the same lane's registers.  Only the source of B's copies and the epilogue differ.
+template <class C, int DT, int LAYOUT, bool QUANT, int SCHED_AT, bool GATED = false>
 TGG_DEV void gemm_fast_body(const GemmParams& p) {
   constexpr bool A_KMAJOR = LAYOUT != LAYOUT_TN;
   constexpr bool B_KMAJOR = LAYOUT == LAYOUT_NT;
@@ -102,6 +105,7 @@ TGG_DEV void gemm_fast_body(const GemmParams& p) {
   // two-buffer scheme is requested only one slab period before it is needed.
   constexpr bool DEEP = C::BST == 3;
   static_assert(!DEEP || !QUANT, "the fused-quantisation epilogue uses the two-buffer configuration");
+  static_assert(!GATED || (!QUANT && LAYOUT != LAYOUT_TN), "the gated block is a forward product");
   typedef Operand<C::BM, A_KMAJOR> OpA;
   typedef Operand<C::BN, B_KMAJOR> OpB;
 
@@ -123,7 +127,15 @@ TGG_DEV void gemm_fast_body(const GemmParams& p) {
 
   // per-lane source offsets of this wave's copies (one swizzle pattern per wave, see FastCfg)
   const int a_voff = OpA::lane_voff(lane, wave % OpA::NPAT, (int)a_ld);
-  const int b_voff = OpB::lane_voff(lane, wave % OpB::NPAT, (int)b_ld);
+  // GATED: column c of the 16 TN that a wave holds in LDS is output column 8 TN w + c mod 8 TN of the tile, of the gate or, in the upper half, of
+  // the up projection F = N / 2 columns further on
+  auto gated_col = [&](int x) { return x / (16 * C::TN) * (8 * C::TN) + x % (8 * C::TN) + (x % (16 * C::TN) >= 8 * C::TN ? p.N / 2 : 0); };
+  int b_voff_ = OpB::lane_voff(lane, wave % OpB::NPAT, (int)b_ld);
+  if (GATED && !B_KMAJOR) {  // token rows: the lane's 16-byte chunk holds columns 8 c ... of the LDS row
+    const int in_row = OpB::lane_voff(lane, wave % OpB::NPAT, 0);
+    b_voff_ += gated_col(in_row / 2) * 2 - in_row;
+  }
+  const int b_voff = b_voff_;
   // K tail (K not a multiple of the slab depth): in a tile's last slab the lanes whose 16-byte chunk of a
   // K-contiguous row starts at or beyond K fetch nothing (zeros); token-row operands end with the descriptor.
   const int tail_chunks = LAYOUT == LAYOUT_TN ? 0 : (p.K % BK) / 8;
@@ -214,7 +226,12 @@ TGG_DEV void gemm_fast_body(const GemmParams& p) {
       // masked_m) reads as zero and its products are never stored
       io.a_base = (uint64_t)p.A + (uint64_t)(t.row0 * a_ld);
       io.a_rem = t.rows * (int)a_ld;
-      if (LAYOUT == LAYOUT_NT) {
+      if (GATED) {  // from the gate's first column of the tile to the end of the group's up projection
+        const int o0 = t.n0 / 2;
+        io.b_base = (uint64_t)p.B + (uint64_t)((LAYOUT == LAYOUT_NT ? ((int64_t)t.g * p.N + o0) * b_ld : (int64_t)t.g * p.K * b_ld + (int64_t)o0 * 2));
+        io.b_rem = LAYOUT == LAYOUT_NT ? (p.N - o0) * (int)b_ld : p.K;
+        if (LAYOUT == LAYOUT_NN) io.b_off = o0 * 2;
+      } else if (LAYOUT == LAYOUT_NT) {
         const int n_left = p.N - t.n0;
         io.b_base = (uint64_t)p.B + (uint64_t)(((int64_t)t.g * p.N + t.n0) * b_ld);
         io.b_rem = (n_left < C::BN ? n_left : C::BN) * (int)b_ld;
@@ -369,7 +386,8 @@ TGG_DEV void gemm_fast_body(const GemmParams& p) {
       copy_b128_to_lds(sc.ra, sc.base + idx * 1024, (sc.tail ? a_voff_tail : a_voff) + idx * OpA::RPI * (int)a_ld);
     } else {
       const int idx = wave + (k - CA) * C::NWAVES;
-      copy_b128_to_lds(sc.rb, sc.base_b + idx * 1024, (sc.tail_b ? b_voff_tail : b_voff) + idx * OpB::RPI * (int)b_ld);
+      const int row = GATED && B_KMAJOR ? gated_col(idx * OpB::RPI) : idx * OpB::RPI;
+      copy_b128_to_lds(sc.rb, sc.base_b + idx * 1024, (sc.tail_b ? b_voff_tail : b_voff) + row * (int)b_ld);
     }
   };
 
@@ -620,6 +638,51 @@ TGG_DEV void gemm_fast_body(const GemmParams& p) {
       }
       continue;
     }
+    if constexpr (GATED) {
+      // Blocks j < TN / 2 of a strip are the gate, the others the up projection of the same outputs.  The projections, where they are asked
+      // for, and then the products pass through the strip's staging rows.
+      constexpr int HN = C::TN / 2, CPH = 2 * C::TN, CPO = C::TN;  // 16-byte chunks of a staged row: both projections, the products
+      const int F = p.N / 2, o0 = (cur.n0 + wn0) / 2;  // the wave's first output column
+      char* const h_tile = (char*)p.H + ((c_row0 + wm0) * (int64_t)p.N + o0) * 2;
+      char* const o_tile = (char*)p.C + ((c_row0 + wm0) * (int64_t)F + o0) * 2;
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        if (p.H) {
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+            *(uint2*)(stage_c + e16 * C::EPI_PITCH + (16 * j + 4 * eg) * 2) = pack4<DT>(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+#pragma unroll
+          for (int it = 0; it < 16 * CPH / 64; ++it) {
+            const int idx = it * 64 + el, r = idx / CPH, ch = idx % CPH, c = (ch % C::TN) * 8;
+            const i32x4_t v = *(const i32x4_t*)(stage_c + r * C::EPI_PITCH + ch * 16);
+            if (o0 + c < F && wm0 + 16 * i + r < cur.rows)
+              store_c((i32x4_t*)(h_tile + ((int64_t)(16 * i + r) * p.N + c + (ch >= C::TN ? F : 0)) * 2), v, 0);
+          }
+        }
+        if (p.act == GATE_SILU) {
+#pragma unroll
+          for (int j = 0; j < HN; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = gate_act<GATE_SILU>(acc[i][j][e]) * acc[i][j + HN][e];
+        } else {
+#pragma unroll
+          for (int j = 0; j < HN; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = gate_act<GATE_GELU_TANH>(acc[i][j][e]) * acc[i][j + HN][e];
+        }
+#pragma unroll
+        for (int j = 0; j < HN; ++j)
+          *(uint2*)(stage_c + e16 * C::EPI_PITCH + (16 * j + 4 * eg) * 2) = pack4<DT>(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+        clear_strip(i);
+#pragma unroll
+        for (int it = 0; it < (16 * CPO + 63) / 64; ++it) {
+          const int idx = it * 64 + el, r = idx / CPO, ch = idx % CPO;
+          if (r < 16 && o0 + ch * 8 < F && wm0 + 16 * i + r < cur.rows)
+            store_c((i32x4_t*)(o_tile + ((int64_t)(16 * i + r) * F + ch * 8) * 2), *(const i32x4_t*)(stage_c + r * C::EPI_PITCH + ch * 16), 0);
+        }
+      }
+      continue;
+    }
     char* const c_tile = (char*)p.C + ((c_row0 + wm0) * (int64_t)p.N + cur.n0 + wn0) * 2;
     constexpr int CPS = 2 * C::TN;        // 16-byte chunks per staged row
     constexpr int PASSES = 16 * CPS / 64;  // wave-wide reads per strip
@@ -692,7 +755,7 @@ __global__ __launch_bounds__(C::THREADS) void gemm_fast_kernel(const GemmParams 
 // Wide and narrow use BM-row tiles, so one group table serves both; for CS the table's tile prefix is rebuilt for
 // its tile height when it differs (some group above 128 rows; sched_init has computed it alongside).  The table sits where the wide configuration keeps
 // it, past everything the others touch.  CS = void: no weight-streaming configuration (K-grouped).
-template <class CW, class CN, class CS, int DT, int LAYOUT>
+template <class CW, class CN, class CS, int DT, int LAYOUT, bool GATED = false>
 __global__ __launch_bounds__(CW::THREADS) void gemm_fast_auto_kernel(const GemmParams p) {
   static_assert(CW::BM == CN::BM && CW::THREADS == CN::THREADS, "one group table, one launch shape");
   static_assert(CN::SMEM_BYTES <= CW::SCHED_OFF, "the narrow configuration must not reach the shared group table");
@@ -716,13 +779,13 @@ __global__ __launch_bounds__(CW::THREADS) void gemm_fast_auto_kernel(const GemmP
         if (sched.pad_ != 0) {  // some group has more than one 128-row tile: the tile prefix for this tile height
           sched_use_half_height(p, sched, half_tile0);
         }
-        gemm_fast_body<CS, DT, LAYOUT, false, CW::SCHED_OFF>(p);
+        gemm_fast_body<CS, DT, LAYOUT, false, CW::SCHED_OFF, GATED>(p);
         return;
       }
     }
-    gemm_fast_body<CW, DT, LAYOUT, false, CW::SCHED_OFF>(p);
+    gemm_fast_body<CW, DT, LAYOUT, false, CW::SCHED_OFF, GATED>(p);
   } else {
-    gemm_fast_body<CN, DT, LAYOUT, false, CW::SCHED_OFF>(p);
+    gemm_fast_body<CN, DT, LAYOUT, false, CW::SCHED_OFF, GATED>(p);
   }
 }
 
@@ -757,10 +820,10 @@ int launch_cfg(const GemmParams& p, hipStream_t s) {
   return launch_kernel(gemm_fast_kernel<C, DT, LAYOUT, QUANT>, C::SMEM_BYTES, C::THREADS, attr_flag(attr_set), p, s, "gemm_fast");
 }
 
-template <class CW, class CN, class CS, int DT, int LAYOUT>
+template <class CW, class CN, class CS, int DT, int LAYOUT, bool GATED = false>
 int launch_auto(const GemmParams& p, hipStream_t s) {
   static bool attr_set[64] = {false};
-  return launch_kernel(gemm_fast_auto_kernel<CW, CN, CS, DT, LAYOUT>, CW::SMEM_BYTES, CW::THREADS, attr_flag(attr_set), p, s, "gemm_fast");
+  return launch_kernel(gemm_fast_auto_kernel<CW, CN, CS, DT, LAYOUT, GATED>, CW::SMEM_BYTES, CW::THREADS, attr_flag(attr_set), p, s, "gemm_fast");
 }
 
 std::atomic<int> g_variant{0};
@@ -823,6 +886,21 @@ bool fast_quant_supported(const GemmParams& p, int dt, int layout) {
   if (p.mode != MODE_MG && p.mode != MODE_MG_PAD) return false;
   if ((p.N & 127) != 0) return false;
   return fast_supported(p, dt, layout);
+}
+
+// The gated block: as the plain product, with one window over a group's gate and up columns, so all of a group's B within the offsets' range.
+bool fast_gated_supported(const GemmParams& p, int dt, int layout) {
+  return (p.N & 15) == 0 && (int64_t)p.N * p.K * 2 < (1ll << 30) && layout != LAYOUT_TN && fast_supported(p, dt, layout);
+}
+
+template <int DT, int LAYOUT>
+static int launch_fast_gated_as(const GemmParams& p, hipStream_t s) {
+  return launch_auto<FastCfg<256, 256, 2, 4>, FastCfg<256, 128, 2, 4>, FastCfg<128, 256, 2, 4, 3>, DT, LAYOUT, true>(p, s);
+}
+
+int launch_fast_gated(const GemmParams& p, int dt, int layout, hipStream_t s) {
+  if (dt == DT_BF16) return layout == LAYOUT_NT ? launch_fast_gated_as<DT_BF16, LAYOUT_NT>(p, s) : launch_fast_gated_as<DT_BF16, LAYOUT_NN>(p, s);
+  return layout == LAYOUT_NT ? launch_fast_gated_as<DT_F16, LAYOUT_NT>(p, s) : launch_fast_gated_as<DT_F16, LAYOUT_NN>(p, s);
 }
 
 int launch_fast_16bit(const GemmParams& p, int dt, int layout, hipStream_t s) {

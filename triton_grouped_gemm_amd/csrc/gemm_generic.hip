@@ -11,6 +11,7 @@
 // gemm_fast.hip take over for the aligned shapes.
 #include "common.hpp"
 #include "sched.hpp"
+#include "gate.hpp"
 #include "generic_addr.hpp"
 #include "launch.hpp"
 
@@ -74,27 +75,30 @@ template <int DT, bool KMAJOR> struct Stager {
   i32x4_t v[NVEC];
 
   // base: element (row 0 of the tile, k = 0 of the whole operand); lim_mn: rows of the tile that may be read
-  TGG_DEV void load(const char* base, int64_t s_row, int64_t s_k, int lim_mn, int64_t k, int64_t k_end) {
+  // up: 0, or for the gated block how many columns behind the gate's the up projection's lie; the tile's rows then take turns, 32 of the gate and
+  // 32 of the up projection of the same outputs (generic_gated_row), and lim_mn counts outputs
+  TGG_DEV void load(const char* base, int64_t s_row, int64_t s_k, int lim_mn, int64_t k, int64_t k_end, int up = 0) {
 #pragma unroll
     for (int i = 0; i < NVEC; ++i) {
       const int idx = threadIdx.x + i * GTHREADS;
       i32x4_t val = {0, 0, 0, 0};
       if (KMAJOR) {
         constexpr int VPR = GBK / VEC;
-        const int row = idx / VPR;
+        const int row = up ? generic_gated_row(idx / VPR) : idx / VPR;
         const int64_t kk = k + (idx % VPR) * VEC;
         if (row < lim_mn && kk < k_end) {
-          const char* src = base + generic_elem_kmajor(row, s_row, kk) * ES;
+          const char* src = base + generic_elem_kmajor(up ? row + generic_gated_up(idx / VPR, up) : row, s_row, kk) * ES;
           if (kk + VEC <= k_end) val = *(const i32x4_t*)src;
           else val = load_partial(src, (int)(k_end - kk) * ES);
         }
       } else {
         constexpr int VPR = 128 / VEC;
         const int krow = idx / VPR;
-        const int mn = (idx % VPR) * VEC;
+        const int at = (idx % VPR) * VEC;
+        const int mn = up ? generic_gated_row(at) : at;
         const int64_t kk = k + krow;
         if (kk < k_end && mn < lim_mn) {
-          const char* src = base + generic_elem_mnmajor(kk, s_k, mn) * ES;
+          const char* src = base + generic_elem_mnmajor(kk, s_k, up ? mn + generic_gated_up(at, up) : mn) * ES;
           if (mn + VEC <= lim_mn) val = *(const i32x4_t*)src;
           else val = load_partial(src, (lim_mn - mn) * ES);
         }
@@ -128,7 +132,7 @@ template <int DT> TGG_DEV typename Frag<DT>::type read_frag(const char* lds, int
   return *(const typename Frag<DT>::type*)(lds + row * PITCH + koff * ES);
 }
 
-enum : int { EPI_PLAIN = 0, EPI_CHANNEL = 1, EPI_BLOCK = 2 };
+enum : int { EPI_PLAIN = 0, EPI_CHANNEL = 1, EPI_BLOCK = 2, EPI_GATED = 3 };
 
 struct GenericSmem {
   SchedTable sched;
@@ -159,7 +163,9 @@ __global__ __launch_bounds__(GTHREADS) void gemm_generic_kernel(const GemmParams
     const char* a_base = (const char*)p.A + io.a_elem * ESA;
     const int a_lim = io.a_lim;
     const char* b_base = (const char*)p.B + io.b_elem * ESB;
-    const int b_lim = io.b_lim;
+    const int b_lim = EPI == EPI_GATED ? io.o_lim : io.b_lim;
+    const int up = EPI == EPI_GATED ? p.N / 2 : 0;
+    if (EPI == EPI_GATED) b_base = (const char*)p.B + io.gate_elem * ESB;
 
     f32x16_t acc[2][2];
     f32x16_t part[2][2];
@@ -176,7 +182,7 @@ __global__ __launch_bounds__(GTHREADS) void gemm_generic_kernel(const GemmParams
     const int kt_n = (int)((klen + GBK - 1) / GBK);
     if (kt_n > 0) {
       sa_.load(a_base, p.a_sm, p.a_sk, a_lim, t.k0, t.k1);
-      sb_.load(b_base, p.b_sn, p.b_sk, b_lim, t.k0, t.k1);
+      sb_.load(b_base, p.b_sn, p.b_sk, b_lim, t.k0, t.k1, up);
       sa_.store(sm.a[0]);
       sb_.store(sm.b[0]);
     }
@@ -185,7 +191,7 @@ __global__ __launch_bounds__(GTHREADS) void gemm_generic_kernel(const GemmParams
       const int cur = kt & 1;
       if (kt + 1 < kt_n) {
         sa_.load(a_base, p.a_sm, p.a_sk, a_lim, t.k0 + (int64_t)(kt + 1) * GBK, t.k1);
-        sb_.load(b_base, p.b_sn, p.b_sk, b_lim, t.k0 + (int64_t)(kt + 1) * GBK, t.k1);
+        sb_.load(b_base, p.b_sn, p.b_sk, b_lim, t.k0 + (int64_t)(kt + 1) * GBK, t.k1, up);
       }
 #pragma unroll
       for (int ks = 0; ks < GBK / 16; ++ks) {
@@ -230,6 +236,32 @@ __global__ __launch_bounds__(GTHREADS) void gemm_generic_kernel(const GemmParams
       __syncthreads();
     }
 
+    if constexpr (EPI == EPI_GATED) {  // column block 0 of a wave is the gate, block 1 the up projection of the same 32 outputs
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int m = wm + i * 32 + l32;
+        if (m >= t.rows) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c = wn / 2 + q * 8 + lh * 4;
+          if (c >= b_lim) continue;
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = acc[i][0][q * 4 + e];
+            v[e] = (p.act == GATE_SILU ? gate_act<GATE_SILU>(x) : gate_act<GATE_GELU_TANH>(x)) * acc[i][1][q * 4 + e];
+          }
+          const int64_t at = (t.row0 + m) * (int64_t)up + t.n0 / 2 + c;
+          *(uint2*)((char*)p.C + at * 2) = pack4<OUT>(v[0], v[1], v[2], v[3]);
+          if (p.H) {
+            uint2* const h = (uint2*)((char*)p.H + ((t.row0 + m) * (int64_t)p.N + t.n0 / 2 + c) * 2);
+            *h = pack4<OUT>(acc[i][0][q * 4], acc[i][0][q * 4 + 1], acc[i][0][q * 4 + 2], acc[i][0][q * 4 + 3]);
+            *(uint2*)((char*)h + (int64_t)up * 2) = pack4<OUT>(acc[i][1][q * 4], acc[i][1][q * 4 + 1], acc[i][1][q * 4 + 2], acc[i][1][q * 4 + 3]);
+          }
+        }
+      }
+      continue;
+    }
     // epilogue: lane owns row m, columns n = wn + j*32 + 8q + 4*lh + (0..3)
     char* c_base = (char*)p.C + io.c_elem * 2;
     const bool vec_ok = (p.N & 3) == 0;
@@ -293,6 +325,12 @@ int launch_generic_16bit(const GemmParams& p, int dt, int layout, hipStream_t s)
     if (layout == 2) return launch_one<DT_F16, DT_F16, false, false, EPI_PLAIN, DT_F16>(p, s);
   }
   return set_error("unsupported dtype/layout (%d, %d)", dt, layout);
+}
+
+// The gated block; layout 0 = NT, 1 = NN
+int launch_generic_gated(const GemmParams& p, int dt, int layout, hipStream_t s) {
+  if (dt == DT_BF16) return layout == 0 ? launch_one<DT_BF16, DT_BF16, true, true, EPI_GATED, DT_BF16>(p, s) : launch_one<DT_BF16, DT_BF16, true, false, EPI_GATED, DT_BF16>(p, s);
+  return layout == 0 ? launch_one<DT_F16, DT_F16, true, true, EPI_GATED, DT_F16>(p, s) : launch_one<DT_F16, DT_F16, true, false, EPI_GATED, DT_F16>(p, s);
 }
 
 int launch_generic_fp8_channel(const GemmParams& p, int ta, int tb, int out_dt, hipStream_t s) {

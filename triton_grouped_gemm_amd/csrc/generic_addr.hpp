@@ -18,6 +18,8 @@ struct GenericTileIo {
   int64_t b_elem;  // element (tile column 0, k = 0) of the group's B
   int b_lim;       // columns of the tile that may be read
   int64_t c_elem;  // element (tile row 0, column 0 of the output matrix) of C
+  int64_t gate_elem;  // the gated block: element (gate column of the tile's first output, k = 0) of the group's B
+  int o_lim;          // and how many of the tile's 64 outputs exist
 };
 
 TGG_HD bool generic_kmode(const GemmParams& p) { return p.mode == MODE_KG || p.mode == MODE_KG_COUNT; }
@@ -31,8 +33,15 @@ TGG_HD GenericTileIo generic_tile_io(const GemmParams& p, const Tile& t) {
   io.b_elem = (int64_t)t.g * p.b_sg + (int64_t)t.n0 * p.b_sn;
   io.b_lim = (p.N - t.n0) < kGenericBN ? (p.N - t.n0) : kGenericBN;
   io.c_elem = generic_kmode(p) ? ((int64_t)t.g * p.c_sg + t.row0 * p.N) : t.row0 * (int64_t)p.N;
+  io.gate_elem = (int64_t)t.g * p.b_sg + (int64_t)(t.n0 / 2) * p.b_sn;
+  io.o_lim = (p.N - t.n0) / 2 < kGenericBN / 2 ? (p.N - t.n0) / 2 : kGenericBN / 2;
   return io;
 }
+
+// The gated block: row r of the tile's 128 rows of B is output (r / 64) * 32 + r % 32 of the tile, of the gate or, in every second run of 32, of the
+// up projection `up` = N / 2 columns behind it
+TGG_HD int generic_gated_row(int r) { return (r >> 6) * 32 + (r & 31); }
+TGG_HD int generic_gated_up(int r, int up) { return (r & 32) ? up : 0; }
 
 // Element offset, from an operand window's start, of (row, k): rows K-contiguous (row stride s_row) ...
 TGG_HD int64_t generic_elem_kmajor(int row, int64_t s_row, int64_t k) { return (int64_t)row * s_row + k; }

@@ -146,6 +146,83 @@ PyObject* m_grouped_gemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// The code of an activation's name; -1 for anything else (the wrapper says what is wrong).
+int activation_code(PyObject* o) {
+  if (!PyUnicode_Check(o)) return -1;
+  if (PyUnicode_CompareWithASCIIString(o, "silu") == 0) return TGG_SILU;
+  return PyUnicode_CompareWithASCIIString(o, "gelu_tanh") == 0 ? TGG_GELU_TANH : -1;
+}
+
+// Gives (first, second) as a Python pair.
+PyObject* pair(const at::Tensor& first, const at::Tensor& second) {
+  PyObject* const t = PyTuple_New(2);
+  if (!t) return nullptr;
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(first));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(second));
+  return t;
+}
+
+// (A, B, sizes, trans_b, activation, num_cu, projections) -> C, or (C, H)
+PyObject* m_grouped_gated_gemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TGG_ARGS(7);
+  TGG_TENSOR(a, 0);
+  TGG_TENSOR(b, 1);
+  TGG_TENSOR(sizes, 2);
+  TGG_TRUTH(trans_b, 3);
+  const int act = activation_code(args[4]);
+  TGG_INT(num_cu, 5);
+  TGG_TRUTH(projections, 6);
+  if (act < 0 || a.dim() != 2 || b.dim() != 3 || records(a) || records(b)) Py_RETURN_NONE;
+  const int64_t m = a.size(0), k = a.size(1), g = b.size(0), n = b.size(trans_b ? 1 : 2);
+  const int dt = code16(a);
+  if (dt < 0 || b.scalar_type() != a.scalar_type() || b.size(trans_b ? 2 : 1) != k || n < 16 || (n & 15) || (k & 7) || g < 1 || g > kMaxGroups ||
+      m == 0 || n >= (1ll << 31) || k >= (1ll << 31) || !sizes_ok(sizes, g) || !a.is_contiguous() || !b.is_contiguous())
+    Py_RETURN_NONE;
+  static const c10::OperatorName plain_op("moe::m_grouped_gated_gemm", ""), both_op("moe::m_grouped_gated_gemm_projections", "");
+  const c10::OperatorName& op = projections ? both_op : plain_op;
+  if (replaced(op)) Py_RETURN_NONE;
+  RECORD_FUNCTION(op.name, std::vector<c10::IValue>({a, b, sizes, trans_b, (int64_t)act, (int64_t)num_cu}));
+  at::Tensor c, h;
+  int rc;
+  {
+    const Unlocked unlocked;
+    c = at::empty({m, n / 2}, a.options());
+    if (projections) h = at::empty({m, n}, a.options());
+    rc = tgg_m_grouped_gated_gemm(a.data_ptr(), b.data_ptr(), c.data_ptr(), projections ? h.data_ptr() : nullptr, sizes.data_ptr(), is64(sizes),
+                                  (int)g, m, (int)(n / 2), (int)k, trans_b, act, dt, (int)num_cu, stream());
+  }
+  return rc == 0 && projections ? pair(c, h) : done("tgg_m_grouped_gated_gemm", rc, c);
+  END_HANDLE_TH_ERRORS
+}
+
+// (grad, h, activation) -> dh
+PyObject* gated_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TGG_ARGS(3);
+  TGG_TENSOR(grad, 0);
+  TGG_TENSOR(h, 1);
+  const int act = activation_code(args[2]);
+  if (act < 0 || grad.dim() != 2 || h.dim() != 2 || records(grad) || records(h)) Py_RETURN_NONE;
+  const int64_t m = grad.size(0), f = grad.size(1);
+  const int dt = code16(h);
+  if (dt < 0 || grad.scalar_type() != h.scalar_type() || m == 0 || h.size(0) != m || h.size(1) != 2 * f || f < 8 || (f & 7) || f >= (1ll << 30) ||
+      !grad.is_contiguous() || !h.is_contiguous())
+    Py_RETURN_NONE;
+  static const c10::OperatorName op("moe::gated_backward", "");
+  if (replaced(op)) Py_RETURN_NONE;
+  RECORD_FUNCTION(op.name, std::vector<c10::IValue>({grad, h, (int64_t)act}));
+  at::Tensor dh;
+  int rc;
+  {
+    const Unlocked unlocked;
+    dh = at::empty({m, 2 * f}, h.options());
+    rc = tgg_gated_backward(grad.data_ptr(), h.data_ptr(), dh.data_ptr(), m, (int)f, act, dt, stream());
+  }
+  return done("tgg_gated_backward", rc, dh);
+  END_HANDLE_TH_ERRORS
+}
+
 // (lhs, rhs, out, masked_m, expected_m, trans_b) -> out
 PyObject* m_grouped_gemm_masked(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -244,14 +321,6 @@ PyObject* m_grouped_gemm_fp8_channel(PyObject*, PyObject* const* args, Py_ssize_
   END_HANDLE_TH_ERRORS
 }
 
-// Gives (first, second) as a Python pair.
-PyObject* pair(const at::Tensor& first, const at::Tensor& second) {
-  PyObject* const t = PyTuple_New(2);
-  if (!t) return nullptr;
-  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(first));
-  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(second));
-  return t;
-}
 
 // The sort's workspace; undefined when it needs none.
 at::Tensor sort_workspace(int64_t tokens, int64_t topk, int64_t experts, const at::Tensor& like, int64_t& bytes) {
@@ -313,6 +382,30 @@ PyObject* permute(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // (input, row_id_map, probs or None) -> out; records nothing
+// (logits, topk, scoring code, renormalize) -> (probs, indices)
+PyObject* topk_router(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TGG_ARGS(4);
+  TGG_TENSOR(logits, 0);
+  TGG_INT(topk, 1);
+  TGG_INT(scoring, 2);
+  TGG_TRUTH(renorm, 3);
+  if (logits.dim() != 2 || logits.numel() == 0 || logits.stride(1) != 1 || logits.size(1) > kMaxExperts || topk < 1 || topk > 64 || topk > logits.size(1)) Py_RETURN_NONE;
+  const int dt = logits.scalar_type() == at::kFloat ? 2 : code16(logits);
+  if (dt < 0) Py_RETURN_NONE;
+  at::Tensor probs, indices;
+  int rc;
+  {
+    const Unlocked unlocked;
+    probs = at::empty({logits.size(0), (int64_t)topk}, logits.options().dtype(at::kFloat));
+    indices = at::empty({logits.size(0), (int64_t)topk}, logits.options().dtype(at::kInt));
+    rc = tgg_moe_router(logits.data_ptr(), logits.stride(0), logits.size(0), (int)logits.size(1), (int)topk, (int)scoring, renorm, dt, (float*)probs.data_ptr(),
+                        (int32_t*)indices.data_ptr(), stream());
+  }
+  return rc != 0 ? done("tgg_moe_router", rc, probs) : pair(probs, indices);
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* unpermute(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   TGG_ARGS(3);
@@ -507,11 +600,14 @@ PyMethodDef methods[] = {
     {"m_grouped_bf16_contiguous", (PyCFunction)(void*)m_grouped_bf16_contiguous, METH_FASTCALL, nullptr},
     {"m_grouped_fp8_contiguous", (PyCFunction)(void*)m_grouped_fp8_contiguous, METH_FASTCALL, nullptr},
     {"m_grouped_gemm", (PyCFunction)(void*)m_grouped_gemm, METH_FASTCALL, nullptr},
+    {"m_grouped_gated_gemm", (PyCFunction)(void*)m_grouped_gated_gemm, METH_FASTCALL, nullptr},
+    {"gated_backward", (PyCFunction)(void*)gated_backward, METH_FASTCALL, nullptr},
     {"m_grouped_gemm_masked", (PyCFunction)(void*)m_grouped_gemm_masked, METH_FASTCALL, nullptr},
     {"k_grouped_gemm", (PyCFunction)(void*)k_grouped_gemm, METH_FASTCALL, nullptr},
     {"m_grouped_gemm_fp8_channel", (PyCFunction)(void*)m_grouped_gemm_fp8_channel, METH_FASTCALL, nullptr},
     {"permute_map", (PyCFunction)(void*)permute_map, METH_FASTCALL, nullptr},
     {"permute", (PyCFunction)(void*)permute, METH_FASTCALL, nullptr},
+    {"topk_router", (PyCFunction)(void*)topk_router, METH_FASTCALL, nullptr},
     {"unpermute", (PyCFunction)(void*)unpermute, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

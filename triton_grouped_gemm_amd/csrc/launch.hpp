@@ -38,4 +38,10 @@ int launch_moe_unpermute_bwd(const void* grad, const void* fwd_in, const int32_t
                              void* act_grad, float* prob_grad, int64_t tokens, int topk, int64_t row_bytes, int dt,
                              hipStream_t s);
 
+// Top-k router (moe_router.hip); dt 0 = bf16, 1 = fp16, 2 = fp32
+int launch_moe_router(const void* logits, int64_t row_bytes, int64_t tokens, int E, int k, int scoring, int renorm, int dt, float* probs,
+                      int32_t* indices, hipStream_t s);
+int launch_moe_router_bwd(const void* logits, int64_t row_bytes, const float* probs, const int32_t* indices, const float* grad, int64_t tokens,
+                          int E, int k, int scoring, int renorm, int dt, void* dlogits, hipStream_t s);
+
 }  // namespace tgg

@@ -1,0 +1,319 @@
+// Top-k router of a mixture-of-experts layer: the k largest of a token's E logits, their probabilities, and the gradient.
+//
+// Order of a row: larger logit first, equal ones (and -0 and +0) by index, NaN above every number.  A logit of -inf is a masked expert and never
+// chosen: what is left of the k entries then has index -1 (an assignment that the token movement drops) and probability 0.
+//   softmax   p_e = exp(l_e - max) / sum over all experts      sigmoid   p_e = 1 / (1 + exp(-l_e))
+//   renormalised: q_k = p_k / sum of the chosen p.  For softmax that is the softmax over the chosen logits, for sigmoid the softmax over the
+//   chosen log sigma(l): no quotient of vanishing numbers.
+// Everything is fp32.
+//
+// LPT lanes work on a token, each on VPL neighbouring logits.  A lane's logits become integer keys that sort like them (for 16-bit logits with the
+// index in the lower half: one 32-bit key says which, and no two are equal; 64 bits for fp32), sorted in registers once by a network; the k
+// largest of the row are then k rounds of a maximum over the lanes' heads (moves between lanes inside the vector unit) after which the one lane that
+// owns the maximum pops its list.  Lane t of a token keeps round t's result, so that probabilities and stores are one step for all of them.
+#include "common.hpp"
+#include "launch.hpp"
+
+namespace tgg {
+
+namespace {
+
+enum : int { RT_BF16 = 0, RT_F16 = 1, RT_F32 = 2 };
+enum : int { SCORE_SOFTMAX = 0, SCORE_SIGMOID = 1 };
+constexpr int kRouterThreads = 256;
+
+// Maximum / sum over the LPT lanes of a token, in every one of them.
+template <int CTRL> TGG_DEV uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false); }
+template <int LPT, class F> TGG_DEV uint32_t over_lanes(uint32_t v, const F& f) {
+  v = f(v, dpp<0xB1>(v));   // quad_perm [1,0,3,2]
+  v = f(v, dpp<0x4E>(v));   // quad_perm [2,3,0,1]
+  v = f(v, dpp<0x141>(v));  // row_half_mirror: the other four of eight
+  v = f(v, dpp<0x140>(v));  // row_mirror: the other eight of sixteen
+  if (LPT > 16) v = f(v, (uint32_t)__shfl_xor((int)v, 16, 64));
+  if (LPT > 32) v = f(v, (uint32_t)__shfl_xor((int)v, 32, 64));
+  return v;
+}
+template <int LPT> TGG_DEV uint32_t max_over(uint32_t v) { return over_lanes<LPT>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); }
+template <int LPT> TGG_DEV uint64_t max_over(uint64_t v) {
+  const uint32_t hi = max_over<LPT>((uint32_t)(v >> 32));
+  const uint32_t lo = max_over<LPT>((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+  return ((uint64_t)hi << 32) | lo;
+}
+template <int LPT> TGG_DEV float sum_over(float v) {
+  return __builtin_bit_cast(float, over_lanes<LPT>(__builtin_bit_cast(uint32_t, v), [](uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b)); }));
+}
+
+// A logit as it was read, in the upper bits of a word.
+template <int RT> TGG_DEV float logit_value(uint32_t u) {
+  if (RT == RT_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
+  return __builtin_bit_cast(float, u);
+}
+// Its place in the order, as an unsigned integer above 0: 16-bit logits fill the upper 16 bits.
+template <int RT> TGG_DEV uint32_t logit_order(uint32_t u) {
+  constexpr uint32_t inf = RT == RT_F16 ? 0x7c000000u : 0x7f800000u, most = RT == RT_F32 ? 0xffffffffu : 0xffff0000u;
+  const uint32_t mag = u & 0x7fffffffu, flip = (uint32_t)((int)u >> 31) | 0x80000000u;
+  uint32_t key = (u ^ flip) & most;
+  if (mag == 0) key = 0x80000000u;  // -0 is +0
+  if (mag > inf) key = most;        // NaN
+  return key;
+}
+template <int RT> TGG_DEV uint32_t logit_of_order(uint32_t key) { return key & 0x80000000u ? key ^ 0x80000000u : ~key & (RT == RT_F32 ? 0xffffffffu : 0xffff0000u); }
+
+template <int RT> struct KeyOf { typedef uint32_t type; };
+template <> struct KeyOf<RT_F32> { typedef uint64_t type; };
+template <int RT> TGG_DEV typename KeyOf<RT>::type make_key(uint32_t u, int e) {
+  if constexpr (RT == RT_F32) return ((uint64_t)logit_order<RT>(u) << 32) | (0xffffffffu - (uint32_t)e);
+  else return logit_order<RT>(u) | (0xffffu - (uint32_t)e);
+}
+template <int RT> TGG_DEV uint32_t key_logit(typename KeyOf<RT>::type key) {
+  if constexpr (RT == RT_F32) return logit_of_order<RT>((uint32_t)(key >> 32));
+  else return logit_of_order<RT>(key & 0xffff0000u);
+}
+template <int RT> TGG_DEV int key_index(typename KeyOf<RT>::type key) {
+  if constexpr (RT == RT_F32) return (int)(0xffffffffu - (uint32_t)key);
+  else return (int)(0xffffu - (key & 0xffffu));
+}
+
+// VPL logits of a row from element e0 on, in the upper bits; those beyond E are -inf.  vec: rows begin on 16 bytes.
+template <int RT, int VPL> TGG_DEV void load_logits(const void* row, int e0, int E, bool vec, uint32_t (&u)[VPL]) {
+  constexpr uint32_t masked = RT == RT_F16 ? 0xfc000000u : 0xff800000u;
+  constexpr int ES = RT == RT_F32 ? 4 : 2, PER = 16 / ES;
+  if constexpr (VPL >= PER) {
+    if (vec && e0 + VPL <= E) {
+#pragma unroll
+      for (int c = 0; c < VPL / PER; ++c) {
+        const uint4 w = *(const uint4*)((const char*)row + (int64_t)e0 * ES + c * 16);
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (RT == RT_F32) u[c * 4 + i] = x[i];
+          else {
+            u[c * 8 + 2 * i] = x[i] << 16;
+            u[c * 8 + 2 * i + 1] = x[i] & 0xffff0000u;
+          }
+        }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    u[i] = masked;
+    if (e0 + i < E) u[i] = RT == RT_F32 ? ((const uint32_t*)row)[e0 + i] : (uint32_t)((const uint16_t*)row)[e0 + i] << 16;
+  }
+}
+
+// Descending order by a merge network of comparisons between fixed places.
+template <int N, class K> TGG_DEV void sort_descending(K (&key)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p <<= 1)
+#pragma unroll
+    for (int q = p; q >= 1; q >>= 1)
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const K a = key[i + j], b = key[i + j + q];
+            key[i + j] = a > b ? a : b;
+            key[i + j + q] = a > b ? b : a;
+          }
+}
+
+TGG_DEV float log_sigmoid(float x) { return fminf(x, 0.f) - log1pf(expf(-fabsf(x))); }
+
+// The row's largest logit for the exponentials; of a row without experts 0, so that every exp(l - max) is 0 there.
+TGG_DEV float shift_of(float top) { return top == -__builtin_inff() ? 0.f : top; }
+
+template <int RT, int LPT, int VPL>
+__global__ __launch_bounds__(kRouterThreads) void router_fwd_kernel(const char* __restrict__ logits, int64_t row_bytes, int64_t tokens, int E, int k,
+                                                                    int scoring, int renorm, int vec, float* __restrict__ probs, int32_t* __restrict__ indices) {
+  typedef typename KeyOf<RT>::type Key;
+  const int lane = threadIdx.x % LPT, e0 = lane * VPL;
+  const int64_t token = (int64_t)blockIdx.x * (kRouterThreads / LPT) + threadIdx.x / LPT;
+  const bool live = token < tokens;
+  uint32_t u[VPL];
+  load_logits<RT, VPL>(logits + token * row_bytes, e0, live ? E : 0, vec, u);
+  Key key[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) key[i] = e0 + i < E ? make_key<RT>(u[i], e0 + i) : 0;
+  sort_descending(key);
+  Key mine = 0;  // lane t: the t-th of the row
+  Key first = 0;
+  for (int t = 0; t < k; ++t) {
+    const Key top = max_over<LPT>(key[0]);
+    if (t == 0) first = top;
+    if (lane == t) mine = top;
+    const bool own = key[0] == top;
+#pragma unroll
+    for (int i = 0; i + 1 < VPL; ++i) key[i] = own ? key[i + 1] : key[i];
+    if (own) key[VPL - 1] = 0;
+  }
+  const float x = logit_value<RT>(key_logit<RT>(mine));
+  const bool chosen = lane < k && !(x == -__builtin_inff());
+  const float top = shift_of(logit_value<RT>(key_logit<RT>(first)));
+  float prob;
+  if (scoring == SCORE_SOFTMAX) {
+    const float e = chosen ? expf(x - top) : 0.f;
+    float sum;
+    if (renorm) {
+      sum = sum_over<LPT>(e);
+    } else {
+      float part = 0.f;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) part += expf(logit_value<RT>(u[i]) - top);  // those beyond E are -inf
+      sum = sum_over<LPT>(part);
+    }
+    prob = e / sum;
+  } else if (renorm) {  // log sigma rises with the logit: the first is the largest
+    const float e = chosen ? expf(log_sigmoid(x) - log_sigmoid(top)) : 0.f;
+    prob = e / sum_over<LPT>(e);
+  } else {
+    prob = 1.f / (1.f + expf(-x));
+  }
+  if (live && lane < k) {
+    probs[token * k + lane] = chosen ? prob : 0.f;
+    indices[token * k + lane] = chosen ? key_index<RT>(mine) : -1;
+  }
+}
+
+template <int RT> TGG_DEV void store_logit(char* row, int e, float v) {
+  if constexpr (RT == RT_F32) ((float*)row)[e] = v;
+  else ((uint16_t*)row)[e] = Out16<RT>::cvt(v);
+}
+
+// Gradient of the logits.  What the chosen experts get, lane t of a token computes from round t's probability; through a row of LDS it reaches the lane
+// that writes that expert's logit.
+template <int RT, int LPT, int VPL>
+__global__ __launch_bounds__(kRouterThreads) void router_bwd_kernel(const char* __restrict__ logits, int64_t row_bytes, const float* __restrict__ probs,
+                                                                    const int32_t* __restrict__ indices, const float* __restrict__ grad, int64_t tokens, int E, int k,
+                                                                    int scoring, int renorm, int vec, char* __restrict__ dlogits, int vec_out) {
+  __shared__ __attribute__((aligned(16))) float part[kRouterThreads / LPT][LPT * VPL];
+  constexpr int ES = RT == RT_F32 ? 4 : 2;
+  const int lane = threadIdx.x % LPT, slot = threadIdx.x / LPT, e0 = lane * VPL;
+  const int64_t token = (int64_t)blockIdx.x * (kRouterThreads / LPT) + slot;
+  const bool live = token < tokens;
+  const char* const row = logits + token * row_bytes;
+  int at = -1;
+  float p = 0.f, d = 0.f, x = 0.f;
+  if (live && lane < k) {
+    at = indices[token * k + lane];
+    if (at >= 0 && at < E) {
+      p = probs[token * k + lane];
+      d = grad[token * k + lane];
+      if (scoring == SCORE_SIGMOID) x = RT == RT_F32 ? ((const float*)row)[at] : logit_value<RT>((uint32_t)((const uint16_t*)row)[at] << 16);
+    } else {
+      at = -1;
+    }
+  }
+  const float pd = p * d, all = sum_over<LPT>(pd);
+  float v = renorm ? p * (d - all) : pd;
+  if (scoring == SCORE_SIGMOID) v *= 1.f / (1.f + expf(x));
+  float* const mine = part[slot];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) mine[i * LPT + lane] = 0.f;
+  if (at >= 0) mine[at % VPL * LPT + at / VPL] = v;  // logit e in place (e mod VPL, e / VPL): the lanes' reads below are neighbours
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // a token's lanes are of one wave: LDS serves them in order
+  float g[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) g[i] = mine[i * LPT + lane];
+  if (scoring == SCORE_SOFTMAX && !renorm) {  // every expert's probability took part in the sum
+    uint32_t u[VPL];
+    load_logits<RT, VPL>(row, e0, live ? E : 0, vec, u);
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const uint32_t o = logit_order<RT>(u[i]);
+      most = o > most ? o : most;
+    }
+    const float top = shift_of(logit_value<RT>(logit_of_order<RT>(max_over<LPT>(most))));
+    float e[VPL], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) sum += e[i] = expf(logit_value<RT>(u[i]) - top);
+    sum = sum_over<LPT>(sum);
+    const float scale = sum > 0.f || sum != sum ? all / sum : 0.f;  // a row without experts has no gradient
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) g[i] -= e[i] * scale;
+  }
+  if (!live) return;
+  char* const out = dlogits + token * (int64_t)E * ES;
+  if constexpr (VPL * ES >= 16) {
+    if (vec_out && e0 + VPL <= E) {
+      if constexpr (RT == RT_F32) {
+#pragma unroll
+        for (int c = 0; c < VPL / 4; ++c) *(float4*)(out + (int64_t)e0 * 4 + c * 16) = make_float4(g[4 * c], g[4 * c + 1], g[4 * c + 2], g[4 * c + 3]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < VPL / 8; ++c) {
+          uint4 w;
+          w.x = pack2<RT>(g[8 * c], g[8 * c + 1]);
+          w.y = pack2<RT>(g[8 * c + 2], g[8 * c + 3]);
+          w.z = pack2<RT>(g[8 * c + 4], g[8 * c + 5]);
+          w.w = pack2<RT>(g[8 * c + 6], g[8 * c + 7]);
+          *(uint4*)(out + (int64_t)e0 * 2 + c * 16) = w;
+        }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VPL; ++i)
+    if (e0 + i < E) store_logit<RT>(out, e0 + i, g[i]);
+}
+
+struct RouterArgs {
+  const char* logits;
+  int64_t row_bytes, tokens;
+  int E, k, scoring, renorm;
+  float* probs;         // forward: written; backward: read
+  int32_t* indices;
+  const float* grad;    // backward
+  char* dlogits;
+};
+
+template <int RT, int LPT, int VPL, bool BWD>
+int launch_router_as(const RouterArgs& a, hipStream_t s) {
+  constexpr int ES = RT == RT_F32 ? 4 : 2, PER = kRouterThreads / LPT;
+  const int64_t blocks = (a.tokens + PER - 1) / PER;
+  if (blocks > 0x7fffffff) return set_error("router over %lld tokens: too many", (long long)a.tokens);
+  const int vec = ((uintptr_t)a.logits & 15) == 0 && (a.row_bytes & 15) == 0;
+  if constexpr (BWD) {
+    const int vec_out = ((uintptr_t)a.dlogits & 15) == 0 && (a.E * ES & 15) == 0;
+    hipLaunchKernelGGL((router_bwd_kernel<RT, LPT, VPL>), dim3((uint32_t)blocks), dim3(kRouterThreads), 0, s, a.logits, a.row_bytes, a.probs, a.indices, a.grad, a.tokens,
+                       a.E, a.k, a.scoring, a.renorm, vec, a.dlogits, vec_out);
+  } else {
+    hipLaunchKernelGGL((router_fwd_kernel<RT, LPT, VPL>), dim3((uint32_t)blocks), dim3(kRouterThreads), 0, s, a.logits, a.row_bytes, a.tokens, a.E, a.k, a.scoring, a.renorm,
+                       vec, a.probs, a.indices);
+  }
+  return check_launch("moe_router");
+}
+
+// As few lanes a token as its experts (eight logits a lane; two in rows of at most 32 experts, sixteen in rows of more than 512) and its k results need.
+template <int RT, bool BWD>
+int launch_router_type(const RouterArgs& a, hipStream_t s) {
+  if (a.E <= 32 && a.k <= 16) return launch_router_as<RT, 16, 2, BWD>(a, s);
+  if (a.E <= 128 && a.k <= 16) return launch_router_as<RT, 16, 8, BWD>(a, s);
+  if (a.E <= 256 && a.k <= 32) return launch_router_as<RT, 32, 8, BWD>(a, s);
+  if (a.E <= 512) return launch_router_as<RT, 64, 8, BWD>(a, s);
+  return launch_router_as<RT, 64, 16, BWD>(a, s);
+}
+
+template <bool BWD>
+int launch_router(const RouterArgs& a, int dt, hipStream_t s) {
+  if (dt == RT_BF16) return launch_router_type<RT_BF16, BWD>(a, s);
+  if (dt == RT_F16) return launch_router_type<RT_F16, BWD>(a, s);
+  return launch_router_type<RT_F32, BWD>(a, s);
+}
+
+}  // namespace
+
+int launch_moe_router(const void* logits, int64_t row_bytes, int64_t tokens, int E, int k, int scoring, int renorm, int dt, float* probs, int32_t* indices, hipStream_t s) {
+  return launch_router<false>(RouterArgs{(const char*)logits, row_bytes, tokens, E, k, scoring, renorm, probs, indices, nullptr, nullptr}, dt, s);
+}
+int launch_moe_router_bwd(const void* logits, int64_t row_bytes, const float* probs, const int32_t* indices, const float* grad, int64_t tokens, int E, int k, int scoring,
+                          int renorm, int dt, void* dlogits, hipStream_t s) {
+  return launch_router<true>(RouterArgs{(const char*)logits, row_bytes, tokens, E, k, scoring, renorm, (float*)probs, (int32_t*)indices, grad, (char*)dlogits}, dt, s);
+}
+
+}  // namespace tgg

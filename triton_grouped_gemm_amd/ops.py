@@ -16,6 +16,7 @@ from . import _native
 from ._native import require_gpu
 from .gemm.BF16.k_grouped_gemm import k_grouped_gemm
 from .gemm.BF16.m_grouped_gemm import m_grouped_gemm
+from .gemm.gated import gated_backward, m_grouped_gated_gemm, m_grouped_gated_gemm_projections
 
 
 def _device_sizes(batch_sizes: torch.Tensor, device: torch.device) -> torch.Tensor:
@@ -66,6 +67,44 @@ def gmm(a, b, batch_sizes, trans_b=False, num_sm=-1):
         if out is not None:
             return out
     return GroupedGemm.apply(a, b, batch_sizes, trans_b, num_sm)
+
+
+class GatedGroupedGemm(torch.autograd.Function):
+    """``gated_gmm`` with the gradients of activations and weights: the projections are kept (in the operands' type), one pass
+    makes their gradient ``dh`` from the output's, and the grouped products of ``dh`` are those of ``gmm``."""
+
+    @staticmethod
+    def forward(ctx, a, b, batch_sizes, activation, trans_b, num_sm):
+        sizes = _device_sizes(batch_sizes, a.device)
+        out, h = m_grouped_gated_gemm_projections(a, b, sizes, bool(trans_b), activation, int(num_sm))
+        ctx.save_for_backward(a, b, sizes, h)
+        ctx.activation, ctx.trans_b, ctx.num_sm = activation, bool(trans_b), int(num_sm)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        a, b, sizes, h = ctx.saved_tensors
+        if not a.shape[0]:  # no rows: nothing to launch
+            return torch.zeros_like(a), torch.zeros_like(b), None, None, None, None
+        dh = gated_backward(grad.contiguous(), h, ctx.activation)
+        agrad = bgrad = None
+        if ctx.needs_input_grad[0]:
+            agrad = m_grouped_gemm(dh, b.contiguous(), sizes, not ctx.trans_b, ctx.num_sm)
+        if ctx.needs_input_grad[1]:
+            lhs, rhs = (dh, a.contiguous()) if ctx.trans_b else (a.contiguous(), dh)
+            bgrad = k_grouped_gemm(lhs, rhs, sizes, numSM=ctx.num_sm)
+        return agrad, bgrad, None, None, None, None
+
+
+def gated_gmm(a, b, batch_sizes, activation="silu", trans_b=False, num_sm=-1):
+    """The gated feed-forward block of every expert: ``act(a_g @ gate_g) * (a_g @ up_g)``, ``[M, F]``, where ``b`` is
+    ``[G, K, 2 F]`` (``[G, 2 F, K]`` with ``trans_b``), gate first, and ``activation`` is ``"silu"`` or ``"gelu_tanh"``.  Stands where
+    ``gmm``, ``chunk``, the activation and the product would; fp32 from the products to the one rounding of the result."""
+    require_gpu(a, b)
+    if not _records(a, b):
+        return m_grouped_gated_gemm(a, b, _device_sizes(batch_sizes, a.device), bool(trans_b), activation, int(num_sm))
+    return GatedGroupedGemm.apply(a, b, batch_sizes, activation, trans_b, num_sm)
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -276,3 +315,76 @@ def unpermute(input_act, row_id_map, probs=None):
         if out is not None:
             return out
     return UnpermuteMoE_topK.apply(input_act, row_id_map, probs)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Top-k router: what permute / unpermute take
+# ---------------------------------------------------------------------------------------------------------------
+_SCORING_CODE = {"softmax": 0, "sigmoid": 1}  # TGG_SOFTMAX, TGG_SIGMOID
+_LOGIT_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_TOPK = 64
+
+
+def _router_forward(logits, topk, scoring, renormalize):
+    result = _native.host().topk_router(logits, topk, scoring, renormalize)
+    if result is not None:
+        return result
+    probs = torch.empty((logits.shape[0], topk), dtype=torch.float32, device=logits.device)
+    indices = torch.empty((logits.shape[0], topk), dtype=torch.int32, device=logits.device)
+    if logits.shape[0]:
+        with torch.cuda.device(logits.device):
+            _native.call("tgg_moe_router", logits.data_ptr(), logits.stride(0), logits.shape[0], logits.shape[1], topk, scoring,
+                         int(renormalize), _LOGIT_CODE[logits.dtype], probs.data_ptr(), indices.data_ptr(),
+                         _native.stream_of(logits))
+    return probs, indices
+
+
+class TopkRouter(torch.autograd.Function):
+    """``topk_router`` with the gradient of the logits; the experts' numbers have none."""
+
+    @staticmethod
+    def forward(ctx, logits, topk, scoring, renormalize):
+        probs, indices = _router_forward(logits.detach(), topk, scoring, renormalize)
+        ctx.mark_non_differentiable(indices)
+        ctx.save_for_backward(logits, probs, indices)
+        ctx.scoring, ctx.renormalize = scoring, renormalize
+        return probs, indices
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):
+        logits, probs, indices = ctx.saved_tensors
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if logits.shape[0]:
+            grad = grad.contiguous()
+            with torch.cuda.device(logits.device):
+                _native.call("tgg_moe_router_bwd", logits.data_ptr(), logits.stride(0), probs.data_ptr(), indices.data_ptr(),
+                             grad.data_ptr(), logits.shape[0], logits.shape[1], probs.shape[1], ctx.scoring,
+                             int(ctx.renormalize), _LOGIT_CODE[logits.dtype], out.data_ptr(), _native.stream_of(logits))
+        return out, None, None, None
+
+
+def topk_router(logits, topk, scoring="softmax", renormalize=True):
+    """The ``topk`` experts of every token and their probabilities: ``(probs [T, topk] fp32, indices [T, topk] int32)``, in the form
+    that ``permute`` (``indices``) and ``unpermute`` (``probs``) take.
+
+    ``logits`` ``[T, E]`` bf16, fp16 or fp32 (E <= 1024, topk <= 64).  Larger logits come first, equal ones by index, NaN above
+    all.  ``scoring``: ``"softmax"`` over all experts or ``"sigmoid"``; ``renormalize`` divides the chosen probabilities by their
+    sum.  A logit of ``-inf`` masks an expert, which is then never chosen: entries left over have index -1, an assignment that ``permute``
+    drops, and probability 0.  Arithmetic is fp32; differentiable in ``logits``."""
+    if scoring not in _SCORING_CODE:
+        raise ValueError(f"scoring must be one of {sorted(_SCORING_CODE)}, got {scoring!r}")
+    require_gpu(logits)
+    if logits.dim() != 2 or logits.dtype not in _LOGIT_CODE:
+        raise ValueError(f"logits must be a [tokens, experts] tensor in bf16, fp16 or fp32, got {tuple(logits.shape)} {logits.dtype}")
+    experts, topk = logits.shape[1], int(topk)
+    if not 1 <= experts <= MAX_EXPERTS:
+        raise ValueError(f"the number of experts must be in [1, {MAX_EXPERTS}], got {experts}")
+    if not 1 <= topk <= min(MAX_TOPK, experts):
+        raise ValueError(f"topk must be in [1, {min(MAX_TOPK, experts)}], got {topk}")
+    if logits.stride(1) != 1 and experts > 1 or logits.stride(0) < experts:
+        logits = logits.contiguous()
+    code, renormalize = _SCORING_CODE[scoring], bool(renormalize)
+    if not _records(logits):
+        return _router_forward(logits, topk, code, renormalize)
+    return TopkRouter.apply(logits, topk, code, renormalize)
