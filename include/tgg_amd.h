@@ -51,6 +51,16 @@ int tgg_m_grouped_gated_gemm(const void* A, const void* B, void* C, void* H, con
  * tgg_k_grouped_gemm_sizes). */
 int tgg_gated_backward(const void* dout, const void* h, void* dh, int64_t M, int F, int activation, int dtype, void* stream);
 
+/* C[r,:] = A[r,:] . W[g(r)]^T with 4-bit weights W[g][n,k] = (q - z[n, k / group_size]) * s[n, k / group_size], q in 0..15; with
+ * activation (TGG_SILU, TGG_GELU_TANH; -1: none) the gated block of N = 2 F columns, C [M,F] = act(gate) * up.
+ *   codes   [G, ceil(N/16), ceil(K/128), 64, 16] bytes: byte 4 s + m of entry 16 lg + c holds the values k = 128 kb + 32 s + 8 lg + e of
+ *           column n = 16 nb + c, low nibble e = 4 m (m < 2) or 4 m - 7, high nibble e + 2; what lies beyond N or K is not used
+ *   scales  [G, ceil(K/group_size), N] in the activations' type;  zeros  the same shape, one byte each (0..15), or NULL: 8
+ * group_size 32, 64 or a multiple of 128.  N and K are multiples of 8, N of 32 with an activation.  fp32 sums, one rounding; the weights are
+ * not rounded.  Meant for few rows a group (a decode step).  Rows past sum(sizes) are not written.  The reference has no counterpart. */
+int tgg_m_grouped_gemm_int4(const void* A, const void* codes, const void* scales, const void* zeros, void* C, const void* sizes, int sizes_i64, int G, int64_t M,
+                            int N, int K, int group_size, int activation, int dtype, int num_cu, void* stream);
+
 /* Same contraction with A/C physically padded: group g starts at sum_{h<g} round_up(sizes[h], align).
  * Replaces deep_gemm.m_grouped_bf16_gemm_nt_contiguous as called from m_grouped_bf16_nt_contiguous
  * (gemm/deep_gemm_ops.py:24-57).  Pad rows of C are not written. */

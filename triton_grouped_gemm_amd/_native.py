@@ -25,6 +25,7 @@ _P, _I, _L = c_void_p, c_int, c_int64
 SIGNATURES = {
     "tgg_m_grouped_gemm": [_P, _P, _P, _P, _I, _I, _L, _I, _I, _I, _I, _I, _P],
     "tgg_m_grouped_gated_gemm": [_P, _P, _P, _P, _P, _I, _I, _L, _I, _I, _I, _I, _I, _I, _P],
+    "tgg_m_grouped_gemm_int4": [_P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _I, _I, _I, _I, _I, _P],
     "tgg_gated_backward": [_P, _P, _P, _L, _I, _I, _I, _P],
     "tgg_m_grouped_gemm_padded": [_P, _P, _P, _P, _I, _I, _L, _I, _I, _I, _I, _I, _P],
     "tgg_m_grouped_gemm_placed": [_P, _P, _P, _P, _I, _P, _I, _L, _I, _I, _I, _I, _P],

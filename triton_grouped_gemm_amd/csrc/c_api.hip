@@ -84,6 +84,7 @@ void set_fp8_variant(int v);
 bool fast_gated_supported(const GemmParams& p, int dt, int layout);
 int launch_fast_gated(const GemmParams& p, int dt, int layout, hipStream_t s);
 int launch_generic_gated(const GemmParams& p, int dt, int layout, hipStream_t s);
+int launch_int4(const GemmParams& g, const void* x, const uint8_t* codes, const void* scales, const uint8_t* zeros, void* out, int gs, bool gated, int dt, hipStream_t s);
 int launch_gated_bwd(const void* dout, const void* h, void* dh, int64_t rows, int F, int act, int dt, hipStream_t s);
 
 static bool aligned16(const void* p) { return (((uintptr_t)p) & 15) == 0; }
@@ -370,6 +371,25 @@ int tgg_gated_backward(const void* dout, const void* h, void* dh, int64_t M, int
   if (activation != TGG_SILU && activation != TGG_GELU_TANH) return set_error("activation code %d not supported", activation);
   if (M == 0) return 0;
   return launch_gated_bwd(dout, h, dh, M, F, activation, dtype, (hipStream_t)stream);
+}
+
+int tgg_m_grouped_gemm_int4(const void* A, const void* codes, const void* scales, const void* zeros, void* C, const void* sizes, int sizes_i64, int G, int64_t M,
+                            int N, int K, int group_size, int activation, int dtype, int num_cu, void* stream) {
+  if (int e = check_common(A, codes, C, sizes, G, N, TGG_MAX_GROUPS)) return e;
+  if (!scales) return set_error("null scale pointer");
+  if (((uintptr_t)scales & 15) != 0) return set_error("operand pointers must be 16-byte aligned");
+  if (M < 0 || K < 0) return set_error("negative M or K");
+  if (dtype != TGG_BF16 && dtype != TGG_F16) return set_error("data type code %d not supported", dtype);
+  if (activation != -1 && activation != TGG_SILU && activation != TGG_GELU_TANH) return set_error("activation code %d not supported", activation);
+  if (group_size != 32 && group_size != 64 && (group_size < 128 || group_size % 128 != 0)) return set_error("group_size must be 32, 64 or a multiple of 128, got %d", group_size);
+  if ((K & 7) || (N & 7)) return set_error("N and K must be multiples of 8 (16-byte rows), got N=%d K=%d", N, K);
+  if (activation != -1 && (N & 31)) return set_error("a gated block needs gate and up columns in multiples of 16, got N=%d", N);
+  // 32-bit offsets within a group's codes and scales and within a tile's rows
+  if ((int64_t)((N + 15) / 16) * ((K + 127) / 128) * 1024 >= (1ll << 30) || (int64_t)K * 2 * 64 >= (1ll << 30)) return set_error("a group of N=%d K=%d is too large", N, K);
+  if (M == 0) return 0;
+  GemmParams p = params_m_grouped(A, codes, C, sizes, sizes_i64, G, M, N, K, 1, num_cu);
+  p.act = activation;
+  return launch_int4(p, A, (const uint8_t*)codes, scales, (const uint8_t*)zeros, C, group_size, activation != -1, dtype, (hipStream_t)stream);
 }
 
 int tgg_m_grouped_gemm_fp8_out(const void* A, const void* B, void* codes, float* scales, const void* sizes,

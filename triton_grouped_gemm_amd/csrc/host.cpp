@@ -196,6 +196,47 @@ PyObject* m_grouped_gated_gemm(PyObject*, PyObject* const* args, Py_ssize_t narg
   END_HANDLE_TH_ERRORS
 }
 
+// (A, codes, scales, sizes, group_size, zeros or None, activation or None, num_cu) -> C
+PyObject* m_grouped_gemm_int4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TGG_ARGS(8);
+  TGG_TENSOR(a, 0);
+  TGG_TENSOR(codes, 1);
+  TGG_TENSOR(scales, 2);
+  TGG_TENSOR(sizes, 3);
+  TGG_INT(gs, 4);
+  const at::Tensor* zeros = nullptr;
+  if (args[5] != Py_None) {
+    zeros = plain(args[5], device);
+    if (!zeros) Py_RETURN_NONE;
+  }
+  const bool gated = args[6] != Py_None;
+  const int act = gated ? activation_code(args[6]) : -1;
+  TGG_INT(num_cu, 7);
+  if ((gated && act < 0) || a.dim() != 2 || codes.dim() != 5 || scales.dim() != 3 || records(a) || records(scales)) Py_RETURN_NONE;
+  const int64_t m = a.size(0), k = a.size(1), g = codes.size(0), n = scales.size(2);
+  const int dt = code16(a);
+  if (dt < 0 || m == 0 || k < 8 || (k & 7) || n < 8 || (n & (gated ? 31 : 7)) || n >= (1ll << 31) || k >= (1ll << 31) || g < 1 || g > kMaxGroups ||
+      !(gs == 32 || gs == 64 || (gs >= 128 && gs % 128 == 0 && gs < (1ll << 31))) || codes.scalar_type() != at::kByte || scales.scalar_type() != a.scalar_type() ||
+      codes.size(1) != (n + 15) / 16 || codes.size(2) != (k + 127) / 128 || codes.size(3) != 64 || codes.size(4) != 16 || scales.size(0) != g ||
+      scales.size(1) != (k + gs - 1) / gs || (zeros && (zeros->scalar_type() != at::kByte || zeros->sizes() != scales.sizes() || !zeros->is_contiguous())) ||
+      !sizes_ok(sizes, g) || !a.is_contiguous() || !codes.is_contiguous() || !scales.is_contiguous())
+    Py_RETURN_NONE;
+  static const c10::OperatorName op("moe::m_grouped_gemm_int4", "");
+  if (replaced(op)) Py_RETURN_NONE;
+  RECORD_FUNCTION(op.name, std::vector<c10::IValue>({a, codes, scales, sizes, (int64_t)gs}));
+  at::Tensor c;
+  int rc;
+  {
+    const Unlocked unlocked;
+    c = at::empty({m, gated ? n / 2 : n}, a.options());
+    rc = tgg_m_grouped_gemm_int4(a.data_ptr(), codes.data_ptr(), scales.data_ptr(), zeros ? zeros->data_ptr() : nullptr, c.data_ptr(), sizes.data_ptr(),
+                                 is64(sizes), (int)g, m, (int)n, (int)k, (int)gs, act, dt, (int)num_cu, stream());
+  }
+  return done("tgg_m_grouped_gemm_int4", rc, c);
+  END_HANDLE_TH_ERRORS
+}
+
 // (grad, h, activation) -> dh
 PyObject* gated_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -601,6 +642,7 @@ PyMethodDef methods[] = {
     {"m_grouped_fp8_contiguous", (PyCFunction)(void*)m_grouped_fp8_contiguous, METH_FASTCALL, nullptr},
     {"m_grouped_gemm", (PyCFunction)(void*)m_grouped_gemm, METH_FASTCALL, nullptr},
     {"m_grouped_gated_gemm", (PyCFunction)(void*)m_grouped_gated_gemm, METH_FASTCALL, nullptr},
+    {"m_grouped_gemm_int4", (PyCFunction)(void*)m_grouped_gemm_int4, METH_FASTCALL, nullptr},
     {"gated_backward", (PyCFunction)(void*)gated_backward, METH_FASTCALL, nullptr},
     {"m_grouped_gemm_masked", (PyCFunction)(void*)m_grouped_gemm_masked, METH_FASTCALL, nullptr},
     {"k_grouped_gemm", (PyCFunction)(void*)k_grouped_gemm, METH_FASTCALL, nullptr},
