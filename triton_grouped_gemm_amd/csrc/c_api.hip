@@ -386,6 +386,7 @@ int tgg_m_grouped_gemm_int4(const void* A, const void* codes, const void* scales
   if (activation != -1 && (N & 31)) return set_error("a gated block needs gate and up columns in multiples of 16, got N=%d", N);
   // 32-bit offsets within a group's codes and scales and within a tile's rows
   if ((int64_t)((N + 15) / 16) * ((K + 127) / 128) * 1024 >= (1ll << 30) || (int64_t)K * 2 * 64 >= (1ll << 30)) return set_error("a group of N=%d K=%d is too large", N, K);
+  if (M >= (1ll << 31)) return set_error("M=%lld does not fit 32 bits", (long long)M);
   if (M == 0) return 0;
   GemmParams p = params_m_grouped(A, codes, C, sizes, sizes_i64, G, M, N, K, 1, num_cu);
   p.act = activation;

@@ -13,9 +13,12 @@
 // difference is taken in integers, 0x4310 + q - z.  Half precision has a packed subtraction: 0x6400 | q is 1024 + q, less 1024 + z exactly.  A scale
 // group's sum then enters the row's accumulator with its scale: weights are never rounded.
 //
-// A tile is up to 64 rows of a group x CB blocks of columns (weights are the multiply's first operand: a lane ends up with four neighbouring columns of a
-// row).  The four waves of a workgroup take every fourth block of 128 values along K and add up in LDS, in order; all loads go through buffer
-// descriptors, whose range check gives zeros for rows and values beyond the operands, and run two blocks ahead.
+// A tile is up to 64 rows of a group x some blocks of columns (weights are the multiply's first operand: a lane ends up with four neighbouring columns of
+// a row).  The tile's activations go through LDS in chunks of 32 KB (16 rows x 1024 values, 32 x 512 or 64 x 256), read whole rows at a time: a fragment
+// read straight from memory touches sixteen rows, a cache line for every lane (that way, with the waves' sums joined in LDS, 128 groups of 64 rows, N = 4096,
+// K = 1536: 604 us, this way 224; 512 rows over 128 groups, N = 2048, K = 768: 46 and 25).  Two chunks alternate; the one after the next waits in registers.  Codes go from memory to registers two blocks ahead.  The four waves
+// of a workgroup take columns side by side, or, where there are too few tiles to go round, every fourth block along K, and add up in LDS, in order.
+// All loads go through buffer descriptors, whose range check gives zeros for rows and values beyond the operands.
 #include <type_traits>
 
 #include "fast_common.hpp"
@@ -37,7 +40,80 @@ struct Int4Params {
 
 namespace {
 
-constexpr int kI4Threads = 256, kI4Waves = 4, kI4Rows = 64;
+constexpr int kI4Threads = 256, kI4Waves = 4, kI4Rows = 64, kI4MaxGroups = 1024;
+constexpr int kI4Chunk = 32 * 1024;  // bytes of a chunk of activations
+
+// The groups' first rows and first row tiles.  (The shared table of sched.hpp keeps 64-bit rows; with it two workgroups do not fit a compute unit.)
+struct Int4Table {
+  int32_t row[kI4MaxGroups + 1], tile[kI4MaxGroups + 1];
+  int32_t scan[2][kI4Waves];
+};
+
+// Built by the whole workgroup, four groups a thread; ends with a barrier.  Rows beyond m_total belong to no group.
+TGG_DEV void int4_table(const GemmParams& g, Int4Table& t) {
+  constexpr int PER = kI4MaxGroups / kI4Threads;
+  const int lane = lane_id(), wave = threadIdx.x >> 6, per = (g.G + kI4Threads - 1) / kI4Threads, g0 = threadIdx.x * per;
+  int64_t size[PER], sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    size[i] = i < per && g0 + i < g.G ? load_size(g.sizes, g.sizes_i64, g0 + i) : 0;
+    size[i] = size[i] < g.m_total ? size[i] : g.m_total;
+    sum += size[i];
+  }
+  // 1024 groups of at most m_total < 2^31 rows: the sum stays within 64 bits
+  __shared__ int64_t wave_rows[kI4Waves];
+  const int64_t rows_incl = sched_wave_scan(sum);
+  if (lane == 63) wave_rows[wave] = rows_incl;
+  __syncthreads();
+  int64_t row = rows_incl - sum;
+  for (int w = 0; w < wave; ++w) row += wave_rows[w];
+  int32_t first[PER], tiles = 0, count[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int64_t begin = row < g.m_total ? row : g.m_total, end = row + size[i] < g.m_total ? row + size[i] : g.m_total;
+    first[i] = (int32_t)begin;
+    count[i] = (int32_t)((end - begin + kI4Rows - 1) / kI4Rows);
+    tiles += count[i];
+    row += size[i];
+  }
+  const int32_t end_row = (int32_t)(row < g.m_total ? row : g.m_total);
+  const int32_t tiles_incl = (int32_t)sched_wave_scan(tiles);
+  if (lane == 63) t.scan[0][wave] = tiles_incl;
+  __syncthreads();
+  int32_t tile = tiles_incl - tiles;
+  for (int w = 0; w < wave; ++w) tile += t.scan[0][w];
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (i < per && g0 + i < g.G) {
+      t.row[g0 + i] = first[i];
+      t.tile[g0 + i] = tile;
+      tile += count[i];
+      if (g0 + i == g.G - 1) {
+        t.row[g.G] = end_row;
+        t.tile[g.G] = tile;
+      }
+    }
+  __syncthreads();
+}
+
+struct Int4Tile { int g, row0, rows, nt; };
+// Tile ids run over (row tile, column tile), columns innermost: what runs together shares activations, and a group's row tiles its weights.
+TGG_DEV Int4Tile int4_tile_at(const Int4Table& t, int G, int id, int tiles_n) {
+  Int4Tile r;
+  const int mt = id / tiles_n;
+  r.nt = id - mt * tiles_n;
+  int lo = 0, hi = G;  // the last group with tile[g] <= mt
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.tile[mid] <= mt) lo = mid; else hi = mid;
+  }
+  r.g = __builtin_amdgcn_readfirstlane(lo);
+  const int at = (mt - t.tile[lo]) * kI4Rows, left = t.row[lo + 1] - t.row[lo] - at;
+  r.row0 = __builtin_amdgcn_readfirstlane(t.row[lo] + at);
+  r.rows = __builtin_amdgcn_readfirstlane(left < kI4Rows ? left : kI4Rows);
+  r.nt = __builtin_amdgcn_readfirstlane(r.nt);
+  return r;
+}
 
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 TGG_DEV rsrc_t window(const void* base, int64_t bytes) {
@@ -73,27 +149,51 @@ template <int DT, bool ZEROS> TGG_DEV i32x4_t operand(uint32_t word, uint32_t zz
   return r;
 }
 
-// GPT: scale groups per 128 values (1 where a group is 128 or more)
-template <int DT, bool GATED, bool ZEROS, int GPT, int RB, int CB>
-TGG_DEV void int4_tile(const Int4Params& p, const Tile& t, float4* red) {
-  const int lane = lane_id(), l16 = lane & 15, lg = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// GPT: scale groups per 128 values (1 where a group is 128 or more).  RB: row blocks, CB: column blocks of a wave.  KSPLIT: the waves share the columns and
+// take every fourth block along K.
+template <int DT, bool GATED, bool ZEROS, int GPT, int RB, int CB, bool KSPLIT>
+TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
+  // (opaque, so that the lane's offsets are made afresh per tile: hoisted out of the tile loop, those of all variants would spill)
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int N = p.g.N, K = p.g.K, F = N / 2;
   const int blocks_n = (N + 15) / 16, blocks_k = (K + 127) / 128;
-  const int g = __builtin_amdgcn_readfirstlane(t.g), rows = __builtin_amdgcn_readfirstlane(t.rows), n0 = __builtin_amdgcn_readfirstlane(t.n0);
-  const int64_t row0 = (int64_t)uniform64((uint64_t)t.row0);
+  const int rows = t.rows;
+  const int64_t row0 = t.row0;
   const int64_t scale_elems = (int64_t)p.scale_groups * N;
-  const rsrc_t cw = window(p.codes + (int64_t)g * blocks_n * blocks_k * 1024, (int64_t)blocks_n * blocks_k * 1024);
+  const rsrc_t cw = window(p.codes + (int64_t)t.g * blocks_n * blocks_k * 1024, (int64_t)blocks_n * blocks_k * 1024);
   const rsrc_t xw = window((const char*)p.x + row0 * K * 2, (int64_t)rows * K * 2);
-  const rsrc_t sw = window((const char*)p.scales + (int64_t)g * scale_elems * 2, scale_elems * 2);
-  const rsrc_t zw = window(ZEROS ? p.zeros + (int64_t)g * scale_elems : nullptr, ZEROS ? scale_elems : 0);
+  const rsrc_t sw = window((const char*)p.scales + (int64_t)t.g * scale_elems * 2, scale_elems * 2);
+  const rsrc_t zw = window(ZEROS ? p.zeros + (int64_t)t.g * scale_elems : nullptr, ZEROS ? scale_elems : 0);
 
-  // first column of column block c: of a gated tile the first half are the gate's, the others the up projection's of the same outputs
-  auto col_of = [&](int c) { return GATED ? n0 / 2 + (c % (CB / 2)) * 16 + (c >= CB / 2 ? F : 0) : n0 + c * 16; };
+  // first column of the wave's column block c: of a gated tile the first half are the gate's, the others the up projection's of the same outputs
+  constexpr int OC = GATED ? CB / 2 : CB;  // column blocks of outputs
+  const int out0 = (t.nt * (KSPLIT ? 1 : kI4Waves) + (KSPLIT ? 0 : wave)) * OC * 16;
+  auto col_of = [&](int c) { return out0 + (c % OC) * 16 + (GATED && c >= OC ? F : 0); };
+  const int out_n = GATED ? F : N;
+
+  // ---- activations: chunks of 16 RB rows x KC values, 16-byte pieces of a row swizzled by the row's number (a fragment read touches 16 rows) ----
+  constexpr int KC = kI4Chunk / 2 / (16 * RB), PIECES = KC / 8, PER = kI4Chunk / 16 / kI4Threads, BLOCKS = KC / 128;
+  i32x4_t xr[PER];
+  auto x_load = [&](int chunk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = tid + i * kI4Threads, r = u / PIECES, k = chunk * KC + (u % PIECES) * 8;
+      xr[i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xw, k < K ? (r * K + k) * 2 : kNowhere, 0, 0));
+    }
+  };
+  auto x_store = [&](int chunk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = tid + i * kI4Threads, r = u / PIECES, c = u % PIECES;
+      *(i32x4_t*)(lds + (chunk & 1) * kI4Chunk + r * (KC * 2) + ((c ^ (r & 15)) << 4)) = xr[i];
+    }
+  };
 
   struct Stage {
     i32x4_t code[CB];
-    i32x4_t x[RB][4];
     uint2 scale[GPT][CB];
     uint8_t zero[ZEROS ? GPT : 1][CB];
   };
@@ -105,15 +205,8 @@ TGG_DEV void int4_tile(const Int4Params& p, const Tile& t, float4* red) {
       st.code[c] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(cw, live && block < blocks_n ? (block * blocks_k + kb) * 1024 + lane * 16 : kNowhere, 0, 2));
     }
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int k = kb * 128 + 32 * s + 8 * lg;
-        st.x[b][s] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xw, k < K ? ((16 * b + l16) * K + k) * 2 : kNowhere, 0, 0));
-      }
-#pragma unroll
     for (int j = 0; j < GPT; ++j) {
-      const int sg = GPT == 1 ? kb / p.blocks_per_scale : kb * GPT + j;
+      const int sg = GPT == 1 ? (p.blocks_per_scale == 1 ? kb : kb / p.blocks_per_scale) : kb * GPT + j;
 #pragma unroll
       for (int c = 0; c < CB; ++c) {
         const int n = col_of(c);
@@ -132,8 +225,14 @@ TGG_DEV void int4_tile(const Int4Params& p, const Tile& t, float4* red) {
   constexpr int bias2 = ZEROS ? (int)0xc310c310u : (int)0xc308c308u;  // -144 or -136, twice
   const i32x4_t bias = {bias2, bias2, bias2, bias2};
 
-  auto compute = [&](const Stage& st) __attribute__((always_inline)) {
+  // block kb of K, the activations' chunk at xs, of which it is block `at`
+  auto compute = [&](const Stage& st, const char* xs, int at) __attribute__((always_inline)) {
     constexpr int SP = 4 / GPT;  // steps of 32 values per scale group
+    i32x4_t x[RB][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int b = 0; b < RB; ++b) x[b][s] = *(const i32x4_t*)(xs + (16 * b + l16) * (KC * 2) + (((16 * at + 4 * s + lg) ^ l16) << 4));
 #pragma unroll
     for (int j = 0; j < GPT; ++j) {
       f32x4_t first[RB];
@@ -142,7 +241,7 @@ TGG_DEV void int4_tile(const Int4Params& p, const Tile& t, float4* red) {
         first[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         if constexpr (DT == DT_BF16) {
 #pragma unroll
-          for (int s = 0; s < SP; ++s) first[b] = mma<DT>(bias, st.x[b][j * SP + s], first[b]);
+          for (int s = 0; s < SP; ++s) first[b] = mma<DT>(bias, x[b][j * SP + s], first[b]);
         }
       }
 #pragma unroll
@@ -162,7 +261,7 @@ TGG_DEV void int4_tile(const Int4Params& p, const Tile& t, float4* red) {
         for (int b = 0; b < RB; ++b) {
           f32x4_t part = first[b];
 #pragma unroll
-          for (int s = 0; s < SP; ++s) part = mma<DT>(w[s], st.x[b][j * SP + s], part);
+          for (int s = 0; s < SP; ++s) part = mma<DT>(w[s], x[b][j * SP + s], part);
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[c][b][e] = __builtin_fmaf(part[e], s4[e], acc[c][b][e]);
         }
@@ -170,69 +269,123 @@ TGG_DEV void int4_tile(const Int4Params& p, const Tile& t, float4* red) {
     }
   };
 
+  constexpr int STEP = KSPLIT ? kI4Waves : 1, OWN = BLOCKS / STEP;  // the wave's blocks of a chunk
+  static_assert(OWN >= 1, "a chunk has a block for every wave");
+  const int kb0 = KSPLIT ? wave : 0;
   Stage st[2];
-  load(st[0], wave);
-  load(st[1], wave + kI4Waves);
-  for (int kb = wave; kb < blocks_k; kb += 2 * kI4Waves) {
-    compute(st[0]);
-    load(st[0], kb + 2 * kI4Waves);
-    if (kb + kI4Waves < blocks_k) {
-      compute(st[1]);
-      load(st[1], kb + 3 * kI4Waves);
+  load(st[0], kb0);
+  load(st[1], kb0 + STEP);
+  x_load(0);
+  __syncthreads();  // the tile before has been read
+  x_store(0);
+  x_load(1);
+  __syncthreads();
+  const int chunks = (blocks_k + BLOCKS - 1) / BLOCKS;
+  for (int q = 0; q < chunks; ++q) {
+    const char* const xs = lds + (q & 1) * kI4Chunk;
+    if constexpr (OWN == 1) {
+      compute(st[0], xs, kb0);
+      st[0] = st[1];
+      load(st[1], (q + 2) * BLOCKS + kb0);
+    } else {
+      const int left = (blocks_k - q * BLOCKS - kb0 + STEP - 1) / STEP, n = left < OWN ? left : OWN;  // OWN is even: every chunk starts with stage 0
+      for (int i = 0; i < n; i += 2) {
+        compute(st[0], xs, kb0 + i * STEP);
+        load(st[0], q * BLOCKS + kb0 + (i + 2) * STEP);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + 1 < n) {
+          compute(st[1], xs, kb0 + (i + 1) * STEP);
+          load(st[1], q * BLOCKS + kb0 + (i + 3) * STEP);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (q + 1 < chunks) {
+      x_store(q + 1);
+      if (q + 2 < chunks) x_load(q + 2);
+      __syncthreads();
     }
   }
 
-  // the waves' sums, added in their order, two row blocks at a time
-  constexpr int OC = GATED ? CB / 2 : CB, HB = RB < 2 ? RB : 2;  // column blocks of outputs; row blocks at a time
-  const int out_n = GATED ? F : N;
+  auto put = [&](int c, int b, f32x4_t v, const f32x4_t& u) __attribute__((always_inline)) {
+    const int row = 16 * b + l16, n = col_of(c) + 4 * lg;
+    if constexpr (GATED) {
 #pragma unroll
-  for (int b0 = 0; b0 < RB; b0 += HB) {
-    __syncthreads();  // what was there before has been read
+      for (int e = 0; e < 4; ++e) v[e] = (p.g.act == GATE_SILU ? gate_act<GATE_SILU>(v[e]) : gate_act<GATE_GELU_TANH>(v[e])) * u[e];
+    }
+    if (row < rows && n < out_n) *(uint2*)((char*)p.out + ((row0 + row) * out_n + n) * 2) = pack4<DT>(v[0], v[1], v[2], v[3]);
+  };
+  if constexpr (!KSPLIT) {
+#pragma unroll
+    for (int c = 0; c < OC; ++c)
+#pragma unroll
+      for (int b = 0; b < RB; ++b) put(c, b, acc[c][b], acc[GATED ? c + OC : c][b]);
+  } else {  // the waves' sums, added in their order
+    float4* const red = (float4*)lds;  // [wave][column block][row block][lane]
+    static_assert(kI4Waves * CB * RB * 1024 <= 2 * kI4Chunk, "the sums fit where the activations were");
+    __syncthreads();
 #pragma unroll
     for (int c = 0; c < CB; ++c)
 #pragma unroll
-      for (int b = 0; b < HB; ++b) red[((wave * CB + c) * HB + b) * 64 + lane] = __builtin_bit_cast(float4, acc[c][b0 + b]);
+      for (int b = 0; b < RB; ++b) red[((wave * CB + c) * RB + b) * 64 + lane] = __builtin_bit_cast(float4, acc[c][b]);
     __syncthreads();
     auto total = [&](int c, int b) __attribute__((always_inline)) {
-      f32x4_t v = __builtin_bit_cast(f32x4_t, red[(c * HB + b) * 64 + lane]);
+      f32x4_t v = __builtin_bit_cast(f32x4_t, red[(c * RB + b) * 64 + lane]);
 #pragma unroll
-      for (int w = 1; w < kI4Waves; ++w) v += __builtin_bit_cast(f32x4_t, red[((w * CB + c) * HB + b) * 64 + lane]);
+      for (int w = 1; w < kI4Waves; ++w) v += __builtin_bit_cast(f32x4_t, red[((w * CB + c) * RB + b) * 64 + lane]);
       return v;
     };
-    for (int i = wave; i < OC * HB; i += kI4Waves) {
-      const int c = i / HB, b = i % HB, row = 16 * (b0 + b) + l16, n = col_of(c) + 4 * lg;
-      f32x4_t v = total(c, b);
-      if constexpr (GATED) {
-        const f32x4_t u = total(c + OC, b);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (p.g.act == GATE_SILU ? gate_act<GATE_SILU>(v[e]) : gate_act<GATE_GELU_TANH>(v[e])) * u[e];
-      }
-      if (row < rows && n < out_n) *(uint2*)((char*)p.out + ((row0 + row) * (int64_t)out_n + n) * 2) = pack4<DT>(v[0], v[1], v[2], v[3]);
+    for (int i = wave; i < OC * RB; i += kI4Waves) {
+      const int c = i / RB, b = i % RB;
+      put(c, b, total(c, b), total(GATED ? c + OC : c, b));
     }
   }
 }
 
-template <int DT, bool GATED, bool ZEROS, int GPT, int CB>
-TGG_DEV void int4_tiles(const Int4Params& p, const SchedTable& sched, float4* red) {
-  const int64_t tiles = sched_num_tiles<kI4Rows, 16 * CB>(p.g, sched);
-  const TileWalk walk = sched_walk(tiles, p.g.tile_split != 0);
+template <int DT, bool GATED, bool ZEROS, int GPT, int CB, bool KSPLIT>
+TGG_DEV void int4_tiles(const Int4Params& p, const Int4Table& table, char* lds) {
+  constexpr int COLS = 16 * CB * (KSPLIT ? 1 : kI4Waves);
+  const int tiles_n = (p.g.N + COLS - 1) / COLS;
+  const TileWalk walk = sched_walk((int64_t)table.tile[p.g.G] * tiles_n, p.g.tile_split != 0);
   for (int64_t id = walk.first; id < walk.end; id += walk.stride) {
-    const Tile t = sched_tile<kI4Rows, 16 * CB>(p.g, sched, id);
-    const int rows = __builtin_amdgcn_readfirstlane(t.rows);
-    if (rows <= 16) int4_tile<DT, GATED, ZEROS, GPT, 1, CB>(p, t, red);
-    else if (rows <= 32) int4_tile<DT, GATED, ZEROS, GPT, 2, CB>(p, t, red);
-    else int4_tile<DT, GATED, ZEROS, GPT, 4, CB>(p, t, red);
+    const Int4Tile t = int4_tile_at(table, p.g.G, (int)id, tiles_n);
+    if (t.rows <= 16) int4_tile<DT, GATED, ZEROS, GPT, 1, CB, KSPLIT>(p, t, lds);
+    else if (t.rows <= 32) int4_tile<DT, GATED, ZEROS, GPT, 2, CB, KSPLIT>(p, t, lds);
+    else if constexpr (!KSPLIT) {  // four column blocks of 64 rows do not fit the registers: two and two
+      Int4Tile h = t;
+#pragma unroll 1
+      for (int half = 0; half < CB / 2; ++half) {
+        h.nt = t.nt * (CB / 2) + half;
+        int4_tile<DT, GATED, ZEROS, GPT, 4, 2, false>(p, h, lds);
+      }
+    }
+    else {  // a chunk of 64 rows has no block for every wave: the tile's halves in turn
+      Int4Tile h = t;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        h.row0 = t.row0 + 32 * half;
+        h.rows = half ? t.rows - 32 : 32;
+        int4_tile<DT, GATED, ZEROS, GPT, 2, CB, true>(p, h, lds);
+      }
+    }
   }
 }
 
 template <int DT, bool GATED, bool ZEROS, int GPT>
 __global__ __launch_bounds__(kI4Threads, 2) void gemm_int4_kernel(const Int4Params p) {
-  __shared__ SchedTable sched;
-  __shared__ __attribute__((aligned(16))) float4 red[kI4Waves * 4 * 2 * 64];  // [wave][column block][row block][lane]
-  sched_init<kI4Rows>(p.g, sched);
-  // Wide tiles read an activation once for twice the columns; narrow ones where the wide ones are too few to go round.
-  if (sched_num_tiles<kI4Rows, 64>(p.g, sched) >= (int64_t)gridDim.x) int4_tiles<DT, GATED, ZEROS, GPT, 4>(p, sched, red);
-  else int4_tiles<DT, GATED, ZEROS, GPT, 2>(p, sched, red);
+  __shared__ Int4Table table;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kI4Chunk];
+  int4_table(p.g, table);
+  // Wide tiles read an activation once for more columns; narrow ones where the wide ones are too few to go round.
+  const int64_t row_tiles = table.tile[p.g.G];
+  if constexpr (GPT < 4) {  // (scale groups of 32: four blocks' scales do not fit the registers)
+    if (row_tiles * ((p.g.N + 255) / 256) >= (int64_t)gridDim.x) {
+      int4_tiles<DT, GATED, ZEROS, GPT, 4, false>(p, table, lds);
+      return;
+    }
+  }
+  if (row_tiles * ((p.g.N + 127) / 128) >= (int64_t)gridDim.x) int4_tiles<DT, GATED, ZEROS, GPT, 2, false>(p, table, lds);
+  else int4_tiles<DT, GATED, ZEROS, GPT, 2, true>(p, table, lds);
 }
 
 template <int DT, bool GATED, bool ZEROS, int GPT>
