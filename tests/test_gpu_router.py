@@ -217,6 +217,24 @@ def test_captured_and_replayed(dev):
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
 
 
+def test_compiled(dev):
+    x, d = draw(30, 48, torch.bfloat16, 4)
+    leaf, dd = x.to(dev).requires_grad_(True), d[:, :4].to(dev)
+    fn = lambda t: ops.topk_router(t, 4, scoring="sigmoid")
+    want, want_idx = fn(leaf)
+    got, got_idx = torch.compile(fn, backend="aot_eager")(leaf)
+    assert torch.equal(got, want) and torch.equal(got_idx, want_idx)
+    assert torch.equal(torch.autograd.grad(got, leaf, dd)[0], torch.autograd.grad(want, leaf, dd)[0])
+
+
+def test_the_gradient_has_no_gradient(dev):
+    x = torch.randn(5, 20, device=dev, requires_grad=True)
+    probs, _ = ops.topk_router(x, 3)
+    (g,) = torch.autograd.grad(probs[:, 0].sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
+
+
 def test_no_tokens(dev):
     x = torch.empty(0, 16, device=dev, requires_grad=True)
     probs, idx = ops.topk_router(x, 4)

@@ -75,32 +75,39 @@ template <int RT> TGG_DEV int key_index(typename KeyOf<RT>::type key) {
   else return (int)(0xffffu - (key & 0xffffu));
 }
 
-// VPL logits of a row from element e0 on, in the upper bits; those beyond E are -inf.  vec: rows begin on 16 bytes.
-template <int RT, int VPL> TGG_DEV void load_logits(const void* row, int e0, int E, bool vec, uint32_t (&u)[VPL]) {
+// Which logits a lane holds.  VEC: VPL neighbouring ones, read 16 bytes at a time (rows begin on 16 bytes and hold whole 16-byte pieces); otherwise
+// every LPT-th one, so that a read instruction covers neighbouring logits (161 fp32 logits a row, 16383 rows: 22 -> 11.3 us forward, 14.3 -> 8.1 backward).
+template <int LPT, int VPL, bool VEC> TGG_DEV int expert_of(int lane, int i) { return VEC ? lane * VPL + i : i * LPT + lane; }
+
+// A lane's logits, in the upper bits; those beyond E are -inf.
+template <int RT, int LPT, int VPL, bool VEC> TGG_DEV void load_logits(const void* row, int lane, int E, uint32_t (&u)[VPL]) {
   constexpr uint32_t masked = RT == RT_F16 ? 0xfc000000u : 0xff800000u;
   constexpr int ES = RT == RT_F32 ? 4 : 2, PER = 16 / ES;
-  if constexpr (VPL >= PER) {
-    if (vec && e0 + VPL <= E) {
+  if constexpr (VEC) {
+    static_assert(VPL % PER == 0, "whole 16-byte pieces");
 #pragma unroll
-      for (int c = 0; c < VPL / PER; ++c) {
-        const uint4 w = *(const uint4*)((const char*)row + (int64_t)e0 * ES + c * 16);
-        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    for (int c = 0; c < VPL / PER; ++c) {
+      const int e = lane * VPL + c * PER;
+      const uint32_t none = RT == RT_F32 ? masked : masked | (masked >> 16);
+      uint4 w = {none, none, none, none};
+      if (e < E) w = *(const uint4*)((const char*)row + (int64_t)e * ES);
+      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (RT == RT_F32) u[c * 4 + i] = x[i];
-          else {
-            u[c * 8 + 2 * i] = x[i] << 16;
-            u[c * 8 + 2 * i + 1] = x[i] & 0xffff0000u;
-          }
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (RT == RT_F32) u[c * 4 + i] = x[i];
+        else {
+          u[c * 8 + 2 * i] = x[i] << 16;
+          u[c * 8 + 2 * i + 1] = x[i] & 0xffff0000u;
         }
       }
-      return;
     }
-  }
+  } else {
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    u[i] = masked;
-    if (e0 + i < E) u[i] = RT == RT_F32 ? ((const uint32_t*)row)[e0 + i] : (uint32_t)((const uint16_t*)row)[e0 + i] << 16;
+    for (int i = 0; i < VPL; ++i) {
+      const int e = expert_of<LPT, VPL, VEC>(lane, i);
+      u[i] = masked;
+      if (e < E) u[i] = RT == RT_F32 ? ((const uint32_t*)row)[e] : (uint32_t)((const uint16_t*)row)[e] << 16;
+    }
   }
 }
 
@@ -126,18 +133,27 @@ TGG_DEV float log_sigmoid(float x) { return fminf(x, 0.f) - log1pf(expf(-fabsf(x
 // The row's largest logit for the exponentials; of a row without experts 0, so that every exp(l - max) is 0 there.
 TGG_DEV float shift_of(float top) { return top == -__builtin_inff() ? 0.f : top; }
 
-template <int RT, int LPT, int VPL>
+// m ? b : a, m all ones or zero.  (Written as a choice, the compiler makes the list below a choice of places: 80 instructions a round in place of 7.)
+TGG_DEV uint32_t choose(uint32_t a, uint32_t b, uint32_t m) { return (b & m) | (a & ~m); }
+TGG_DEV uint64_t choose(uint64_t a, uint64_t b, uint32_t m) {
+  return ((uint64_t)choose((uint32_t)(a >> 32), (uint32_t)(b >> 32), m) << 32) | choose((uint32_t)a, (uint32_t)b, m);
+}
+
+template <int RT, int LPT, int VPL, bool VEC>
 __global__ __launch_bounds__(kRouterThreads) void router_fwd_kernel(const char* __restrict__ logits, int64_t row_bytes, int64_t tokens, int E, int k,
-                                                                    int scoring, int renorm, int vec, float* __restrict__ probs, int32_t* __restrict__ indices) {
+                                                                    int scoring, int renorm, float* __restrict__ probs, int32_t* __restrict__ indices) {
   typedef typename KeyOf<RT>::type Key;
-  const int lane = threadIdx.x % LPT, e0 = lane * VPL;
+  const int lane = threadIdx.x % LPT;
   const int64_t token = (int64_t)blockIdx.x * (kRouterThreads / LPT) + threadIdx.x / LPT;
   const bool live = token < tokens;
   uint32_t u[VPL];
-  load_logits<RT, VPL>(logits + token * row_bytes, e0, live ? E : 0, vec, u);
+  load_logits<RT, LPT, VPL, VEC>(logits + token * row_bytes, lane, live ? E : 0, u);
   Key key[VPL];
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) key[i] = e0 + i < E ? make_key<RT>(u[i], e0 + i) : 0;
+  for (int i = 0; i < VPL; ++i) {
+    const int e = expert_of<LPT, VPL, VEC>(lane, i);
+    key[i] = e < E ? make_key<RT>(u[i], e) : 0;
+  }
   sort_descending(key);
   Key mine = 0;  // lane t: the t-th of the row
   Key first = 0;
@@ -145,10 +161,10 @@ __global__ __launch_bounds__(kRouterThreads) void router_fwd_kernel(const char* 
     const Key top = max_over<LPT>(key[0]);
     if (t == 0) first = top;
     if (lane == t) mine = top;
-    const bool own = key[0] == top;
+    const uint32_t own = key[0] == top ? 0xffffffffu : 0u;
 #pragma unroll
-    for (int i = 0; i + 1 < VPL; ++i) key[i] = own ? key[i + 1] : key[i];
-    if (own) key[VPL - 1] = 0;
+    for (int i = 0; i + 1 < VPL; ++i) key[i] = choose(key[i], key[i + 1], own);
+    key[VPL - 1] = choose(key[VPL - 1], Key(0), own);
   }
   const float x = logit_value<RT>(key_logit<RT>(mine));
   const bool chosen = lane < k && !(x == -__builtin_inff());
@@ -185,13 +201,13 @@ template <int RT> TGG_DEV void store_logit(char* row, int e, float v) {
 
 // Gradient of the logits.  What the chosen experts get, lane t of a token computes from round t's probability; through a row of LDS it reaches the lane
 // that writes that expert's logit.
-template <int RT, int LPT, int VPL>
+template <int RT, int LPT, int VPL, bool VEC>
 __global__ __launch_bounds__(kRouterThreads) void router_bwd_kernel(const char* __restrict__ logits, int64_t row_bytes, const float* __restrict__ probs,
                                                                     const int32_t* __restrict__ indices, const float* __restrict__ grad, int64_t tokens, int E, int k,
-                                                                    int scoring, int renorm, int vec, char* __restrict__ dlogits, int vec_out) {
+                                                                    int scoring, int renorm, char* __restrict__ dlogits) {
   __shared__ __attribute__((aligned(16))) float part[kRouterThreads / LPT][LPT * VPL];
   constexpr int ES = RT == RT_F32 ? 4 : 2;
-  const int lane = threadIdx.x % LPT, slot = threadIdx.x / LPT, e0 = lane * VPL;
+  const int lane = threadIdx.x % LPT, slot = threadIdx.x / LPT;
   const int64_t token = (int64_t)blockIdx.x * (kRouterThreads / LPT) + slot;
   const bool live = token < tokens;
   const char* const row = logits + token * row_bytes;
@@ -213,14 +229,14 @@ __global__ __launch_bounds__(kRouterThreads) void router_bwd_kernel(const char* 
   float* const mine = part[slot];
 #pragma unroll
   for (int i = 0; i < VPL; ++i) mine[i * LPT + lane] = 0.f;
-  if (at >= 0) mine[at % VPL * LPT + at / VPL] = v;  // logit e in place (e mod VPL, e / VPL): the lanes' reads below are neighbours
+  if (at >= 0) mine[VEC ? at % VPL * LPT + at / VPL : at] = v;  // where the lane that holds this logit reads below
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // a token's lanes are of one wave: LDS serves them in order
   float g[VPL];
 #pragma unroll
   for (int i = 0; i < VPL; ++i) g[i] = mine[i * LPT + lane];
   if (scoring == SCORE_SOFTMAX && !renorm) {  // every expert's probability took part in the sum
     uint32_t u[VPL];
-    load_logits<RT, VPL>(row, e0, live ? E : 0, vec, u);
+    load_logits<RT, LPT, VPL, VEC>(row, lane, live ? E : 0, u);
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
@@ -238,28 +254,30 @@ __global__ __launch_bounds__(kRouterThreads) void router_bwd_kernel(const char* 
   }
   if (!live) return;
   char* const out = dlogits + token * (int64_t)E * ES;
-  if constexpr (VPL * ES >= 16) {
-    if (vec_out && e0 + VPL <= E) {
+  if constexpr (VEC) {
+    constexpr int PER = 16 / ES;
+#pragma unroll
+    for (int c = 0; c < VPL / PER; ++c) {
+      const int e = lane * VPL + c * PER;
+      if (e >= E) continue;
       if constexpr (RT == RT_F32) {
-#pragma unroll
-        for (int c = 0; c < VPL / 4; ++c) *(float4*)(out + (int64_t)e0 * 4 + c * 16) = make_float4(g[4 * c], g[4 * c + 1], g[4 * c + 2], g[4 * c + 3]);
+        *(float4*)(out + (int64_t)e * 4) = make_float4(g[4 * c], g[4 * c + 1], g[4 * c + 2], g[4 * c + 3]);
       } else {
-#pragma unroll
-        for (int c = 0; c < VPL / 8; ++c) {
-          uint4 w;
-          w.x = pack2<RT>(g[8 * c], g[8 * c + 1]);
-          w.y = pack2<RT>(g[8 * c + 2], g[8 * c + 3]);
-          w.z = pack2<RT>(g[8 * c + 4], g[8 * c + 5]);
-          w.w = pack2<RT>(g[8 * c + 6], g[8 * c + 7]);
-          *(uint4*)(out + (int64_t)e0 * 2 + c * 16) = w;
-        }
+        uint4 w;
+        w.x = pack2<RT>(g[8 * c], g[8 * c + 1]);
+        w.y = pack2<RT>(g[8 * c + 2], g[8 * c + 3]);
+        w.z = pack2<RT>(g[8 * c + 4], g[8 * c + 5]);
+        w.w = pack2<RT>(g[8 * c + 6], g[8 * c + 7]);
+        *(uint4*)(out + (int64_t)e * 2) = w;
       }
-      return;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = expert_of<LPT, VPL, VEC>(lane, i);
+      if (e < E) store_logit<RT>(out, e, g[i]);
     }
   }
-#pragma unroll
-  for (int i = 0; i < VPL; ++i)
-    if (e0 + i < E) store_logit<RT>(out, e0 + i, g[i]);
 }
 
 struct RouterArgs {
@@ -272,21 +290,29 @@ struct RouterArgs {
   char* dlogits;
 };
 
-template <int RT, int LPT, int VPL, bool BWD>
-int launch_router_as(const RouterArgs& a, hipStream_t s) {
-  constexpr int ES = RT == RT_F32 ? 4 : 2, PER = kRouterThreads / LPT;
+template <int RT, int LPT, int VPL, bool VEC, bool BWD>
+int launch_router_kernel(const RouterArgs& a, hipStream_t s) {
+  constexpr int PER = kRouterThreads / LPT;
   const int64_t blocks = (a.tokens + PER - 1) / PER;
   if (blocks > 0x7fffffff) return set_error("router over %lld tokens: too many", (long long)a.tokens);
-  const int vec = ((uintptr_t)a.logits & 15) == 0 && (a.row_bytes & 15) == 0;
   if constexpr (BWD) {
-    const int vec_out = ((uintptr_t)a.dlogits & 15) == 0 && (a.E * ES & 15) == 0;
-    hipLaunchKernelGGL((router_bwd_kernel<RT, LPT, VPL>), dim3((uint32_t)blocks), dim3(kRouterThreads), 0, s, a.logits, a.row_bytes, a.probs, a.indices, a.grad, a.tokens,
-                       a.E, a.k, a.scoring, a.renorm, vec, a.dlogits, vec_out);
+    hipLaunchKernelGGL((router_bwd_kernel<RT, LPT, VPL, VEC>), dim3((uint32_t)blocks), dim3(kRouterThreads), 0, s, a.logits, a.row_bytes, a.probs, a.indices, a.grad, a.tokens,
+                       a.E, a.k, a.scoring, a.renorm, a.dlogits);
   } else {
-    hipLaunchKernelGGL((router_fwd_kernel<RT, LPT, VPL>), dim3((uint32_t)blocks), dim3(kRouterThreads), 0, s, a.logits, a.row_bytes, a.tokens, a.E, a.k, a.scoring, a.renorm,
-                       vec, a.probs, a.indices);
+    hipLaunchKernelGGL((router_fwd_kernel<RT, LPT, VPL, VEC>), dim3((uint32_t)blocks), dim3(kRouterThreads), 0, s, a.logits, a.row_bytes, a.tokens, a.E, a.k, a.scoring,
+                       a.renorm, a.probs, a.indices);
   }
   return check_launch("moe_router");
+}
+
+template <int RT, int LPT, int VPL, bool BWD>
+int launch_router_as(const RouterArgs& a, hipStream_t s) {
+  constexpr int ES = RT == RT_F32 ? 4 : 2;
+  if constexpr (VPL * ES >= 16) {
+    const bool rows = ((uintptr_t)a.logits & 15) == 0 && (a.row_bytes & 15) == 0 && (a.E * ES & 15) == 0;
+    if (rows && (!BWD || ((uintptr_t)a.dlogits & 15) == 0)) return launch_router_kernel<RT, LPT, VPL, true, BWD>(a, s);
+  }
+  return launch_router_kernel<RT, LPT, VPL, false, BWD>(a, s);
 }
 
 // As few lanes a token as its experts (eight logits a lane; two in rows of at most 32 experts, sixteen in rows of more than 512) and its k results need.

@@ -10,7 +10,10 @@ Mirrors the autograd wrapper of the reference's baseline extension (grouped_gemm
 ``batch_sizes`` may live on the host (as the reference's extension requires) or on the device; a device tensor
 is used as is, with no host synchronisation.
 """
+from typing import Tuple
+
 import torch
+from torch import Tensor
 
 from . import _native
 from ._native import require_gpu
@@ -325,10 +328,8 @@ _LOGIT_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_TOPK = 64
 
 
-def _router_forward(logits, topk, scoring, renormalize):
-    result = _native.host().topk_router(logits, topk, scoring, renormalize)
-    if result is not None:
-        return result
+@torch.library.custom_op("moe::topk_router", mutates_args=())
+def _router_forward(logits: Tensor, topk: int, scoring: int, renormalize: bool) -> Tuple[Tensor, Tensor]:
     probs = torch.empty((logits.shape[0], topk), dtype=torch.float32, device=logits.device)
     indices = torch.empty((logits.shape[0], topk), dtype=torch.int32, device=logits.device)
     if logits.shape[0]:
@@ -339,12 +340,36 @@ def _router_forward(logits, topk, scoring, renormalize):
     return probs, indices
 
 
+@_router_forward.register_fake
+def _(logits, topk, scoring, renormalize):
+    return (logits.new_empty((logits.shape[0], topk), dtype=torch.float32),
+            logits.new_empty((logits.shape[0], topk), dtype=torch.int32))
+
+
+@torch.library.custom_op("moe::topk_router_backward", mutates_args=())
+def _router_backward(logits: Tensor, probs: Tensor, indices: Tensor, grad: Tensor, scoring: int, renormalize: bool) -> Tensor:
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if logits.shape[0]:
+        grad = grad.float().contiguous()
+        with torch.cuda.device(logits.device):
+            _native.call("tgg_moe_router_bwd", logits.data_ptr(), logits.stride(0), probs.data_ptr(), indices.data_ptr(),
+                         grad.data_ptr(), logits.shape[0], logits.shape[1], probs.shape[1], scoring, int(renormalize),
+                         _LOGIT_CODE[logits.dtype], out.data_ptr(), _native.stream_of(logits))
+    return out
+
+
+@_router_backward.register_fake
+def _(logits, probs, indices, grad, scoring, renormalize):
+    return logits.new_empty(logits.shape)
+
+
 class TopkRouter(torch.autograd.Function):
-    """``topk_router`` with the gradient of the logits; the experts' numbers have none."""
+    """``topk_router`` with the gradient of the logits; the experts' numbers have none.  (An ordinary eager call is recorded by the
+    native call path instead, with the same two launches.)"""
 
     @staticmethod
     def forward(ctx, logits, topk, scoring, renormalize):
-        probs, indices = _router_forward(logits.detach(), topk, scoring, renormalize)
+        probs, indices = _router_forward(logits, topk, scoring, renormalize)
         ctx.mark_non_differentiable(indices)
         ctx.save_for_backward(logits, probs, indices)
         ctx.scoring, ctx.renormalize = scoring, renormalize
@@ -354,14 +379,7 @@ class TopkRouter(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _):
         logits, probs, indices = ctx.saved_tensors
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        if logits.shape[0]:
-            grad = grad.contiguous()
-            with torch.cuda.device(logits.device):
-                _native.call("tgg_moe_router_bwd", logits.data_ptr(), logits.stride(0), probs.data_ptr(), indices.data_ptr(),
-                             grad.data_ptr(), logits.shape[0], logits.shape[1], probs.shape[1], ctx.scoring,
-                             int(ctx.renormalize), _LOGIT_CODE[logits.dtype], out.data_ptr(), _native.stream_of(logits))
-        return out, None, None, None
+        return _router_backward(logits, probs, indices, grad, ctx.scoring, ctx.renormalize), None, None, None
 
 
 def topk_router(logits, topk, scoring="softmax", renormalize=True):
@@ -372,6 +390,10 @@ def topk_router(logits, topk, scoring="softmax", renormalize=True):
     all.  ``scoring``: ``"softmax"`` over all experts or ``"sigmoid"``; ``renormalize`` divides the chosen probabilities by their
     sum.  A logit of ``-inf`` masks an expert, which is then never chosen: entries left over have index -1, an assignment that ``permute``
     drops, and probability 0.  Arithmetic is fp32; differentiable in ``logits``."""
+    if not torch.compiler.is_compiling():
+        result = (_native._host or _native.host()).topk_router(logits, topk, _SCORING_CODE.get(scoring), renormalize)
+        if result is not None:
+            return result
     if scoring not in _SCORING_CODE:
         raise ValueError(f"scoring must be one of {sorted(_SCORING_CODE)}, got {scoring!r}")
     require_gpu(logits)
