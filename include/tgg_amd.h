@@ -39,15 +39,15 @@ int tgg_m_grouped_gemm(const void* A, const void* B, void* C, const void* sizes,
 /* Gated feed-forward block: H[r,:] = A[r,:] . B[g(r)]^T (trans_b=1, B is [G,2F,K]) or A[r,:] . B[g(r)] (trans_b=0, B is
  * [G,K,2F]), whose first F columns are the gate and last F the up projection, and C[r,:] = act(gate) * up, [M,F], with
  * everything between the products and the one rounding to `dtype` in fp32.  H [M,2F] may be NULL; otherwise it receives both
- * projections, rounded to `dtype`: what tgg_gated_backward takes.  Rows past sum(sizes) are not written.  F and K are
+ * projections in fp32: what tgg_gated_backward takes.  Rows past sum(sizes) are not written.  F and K are
  * multiples of 8.  The reference has no counterpart: its layers run the grouped product and the activation as separate operators. */
 #define TGG_SILU 0      /* x sigma(x) */
 #define TGG_GELU_TANH 1 /* x sigma(2 sqrt(2/pi) (x + 0.044715 x^3)) */
 int tgg_m_grouped_gated_gemm(const void* A, const void* B, void* C, void* H, const void* sizes, int sizes_i64, int G, int64_t M,
                              int F, int K, int trans_b, int activation, int dtype, int num_cu, void* stream);
 
-/* Gradient of C = act(gate) * up with respect to H: dh[r,:] = [dout up act'(gate) | dout act(gate)] for all M rows, dout [M,F],
- * h and dh [M,2F].  The gradients of A and B are the grouped products of dh (tgg_m_grouped_gemm with trans_b flipped,
+/* Gradient of C = act(gate) * up with respect to H: dh[r,:] = [dout up act'(gate) | dout act(gate)] for all M rows, dout [M,F]
+ * and dh [M,2F] in `dtype`, h [M,2F] fp32.  The gradients of A and B are the grouped products of dh (tgg_m_grouped_gemm with trans_b flipped,
  * tgg_k_grouped_gemm_sizes). */
 int tgg_gated_backward(const void* dout, const void* h, void* dh, int64_t M, int F, int activation, int dtype, void* stream);
 

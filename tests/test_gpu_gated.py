@@ -2,13 +2,13 @@
 formulas in 64 bits.
 
 Bounds, with u the half step of the operands' type (torch.finfo(t).eps / 2):
-  projections  a sum of K products in fp32 is off by at most (K + 8) 2^-24 times the sum of the products' magnitudes (S), the
-               stored projection by u of its value more;
+  projections  a sum of K products in fp32 is off by at most (K + 8) 2^-24 times the sum of the products' magnitudes; they are
+               stored in fp32;
   outputs      act(gate) up: the slopes of both activations stay within 1.13, so the sums' errors arrive as
                1.13 |up| e_gate + |act| e_up; the activation itself (exp2 and reciprocal good to an ulp, its argument rounded) is
                off by at most 2^-19 of its value for |gate| up to 16; then u of the value for the one rounding;
-  gradients    dh is made from stored projections, so each of its values carries u of the projections' slopes besides its own
-               rounding; sums of it are bounded with the magnitudes.
+  gradients    dh is rounded to the operands' type before it enters the products, u of each of its values; sums of it are
+               bounded with the magnitudes.
 """
 import pytest
 import torch
@@ -74,26 +74,40 @@ CASES = [
     ([600, 1, 255], 256, 264, torch.bfloat16, False, "gelu_tanh"),
     ([512, 700], 1000, 520, torch.bfloat16, True, "silu"),
     ([4] * 64, 256, 768, torch.bfloat16, True, "silu"),
+    # whole slabs of K and, for [K, 2 F] weights, whole tiles of columns: the four-wave kernel's; half tiles, full ones and both in turn
+    ([700, 0, 128, 129, 1], 256, 200, torch.bfloat16, True, "gelu_tanh"),
+    ([300, 513, 20, 256], 384, 256, torch.float16, False, "silu"),
+    ([60, 100, 3], 512, 128, torch.bfloat16, False, "gelu_tanh"),
+    ([1000], 640, 264, torch.float16, True, "silu"),
+    ([520, 40, 700], 256, 384, torch.bfloat16, False, "silu"),
+    ([256, 256, 384], 256, 128, torch.float16, False, "gelu_tanh"),
 ]
 
 
-@pytest.mark.parametrize("generic", [True, False])
+# the shape-agnostic kernel, the routes of ordinary calls, the eight-wave kernel alone, the four-wave kernel wherever it can
+PATHS = {"generic": ("force_generic", 1, 0), "routed": ("four_wave", 1, 1), "eight_wave": ("four_wave", 0, 1), "four_wave": ("four_wave", 2, 1)}
+
+
+@pytest.fixture(params=sorted(PATHS))
+def path(request):
+    key, value, back = PATHS[request.param]
+    _native.set_option(key, value)
+    yield request.param
+    _native.set_option(key, back)
+
+
 @pytest.mark.parametrize("case", CASES, ids=[f"{len(c[0])}g{sum(c[0])}r_k{c[1]}_f{c[2]}_{'nt' if c[4] else 'nn'}" for c in CASES])
-def test_forward(dev, case, generic):
+def test_forward(dev, case, path):
     sizes, k, f, dtype, trans_b, kind = case
     a, b, _ = make(sizes, k, f, dtype, trans_b, 7 * k + f)
     want, h64, eo, eh = reference(a, b, sizes, trans_b, kind)
     ad, bd = a.to(dev), b.to(dev)
     counts = torch.tensor(sizes, dtype=torch.int64 if k % 16 else torch.int32, device=dev)
-    try:
-        _native.set_option("force_generic", int(generic))
-        out = m_grouped_gated_gemm(ad, bd, counts, trans_b, kind)
-        both, h = m_grouped_gated_gemm_projections(ad, bd, counts, trans_b, kind)
-    finally:
-        _native.set_option("force_generic", 0)
+    out = m_grouped_gated_gemm(ad, bd, counts, trans_b, kind)
+    both, h = m_grouped_gated_gemm_projections(ad, bd, counts, trans_b, kind)
     check(out, want, eo, dtype, "out")
-    assert torch.equal(out, both)
-    check(h, h64, eh, dtype, "projections")
+    assert torch.equal(out, both) and h.dtype == torch.float32
+    check(h, h64, eh, torch.float32, "projections")
 
 
 def _window(rows, cols, dtype, dev, fill):
@@ -102,26 +116,21 @@ def _window(rows, cols, dtype, dev, fill):
     return base, base[256:256 + rows * cols].view(rows, cols)
 
 
-@pytest.mark.parametrize("generic", [True, False])
 @pytest.mark.parametrize("trans_b", [True, False])
-@pytest.mark.parametrize("rows,f", [(5, 24), (700, 136)])
-def test_rows_behind_the_last_group_and_neighbours_are_left_alone(dev, generic, trans_b, rows, f):
-    k, extra = 136, 9
+@pytest.mark.parametrize("rows,f,k", [(5, 24, 136), (700, 136, 136), (90, 128, 256), (900, 256, 384)])
+def test_rows_behind_the_last_group_and_neighbours_are_left_alone(dev, path, trans_b, rows, f, k):
+    extra = 9
     sizes = [rows // 3, 0, rows - rows // 3]
     a, b, _ = make(sizes, k, f, torch.bfloat16, trans_b, 3, extra)
     a[rows:] = float("nan")
     out_base, out = _window(rows + extra, f, torch.bfloat16, dev, 7.0)
-    h_base, h = _window(rows + extra, 2 * f, torch.bfloat16, dev, 9.0)
+    h_base, h = _window(rows + extra, 2 * f, torch.float32, dev, 9.0)
     ad, bd, counts = a.to(dev), b.to(dev), torch.tensor(sizes, dtype=torch.int32, device=dev)
-    try:
-        _native.set_option("force_generic", int(generic))
-        _native.call("tgg_m_grouped_gated_gemm", ad.data_ptr(), bd.data_ptr(), out.data_ptr(), h.data_ptr(), counts.data_ptr(), 0,
-                     3, rows + extra, f, k, int(trans_b), 0, _native.BF16, -1, _native.stream_of(ad))
-    finally:
-        _native.set_option("force_generic", 0)
+    _native.call("tgg_m_grouped_gated_gemm", ad.data_ptr(), bd.data_ptr(), out.data_ptr(), h.data_ptr(), counts.data_ptr(), 0,
+                 3, rows + extra, f, k, int(trans_b), 0, _native.BF16, -1, _native.stream_of(ad))
     want, h64, eo, eh = reference(a, b, sizes, trans_b, "silu")
     check(out[:rows], want, eo, torch.bfloat16, "out")
-    check(h[:rows], h64, eh, torch.bfloat16, "projections")
+    check(h[:rows], h64, eh, torch.float32, "projections")
     assert (out[rows:] == 7.0).all() and (h[rows:] == 9.0).all()
     assert (out_base[:256] == 7.0).all() and (out_base[-256:] == 7.0).all() and (h_base[:256] == 9.0).all() and (h_base[-256:] == 9.0).all()
 
@@ -131,8 +140,8 @@ def test_rows_behind_the_last_group_and_neighbours_are_left_alone(dev, generic, 
 @pytest.mark.parametrize("rows,f", [(1, 8), (3, 344), (129, 768), (1000, 40)])
 def test_gradient_of_the_projections(dev, rows, f, dtype, kind):
     gen = torch.Generator().manual_seed(rows + f)
-    h = (torch.randn(rows, 2 * f, generator=gen) * 3).to(dtype)
-    h[0, :8] = torch.tensor([0.0, -0.0, 16.0, -16.0, 1e-3, -1e-3, 5.0, -5.0], dtype=dtype)
+    h = (torch.randn(rows, 2 * f, generator=gen) * 3).clamp(-16, 16)
+    h[0, :8] = torch.tensor([0.0, -0.0, 16.0, -16.0, 1e-3, -1e-3, 5.0, -5.0])
     d = torch.randn(rows, f, generator=gen).to(dtype)
     leaf = h.double().requires_grad_(True)
     (act64(leaf[:, :f], kind) * leaf[:, f:] * d.double()).sum().backward()
@@ -147,7 +156,7 @@ def test_gradient_of_the_projections(dev, rows, f, dtype, kind):
 
 
 def _gradients64(a, b, grad, sizes, trans_b, kind):
-    """Gradients in 64 bits and bounds for those made from rounded projections and a rounded dh."""
+    """Gradients in 64 bits and bounds for those made from fp32 projections and a rounded dh."""
     f, u = grad.shape[1], half_step(a.dtype)
     das, ea, dbs, eb = [], [], [], []
     row = 0
@@ -162,9 +171,11 @@ def _gradients64(a, b, grad, sizes, trans_b, kind):
         das.append(x.grad)
         dbs.append(w.grad)
         gate, up = h[:, :f].detach().abs(), h[:, f:].detach().abs()
-        # |second derivative| <= 1.2 for both activations; u of each stored projection, u of dh itself
-        e = torch.cat([d.abs() * (1.13 * up * u + 1.2 * up * gate * u), d.abs() * 1.13 * gate * u], 1) + u * h.grad.abs()
-        e = e * (1 + 2 ** -5) + h.grad.abs() * (a.shape[1] * 2.0 ** -22)
+        # u of dh itself; |second derivative| <= 1.2 for both activations, each projection off by (K + 8) 2^-24 of its products' magnitudes, the slopes
+        # good to 2^-19 of theirs
+        eh = (x.detach().abs() @ wt.detach().abs()) * (a.shape[1] + 8) * 2.0 ** -24
+        e = torch.cat([d.abs() * (1.13 * eh[:, f:] + 1.2 * up * eh[:, :f] + 3 * up * 2.0 ** -19), d.abs() * (1.13 * eh[:, :f] + gate * 2.0 ** -19)], 1)
+        e = (e + u * h.grad.abs()) * (1 + 2 ** -6)
         wa, xa, dha = wt.detach().abs(), x.detach().abs(), h.grad.abs()
         ea.append(e @ wa.t() + (dha @ wa.t()) * (2 * f + 8) * 2.0 ** -24)
         ew = xa.t() @ e + (xa.t() @ dha) * (n + 8) * 2.0 ** -24

@@ -142,6 +142,8 @@ def accumulator_reads_too_early(text: str):
     return bad
 
 
+FOUR_WAVE = ("gemm_w4", "gated_w4")  # source files with instantiations of gemm_w4_kernel
+
 # The K-grouped four-wave kernels hold a work-queue draw that is in flight across K steps in v255 (KgDraw, w4_common.hpp).
 K_GROUPED = {"gemm_wgrad": "gemm_wgrad_kernel", "fp8_w4": "fp8_w4_kernel"}  # source file, kernel
 
@@ -210,7 +212,7 @@ def compiler_uses_of_named_registers(text: str):
 def findings(stem: str, text: str):
     """What is wrong with the device assembly of csrc/<stem>.hip, one line each."""
     checks = [("wait states missing", scan(text))]
-    if stem == "gemm_w4":
+    if stem in FOUR_WAVE:
         checks += [("compiler-generated uses of v[192:255]", stray_uses_of_reserved_registers(text)),
                    ("compiler-generated uses of named registers", compiler_uses_of_named_registers(text)),
                    ("accumulator reads too close behind the multiply", accumulator_reads_too_early(text))]
@@ -221,7 +223,7 @@ def findings(stem: str, text: str):
                    ("accumulator reads too close behind the multiply", accumulator_reads_too_early(text.replace(kernel, "gemm_w4_kernel"))),
                    # a spilled value would be reloaded behind the copies
                    ("uses of scratch memory", [line for line, _ in _kernel_lines(text, kernel) if "scratch_" in line])]
-    expected = {"gemm_w4": "gemm_w4_kernel", **K_GROUPED}.get(stem)
+    expected = {**dict.fromkeys(FOUR_WAVE, "gemm_w4_kernel"), **K_GROUPED}.get(stem)
     if expected and expected not in text:
         checks.append(("no kernel of this name", [expected]))
     return [f"{stem}: {len(found)} {what}, first: {found[0]}" for what, found in checks if found]

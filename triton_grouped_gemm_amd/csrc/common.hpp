@@ -120,7 +120,7 @@ struct GemmParams {
   // gated feed-forward block (kernels instantiated for it): N = 2 F columns of B are F of the gate and F of the up
   // projection, C is [rows, F] = act(gate) * up, and a tile of BN columns covers BN / 2 outputs, the gate's columns n0 / 2 ... and the
   // up projection's F + n0 / 2 ...; both sums of an output meet in one lane.
-  void* H;                // the projections themselves, [rows, 2 F] in the outputs' type (what the backward pass needs), or null
+  void* H;                // the projections themselves, [rows, 2 F] in fp32 (what the backward pass needs), or null
   int act;                // GATE_SILU / GATE_GELU_TANH (gate.hpp)
 };
 

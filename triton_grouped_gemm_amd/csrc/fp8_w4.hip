@@ -19,7 +19,7 @@
 // in groups 8-15.  The buffers alternate by a toggled address bit, so any number of slabs per tile will do (two at least: of
 // nothing, if need be).
 //
-// The epilogue needs no LDS staging: B's rows sit in LDS in the order of gemm_w4.hip, so that a lane's results of the eight column
+// The epilogue needs no LDS staging: B's rows sit in LDS in the order of gemm_w4.hpp, so that a lane's results of the eight column
 // blocks are eight neighbouring outputs of a row.  Row blocks 0-3 are complete after group 7 of a tile's last slab and leave between
 // the multiplies of its groups 8-15; row blocks 4-7 leave in groups 0-7 of the next tile's first slab, where they are not
 // touched.  The tile's 256 + 256 scales are copied to LDS in its first slab.
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(Fp8W4Cfg::THREADS) void fp8_w4_kernel(const GemmPar
   const int ld = (int)p.k_total;  // bytes between consecutive rows of either operand
 
   // Copy k (0..7) of an operand's slab by this wave is copy instruction wave + 4 k: LDS rows 8 (wave + 4 k) ... + 7.  A's rows are in order,
-  // B's permuted as in gemm_w4.hip: LDS row 128 h + 16 j + c holds column 128 h + 8 c + j of the tile.
+  // B's permuted as in gemm_w4.hpp: LDS row 128 h + 16 j + c holds column 128 h + 8 c + j of the tile.
   int vo_a[8], vo_b[8];
   static_assert(Op::NPAT == 2, "the swizzle pattern of copy wave + 4 k is that of copy wave");
 #pragma unroll

@@ -640,23 +640,18 @@ TGG_DEV void gemm_fast_body(const GemmParams& p) {
     }
     if constexpr (GATED) {
       // Blocks j < TN / 2 of a strip are the gate, the others the up projection of the same outputs.  The projections, where they are asked
-      // for, and then the products pass through the strip's staging rows.
-      constexpr int HN = C::TN / 2, CPH = 2 * C::TN, CPO = C::TN;  // 16-byte chunks of a staged row: both projections, the products
+      // for, leave as fp32, 16 bytes a lane; the products pass through the strip's staging rows.
+      constexpr int HN = C::TN / 2, CPO = C::TN;  // CPO: 16-byte chunks of a staged row
       const int F = p.N / 2, o0 = (cur.n0 + wn0) / 2;  // the wave's first output column
-      char* const h_tile = (char*)p.H + ((c_row0 + wm0) * (int64_t)p.N + o0) * 2;
+      char* const h_tile = (char*)p.H + ((c_row0 + wm0) * (int64_t)p.N + o0) * 4;
       char* const o_tile = (char*)p.C + ((c_row0 + wm0) * (int64_t)F + o0) * 2;
 #pragma unroll
       for (int i = 0; i < C::TM; ++i) {
-        if (p.H) {
+        if (p.H && wm0 + 16 * i + e16 < cur.rows) {
 #pragma unroll
-          for (int j = 0; j < C::TN; ++j)
-            *(uint2*)(stage_c + e16 * C::EPI_PITCH + (16 * j + 4 * eg) * 2) = pack4<DT>(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
-#pragma unroll
-          for (int it = 0; it < 16 * CPH / 64; ++it) {
-            const int idx = it * 64 + el, r = idx / CPH, ch = idx % CPH, c = (ch % C::TN) * 8;
-            const i32x4_t v = *(const i32x4_t*)(stage_c + r * C::EPI_PITCH + ch * 16);
-            if (o0 + c < F && wm0 + 16 * i + r < cur.rows)
-              store_c((i32x4_t*)(h_tile + ((int64_t)(16 * i + r) * p.N + c + (ch >= C::TN ? F : 0)) * 2), v, 0);
+          for (int j = 0; j < C::TN; ++j) {
+            const int c = 16 * (j % HN) + 4 * eg;
+            if (o0 + c < F) store_c((i32x4_t*)(h_tile + ((int64_t)(16 * i + e16) * p.N + c + (j >= HN ? F : 0)) * 4), __builtin_bit_cast(i32x4_t, acc[i][j]), 1);
           }
         }
         if (p.act == GATE_SILU) {
@@ -678,7 +673,9 @@ TGG_DEV void gemm_fast_body(const GemmParams& p) {
         for (int it = 0; it < (16 * CPO + 63) / 64; ++it) {
           const int idx = it * 64 + el, r = idx / CPO, ch = idx % CPO;
           if (r < 16 && o0 + ch * 8 < F && wm0 + 16 * i + r < cur.rows)
-            store_c((i32x4_t*)(o_tile + ((int64_t)(16 * i + r) * F + ch * 8) * 2), *(const i32x4_t*)(stage_c + r * C::EPI_PITCH + ch * 16), 0);
+            // (through L2: 64-byte row segments, see the quantised output; its own wait states as in store_c)
+            asm volatile("global_store_dwordx4 %0, %1, off\n\ts_nop 1"
+                         : : "v"(o_tile + ((int64_t)(16 * i + r) * F + ch * 8) * 2), "v"(*(const i32x4_t*)(stage_c + r * C::EPI_PITCH + ch * 16)) : "memory");
         }
       }
       continue;

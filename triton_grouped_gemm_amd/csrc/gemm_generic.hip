@@ -254,9 +254,9 @@ __global__ __launch_bounds__(GTHREADS) void gemm_generic_kernel(const GemmParams
           const int64_t at = (t.row0 + m) * (int64_t)up + t.n0 / 2 + c;
           *(uint2*)((char*)p.C + at * 2) = pack4<OUT>(v[0], v[1], v[2], v[3]);
           if (p.H) {
-            uint2* const h = (uint2*)((char*)p.H + ((t.row0 + m) * (int64_t)p.N + t.n0 / 2 + c) * 2);
-            *h = pack4<OUT>(acc[i][0][q * 4], acc[i][0][q * 4 + 1], acc[i][0][q * 4 + 2], acc[i][0][q * 4 + 3]);
-            *(uint2*)((char*)h + (int64_t)up * 2) = pack4<OUT>(acc[i][1][q * 4], acc[i][1][q * 4 + 1], acc[i][1][q * 4 + 2], acc[i][1][q * 4 + 3]);
+            float4* const h = (float4*)((float*)p.H + (t.row0 + m) * (int64_t)p.N + t.n0 / 2 + c);
+            *h = make_float4(acc[i][0][q * 4], acc[i][0][q * 4 + 1], acc[i][0][q * 4 + 2], acc[i][0][q * 4 + 3]);
+            *(float4*)((float*)h + up) = make_float4(acc[i][1][q * 4], acc[i][1][q * 4 + 1], acc[i][1][q * 4 + 2], acc[i][1][q * 4 + 3]);
           }
         }
       }

@@ -2,7 +2,7 @@
 // A [Ktot, Mdim], B [Ktot, N], C [G, Mdim, N].
 //
 // One workgroup per CU, four waves, one per SIMD; tile 256x256, every wave owns a 128x128 block of 16x16x32 MFMA tiles with
-// its 256 accumulator registers in AGPRs (see gemm_w4.hip for why, and for the rules that the order of the instructions
+// its 256 accumulator registers in AGPRs (see gemm_w4.hpp for why, and for the rules that the order of the instructions
 // follows).  A K step is 32 tokens, and so is a slab: 16 KB of A and 16 KB of B, token rows of 512 bytes, four slab buffers
 // in LDS.  Per K step q, per wave:
 //   64 multiplies on fragment set q % 2; meanwhile the 16 fragments of slab q + 1 are read into the other set (two
@@ -13,7 +13,7 @@
 // Token rows are 512 bytes whatever the slab's depth, so that the shallow slabs cost no extra requests here (operands whose
 // rows run along K would fetch half lines), and a segment's last slab is padded to 32 tokens and not to 64.
 //
-// The epilogue rides on multiplies as in gemm_w4.hip: strips 0-3 of a wave's block are converted and stored between the
+// The epilogue rides on multiplies as in gemm_w4.hpp: strips 0-3 of a wave's block are converted and stored between the
 // multiplies of the tile's last K step, strips 4-7 between those of the next tile's first, whose multiplies start from a
 // zero addend.  Against the eight-wave kernel (gemm_fast.hip, TN), 128 groups of 2048 x 1536 with 64 /
 // 128 / 256 / 512 / 1024 tokens on average, operands in no cache: 190 / 237 / 325 / 488 / 815 -> 179 / 212 / 287 / 432 / 721 us (5120 tokens:
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(WgradCfg::THREADS) void gemm_wgrad_kernel(const Gem
     else lds_read_tr<off, off + 4 * 512>(sa[Q & 7], a_rd[Q & 7]);
   };
 
-  // ---- epilogue (see gemm_w4.hip, B as [G, K, N]): a lane owns row l16 and columns 16 j + 4 lg + (0..3) of block (i, j); a strip
+  // ---- epilogue (see gemm_w4.hpp, B as [G, K, N]): a lane owns row l16 and columns 16 j + 4 lg + (0..3) of block (i, j); a strip
   // goes through the wave's LDS staging as two pieces of 64 columns and leaves as 16-byte stores of 128-byte row segments
   i32x4_t pend_rs = make_rsrc32(0, 0);
   int pend_cols = 0;
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(WgradCfg::THREADS) void gemm_wgrad_kernel(const Gem
     constexpr int EPI_S0 = EPI == 2 ? 0 : 4, EPI_G0 = EPI == 2 ? 4 : 0;
     for_each<64>([&](auto Nc) __attribute__((always_inline)) {
       constexpr int n = decltype(Nc)::value, i = n / 8, j = (i & 1) ? 7 - n % 8 : n % 8;  // snake order: one operand register changes per multiply
-      if constexpr (EPI != 0) {  // block bb of the half in the gap in front of multiply G0 + 7 bb / 4, as in gemm_w4.hip
+      if constexpr (EPI != 0) {  // block bb of the half in the gap in front of multiply G0 + 7 bb / 4, as in gemm_w4.hpp
 #pragma unroll
         for (int bb = 0; bb < 32; ++bb) {
           const int g = EPI_G0 + 7 * bb / 4, si = EPI_S0 + bb / 8, sj = (si & 1) ? 7 - bb % 8 : bb % 8;

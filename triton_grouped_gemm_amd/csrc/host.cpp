@@ -190,7 +190,7 @@ PyObject* m_grouped_gated_gemm(PyObject*, PyObject* const* args, Py_ssize_t narg
   {
     const Unlocked unlocked;
     c = at::empty({m, n / 2}, a.options());
-    if (projections) h = at::empty({m, n}, a.options());
+    if (projections) h = at::empty({m, n}, a.options().dtype(at::kFloat));
     rc = tgg_m_grouped_gated_gemm(a.data_ptr(), b.data_ptr(), c.data_ptr(), projections ? h.data_ptr() : nullptr, sizes.data_ptr(), is64(sizes),
                                   (int)g, m, (int)(n / 2), (int)k, trans_b, act, dt, (int)num_cu, stream());
   }
@@ -248,8 +248,8 @@ PyObject* gated_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int act = activation_code(args[2]);
   if (act < 0 || grad.dim() != 2 || h.dim() != 2 || records(grad) || records(h)) Py_RETURN_NONE;
   const int64_t m = grad.size(0), f = grad.size(1);
-  const int dt = code16(h);
-  if (dt < 0 || grad.scalar_type() != h.scalar_type() || m == 0 || h.size(0) != m || h.size(1) != 2 * f || f < 8 || (f & 7) || f >= (1ll << 30) ||
+  const int dt = code16(grad);
+  if (dt < 0 || h.scalar_type() != at::kFloat || m == 0 || h.size(0) != m || h.size(1) != 2 * f || f < 8 || (f & 7) || f >= (1ll << 30) ||
       !grad.is_contiguous() || !h.is_contiguous())
     Py_RETURN_NONE;
   static const c10::OperatorName op("moe::gated_backward", "");
@@ -259,7 +259,7 @@ PyObject* gated_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   int rc;
   {
     const Unlocked unlocked;
-    dh = at::empty({m, 2 * f}, h.options());
+    dh = at::empty({m, 2 * f}, grad.options());
     rc = tgg_gated_backward(grad.data_ptr(), h.data_ptr(), dh.data_ptr(), m, (int)f, act, dt, stream());
   }
   return done("tgg_gated_backward", rc, dh);

@@ -1,4 +1,4 @@
-// Building blocks shared by the four-wave gfx950 kernels (gemm_w4.hip, gemm_wgrad.hip): multiplies and fragment reads as
+// Building blocks shared by the four-wave gfx950 kernels (gemm_w4.hpp, gemm_wgrad.hip): multiplies and fragment reads as
 // single inline-assembly statements, which the compiler keeps in source order and only allocates registers for.
 #pragma once
 #include "fast_common.hpp"

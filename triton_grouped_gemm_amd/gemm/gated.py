@@ -42,7 +42,7 @@ def _gated_launch(A: Tensor, B: Tensor, size_per_group: Tensor, trans_b: bool, a
     assert A.device == B.device, "A and B must live on one GPU"
     A, B = A.contiguous(), B.contiguous()
     out = A.new_empty(M, N // 2)
-    h = A.new_empty(M, N) if projections else None
+    h = A.new_empty(M, N, dtype=torch.float32) if projections else None
     if M == 0:
         return out, h
     with torch.cuda.device(A.device):
@@ -73,7 +73,7 @@ def m_grouped_gated_gemm_projections(A: Tensor, B: Tensor, size_per_group: Tenso
 @m_grouped_gated_gemm_projections.register_fake
 def _(A, B, size_per_group, trans_b=False, activation="silu", numSM=-1):
     N = B.shape[1] if trans_b else B.shape[2]
-    return A.new_empty(A.shape[0], N // 2), A.new_empty(A.shape[0], N)
+    return A.new_empty(A.shape[0], N // 2), A.new_empty(A.shape[0], N, dtype=torch.float32)
 
 
 @torch.library.custom_op("moe::gated_backward", mutates_args=())
@@ -81,23 +81,23 @@ def gated_backward(grad: Tensor, h: Tensor, activation: str = "silu") -> Tensor:
     code = _activation_code(activation)
     assert grad.dim() == 2 and h.dim() == 2 and h.shape == (grad.shape[0], 2 * grad.shape[1]), \
         "grad must be [M, F] and h [M, 2 F]"
-    assert h.dtype in _native.DTYPE_CODE and grad.dtype == h.dtype, f"data types {grad.dtype} and {h.dtype} not supported"
+    assert grad.dtype in _native.DTYPE_CODE and h.dtype == torch.float32, f"data types {grad.dtype} and {h.dtype} not supported"
     assert grad.shape[1] % 8 == 0 and grad.shape[1] > 0, "F must be a multiple of 8 (16-byte rows)"
     _native.require_gpu(grad, h)
     assert grad.device == h.device, "grad and h must live on one GPU"
     grad, h = grad.contiguous(), h.contiguous()
-    dh = torch.empty_like(h)
+    dh = grad.new_empty(h.shape)
     if not h.shape[0]:
         return dh
     with torch.cuda.device(h.device):
         _native.call("tgg_gated_backward", grad.data_ptr(), h.data_ptr(), dh.data_ptr(), grad.shape[0], grad.shape[1], code,
-                     _native.DTYPE_CODE[h.dtype], _native.stream_of(h))
+                     _native.DTYPE_CODE[grad.dtype], _native.stream_of(h))
     return dh
 
 
 @gated_backward.register_fake
 def _(grad, h, activation="silu"):
-    return torch.empty_like(h)
+    return grad.new_empty(h.shape)
 
 
 class _Gated(_native.EagerOp):
@@ -115,8 +115,8 @@ class _Gated(_native.EagerOp):
 
 
 class _GatedProjections(_native.EagerOp):
-    """The operator ``moe::m_grouped_gated_gemm_projections``: ``(out [M, F], h [M, 2 F])``, h the projections rounded to the
-    operands' type, which ``gated_backward`` takes."""
+    """The operator ``moe::m_grouped_gated_gemm_projections``: ``(out [M, F], h [M, 2 F])``, h the projections in fp32,
+    which ``gated_backward`` takes."""
     __name__ = "m_grouped_gated_gemm_projections"
 
     def __call__(self, A: Tensor, B: Tensor, size_per_group: Tensor, trans_b: bool = False, activation: str = "silu",

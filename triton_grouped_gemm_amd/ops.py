@@ -73,7 +73,8 @@ def gmm(a, b, batch_sizes, trans_b=False, num_sm=-1):
 
 
 class GatedGroupedGemm(torch.autograd.Function):
-    """``gated_gmm`` with the gradients of activations and weights: the projections are kept (in the operands' type), one pass
+    """``gated_gmm`` with the gradients of activations and weights: the projections are kept (in fp32: their rounding would be a
+    third one in the gradients, beside that of ``dh`` and their own), one pass
     makes their gradient ``dh`` from the output's, and the grouped products of ``dh`` are those of ``gmm``."""
 
     @staticmethod
