@@ -84,8 +84,9 @@ CASES = [
 ]
 
 
-# the shape-agnostic kernel, the routes of ordinary calls, the eight-wave kernel alone, the four-wave kernel wherever it can
-PATHS = {"generic": ("force_generic", 1, 0), "routed": ("four_wave", 1, 1), "eight_wave": ("four_wave", 0, 1), "four_wave": ("four_wave", 2, 1)}
+# the shape-agnostic kernel, the routes of ordinary calls, the eight-wave kernel alone, the four-wave and the deep-ring kernel wherever they can
+PATHS = {"generic": ("force_generic", 1, 0), "routed": ("four_wave", 1, 1), "eight_wave": ("four_wave", 0, 1), "four_wave": ("four_wave", 2, 1),
+         "deep": ("deep", 2, 1)}
 
 
 @pytest.fixture(params=sorted(PATHS))

@@ -81,6 +81,8 @@ bool fast_quant_supported(const GemmParams& p, int dt, int layout);
 int launch_fast_16bit_quant(const GemmParams& p, int dt, int layout, hipStream_t s);
 void set_fast_variant(int v);
 void set_fp8_variant(int v);
+bool deep_gated_supported(const GemmParams& p, int dt, int layout, bool any_size);
+int launch_deep_gated(const GemmParams& p, int dt, int layout, hipStream_t s);
 bool w4_gated_supported(const GemmParams& p, int dt, int layout, bool any_size);
 int launch_w4_gated(const GemmParams& p, int dt, int layout, hipStream_t s);
 bool fast_gated_supported(const GemmParams& p, int dt, int layout);
@@ -246,7 +248,8 @@ static int dispatch_16bit(const GemmParams& p, int dt, int layout, hipStream_t s
 // The gated block (GemmParams::H): the plain product's routes, of the kernels that are instantiated for it
 static int dispatch_gated(const GemmParams& p, int dt, int layout, hipStream_t s) {
   if (g_force_generic.load() || !fast_gated_supported(p, dt, layout)) return launch_generic_gated(p, dt, layout, s);
-  const int four_wave = g_four_wave.load();
+  const int four_wave = g_four_wave.load(), deep = g_deep.load();
+  if ((deep == 2 || (deep == 1 && four_wave == 1)) && deep_gated_supported(p, dt, layout, deep == 2)) return launch_deep_gated(p, dt, layout, s);
   if (four_wave && w4_gated_supported(p, dt, layout, four_wave == 2)) {
     if (!w4_decided_on_device(p) || four_wave == 2) return launch_w4_gated(p, dt, layout, s);
     GemmParams q = p;

@@ -21,6 +21,7 @@
 // rounds a small tile's operands cost more than its fit gains (128 groups, 32768 rows, N = 1536, K = 2048: 256 us by the larger tiles, 381 here).
 // FP8 with per-channel scales, 100 random launches of up to 8192 rows: 0.62 of the eight-wave kernel's time (0.42-0.87), the same bits.  4 groups of 270
 // rows, N = 2048, K = 4096: 35 -> 16 us; 16 of 3393, N = 768, K = 768: 16.1 -> 12.7.
+#include "gate.hpp"
 #include "launch.hpp"
 #include "w4_common.hpp"
 
@@ -60,10 +61,14 @@ TGG_DEV void copy_slab_b128(const i32x4_t& rsrc, uint32_t lds_addr, int voff, in
 // FP8: a slab is 128 bytes of every row as well, but its multiplies take all 128 values at once (32 per lane: 16-byte chunks lg and lg + 4 of a row,
 // see gemm_fp8.hip).  The two steps of a slab are the two halves of the wave's row blocks; the second one goes column block by
 // column block, and the next slab's fragment takes the place of the one that has been used.
-template <class C, int DT, int LAYOUT, int FA, int FB>
+// GATED: the gated feed-forward block (GemmParams::H).  A wave's columns are half gate, half up projection of the same outputs (column blocks j < TN / 2 and the
+// others), so a lane holds both sums; only where B's rows or columns come from and the epilogue differ.
+template <class C, int DT, int LAYOUT, int FA, int FB, bool GATED = false>
 TGG_DEV void gemm_deep_body(const GemmParams& p) {
   constexpr bool FP8 = LAYOUT == DEEP_FP8;
   constexpr bool B_KMAJOR = LAYOUT != DEEP_NN;
+  static_assert(!GATED || !FP8, "the gated block is 16-bit");
+  const int F = p.N / 2;  // GATED: outputs of a row
   constexpr int ES = FP8 ? 1 : 2, KS = BKD * 2 / ES;  // bytes of an operand's value, values of a slab row
   typedef Operand<C::BM, true> OpA;
   typedef Operand<C::BN, B_KMAJOR> OpB;
@@ -91,10 +96,18 @@ TGG_DEV void gemm_deep_body(const GemmParams& p) {
   for (int k = 0; k < C::CB; ++k) {
     if (B_KMAJOR) {
       const int r_local = lane / OpB::CPR, row = (wave + 4 * k) * OpB::RPI + r_local;
-      const int col = (row & ~(16 * C::TN - 1)) + C::TN * (row & 15) + ((row >> 4) & (C::TN - 1));
+      int col = (row & ~(16 * C::TN - 1)) + C::TN * (row & 15) + ((row >> 4) & (C::TN - 1));
+      if (GATED) {
+        const int j = (row >> 4) & (C::TN - 1);
+        col = (row & ~(16 * C::TN - 1)) / 2 + C::TN / 2 * (row & 15) + j % (C::TN / 2) + (j >= C::TN / 2 ? F : 0);
+      }
       vo_b[k] = OpB::lane_voff(lane, wave % OpB::NPAT, ld) + (col - r_local) * ld;
     } else {
       vo_b[k] = OpB::lane_voff(lane, wave % OpB::NPAT, ld_b) + (wave + 4 * k) * OpB::RPI * ld_b;
+      if (GATED) {
+        const int x = OpB::lane_voff(lane, wave % OpB::NPAT, 0) / 2, y = x % (16 * C::TN);  // the chunk's first column in its LDS row
+        vo_b[k] += ((x - y) / 2 + y % (8 * C::TN) + (y >= 8 * C::TN ? F : 0) - x) * 2;
+      }
     }
   }
   // K tail: lanes whose chunk of a K-contiguous row starts at or beyond K fetch nothing in a tile's last slab
@@ -144,7 +157,11 @@ TGG_DEV void gemm_deep_body(const GemmParams& p) {
       seen_g = t.g;
       const int n_left = p.N - t.n0;
       ra = make_rsrc32(uniform64((uint64_t)p.A + (uint64_t)(t.row0 * ld)), t.rows * ld);
-      if (B_KMAJOR) rb = make_rsrc32(uniform64((uint64_t)p.B + (uint64_t)(((int64_t)t.g * p.N + t.n0) * ld)), (n_left < C::BN ? n_left : C::BN) * ld);
+      // (the gated block: from the gate's first column of the tile to the end of the group's up projection)
+      const int o0 = t.n0 / 2;
+      if (GATED && B_KMAJOR) rb = make_rsrc32(uniform64((uint64_t)p.B + (uint64_t)(((int64_t)t.g * p.N + o0) * ld)), (p.N - o0) * ld);
+      else if (GATED) rb = make_rsrc32(uniform64((uint64_t)p.B + (uint64_t)(((int64_t)t.g * p.K * p.N + o0) * 2)), p.K * ld_b - o0 * 2);
+      else if (B_KMAJOR) rb = make_rsrc32(uniform64((uint64_t)p.B + (uint64_t)(((int64_t)t.g * p.N + t.n0) * ld)), (n_left < C::BN ? n_left : C::BN) * ld);
       // NN: to the end of the group's last token row; what a row segment reads beyond its row are columns that are not stored
       else rb = make_rsrc32(uniform64((uint64_t)p.B + (uint64_t)(((int64_t)t.g * p.K * p.N + t.n0) * 2)), p.K * ld_b - t.n0 * 2);
       left = kt_n;
@@ -283,7 +300,9 @@ TGG_DEV void gemm_deep_body(const GemmParams& p) {
       advance();
       // this wave's copies of the next slab have landed (a tile's stores, younger than those copies for ST - 2 slabs, may be in flight as well),
       // and it has read all it needs of this one
-      if (kt < C::ST - 2 && tile_id != w_first) wait_vmcnt<(C::ST - 2) * C::NC + (B_KMAJOR ? C::STORES_NT : C::STORES_NN)>();
+      // (the gated block stores as often as the plain product with [G, N, K] weights, half as often or once a strip with the others; more with projections)
+      constexpr int STORES = B_KMAJOR ? C::STORES_NT : GATED ? C::TM : C::STORES_NN;
+      if (kt < C::ST - 2 && tile_id != w_first) wait_vmcnt<(C::ST - 2) * C::NC + STORES>();
       else wait_vmcnt<(C::ST - 2) * C::NC>();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __syncthreads();
@@ -299,6 +318,61 @@ TGG_DEV void gemm_deep_body(const GemmParams& p) {
     }
     // ---- epilogue ----
     const int rows_left = cur.rows - wm0;
+    if constexpr (GATED) {
+      constexpr int HN = C::TN / 2;
+      const int o0 = (cur.n0 + wn0) / 2, out_rows = rows_left < C::BM / 2 ? rows_left : C::BM / 2, cols = F - o0;
+      const i32x4_t rc = make_rsrc32(uniform64((uint64_t)p.C + (uint64_t)(((cur.row0 + wm0) * (int64_t)F + o0) * 2)), cols > 0 ? out_rows * F * 2 : 0);
+      int el = lane;
+      asm volatile("s_nop 4" : "+v"(el) : "s"(rc));
+      const int e16 = el & 15, eg = el >> 4;
+      if (p.H) {  // NT: row 4 eg + r, HN neighbouring columns of each; NN: row e16, four
+        float* const h = (float*)p.H + (cur.row0 + wm0) * (int64_t)p.N + o0;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int row = B_KMAJOR ? 4 * eg + r : e16, col = B_KMAJOR ? HN * e16 + j % HN : 16 * (j % HN) + 4 * eg + r;
+              if (col < cols && 16 * i + row < rows_left) h[(int64_t)(16 * i + row) * p.N + col + (j >= HN ? F : 0)] = acc[i][j][r];
+            }
+      }
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < HN; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float x = acc[i][j][r];
+            acc[i][j][r] = (p.act == GATE_SILU ? gate_act<GATE_SILU>(x) : gate_act<GATE_GELU_TANH>(x)) * acc[i][j + HN][r];
+          }
+      if (B_KMAJOR) {
+        const int off0 = HN * e16 < cols ? (4 * eg * F + HN * e16) * 2 : kNoFetch;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int off = off0 + (16 * i + r) * F * 2;
+            const uint32_t w = pack2<DT>(acc[i][0][r], acc[i][HN - 1][r]);
+            if constexpr (HN == 2) asm volatile("buffer_store_dword %0, %1, %2, 0 offen\n\ts_nop 1" : : "v"(w), "v"(off), "s"(rc) : "memory");
+            else asm volatile("buffer_store_short %0, %1, %2, 0 offen\n\ts_nop 1" : : "v"(w), "v"(off), "s"(rc) : "memory");
+          }
+      } else {
+        char* const stage = smem + kDeepEpiOff + wave * C::EPI_WAVE_BYTES;
+        constexpr int CPS = C::TN;  // 16-byte chunks of a staged row; 16 rows are at most one wave's worth
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) {
+#pragma unroll
+          for (int j = 0; j < HN; ++j)
+            *(uint2*)(stage + e16 * C::EPI_PITCH + (16 * j + 4 * eg) * 2) = pack4<DT>(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+          const int r = el / CPS, ch = el % CPS;
+          const i32x4_t v = *(const i32x4_t*)(stage + (r & 15) * C::EPI_PITCH + ch * 16);
+          store_b128<false, 1>(v, r < 16 && ch * 8 < cols ? ((16 * i + r) * F + ch * 8) * 2 : kNoFetch, rc);
+        }
+      }
+      clear();
+      continue;
+    }
     const i32x4_t rc = make_rsrc32(uniform64((uint64_t)p.C + (uint64_t)(((cur.row0 + wm0) * (int64_t)p.N + cur.n0 + wn0) * 2)),
                                    (rows_left < C::BM / 2 ? rows_left : C::BM / 2) * p.N * 2);
     const int cols = p.N - cur.n0 - wn0;
@@ -354,7 +428,7 @@ TGG_DEV void gemm_deep_body(const GemmParams& p) {
 }
 
 // The tile height of the table is 128; the small tiles take the half-height cut that sched_init leaves.
-template <int DT, int LAYOUT, int FA = 0, int FB = 0>
+template <int DT, int LAYOUT, int FA = 0, int FB = 0, bool GATED = false>
 __global__ __launch_bounds__(256) void gemm_deep_kernel(const GemmParams p) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   auto& sched = *reinterpret_cast<SchedTableT<kFastMaxGroups>*>(smem + kDeepSchedOff);
@@ -367,21 +441,21 @@ __global__ __launch_bounds__(256) void gemm_deep_kernel(const GemmParams p) {
   auto rounds = [&](int64_t tiles) { return (int)((tiles + wgs - 1) / wgs); };
   const int small = rounds((int64_t)rows64 * cols64) * 16, mid = rounds((int64_t)rows64 * cols128) * 24, wide = rounds((int64_t)rows128 * cols128) * 32;
   if (wide <= mid && wide < small) {
-    gemm_deep_body<Wide, DT, LAYOUT, FA, FB>(p);
+    gemm_deep_body<Wide, DT, LAYOUT, FA, FB, GATED>(p);
   } else {
     sched_use_half_height(p, sched, half_tile0);
-    if (small <= mid) gemm_deep_body<Small, DT, LAYOUT, FA, FB>(p);
-    else gemm_deep_body<Mid, DT, LAYOUT, FA, FB>(p);
+    if (small <= mid) gemm_deep_body<Small, DT, LAYOUT, FA, FB, GATED>(p);
+    else gemm_deep_body<Mid, DT, LAYOUT, FA, FB, GATED>(p);
   }
 }
 
-template <int DT, int LAYOUT, int FA = 0, int FB = 0>
+template <int DT, int LAYOUT, int FA = 0, int FB = 0, bool GATED = false>
 int launch_deep(const GemmParams& p, hipStream_t s) {
   static bool attr_set[64] = {false};
   int dev = 0;
   (void)hipGetDevice(&dev);
   const bool listed = dev >= 0 && dev < 64;
-  auto kern = gemm_deep_kernel<DT, LAYOUT, FA, FB>;
+  auto kern = gemm_deep_kernel<DT, LAYOUT, FA, FB, GATED>;
   if (!listed || !attr_set[dev]) {
     if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, kDeepSmemBytes) != hipSuccess)
       return check_launch("hipFuncSetAttribute(gemm_deep)");
@@ -434,6 +508,16 @@ static int launch_deep_fp8_out(const GemmParams& p, int out_dt, hipStream_t s) {
 int launch_deep_fp8(const GemmParams& p, int ta, int tb, int out_dt, hipStream_t s) {
   if (ta == DT_E4M3) return tb == DT_E4M3 ? launch_deep_fp8_out<0, 0>(p, out_dt, s) : launch_deep_fp8_out<0, 1>(p, out_dt, s);
   return tb == DT_E4M3 ? launch_deep_fp8_out<1, 0>(p, out_dt, s) : launch_deep_fp8_out<1, 1>(p, out_dt, s);
+}
+
+// The gated block: as the plain product, with one window over a group's gate and up columns.
+bool deep_gated_supported(const GemmParams& p, int dt, int layout, bool any_size) {
+  return (p.N & 15) == 0 && (int64_t)p.N * p.K * 2 < (1ll << 30) && deep_supported(p, dt, layout, any_size);
+}
+
+int launch_deep_gated(const GemmParams& p, int dt, int layout, hipStream_t s) {
+  if (layout == DEEP_NT) return dt == DT_BF16 ? launch_deep<DT_BF16, DEEP_NT, 0, 0, true>(p, s) : launch_deep<DT_F16, DEEP_NT, 0, 0, true>(p, s);
+  return dt == DT_BF16 ? launch_deep<DT_BF16, DEEP_NN, 0, 0, true>(p, s) : launch_deep<DT_F16, DEEP_NN, 0, 0, true>(p, s);
 }
 
 int launch_deep_16bit(const GemmParams& p, int dt, int layout, hipStream_t s) {
