@@ -13,10 +13,12 @@
 // difference is taken in integers, 0x4310 + q - z.  Half precision has a packed subtraction: 0x6400 | q is 1024 + q, less 1024 + z exactly.  A scale
 // group's sum then enters the row's accumulator with its scale: weights are never rounded.
 //
-// A tile is up to 64 rows of a group x some blocks of columns (weights are the multiply's first operand: a lane ends up with four neighbouring columns of
-// a row).  The tile's activations go through LDS in chunks of 32 KB (16 rows x 1024 values, 32 x 512 or 64 x 256), read whole rows at a time: a fragment
+// A tile is up to 64 rows of a group x some blocks of columns.  The activations are the multiply's first operand, so a lane ends up with four rows of one
+// column: it needs one scale (and zero point) of a scale group, not four.  What bounds a launch with small scale groups is the number of load instructions, 16
+// cycles of the address unit each: with weights first and a load per scale group and block, 2047 rows over 64 groups, N = 1544, K = 2080, groups of 32 with zero points
+// took 79 us; the lanes' four quarters now load four groups' scales at once and hand them round.  The tile's activations go through LDS in chunks of 32 KB (16 rows x 1024 values, 32 x 512 or 64 x 256), read whole rows at a time: a fragment
 // read straight from memory touches sixteen rows, a cache line for every lane (that way, with the waves' sums joined in LDS, 128 groups of 64 rows, N = 4096,
-// K = 1536: 604 us, this way 224; 512 rows over 128 groups, N = 2048, K = 768: 46 and 25).  Two chunks alternate; the one after the next waits in registers.  Codes go from memory to registers two blocks ahead.  The four waves
+// K = 1536: 604 us, this way 224; 512 rows over 128 groups, N = 2048, K = 768: 46 and 25).  Two chunks alternate; the one after the next waits in registers.  Codes go from memory to registers two or four blocks ahead.  The four waves
 // of a workgroup take columns side by side, or, where there are too few tiles to go round, every fourth block along K, and add up in LDS, in order.
 // All loads go through buffer descriptors, whose range check gives zeros for rows and values beyond the operands.
 #include <type_traits>
@@ -122,9 +124,10 @@ TGG_DEV rsrc_t window(const void* base, int64_t bytes) {
 }
 constexpr int kNowhere = 0x7ffffff0;  // beyond every window
 
-template <int DT> TGG_DEV f32x4_t mma(const i32x4_t& w, const i32x4_t& x, const f32x4_t& c) {
-  if constexpr (DT == DT_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), __builtin_bit_cast(bf16x8_t, x), c, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w), __builtin_bit_cast(f16x8_t, x), c, 0, 0, 0);
+// c[row][column] += x[row][k] w[column][k]: the lane's rows 4 lg + (0..3) of column l16
+template <int DT> TGG_DEV f32x4_t mma(const i32x4_t& x, const i32x4_t& w, const f32x4_t& c) {
+  if constexpr (DT == DT_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, w), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, x), __builtin_bit_cast(f16x8_t, w), c, 0, 0, 0);
 }
 
 template <int DT> TGG_DEV float scale_value(uint32_t bits) {
@@ -174,46 +177,41 @@ TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
   auto col_of = [&](int c) { return out0 + (c % OC) * 16 + (GATED && c >= OC ? F : 0); };
   const int out_n = GATED ? F : N;
 
-  // ---- activations: chunks of 16 RB rows x KC values, 16-byte pieces of a row swizzled by the row's number (a fragment read touches 16 rows) ----
-  constexpr int KC = kI4Chunk / 2 / (16 * RB), PIECES = KC / 8, PER = kI4Chunk / 16 / kI4Threads, BLOCKS = KC / 128;
+  // ---- activations: chunks of 16 RB rows x KC values (32 KB, or 24 where RB = 3), 16-byte pieces of a row swizzled by the row's number (a fragment read touches 16 rows) ----
+  constexpr int KC = RB == 1 ? 1024 : RB == 2 ? 512 : 256, PIECES = KC / 8, PER = 16 * RB * PIECES / kI4Threads, BLOCKS = KC / 128;
+  static_assert(16 * RB * KC * 2 <= kI4Chunk, "a chunk's place");
   i32x4_t xr[PER];
+  static_assert(PIECES % 16 == 0 && (KC == 256 || kI4Threads % PIECES == 0 || PIECES % kI4Threads == 0), "a thread keeps its place in a row");
+  constexpr int TPR = PIECES < kI4Threads ? PIECES : kI4Threads, ROWS_PER = kI4Threads / TPR;  // threads of a row, rows of one go
+  const int xt_row = tid / TPR, xt_col = tid % TPR;
   auto x_load = [&](int chunk) __attribute__((always_inline)) {
+    const int k = chunk * KC + xt_col * 8;
+    const uint32_t at = k < K ? (uint32_t)((xt_row * K + k) * 2) : (uint32_t)kNowhere;  // (beyond every window also with 64 rows' distance added)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = tid + i * kI4Threads, r = u / PIECES, k = chunk * KC + (u % PIECES) * 8;
-      xr[i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xw, k < K ? (r * K + k) * 2 : kNowhere, 0, 0));
-    }
+    for (int i = 0; i < PER; ++i)
+      xr[i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xw, (int)(at + (uint32_t)(i * ROWS_PER * K * 2)), 0, 0));
   };
   auto x_store = [&](int chunk) __attribute__((always_inline)) {
+    char* const to = lds + (chunk & 1) * kI4Chunk + xt_row * (KC * 2);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = tid + i * kI4Threads, r = u / PIECES, c = u % PIECES;
-      *(i32x4_t*)(lds + (chunk & 1) * kI4Chunk + r * (KC * 2) + ((c ^ (r & 15)) << 4)) = xr[i];
-    }
+    for (int i = 0; i < PER; ++i) *(i32x4_t*)(to + i * ROWS_PER * (KC * 2) + ((xt_col ^ ((xt_row + i * ROWS_PER) & 15)) << 4)) = xr[i];
   };
 
   struct Stage {
     i32x4_t code[CB];
-    uint2 scale[GPT][CB];
-    uint8_t zero[ZEROS ? GPT : 1][CB];
+    uint16_t scale[CB];  // of the lane's column in scale group lg mod GPT of the block
+    uint8_t zero[ZEROS ? CB : 1];
   };
   auto load = [&](Stage& st, int kb) __attribute__((always_inline)) {
     const bool live = kb < blocks_k;
+    const int sg = GPT == 1 ? (p.blocks_per_scale == 1 ? kb : kb / p.blocks_per_scale) : kb * GPT + (lg & (GPT - 1));
+    const bool there = sg < p.scale_groups;
 #pragma unroll
     for (int c = 0; c < CB; ++c) {
-      const int block = col_of(c) >> 4;
+      const int block = col_of(c) >> 4, at = sg * N + col_of(c) + l16;
       st.code[c] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(cw, live && block < blocks_n ? (block * blocks_k + kb) * 1024 + lane * 16 : kNowhere, 0, 2));
-    }
-#pragma unroll
-    for (int j = 0; j < GPT; ++j) {
-      const int sg = GPT == 1 ? (p.blocks_per_scale == 1 ? kb : kb / p.blocks_per_scale) : kb * GPT + j;
-#pragma unroll
-      for (int c = 0; c < CB; ++c) {
-        const int n = col_of(c);
-        const bool there = sg < p.scale_groups;
-        st.scale[j][c] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(sw, there ? (sg * N + n + 4 * lg) * 2 : kNowhere, 0, 0));
-        if (ZEROS) st.zero[j][c] = __builtin_amdgcn_raw_buffer_load_b8(zw, there ? sg * N + n + l16 : kNowhere, 0, 0);
-      }
+      st.scale[c] = __builtin_amdgcn_raw_buffer_load_b16(sw, there ? at * 2 : kNowhere, 0, 0);
+      if (ZEROS) st.zero[c] = __builtin_amdgcn_raw_buffer_load_b8(zw, there ? at : kNowhere, 0, 0);
     }
   };
 
@@ -225,77 +223,79 @@ TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
   constexpr int bias2 = ZEROS ? (int)0xc310c310u : (int)0xc308c308u;  // -144 or -136, twice
   const i32x4_t bias = {bias2, bias2, bias2, bias2};
 
-  // block kb of K, the activations' chunk at xs, of which it is block `at`
+  // a block of K whose activations are block `at` of the chunk at xs
   auto compute = [&](const Stage& st, const char* xs, int at) __attribute__((always_inline)) {
     constexpr int SP = 4 / GPT;  // steps of 32 values per scale group
-    i32x4_t x[RB][4];
+    uint32_t meta[CB];
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int b = 0; b < RB; ++b) x[b][s] = *(const i32x4_t*)(xs + (16 * b + l16) * (KC * 2) + (((16 * at + 4 * s + lg) ^ l16) << 4));
+    for (int c = 0; c < CB; ++c) meta[c] = st.scale[c] | (ZEROS ? (uint32_t)st.zero[c] << 16 : 0u);
 #pragma unroll
     for (int j = 0; j < GPT; ++j) {
+      i32x4_t x[RB][SP];
+#pragma unroll
+      for (int s = 0; s < SP; ++s)
+#pragma unroll
+        for (int b = 0; b < RB; ++b) x[b][s] = *(const i32x4_t*)(xs + (16 * b + l16) * (KC * 2) + at * 256 + (((4 * (j * SP + s) + lg) ^ l16) << 4));
       f32x4_t first[RB];
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
         first[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         if constexpr (DT == DT_BF16) {
 #pragma unroll
-          for (int s = 0; s < SP; ++s) first[b] = mma<DT>(bias, x[b][j * SP + s], first[b]);
+          for (int s = 0; s < SP; ++s) first[b] = mma<DT>(x[b][s], bias, first[b]);
         }
       }
 #pragma unroll
       for (int c = 0; c < CB; ++c) {
+        const uint32_t m = GPT == 1 ? meta[c] : (uint32_t)__builtin_amdgcn_ds_bpermute((16 * j + l16) * 4, (int)meta[c]);
         uint32_t zz = 0;
         if constexpr (DT == DT_BF16) {
-          if (ZEROS) zz = st.zero[j][c] * 0x00010001u;
+          if (ZEROS) zz = (m >> 16) * 0x00010001u;
         } else {  // minus (1024 + z): 0xe400 | z
-          zz = ZEROS ? 0xe400e400u + st.zero[j][c] * 0x00010001u : 0xe408e408u;
+          zz = ZEROS ? 0xe400e400u + (m >> 16) * 0x00010001u : 0xe408e408u;
         }
         i32x4_t w[SP];
 #pragma unroll
         for (int s = 0; s < SP; ++s) w[s] = operand<DT, ZEROS>((uint32_t)st.code[c][j * SP + s], zz);
-        const float s4[4] = {scale_value<DT>(st.scale[j][c].x & 0xffff), scale_value<DT>(st.scale[j][c].x >> 16),
-                             scale_value<DT>(st.scale[j][c].y & 0xffff), scale_value<DT>(st.scale[j][c].y >> 16)};
+        const float scale = scale_value<DT>(m & 0xffff);
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
           f32x4_t part = first[b];
 #pragma unroll
-          for (int s = 0; s < SP; ++s) part = mma<DT>(w[s], x[b][j * SP + s], part);
+          for (int s = 0; s < SP; ++s) part = mma<DT>(x[b][s], w[s], part);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[c][b][e] = __builtin_fmaf(part[e], s4[e], acc[c][b][e]);
+          for (int e = 0; e < 4; ++e) acc[c][b][e] = __builtin_fmaf(part[e], scale, acc[c][b][e]);
         }
       }
+      if (GPT == 4) __builtin_amdgcn_sched_barrier(0);  // all groups' operands at once do not fit the registers
     }
   };
 
   constexpr int STEP = KSPLIT ? kI4Waves : 1, OWN = BLOCKS / STEP;  // the wave's blocks of a chunk
   static_assert(OWN >= 1, "a chunk has a block for every wave");
+  constexpr int D = !KSPLIT && CB == 2 && RB <= 2 ? 4 : 2;  // blocks in flight
   const int kb0 = KSPLIT ? wave : 0;
-  Stage st[2];
-  load(st[0], kb0);
-  load(st[1], kb0 + STEP);
+  Stage st[D];
+#pragma unroll
+  for (int i = 0; i < D; ++i) load(st[i], kb0 + i * STEP);
   x_load(0);
   __syncthreads();  // the tile before has been read
   x_store(0);
   x_load(1);
   __syncthreads();
   const int chunks = (blocks_k + BLOCKS - 1) / BLOCKS;
-  for (int q = 0; q < chunks; ++q) {
+  // chunk q, whose first block is in stage S
+  auto chunk = [&](auto Sc, int q) __attribute__((always_inline)) {
+    constexpr int S = decltype(Sc)::value, RUN = OWN < D ? OWN : D;
     const char* const xs = lds + (q & 1) * kI4Chunk;
-    if constexpr (OWN == 1) {
-      compute(st[0], xs, kb0);
-      st[0] = st[1];
-      load(st[1], (q + 2) * BLOCKS + kb0);
-    } else {
-      const int left = (blocks_k - q * BLOCKS - kb0 + STEP - 1) / STEP, n = left < OWN ? left : OWN;  // OWN is even: every chunk starts with stage 0
-      for (int i = 0; i < n; i += 2) {
-        compute(st[0], xs, kb0 + i * STEP);
-        load(st[0], q * BLOCKS + kb0 + (i + 2) * STEP);
-        __builtin_amdgcn_sched_barrier(0);
-        if (i + 1 < n) {
-          compute(st[1], xs, kb0 + (i + 1) * STEP);
-          load(st[1], q * BLOCKS + kb0 + (i + 3) * STEP);
+    const int left = (blocks_k - q * BLOCKS - kb0 + STEP - 1) / STEP, n = left < OWN ? left : OWN;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += RUN) {
+#pragma unroll
+      for (int i = 0; i < RUN; ++i) {
+        if (i == 0 || i0 + i < n) {
+          compute(st[(S + i) % D], xs, kb0 + (i0 + i) * STEP);
+          load(st[(S + i) % D], q * BLOCKS + kb0 + (i0 + i + D) * STEP);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -305,15 +305,31 @@ TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
       if (q + 2 < chunks) x_load(q + 2);
       __syncthreads();
     }
+  };
+  constexpr int TURNS = OWN < D ? D / OWN : 1;  // chunks until the first block is in stage 0 again
+  static_assert(TURNS <= 2, "two chunks in turn");
+  for (int q = 0; q < chunks; q += TURNS) {
+    chunk(std::integral_constant<int, 0>(), q);
+    if constexpr (TURNS == 2) {
+      if (q + 1 < chunks) chunk(std::integral_constant<int, OWN % D>(), q + 1);
+    }
   }
 
+  // Rows 4 lg + e of block b, column l16: neighbouring lanes exchange halves, so that a store is two columns of a row.
   auto put = [&](int c, int b, f32x4_t v, const f32x4_t& u) __attribute__((always_inline)) {
-    const int row = 16 * b + l16, n = col_of(c) + 4 * lg;
     if constexpr (GATED) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = (p.g.act == GATE_SILU ? gate_act<GATE_SILU>(v[e]) : gate_act<GATE_GELU_TANH>(v[e])) * u[e];
     }
-    if (row < rows && n < out_n) *(uint2*)((char*)p.out + ((row0 + row) * out_n + n) * 2) = pack4<DT>(v[0], v[1], v[2], v[3]);
+    const bool odd = l16 & 1;
+    const int n = col_of(c) + (l16 & ~1), row = 16 * b + 4 * lg + (odd ? 2 : 0);
+    char* const at = (char*)p.out + ((row0 + row) * out_n + n) * 2;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float give = odd ? v[e] : v[e + 2], keep = odd ? v[e + 2] : v[e];
+      const float got = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, give), 0xB1, 0xf, 0xf, false));  // quad_perm [1,0,3,2]
+      if (row + e < rows && n < out_n) *(uint32_t*)(at + (int64_t)e * out_n * 2) = odd ? pack2<DT>(got, keep) : pack2<DT>(keep, got);
+    }
   };
   if constexpr (!KSPLIT) {
 #pragma unroll
@@ -351,12 +367,13 @@ TGG_DEV void int4_tiles(const Int4Params& p, const Int4Table& table, char* lds) 
     const Int4Tile t = int4_tile_at(table, p.g.G, (int)id, tiles_n);
     if (t.rows <= 16) int4_tile<DT, GATED, ZEROS, GPT, 1, CB, KSPLIT>(p, t, lds);
     else if (t.rows <= 32) int4_tile<DT, GATED, ZEROS, GPT, 2, CB, KSPLIT>(p, t, lds);
-    else if constexpr (!KSPLIT) {  // four column blocks of 64 rows do not fit the registers: two and two
+    else if constexpr (!KSPLIT) {  // four column blocks of more rows do not fit the registers: two and two
       Int4Tile h = t;
 #pragma unroll 1
       for (int half = 0; half < CB / 2; ++half) {
         h.nt = t.nt * (CB / 2) + half;
-        int4_tile<DT, GATED, ZEROS, GPT, 4, 2, false>(p, h, lds);
+        if (t.rows <= 48) int4_tile<DT, GATED, ZEROS, GPT, 3, 2, false>(p, h, lds);
+        else int4_tile<DT, GATED, ZEROS, GPT, 4, 2, false>(p, h, lds);
       }
     }
     else {  // a chunk of 64 rows has no block for every wave: the tile's halves in turn
@@ -378,13 +395,8 @@ __global__ __launch_bounds__(kI4Threads, 2) void gemm_int4_kernel(const Int4Para
   int4_table(p.g, table);
   // Wide tiles read an activation once for more columns; narrow ones where the wide ones are too few to go round.
   const int64_t row_tiles = table.tile[p.g.G];
-  if constexpr (GPT < 4) {  // (scale groups of 32: four blocks' scales do not fit the registers)
-    if (row_tiles * ((p.g.N + 255) / 256) >= (int64_t)gridDim.x) {
-      int4_tiles<DT, GATED, ZEROS, GPT, 4, false>(p, table, lds);
-      return;
-    }
-  }
-  if (row_tiles * ((p.g.N + 127) / 128) >= (int64_t)gridDim.x) int4_tiles<DT, GATED, ZEROS, GPT, 2, false>(p, table, lds);
+  if (row_tiles * ((p.g.N + 255) / 256) >= (int64_t)gridDim.x) int4_tiles<DT, GATED, ZEROS, GPT, 4, false>(p, table, lds);
+  else if (row_tiles * ((p.g.N + 127) / 128) >= (int64_t)gridDim.x) int4_tiles<DT, GATED, ZEROS, GPT, 2, false>(p, table, lds);
   else int4_tiles<DT, GATED, ZEROS, GPT, 2, true>(p, table, lds);
 }
 
