@@ -350,3 +350,48 @@ def test_refusals(dev, change):
                  lambda: ops.gated_gmm(a.clone().requires_grad_(True), b, sizes, kind, True)):
         with pytest.raises(error):
             call()
+
+
+@pytest.mark.parametrize("tokens,hidden,ffn,experts,topk,scoring", [(300, 256, 128, 8, 2, "softmax"), (77, 128, 64, 16, 4, "sigmoid")])
+def test_a_training_layer(dev, tokens, hidden, ffn, experts, topk, scoring):
+    """Router, movement, gated block, down projection and combination with all gradients, against the layer in 64 bits with the same
+    choice of experts.  Rows are rounded to bfloat16 after the block, after the down projection and at the end, gradients after every
+    product: at most five roundings on a way, each 2^-9.2 of the norm, which add like squares to 0.0038; the bound leaves as much again
+    for sums that cancel."""
+    gen = torch.Generator().manual_seed(tokens)
+    x = torch.randn(tokens, hidden, generator=gen).to(torch.bfloat16)
+    wr = (torch.randn(hidden, experts, generator=gen) * hidden ** -0.5).to(torch.bfloat16)
+    w1 = (torch.randn(experts, 2 * ffn, hidden, generator=gen) * hidden ** -0.5).to(torch.bfloat16)
+    w2 = (torch.randn(experts, hidden, ffn, generator=gen) * ffn ** -0.5).to(torch.bfloat16)
+    logits = (x.float() @ wr.float())
+    logits[:, 3] = float("-inf")  # an expert without tokens
+    grad = torch.randn(tokens, hidden, generator=gen).to(torch.bfloat16)
+
+    leaves = [t.to(dev).requires_grad_(True) for t in (x, logits, w1, w2)]
+    xd, ld, w1d, w2d = leaves
+    probs, idx = ops.topk_router(ld, topk, scoring=scoring)
+    rows, row_map = ops.permute(xd, idx, num_experts=experts)
+    _, counts = ops.permute_map(idx, num_experts=experts)
+    y = ops.gmm(ops.gated_gmm(rows, w1d, counts, trans_b=True), w2d, counts, trans_b=True)
+    out = ops.unpermute(y, row_map, probs)
+    got = torch.autograd.grad(out, leaves, grad.to(dev))
+
+    exact = [t.double().requires_grad_(True) for t in (x, logits.clamp_min(-1e9), w1, w2)]
+    xe, le, w1e, w2e = exact
+    chosen = torch.gather(le, 1, idx.cpu().long())
+    if scoring == "softmax":
+        p = torch.softmax(chosen, 1)
+    else:
+        p = torch.sigmoid(chosen)
+        p = p / p.sum(1, keepdim=True)
+    want = 0
+    for j in range(topk):
+        e = idx[:, j].cpu().long()
+        h = torch.stack([w1e[e[t]] @ xe[t] for t in range(tokens)])
+        a = act64(h[:, :ffn], "silu") * h[:, ffn:]
+        want = want + p[:, j:j + 1] * torch.stack([w2e[e[t]] @ a[t] for t in range(tokens)])
+    grads = torch.autograd.grad(want, exact, grad.double())
+    for name, a, b in (("out", out, want), *zip(("dx", "dlogits", "dw1", "dw2"), got, grads)):
+        a, b = a.detach().double().cpu(), b.detach()
+        assert (a - b).norm() <= 7.6e-3 * b.norm(), f"{name}: {((a - b).norm() / b.norm()).item():.2e}"
+    assert torch.count_nonzero(got[2][3]) == 0 and torch.count_nonzero(got[1][:, 3]) == 0

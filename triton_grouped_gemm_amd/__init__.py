@@ -15,8 +15,8 @@ _ALIASED = [
     "gemm", "gemm.layout", "gemm.deep_gemm_ops", "gemm.BF16", "gemm.BF16.m_grouped_gemm",
     "gemm.BF16.m_grouped_gemm_TMA", "gemm.BF16.m_grouped_gemm_masked_TMA", "gemm.BF16.k_grouped_gemm",
     "gemm.BF16.k_grouped_gemm_TMA", "gemm.BF16.utils", "gemm.FP8", "gemm.FP8.m_grouped_gemm_channel_expert",
-    "gemm.FP8.k_grouped_gemm_channel_expert", "quant", "quant.trans_per_block_quant_expand_128x",
-    "quant.fp8_cast",
+    "gemm.FP8.k_grouped_gemm_channel_expert", "gemm.gated", "gemm.INT4", "gemm.INT4.m_grouped_gemm_int4", "quant",
+    "quant.trans_per_block_quant_expand_128x", "quant.fp8_cast", "quant.int4_cast",
 ]
 
 
