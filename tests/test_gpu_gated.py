@@ -156,6 +156,17 @@ def test_gradient_of_the_projections(dev, rows, f, dtype, kind):
     check(got, leaf.grad, slack, dtype, "dh")
 
 
+@pytest.mark.parametrize("kind", ["silu", "gelu_tanh"])
+def test_gradient_far_out(dev, kind):
+    """Beyond |gate| = 100 the activations are x or 0 and their slopes 1 or 0, up to the largest numbers."""
+    x = torch.tensor([1e2, 1e10, 1e25, 3e38, -1e2, -1e10, -1e25, -3e38])
+    h = torch.cat([x, torch.ones(8)])[None].to(dev)
+    d = torch.ones(1, 8, dtype=torch.bfloat16, device=dev)
+    got = gated_backward(d, h, kind).float().cpu()[0]
+    assert torch.equal(got[:8], torch.tensor([1.0] * 4 + [0.0] * 4))
+    assert torch.equal(got[8:12], x[:4].bfloat16().float()) and (got[12:].abs() <= 1e-30).all()
+
+
 def _gradients64(a, b, grad, sizes, trans_b, kind):
     """Gradients in 64 bits and bounds for those made from fp32 projections and a rounded dh."""
     f, u = grad.shape[1], half_step(a.dtype)

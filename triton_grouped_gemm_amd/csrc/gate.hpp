@@ -24,7 +24,8 @@ template <int ACT> TGG_DEV float gate_act(float x) { return x * gate_sigma<ACT>(
 // Activation and its slope at x: sigma + x sigma (1 - sigma) z'(x)
 template <int ACT> TGG_DEV void gate_act_slope(float x, float& act, float& slope) {
   const float s = gate_sigma<ACT>(x);
-  const float dz = ACT == GATE_SILU ? 1.0f : kGelu1 + 3.0f * kGelu3 * (x * x);
+  // (the square kept finite: for |x| beyond 1.8e19 the slope of sigma is an exact 0 and must stay one)
+  const float dz = ACT == GATE_SILU ? 1.0f : kGelu1 + 3.0f * kGelu3 * fminf(x * x, 1e30f);
   act = x * s;
   slope = s + act * (1.0f - s) * dz;
 }
