@@ -49,23 +49,31 @@ template <int RT> TGG_DEV float logit_value(uint32_t u) {
   if (RT == RT_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
   return __builtin_bit_cast(float, u);
 }
-// Its place in the order, as an unsigned integer above 0: 16-bit logits fill the upper 16 bits.
+// Its place in the order, as an unsigned integer above 0 (16-bit logits fill the upper 16 bits): the signed value of sign and magnitude, which is the same for
+// -0 and +0, with the sign bit turned; NaN is the first magnitude behind infinity.
 template <int RT> TGG_DEV uint32_t logit_order(uint32_t u) {
-  constexpr uint32_t inf = RT == RT_F16 ? 0x7c000000u : 0x7f800000u, most = RT == RT_F32 ? 0xffffffffu : 0xffff0000u;
-  const uint32_t mag = u & 0x7fffffffu, flip = (uint32_t)((int)u >> 31) | 0x80000000u;
-  uint32_t key = (u ^ flip) & most;
-  if (mag == 0) key = 0x80000000u;  // -0 is +0
-  if (mag > inf) key = most;        // NaN
-  return key;
+  constexpr uint32_t inf = RT == RT_F16 ? 0x7c000000u : 0x7f800000u, step = RT == RT_F32 ? 1u : 0x10000u;
+  const uint32_t mag = u & 0x7fffffffu, sign = mag > inf ? 0u : (uint32_t)((int)u >> 31);
+  return (((mag > inf ? inf + step : mag) ^ sign) - sign) ^ 0x80000000u;
 }
-template <int RT> TGG_DEV uint32_t logit_of_order(uint32_t key) { return key & 0x80000000u ? key ^ 0x80000000u : ~key & (RT == RT_F32 ? 0xffffffffu : 0xffff0000u); }
+// The same for two 16-bit logits at once, in packed 16-bit instructions (five a logit in place of nine).
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
+typedef __attribute__((ext_vector_type(2))) short s16x2_t;
+template <int RT> TGG_DEV uint32_t logit_order_pair(uint32_t w) {
+  constexpr unsigned short inf = RT == RT_F16 ? 0x7c00 : 0x7f80;
+  const u16x2_t infs = {inf, inf}, behind = {inf + 1, inf + 1}, one = {1, 1};
+  const u16x2_t mag = __builtin_bit_cast(u16x2_t, w & 0x7fff7fffu);
+  const u16x2_t nan = (u16x2_t)0 - __builtin_elementwise_min(__builtin_elementwise_sub_sat(mag, infs), one);  // all ones where NaN
+  const u16x2_t sign = __builtin_bit_cast(u16x2_t, (s16x2_t)(__builtin_bit_cast(s16x2_t, w) >> 15)) & ~nan;
+  return __builtin_bit_cast(uint32_t, (u16x2_t)((__builtin_elementwise_min(mag, behind) ^ sign) - sign)) ^ 0x80008000u;
+}
+template <int RT> TGG_DEV uint32_t logit_of_order(uint32_t key) {
+  const uint32_t value = key ^ 0x80000000u, sign = (uint32_t)((int)value >> 31);
+  return ((value ^ sign) - sign) | (sign & 0x80000000u);
+}
 
 template <int RT> struct KeyOf { typedef uint32_t type; };
 template <> struct KeyOf<RT_F32> { typedef uint64_t type; };
-template <int RT> TGG_DEV typename KeyOf<RT>::type make_key(uint32_t u, int e) {
-  if constexpr (RT == RT_F32) return ((uint64_t)logit_order<RT>(u) << 32) | (0xffffffffu - (uint32_t)e);
-  else return logit_order<RT>(u) | (0xffffu - (uint32_t)e);
-}
 template <int RT> TGG_DEV uint32_t key_logit(typename KeyOf<RT>::type key) {
   if constexpr (RT == RT_F32) return logit_of_order<RT>((uint32_t)(key >> 32));
   else return logit_of_order<RT>(key & 0xffff0000u);
@@ -148,11 +156,19 @@ __global__ __launch_bounds__(kRouterThreads) void router_fwd_kernel(const char* 
   const bool live = token < tokens;
   uint32_t u[VPL];
   load_logits<RT, LPT, VPL, VEC>(logits + token * row_bytes, lane, live ? E : 0, u);
+  // (places beyond E hold -inf behind every real one: they are never chosen)
   Key key[VPL];
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    const int e = expert_of<LPT, VPL, VEC>(lane, i);
-    key[i] = e < E ? make_key<RT>(u[i], e) : 0;
+  for (int i = 0; i < VPL; i += 2) {
+    const uint32_t e = (uint32_t)expert_of<LPT, VPL, VEC>(lane, i), f = (uint32_t)expert_of<LPT, VPL, VEC>(lane, i + 1);
+    if constexpr (RT == RT_F32) {
+      key[i] = ((uint64_t)logit_order<RT>(u[i]) << 32) | (0xffffffffu - e);
+      key[i + 1] = ((uint64_t)logit_order<RT>(u[i + 1]) << 32) | (0xffffffffu - f);
+    } else {
+      const uint32_t both = logit_order_pair<RT>((u[i] >> 16) | u[i + 1]);
+      key[i] = (both << 16) | (0xffffu - e);
+      key[i + 1] = (both & 0xffff0000u) | (0xffffu - f);
+    }
   }
   sort_descending(key);
   Key mine = 0;  // lane t: the t-th of the row
