@@ -18,7 +18,8 @@
 // cycles of the address unit each: with weights first and a load per scale group and block, 2047 rows over 64 groups, N = 1544, K = 2080, groups of 32 with zero points
 // took 79 us; the lanes' four quarters now load four groups' scales at once and hand them round.  The tile's activations go through LDS in chunks of 32 KB (16 rows x 1024 values, 32 x 512 or 64 x 256), read whole rows at a time: a fragment
 // read straight from memory touches sixteen rows, a cache line for every lane (that way, with the waves' sums joined in LDS, 128 groups of 64 rows, N = 4096,
-// K = 1536: 604 us, this way 224; 512 rows over 128 groups, N = 2048, K = 768: 46 and 25).  Two chunks alternate; the one after the next waits in registers.  Codes go from memory to registers two or four blocks ahead.  The four waves
+// K = 1536: 604 us, this way 204; 512 rows over 128 groups, N = 2048, K = 768: 46 and 23).  Two chunks alternate, one multiplied while the other is copied, straight to LDS (through
+// registers 226 and 24.5 us, and scale groups of 32 spilled).  Codes go from memory to registers two or four blocks ahead.  The four waves
 // of a workgroup take columns side by side, or, where there are too few tiles to go round, every fourth block along K, and add up in LDS, in order.
 // All loads go through buffer descriptors, whose range check gives zeros for rows and values beyond the operands.
 #include <type_traits>
@@ -137,15 +138,16 @@ template <int DT> TGG_DEV float scale_value(uint32_t bits) {
 
 // The eight values of a word of codes as a multiply's operand, plus 128 (or 144) in bfloat16.  zz: the zero point in both halves (bfloat16, ZEROS), or
 // minus (1024 + zero point) as a pair of half precision values.
-template <int DT, bool ZEROS> TGG_DEV i32x4_t operand(uint32_t word, uint32_t zz) {
+// mask and base are 0x000f000f and the exponents' bits, in registers: as literals the two would take an instruction each (the 64 rows of above: 204 us for 213).
+template <int DT, bool ZEROS> TGG_DEV i32x4_t operand(uint32_t word, uint32_t zz, uint32_t mask, uint32_t base) {
   i32x4_t r;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    const uint32_t q = (word >> (4 * t)) & 0x000f000fu;
+    const uint32_t q = ((word >> (4 * t)) & mask) | base;
     if constexpr (DT == DT_BF16) {
-      r[t] = (int)(ZEROS ? (q | 0x43104310u) - zz : (q | 0x43004300u));
+      r[t] = (int)(ZEROS ? q - zz : q);
     } else {
-      const f16x2_t v = __builtin_bit_cast(f16x2_t, q | 0x64006400u) + __builtin_bit_cast(f16x2_t, zz);
+      const f16x2_t v = __builtin_bit_cast(f16x2_t, q) + __builtin_bit_cast(f16x2_t, zz);
       r[t] = __builtin_bit_cast(int, v);
     }
   }
@@ -155,7 +157,7 @@ template <int DT, bool ZEROS> TGG_DEV i32x4_t operand(uint32_t word, uint32_t zz
 // GPT: scale groups per 128 values (1 where a group is 128 or more).  RB: row blocks, CB: column blocks of a wave.  KSPLIT: the waves share the columns and
 // take every fourth block along K.
 template <int DT, bool GATED, bool ZEROS, int GPT, int RB, int CB, bool KSPLIT>
-TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
+TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* buf0, char* buf1) {
   // (opaque, so that the lane's offsets are made afresh per tile: hoisted out of the tile loop, those of all variants would spill)
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));
@@ -180,21 +182,24 @@ TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
   // ---- activations: chunks of 16 RB rows x KC values (32 KB, or 24 where RB = 3), 16-byte pieces of a row swizzled by the row's number (a fragment read touches 16 rows) ----
   constexpr int KC = RB == 1 ? 1024 : RB == 2 ? 512 : 256, PIECES = KC / 8, PER = 16 * RB * PIECES / kI4Threads, BLOCKS = KC / 128;
   static_assert(16 * RB * KC * 2 <= kI4Chunk, "a chunk's place");
-  i32x4_t xr[PER];
   static_assert(PIECES % 16 == 0 && (KC == 256 || kI4Threads % PIECES == 0 || PIECES % kI4Threads == 0), "a thread keeps its place in a row");
   constexpr int TPR = PIECES < kI4Threads ? PIECES : kI4Threads, ROWS_PER = kI4Threads / TPR;  // threads of a row, rows of one go
-  const int xt_row = tid / TPR, xt_col = tid % TPR;
-  auto x_load = [&](int chunk) __attribute__((always_inline)) {
-    const int k = chunk * KC + xt_col * 8;
-    const uint32_t at = k < K ? (uint32_t)((xt_row * K + k) * 2) : (uint32_t)kNowhere;  // (beyond every window also with 64 rows' distance added)
+  const int xt_row = tid / TPR, xt_piece = (tid % TPR) ^ (xt_row & 15);
+  // straight to LDS: a wave's instruction fills a kilobyte in the lanes' order, so the swizzle is in which piece a lane fetches
+  auto x_copy = [&](int chunk, char* buf) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      xr[i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xw, (int)(at + (uint32_t)(i * ROWS_PER * K * 2)), 0, 0));
+    for (int i = 0; i < PER; ++i) {
+      const int k = chunk * KC + (xt_piece ^ (i * ROWS_PER & 15)) * 8;
+      const uint32_t at = (k < K ? (uint32_t)((xt_row * K + k) * 2) : (uint32_t)kNowhere) + (uint32_t)(i * ROWS_PER * K * 2);  // (beyond every window also with 64 rows' distance added)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(xw, (lds_ptr_t)(buf + wave * 1024 + i * (kI4Threads * 16)), 16, (int)at, 0, 0, 0);
+    }
   };
-  auto x_store = [&](int chunk) __attribute__((always_inline)) {
-    char* const to = lds + (chunk & 1) * kI4Chunk + xt_row * (KC * 2);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) *(i32x4_t*)(to + i * ROWS_PER * (KC * 2) + ((xt_col ^ ((xt_row + i * ROWS_PER) & 15)) << 4)) = xr[i];
+
+  // the wave's own copies have landed, by a read behind them that the compiler waits for, and then everybody's
+  auto x_landed = [&](const char* buf) __attribute__((always_inline)) {
+    const int last = *(const int*)(buf + (PER - 1) * (kI4Threads * 16) + tid * 16);
+    asm volatile("" : : "v"(last));
+    __syncthreads();
   };
 
   struct Stage {
@@ -221,6 +226,8 @@ TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
 #pragma unroll
     for (int b = 0; b < RB; ++b) acc[c][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   constexpr int bias2 = ZEROS ? (int)0xc310c310u : (int)0xc308c308u;  // -144 or -136, twice
+  uint32_t mask = 0x000f000fu, base = DT != DT_BF16 ? 0x64006400u : ZEROS ? 0x43104310u : 0x43004300u;
+  asm volatile("" : "+s"(mask), "+v"(base));
   const i32x4_t bias = {bias2, bias2, bias2, bias2};
 
   // a block of K whose activations are block `at` of the chunk at xs
@@ -256,7 +263,7 @@ TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
         }
         i32x4_t w[SP];
 #pragma unroll
-        for (int s = 0; s < SP; ++s) w[s] = operand<DT, ZEROS>((uint32_t)st.code[c][j * SP + s], zz);
+        for (int s = 0; s < SP; ++s) w[s] = operand<DT, ZEROS>((uint32_t)st.code[c][j * SP + s], zz, mask, base);
         const float scale = scale_value<DT>(m & 0xffff);
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
@@ -267,7 +274,15 @@ TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
           for (int e = 0; e < 4; ++e) acc[c][b][e] = __builtin_fmaf(part[e], scale, acc[c][b][e]);
         }
       }
-      if (GPT == 4) __builtin_amdgcn_sched_barrier(0);  // all groups' operands at once do not fit the registers
+      // Several scale groups' sums are added in time: all of them at once do not fit the registers.  (Where a block is one group this costs an
+      // overlap of blocks: the 64 rows of above 226 us for 213.)
+      if (GPT == 2 || (GPT == 4 && (j & 1))) {
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+          for (int b = 0; b < RB; ++b) asm volatile("" : "+v"(acc[c][b]));
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   };
 
@@ -278,16 +293,29 @@ TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
   Stage st[D];
 #pragma unroll
   for (int i = 0; i < D; ++i) load(st[i], kb0 + i * STEP);
-  x_load(0);
   __syncthreads();  // the tile before has been read
-  x_store(0);
-  x_load(1);
-  __syncthreads();
+  x_copy(0, buf0);
+  x_landed(buf0);
   const int chunks = (blocks_k + BLOCKS - 1) / BLOCKS;
-  // chunk q, whose first block is in stage S
-  auto chunk = [&](auto Sc, int q) __attribute__((always_inline)) {
-    constexpr int S = decltype(Sc)::value, RUN = OWN < D ? OWN : D;
-    const char* const xs = lds + (q & 1) * kI4Chunk;
+  // Chunk q, in xs, whose first block is in stage S.  All but the last one have all their blocks: without branches around the loads the compiler
+  // can tell how many of them are behind the copies it waits for.
+  constexpr int RUN = OWN < D ? OWN : D;
+  auto whole = [&](auto Sc, int q, const char* xs, char* next) __attribute__((always_inline)) {
+    constexpr int S = decltype(Sc)::value;
+    x_copy(q + 1, next);
+#pragma unroll 1
+    for (int i0 = 0; i0 < OWN; i0 += RUN) {
+#pragma unroll
+      for (int i = 0; i < RUN; ++i) {
+        compute(st[(S + i) % D], xs, kb0 + (i0 + i) * STEP);
+        load(st[(S + i) % D], q * BLOCKS + kb0 + (i0 + i + D) * STEP);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    x_landed(next);
+  };
+  auto last = [&](auto Sc, int q, const char* xs) __attribute__((always_inline)) {
+    constexpr int S = decltype(Sc)::value;
     const int left = (blocks_k - q * BLOCKS - kb0 + STEP - 1) / STEP, n = left < OWN ? left : OWN;
 #pragma unroll 1
     for (int i0 = 0; i0 < n; i0 += RUN) {
@@ -295,25 +323,25 @@ TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
       for (int i = 0; i < RUN; ++i) {
         if (i == 0 || i0 + i < n) {
           compute(st[(S + i) % D], xs, kb0 + (i0 + i) * STEP);
-          load(st[(S + i) % D], q * BLOCKS + kb0 + (i0 + i + D) * STEP);
+          if (OWN > D) load(st[(S + i) % D], q * BLOCKS + kb0 + (i0 + i + D) * STEP);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (q + 1 < chunks) {
-      x_store(q + 1);
-      if (q + 2 < chunks) x_load(q + 2);
-      __syncthreads();
-    }
   };
-  constexpr int TURNS = OWN < D ? D / OWN : 1;  // chunks until the first block is in stage 0 again
-  static_assert(TURNS <= 2, "two chunks in turn");
-  for (int q = 0; q < chunks; q += TURNS) {
-    chunk(std::integral_constant<int, 0>(), q);
-    if constexpr (TURNS == 2) {
-      if (q + 1 < chunks) chunk(std::integral_constant<int, OWN % D>(), q + 1);
-    }
+  static_assert(2 * OWN % D == 0, "after two chunks the first block is in stage 0 again");
+  typedef std::integral_constant<int, 0> Even;
+  typedef std::integral_constant<int, OWN % D> Odd;
+  int q = 0;
+  while (q + 1 < chunks) {
+    whole(Even(), q, buf0, buf1);
+    if (++q + 1 == chunks) break;
+    whole(Odd(), q, buf1, buf0);
+    ++q;
   }
+  if constexpr (OWN % D == 0) last(Even(), q, q & 1 ? buf1 : buf0);
+  else if (q & 1) last(Odd(), q, buf1);
+  else last(Even(), q, buf0);
 
   // Rows 4 lg + e of block b, column l16: neighbouring lanes exchange halves, so that a store is two columns of a row.
   auto put = [&](int c, int b, f32x4_t v, const f32x4_t& u) __attribute__((always_inline)) {
@@ -337,8 +365,8 @@ TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
 #pragma unroll
       for (int b = 0; b < RB; ++b) put(c, b, acc[c][b], acc[GATED ? c + OC : c][b]);
   } else {  // the waves' sums, added in their order
-    float4* const red = (float4*)lds;  // [wave][column block][row block][lane]
-    static_assert(kI4Waves * CB * RB * 1024 <= 2 * kI4Chunk, "the sums fit where the activations were");
+    float4* const red = (float4*)buf0;  // [wave][column block][row block][lane]
+    static_assert(kI4Waves * CB * RB * 1024 <= kI4Chunk, "the sums fit where the activations were");
     __syncthreads();
 #pragma unroll
     for (int c = 0; c < CB; ++c)
@@ -359,21 +387,21 @@ TGG_DEV void int4_tile(const Int4Params& p, const Int4Tile& t, char* lds) {
 }
 
 template <int DT, bool GATED, bool ZEROS, int GPT, int CB, bool KSPLIT>
-TGG_DEV void int4_tiles(const Int4Params& p, const Int4Table& table, char* lds) {
+TGG_DEV void int4_tiles(const Int4Params& p, const Int4Table& table, char* buf0, char* buf1) {
   constexpr int COLS = 16 * CB * (KSPLIT ? 1 : kI4Waves);
   const int tiles_n = (p.g.N + COLS - 1) / COLS;
   const TileWalk walk = sched_walk((int64_t)table.tile[p.g.G] * tiles_n, p.g.tile_split != 0);
   for (int64_t id = walk.first; id < walk.end; id += walk.stride) {
     const Int4Tile t = int4_tile_at(table, p.g.G, (int)id, tiles_n);
-    if (t.rows <= 16) int4_tile<DT, GATED, ZEROS, GPT, 1, CB, KSPLIT>(p, t, lds);
-    else if (t.rows <= 32) int4_tile<DT, GATED, ZEROS, GPT, 2, CB, KSPLIT>(p, t, lds);
+    if (t.rows <= 16) int4_tile<DT, GATED, ZEROS, GPT, 1, CB, KSPLIT>(p, t, buf0, buf1);
+    else if (t.rows <= 32) int4_tile<DT, GATED, ZEROS, GPT, 2, CB, KSPLIT>(p, t, buf0, buf1);
     else if constexpr (!KSPLIT) {  // four column blocks of more rows do not fit the registers: two and two
       Int4Tile h = t;
 #pragma unroll 1
       for (int half = 0; half < CB / 2; ++half) {
         h.nt = t.nt * (CB / 2) + half;
-        if (t.rows <= 48) int4_tile<DT, GATED, ZEROS, GPT, 3, 2, false>(p, h, lds);
-        else int4_tile<DT, GATED, ZEROS, GPT, 4, 2, false>(p, h, lds);
+        if (t.rows <= 48) int4_tile<DT, GATED, ZEROS, GPT, 3, 2, false>(p, h, buf0, buf1);
+        else int4_tile<DT, GATED, ZEROS, GPT, 4, 2, false>(p, h, buf0, buf1);
       }
     }
     else {  // a chunk of 64 rows has no block for every wave: the tile's halves in turn
@@ -382,7 +410,7 @@ TGG_DEV void int4_tiles(const Int4Params& p, const Int4Table& table, char* lds) 
       for (int half = 0; half < 2; ++half) {
         h.row0 = t.row0 + 32 * half;
         h.rows = half ? t.rows - 32 : 32;
-        int4_tile<DT, GATED, ZEROS, GPT, 2, CB, true>(p, h, lds);
+        int4_tile<DT, GATED, ZEROS, GPT, 2, CB, true>(p, h, buf0, buf1);
       }
     }
   }
@@ -391,13 +419,14 @@ TGG_DEV void int4_tiles(const Int4Params& p, const Int4Table& table, char* lds) 
 template <int DT, bool GATED, bool ZEROS, int GPT>
 __global__ __launch_bounds__(kI4Threads, 2) void gemm_int4_kernel(const Int4Params p) {
   __shared__ Int4Table table;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kI4Chunk];
+  __shared__ __attribute__((aligned(1024))) char buf0[kI4Chunk];
+  __shared__ __attribute__((aligned(1024))) char buf1[kI4Chunk];
   int4_table(p.g, table);
   // Wide tiles read an activation once for more columns; narrow ones where the wide ones are too few to go round.
   const int64_t row_tiles = table.tile[p.g.G];
-  if (row_tiles * ((p.g.N + 255) / 256) >= (int64_t)gridDim.x) int4_tiles<DT, GATED, ZEROS, GPT, 4, false>(p, table, lds);
-  else if (row_tiles * ((p.g.N + 127) / 128) >= (int64_t)gridDim.x) int4_tiles<DT, GATED, ZEROS, GPT, 2, false>(p, table, lds);
-  else int4_tiles<DT, GATED, ZEROS, GPT, 2, true>(p, table, lds);
+  if (row_tiles * ((p.g.N + 255) / 256) >= (int64_t)gridDim.x) int4_tiles<DT, GATED, ZEROS, GPT, 4, false>(p, table, buf0, buf1);
+  else if (row_tiles * ((p.g.N + 127) / 128) >= (int64_t)gridDim.x) int4_tiles<DT, GATED, ZEROS, GPT, 2, false>(p, table, buf0, buf1);
+  else int4_tiles<DT, GATED, ZEROS, GPT, 2, true>(p, table, buf0, buf1);
 }
 
 template <int DT, bool GATED, bool ZEROS, int GPT>
