@@ -92,6 +92,19 @@ def test_forward(dev, case):
     check(capped, want, slack, dtype)
 
 
+@pytest.mark.parametrize("dtype,gs,zeros", [(torch.bfloat16, 128, False), (torch.float16, 32, True), (torch.bfloat16, 64, True)], ids=["bf16_128", "fp16_32z", "bf16_64z"])
+@pytest.mark.parametrize("k", [256, 264, 768, 1024, 1032, 1544, 2176, 3088, 4112])
+def test_lengths_around_the_chunks_of_activations(dev, k, dtype, gs, zeros):
+    """Tiles of up to 16, 32, 48 and 64 rows, whose activations pass through shared memory 1024, 512 and 256 values at a time, side by side and split along K."""
+    sizes, n = [16, 64, 2, 32, 48, 77], 264
+    x, q, scales, points = make(sizes, n, k, gs, zeros, dtype, k)
+    want, slack = reference(x, q, scales, points, sizes, gs, None)
+    args = (x.to(dev), pack_int4(q.to(dev)), scales.to(dev), torch.tensor(sizes, dtype=torch.int32, device=dev), gs, None if points is None else points.to(dev))
+    for cap in (None, 16, 8, 3):  # 7 row tiles: split along K, 128 columns a tile, 256, and several tiles a workgroup
+        got = m_grouped_gemm_int4(*args) if cap is None else m_grouped_gemm_int4(*args, numSM=cap)
+        check(got, want, slack, dtype)
+
+
 @pytest.mark.parametrize("kind", [None, "silu"])
 @pytest.mark.parametrize("rows", [5, 90])
 def test_rows_behind_the_last_group_and_neighbours_are_left_alone(dev, rows, kind):
