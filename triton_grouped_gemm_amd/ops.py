@@ -329,8 +329,29 @@ _LOGIT_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_TOPK = 64
 
 
+def _check_router(logits: Tensor, topk: int, scoring: int) -> None:
+    if logits.dim() != 2 or logits.dtype not in _LOGIT_CODE:
+        raise ValueError(f"logits must be a [tokens, experts] tensor in bf16, fp16 or fp32, got {tuple(logits.shape)} {logits.dtype}")
+    experts = logits.shape[1]
+    if not 1 <= experts <= MAX_EXPERTS:
+        raise ValueError(f"the number of experts must be in [1, {MAX_EXPERTS}], got {experts}")
+    if not 1 <= topk <= min(MAX_TOPK, experts):
+        raise ValueError(f"topk must be in [1, {min(MAX_TOPK, experts)}], got {topk}")
+    if scoring not in _SCORING_CODE.values():
+        raise ValueError(f"scoring code {scoring} not supported")
+
+
+def _router_rows(logits: Tensor) -> Tensor:
+    """``logits`` as the kernels read them: neighbouring experts in neighbouring places, rows any distance apart."""
+    strided = logits.stride(1) != 1 and logits.shape[1] > 1 or logits.stride(0) < logits.shape[1]
+    return logits.contiguous() if strided else logits
+
+
 @torch.library.custom_op("moe::topk_router", mutates_args=())
 def _router_forward(logits: Tensor, topk: int, scoring: int, renormalize: bool) -> Tuple[Tensor, Tensor]:
+    _check_router(logits, topk, scoring)
+    require_gpu(logits)
+    logits = _router_rows(logits)
     probs = torch.empty((logits.shape[0], topk), dtype=torch.float32, device=logits.device)
     indices = torch.empty((logits.shape[0], topk), dtype=torch.int32, device=logits.device)
     if logits.shape[0]:
@@ -349,9 +370,22 @@ def _(logits, topk, scoring, renormalize):
 
 @torch.library.custom_op("moe::topk_router_backward", mutates_args=())
 def _router_backward(logits: Tensor, probs: Tensor, indices: Tensor, grad: Tensor, scoring: int, renormalize: bool) -> Tensor:
+    if probs.dim() != 2 or probs.dtype != torch.float32:
+        raise ValueError(f"probs must be the [tokens, topk] fp32 tensor of the forward call, got {tuple(probs.shape)} {probs.dtype}")
+    _check_router(logits, probs.shape[1], scoring)
+    if probs.shape[0] != logits.shape[0]:
+        raise ValueError(f"probs must hold one row per token, got {probs.shape[0]} for {logits.shape[0]}")
+    if indices.shape != probs.shape or indices.dtype != torch.int32:
+        raise ValueError(f"indices must be the int32 tensor of the forward call, got {tuple(indices.shape)} {indices.dtype}")
+    if grad.shape != probs.shape or not grad.dtype.is_floating_point:
+        raise ValueError(f"grad must be a floating-point tensor of the shape of probs, got {tuple(grad.shape)} {grad.dtype}")
+    if not probs.device == indices.device == grad.device == logits.device:
+        raise ValueError("all operands must live on one GPU")
+    require_gpu(logits)
+    logits = _router_rows(logits)
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     if logits.shape[0]:
-        grad = grad.float().contiguous()
+        probs, indices, grad = probs.contiguous(), indices.contiguous(), grad.float().contiguous()
         with torch.cuda.device(logits.device):
             _native.call("tgg_moe_router_bwd", logits.data_ptr(), logits.stride(0), probs.data_ptr(), indices.data_ptr(),
                          grad.data_ptr(), logits.shape[0], logits.shape[1], probs.shape[1], scoring, int(renormalize),
@@ -397,17 +431,10 @@ def topk_router(logits, topk, scoring="softmax", renormalize=True):
             return result
     if scoring not in _SCORING_CODE:
         raise ValueError(f"scoring must be one of {sorted(_SCORING_CODE)}, got {scoring!r}")
+    topk, code, renormalize = int(topk), _SCORING_CODE[scoring], bool(renormalize)
+    _check_router(logits, topk, code)
     require_gpu(logits)
-    if logits.dim() != 2 or logits.dtype not in _LOGIT_CODE:
-        raise ValueError(f"logits must be a [tokens, experts] tensor in bf16, fp16 or fp32, got {tuple(logits.shape)} {logits.dtype}")
-    experts, topk = logits.shape[1], int(topk)
-    if not 1 <= experts <= MAX_EXPERTS:
-        raise ValueError(f"the number of experts must be in [1, {MAX_EXPERTS}], got {experts}")
-    if not 1 <= topk <= min(MAX_TOPK, experts):
-        raise ValueError(f"topk must be in [1, {min(MAX_TOPK, experts)}], got {topk}")
-    if logits.stride(1) != 1 and experts > 1 or logits.stride(0) < experts:
-        logits = logits.contiguous()
-    code, renormalize = _SCORING_CODE[scoring], bool(renormalize)
+    logits = _router_rows(logits)  # recorded, so that a copy's gradient has the logits' strides
     if not _records(logits):
         return _router_forward(logits, topk, code, renormalize)
     return TopkRouter.apply(logits, topk, code, renormalize)
