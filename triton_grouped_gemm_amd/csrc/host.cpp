@@ -433,6 +433,7 @@ int router_forward(const at::Tensor& logits, int64_t topk, int64_t scoring, bool
   return tgg_moe_router(logits.data_ptr(), logits.stride(0), logits.size(0), (int)logits.size(1), (int)topk, (int)scoring, renorm, router_code(logits),
                         (float*)probs.data_ptr(), (int32_t*)indices.data_ptr(), stream());
 }
+const c10::OperatorName kRouterOp("moe::topk_router", ""), kRouterBackwardOp("moe::topk_router_backward", "");
 struct RouterFunction : torch::autograd::Function<RouterFunction> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, int64_t topk, int64_t scoring, bool renorm) {
     at::Tensor probs, indices;
@@ -450,6 +451,7 @@ struct RouterFunction : torch::autograd::Function<RouterFunction> {
       const at::AutoGradMode no_graph(false);
       const torch::autograd::variable_list saved = ctx->get_saved_variables();
       const at::Tensor &logits = saved[0], &probs = saved[1], &indices = saved[2], grad = grads[0].to(at::kFloat).contiguous();
+      RECORD_FUNCTION(kRouterBackwardOp.name, std::vector<c10::IValue>({logits, probs, indices, grad}));
       out = at::empty(logits.sizes(), logits.options());
       TORCH_CHECK(tgg_moe_router_bwd(logits.data_ptr(), logits.stride(0), (const float*)probs.data_ptr(), (const int32_t*)indices.data_ptr(),
                                      (const float*)grad.data_ptr(), logits.size(0), (int)logits.size(1), (int)probs.size(1),
@@ -474,11 +476,14 @@ PyObject* topk_router(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (logits.dim() != 2 || logits.numel() == 0 || logits.stride(1) != 1 || logits.stride(0) < logits.size(1) || logits.size(1) > kMaxExperts || topk < 1 ||
       topk > 64 || topk > logits.size(1) || router_code(logits) < 0)
     Py_RETURN_NONE;
+  const bool recorded = records(logits);
+  if (replaced(kRouterOp) || (recorded && replaced(kRouterBackwardOp))) Py_RETURN_NONE;
+  RECORD_FUNCTION(kRouterOp.name, std::vector<c10::IValue>({logits, (int64_t)topk, (int64_t)scoring, renorm}));
   at::Tensor probs, indices;
   int rc = 0;
   {
     const Unlocked unlocked;
-    if (records(logits)) {
+    if (recorded) {
       const torch::autograd::variable_list both = RouterFunction::apply(logits, (int64_t)topk, (int64_t)scoring, renorm);
       probs = both[0];
       indices = both[1];

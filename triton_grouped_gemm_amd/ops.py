@@ -398,6 +398,10 @@ def _(logits, probs, indices, grad, scoring, renormalize):
     return logits.new_empty(logits.shape)
 
 
+# (what is registered for them runs in ``topk_router`` too: see EagerOp)
+_router_forward.__class__ = _router_backward.__class__ = _native.EagerOp
+
+
 class TopkRouter(torch.autograd.Function):
     """``topk_router`` with the gradient of the logits; the experts' numbers have none.  (An ordinary eager call is recorded by the
     native call path instead, with the same two launches.)"""
@@ -425,7 +429,7 @@ def topk_router(logits, topk, scoring="softmax", renormalize=True):
     all.  ``scoring``: ``"softmax"`` over all experts or ``"sigmoid"``; ``renormalize`` divides the chosen probabilities by their
     sum.  A logit of ``-inf`` masks an expert, which is then never chosen: entries left over have index -1, an assignment that ``permute``
     drops, and probability 0.  Arithmetic is fp32; differentiable in ``logits``."""
-    if not torch.compiler.is_compiling():
+    if not (_router_forward.replaced or _router_backward.replaced or torch.compiler.is_compiling()):
         result = (_native._host or _native.host()).topk_router(logits, topk, _SCORING_CODE.get(scoring), renormalize)
         if result is not None:
             return result
