@@ -26,14 +26,15 @@ def m_grouped_gemm_int4(A: Tensor, codes: Tensor, scales: Tensor, size_per_group
                         zeros: Optional[Tensor] = None, activation: Optional[str] = None, numSM: int = -1) -> Tensor:
     if activation is not None and activation not in _native.ACTIVATION_CODE:
         raise ValueError(f"activation must be None or one of {sorted(_native.ACTIVATION_CODE)}, got {activation!r}")
-    if group_size not in (32, 64) and (group_size < 128 or group_size % 128):
-        raise ValueError(f"group_size must be 32, 64 or a multiple of 128, got {group_size}")
+    if group_size not in (32, 64) and (not 128 <= group_size < 1 << 31 or group_size % 128):
+        raise ValueError(f"group_size must be 32, 64 or a multiple of 128 below 2^31, got {group_size}")
     assert A.dim() == 2, "A must be [M, K]"
     assert A.dtype in _native.DTYPE_CODE, f"data type {A.dtype} not supported"
     assert scales.dim() == 3 and scales.dtype == A.dtype, "scales must be [G, ceil(K / group_size), N] in A's type"
     M, K = A.shape
     num_groups, scale_groups, N = scales.shape
     assert K % 8 == 0 and K > 0 and N % 8 == 0 and N > 0, "K and N must be multiples of 8 (16-byte rows)"
+    assert K < 1 << 31 and N < 1 << 31, "K and N must fit 32 bits"
     assert scale_groups == -(-K // group_size), "scales must hold one row per group of group_size values of K"
     assert codes.dtype == torch.uint8 and codes.shape == (num_groups, -(-N // 16), -(-K // 128), 64, 16), \
         "codes must be what pack_int4 returns for [G, N, K] values"

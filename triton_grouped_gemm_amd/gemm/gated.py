@@ -35,6 +35,7 @@ def _gated_launch(A: Tensor, B: Tensor, size_per_group: Tensor, trans_b: bool, a
     assert A.dtype == B.dtype, "A and B must share one data type"
     assert N % 16 == 0 and N > 0, "B must hold F gate and F up columns, F a multiple of 8 (16-byte rows)"
     assert K % 8 == 0, "K must be a multiple of 8 (16-byte rows)"
+    assert K < 1 << 31 and N < 1 << 31, "K and 2 F must fit 32 bits"
     assert size_per_group.dim() == 1 and size_per_group.shape[0] == num_groups, \
         "size_per_group must hold one entry per group of B"
     assert 1 <= num_groups <= _native.MAX_GROUPS, f"at most {_native.MAX_GROUPS} groups are supported"
@@ -83,6 +84,7 @@ def gated_backward(grad: Tensor, h: Tensor, activation: str = "silu") -> Tensor:
         "grad must be [M, F] and h [M, 2 F]"
     assert grad.dtype in _native.DTYPE_CODE and h.dtype == torch.float32, f"data types {grad.dtype} and {h.dtype} not supported"
     assert grad.shape[1] % 8 == 0 and grad.shape[1] > 0, "F must be a multiple of 8 (16-byte rows)"
+    assert grad.shape[1] < 1 << 30, "2 F must fit 32 bits"
     _native.require_gpu(grad, h)
     assert grad.device == h.device, "grad and h must live on one GPU"
     grad, h = grad.contiguous(), h.contiguous()
