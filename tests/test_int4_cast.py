@@ -77,3 +77,14 @@ def test_the_product_refuses(change):
         activation = "silu"
     with pytest.raises(error):
         m_grouped_gemm_int4(x, codes, scales, sizes, gs, zeros, activation)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_weights_that_are_trained_give_operands_without_a_graph(dtype, zeros):
+    w = torch.randn(2, 24, 96, generator=torch.Generator().manual_seed(1)).to(dtype)
+    want = per_group_cast_to_int4(w, 32, zeros)
+    got = per_group_cast_to_int4(torch.nn.Parameter(w.clone()), 32, zeros)
+    for x, y in zip(got, want):
+        assert (x is None) == (y is None)
+        assert x is None or (not x.requires_grad and torch.equal(x, y))

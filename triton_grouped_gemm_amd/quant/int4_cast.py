@@ -46,10 +46,11 @@ def unpack_int4(codes: torch.Tensor, N: int, K: int) -> torch.Tensor:
     return q.permute(0, 1, 4, 2, 5, 3, 6).reshape(G, nb * 16, kb * 128)[:, :N, :K].contiguous()
 
 
+@torch.no_grad()
 def per_group_cast_to_int4(w: torch.Tensor, group_size: int = 128, zeros: bool = False,
                            ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """``w`` ``[G, N, K]`` -> ``(codes, scales [G, ceil(K/group_size), N], zeros or None)`` for ``m_grouped_gemm_int4``, scales in the
-    weights' type (bf16 or fp16; fp32 weights give bf16 scales).
+    weights' type (bf16 or fp16; fp32 weights give bf16 scales).  No gradient is recorded, whether the weights are trained or not.
 
     Without zero points a group's values are ``(q - 8) s`` with s the largest magnitude over 7; with them the group's range, extended
     to hold 0, is divided into 15 steps.  Codes are rounded to nearest against the rounded scale, so that a value is off by at most half
