@@ -83,3 +83,34 @@ def test_lengths_around_the_chunks_of_activations(dev, k, dtype, gs, zeros):
     args = (x.to(dev), pack_int4(q.to(dev)), scales.to(dev), torch.tensor(sizes, dtype=torch.int32, device=dev), gs, None if points is None else points.to(dev))
     for cap in (-1, 16, 8, 3):
         check(m_grouped_gemm_int4(*args, numSM=cap), want, slack)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,gs,zeros,kind", [(torch.bfloat16, 128, False, "silu"), (torch.bfloat16, 32, True, "gelu_tanh"), (torch.float16, 64, True, "silu"),
+                                                 (torch.float16, 128, False, "gelu_tanh")], ids=["bf16_128", "bf16_32z", "fp16_64z", "fp16_128"])
+@pytest.mark.parametrize("n", [288, 416])
+@pytest.mark.parametrize("k", [256, 264, 1032])
+def test_gated_tiles_of_many_rows_and_columns(dev, k, n, dtype, gs, zeros, kind):
+    """Gate and up columns of every width of tile, several tiles of columns, the last one cut: 144 and 208 outputs are no whole tile of 32, 64 or 128.  Tiles
+    of more than 32 rows are worked on as two half tiles of 64 outputs where they are 256 columns wide (14 of them: up to 14 workgroups), as two halves of
+    their rows where they are split along K (a whole GPU)."""
+    sizes = [16, 64, 2, 32, 48, 77]
+    x, q, scales, points = make(sizes, n, k, gs, zeros, dtype, k + n)
+    want, slack = reference(x, q, scales, points, sizes, gs, kind)
+    args = (x.to(dev), pack_int4(q.to(dev)), scales.to(dev), torch.tensor(sizes, dtype=torch.int32, device=dev), gs, None if points is None else points.to(dev), kind)
+    for cap in (-1, 20, 14, 3):
+        check(m_grouped_gemm_int4(*args, numSM=cap), want, slack)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("gs", [32, 64, 128])
+def test_every_code_with_every_zero_point(dev, gs, dtype):
+    """q - z for all q and z in 0..15 in every place of a block, exact: rows of the identity, scales of one."""
+    k, n = 128, 256
+    q = torch.arange(n)[:, None].expand(n, k) % 16
+    points = (torch.arange(n) // 16).to(torch.uint8)
+    args = (torch.eye(k, dtype=dtype, device=dev), pack_int4(q[None].to(dev)), torch.ones(1, k // gs, n, dtype=dtype, device=dev), torch.tensor([k], device=dev), gs)
+    got = m_grouped_gemm_int4(*args, points.expand(1, k // gs, n).contiguous().to(dev))
+    assert torch.equal(got.float().cpu(), (q.t() - points.float()))
+    assert torch.equal(m_grouped_gemm_int4(*args).float().cpu(), q.t() - 8.0)
