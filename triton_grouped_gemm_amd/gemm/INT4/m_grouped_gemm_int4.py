@@ -4,9 +4,13 @@
 
     y[r] = A[r] @ W[g(r)]^T,    W[g][n, k] = (q[n, k] - z[n, k // group_size]) * s[n, k // group_size],    q in 0..15
 
-(z = 8 unless ``zeros`` is given) and returns ``y``, or with ``activation`` the gated block ``act(y[:F]) * y[F:]`` of N = 2 F columns,
-as ``m_grouped_gated_gemm`` does.  Sums are fp32, the weights are not rounded, the result is rounded once.  ``quant.int4_cast`` makes
-the operands: ``per_group_cast_to_int4`` from 16-bit weights, ``pack_int4`` from 4-bit values.
+(z = 8 unless ``zeros`` is given, whose bytes are 0..15 like the codes) and returns ``y``, or with ``activation`` the gated block
+``act(y[:F]) * y[F:]`` of N = 2 F columns, as ``m_grouped_gated_gemm`` does.  Sums are fp32, the weights are not rounded, the result is
+rounded once.  ``quant.int4_cast`` makes the operands: ``per_group_cast_to_int4`` from 16-bit weights, ``pack_int4`` from 4-bit values.
+
+Two limits, because bfloat16 operands are biased codes, 128 + q or 144 + q - z, whose bias is taken back in the fp32 sums: zero points lie on the
+device and are not checked, and one above 15 gives wrong weights; and a row of A with infinities, or with magnitudes that add up to more than
+2e36 within 128 values of K, gives NaN.
 
 It stands beside ``m_grouped_gemm`` (gemm/BF16/m_grouped_gemm_TMA.py:297-462 of the reference, which has no 4-bit weights) and
 is meant for few rows a group: the codes are read once for up to 64 rows of a group.
@@ -66,7 +70,7 @@ def _(A, codes, scales, size_per_group, group_size=128, zeros=None, activation=N
 
 
 class _MGroupedGemmInt4(_native.EagerOp):
-    """The operator ``moe::m_grouped_gemm_int4``; rows past ``sum(size_per_group)`` are left uninitialised, as in
+    """The operator ``moe::m_grouped_gemm_int4``: ``zeros`` are bytes 0..15 (not looked at: others give wrong weights in bfloat16); rows past ``sum(size_per_group)`` are left uninitialised, as in
     ``m_grouped_gemm``.  An ordinary eager call goes to the kernel directly."""
     __name__ = "m_grouped_gemm_int4"
 
