@@ -58,7 +58,7 @@ int tgg_gated_backward(const void* dout, const void* h, void* dh, int64_t M, int
  *   scales  [G, ceil(K/group_size), N] in the activations' type;  zeros  the same shape, one byte each (0..15), or NULL: 8
  * group_size 32, 64 or a multiple of 128.  N and K are multiples of 8, N of 32 with an activation.  fp32 sums, one rounding; the weights are
  * not rounded.  TGG_BF16 multiplies biased codes: zero points above 15 give wrong weights, rows of A with infinities, or with magnitudes that add up to more than
- * 2e36 within 128 values, NaN.  Meant for few rows a group (a decode step).  Rows past sum(sizes) are not written.  The reference has no counterpart. */
+ * 2e36 within 128 values, NaN or infinity.  Meant for few rows a group (a decode step).  Rows past sum(sizes) are not written.  The reference has no counterpart. */
 int tgg_m_grouped_gemm_int4(const void* A, const void* codes, const void* scales, const void* zeros, void* C, const void* sizes, int sizes_i64, int G, int64_t M,
                             int N, int K, int group_size, int activation, int dtype, int num_cu, void* stream);
 

@@ -18,7 +18,7 @@
 // cycles of the address unit each: with weights first and a load per scale group and block, 2047 rows over 64 groups, N = 1544, K = 2080, groups of 32 with zero points
 // took 79 us; the lanes' four quarters now load four groups' scales at once and hand them round.  The tile's activations go through LDS in chunks of 32 KB (16 rows x 1024 values, 32 x 512 or 64 x 256), read whole rows at a time: a fragment
 // read straight from memory touches sixteen rows, a cache line for every lane (that way, with the waves' sums joined in LDS, 128 groups of 64 rows, N = 4096,
-// K = 1536: 604 us, this way 204; 512 rows over 128 groups, N = 2048, K = 768: 46 and 23).  Two chunks alternate, one multiplied while the other is copied, straight to LDS (through
+// K = 1536: 604 us, this way 204-213 by run; 512 rows over 128 groups, N = 2048, K = 768: 46 and 23).  Two chunks alternate, one multiplied while the other is copied, straight to LDS (through
 // registers 226 and 24.5 us, and scale groups of 32 spilled).  Codes go from memory to registers two or four blocks ahead.  The four waves
 // of a workgroup take columns side by side, or, where there are too few tiles to go round, every fourth block along K, and add up in LDS, in order.
 // All loads go through buffer descriptors, whose range check gives zeros for rows and values beyond the operands.

@@ -424,8 +424,8 @@ PyObject* permute(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// (input, row_id_map, probs or None) -> out; records nothing
-// The router with its gradient: what ops.TopkRouter is, recorded and run without Python (26 us of host time for a forward and backward pass in place of 60).
+// The router with its gradient: what ops.TopkRouter is, recorded and run without Python (a forward and backward pass takes 49-51 us of host time in place of
+// 145; torch's own exp takes 42-44, the engine's share of any recorded call).
 int router_code(const at::Tensor& logits) { return logits.scalar_type() == at::kFloat ? 2 : code16(logits); }
 int router_forward(const at::Tensor& logits, int64_t topk, int64_t scoring, bool renorm, at::Tensor& probs, at::Tensor& indices) {
   probs = at::empty({logits.size(0), topk}, logits.options().dtype(at::kFloat));
@@ -495,6 +495,7 @@ PyObject* topk_router(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// (input, row_id_map, probs or None) -> out; records nothing
 PyObject* unpermute(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   TGG_ARGS(3);

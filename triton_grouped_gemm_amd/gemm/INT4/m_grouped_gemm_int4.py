@@ -10,7 +10,7 @@ rounded once.  ``quant.int4_cast`` makes the operands: ``per_group_cast_to_int4`
 
 Two limits, because bfloat16 operands are biased codes, 128 + q or 144 + q - z, whose bias is taken back in the fp32 sums: zero points lie on the
 device and are not checked, and one above 15 gives wrong weights; and a row of A with infinities, or with magnitudes that add up to more than
-2e36 within 128 values of K, gives NaN.
+2e36 within 128 values of K, gives NaN or infinity.
 
 It stands beside ``m_grouped_gemm`` (gemm/BF16/m_grouped_gemm_TMA.py:297-462 of the reference, which has no 4-bit weights) and
 is meant for few rows a group: the codes are read once for up to 64 rows of a group.
