@@ -118,3 +118,29 @@ def test_the_router_s_gradient_with_saved_tensors_elsewhere(dev):
     assert torch.equal(torch.autograd.grad(probs, logits, grad)[0], want)
     got = torch.utils.checkpoint.checkpoint(lambda t: ops.topk_router(t, 6)[0], logits, use_reentrant=False)
     assert torch.equal(torch.autograd.grad(got, logits, grad)[0], want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scoring,renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True)])
+def test_what_hooks_of_saved_tensors_give_back(dev, scoring, renormalize):
+    """Other strides are the same values; another device, type or shape is refused, before the launch where the kernel could read out of range."""
+    logits, grad = torch.randn(40, 24, device=dev, requires_grad=True), torch.randn(40, 3, device=dev)
+
+    def gradient(unpack):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), unpack):
+            probs, _ = ops.topk_router(logits, 3, scoring=scoring, renormalize=renormalize)
+        return torch.autograd.grad(probs, logits, grad)[0]
+
+    want = gradient(lambda t: t)
+    assert torch.equal(gradient(lambda t: t.t().contiguous().t()), want)
+    wide = lambda t: torch.cat([t, t], 1)[:, :t.shape[1]]
+    assert torch.equal(gradient(wide), want)
+    for unpack in (lambda t: t.cpu(), lambda t: t.cpu() if t.dtype is torch.int32 else t):
+        with pytest.raises(RuntimeError, match="must be on cuda"):
+            gradient(unpack)
+    for unpack in (lambda t: t.double(), lambda t: t[:39], lambda t: t[:, :2] if t.shape[1] == 3 else t, lambda t: t.long() if t.dtype is torch.int32 else t,
+                   lambda t: t.reshape(-1)):
+        with pytest.raises(RuntimeError, match="changed in shape or type"):
+            gradient(unpack)
+    with pytest.raises(RuntimeError, match="invalid gradient"):
+        gradient(lambda t: t[:, :20] if t.shape[1] == 24 else t)

@@ -450,7 +450,17 @@ struct RouterFunction : torch::autograd::Function<RouterFunction> {
     if (grads[0].defined()) {
       const at::AutoGradMode no_graph(false);
       const torch::autograd::variable_list saved = ctx->get_saved_variables();
-      const at::Tensor &logits = saved[0], &probs = saved[1], &indices = saved[2], grad = grads[0].to(at::kFloat).contiguous();
+      // What a hook of saved tensors gives back need not be what was saved.  Strides do not matter, and the engine compares the result with the logits.
+      const at::IntArrayRef chosen = grads[0].sizes();
+      TORCH_CHECK(saved[0].dim() == 2 && saved[0].size(0) == chosen[0] && router_code(saved[0]) >= 0 && saved[1].sizes() == chosen &&
+                      saved[1].scalar_type() == at::kFloat && saved[2].sizes() == chosen && saved[2].scalar_type() == at::kInt,
+                  "topk_router: the tensors saved for its backward pass have changed in shape or type");
+      for (const at::Tensor& t : saved)
+        TORCH_CHECK(t.layout() == at::kStrided && t.device() == grads[0].device(), "topk_router: the tensors saved for its backward pass must be on ", grads[0].device(),
+                    ", got ", t.device());
+      const bool rows = saved[0].stride(1) == 1 && saved[0].stride(0) >= saved[0].size(1);
+      const at::Tensor logits = rows ? saved[0] : saved[0].contiguous(), probs = saved[1].contiguous(), indices = saved[2].contiguous(),
+                       grad = grads[0].to(at::kFloat).contiguous();
       RECORD_FUNCTION(kRouterBackwardOp.name, std::vector<c10::IValue>({logits, probs, indices, grad}));
       out = at::empty(logits.sizes(), logits.options());
       TORCH_CHECK(tgg_moe_router_bwd(logits.data_ptr(), logits.stride(0), (const float*)probs.data_ptr(), (const int32_t*)indices.data_ptr(),
