@@ -265,6 +265,22 @@ int tgg_moe_router(const void* logits, int64_t row_stride, int64_t num_tokens, i
 int tgg_moe_router_bwd(const void* logits, int64_t row_stride, const float* probs, const int32_t* indices, const float* grad, int64_t num_tokens, int num_experts,
                        int topk, int scoring, int renormalize, int dtype, void* dlogits, void* stream);
 
+/* Newton-Schulz orthogonalisation of every matrix of a stack [batch, rows, cols] (contiguous; dtype TGG_BF16, TGG_F16 or 2 = fp32):
+ *   X = x / (|x|_F + eps), then `steps` times  G = X X^T, X = a X + (b G + c G^2) X   (of the transposed matrix where rows > cols: the same matrix),
+ * out in x's type.  Held in 22 bits or more throughout; results in fp16 and fp32 are as good as fp32 products, those in bf16
+ * are multiplied in half precision where that stays below their own rounding.  Values must keep |X| entries below 64 and those of the polynomial
+ * below 64 (any coefficients that keep singular values near 1 do); beyond, results are not finite.
+ * tgg_muon_update: the optimiser's step, in place:
+ *   momentum = beta momentum + (1 - beta) grad (fp32);  u = nesterov ? beta momentum + (1 - beta) grad : momentum;
+ *   weight = keep weight - step X(u), rounded once to its type
+ * grad and weight in types of their own.  Rows and columns up to 65536.  The workspace (256-byte aligned; size from
+ * tgg_newton_schulz_workspace_bytes) is in use until the call's kernels are done.  The reference has no optimiser. */
+int tgg_newton_schulz_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int64_t* bytes);
+int tgg_newton_schulz(const void* x, void* out, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c, float eps, int dtype, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+int tgg_muon_update(void* weight, int weight_dtype, const void* grad, int grad_dtype, float* momentum, int64_t batch, int64_t rows, int64_t cols, float keep, float step,
+                    float beta, int nesterov, int steps, float a, float b, float c, float eps, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Test hook, runs entirely on the host (no GPU needed): the order in which `grid` persistent workgroups walk
  * the output tiles of a launch, computed by the same scheduler functions the kernels execute.  It restates
  * what the reference's grouped_launch / m_indices_pad tile enumeration guarantees

@@ -795,6 +795,52 @@ int tgg_moe_router_bwd(const void* logits, int64_t row_stride, const float* prob
                                (hipStream_t)stream);
 }
 
+// ---- Newton-Schulz orthogonalisation --------------------------------------------------------------------------
+static int newton_schulz_check(int64_t batch, int64_t rows, int64_t cols) {
+  constexpr int64_t most = 1 << 16;
+  if (batch < 0 || rows < 1 || cols < 1) return set_error("bad stack of %lld matrices of %lld x %lld", (long long)batch, (long long)rows, (long long)cols);
+  if (rows > most || cols > most) return set_error("matrices of %lld x %lld: at most %lld rows and columns are supported", (long long)rows, (long long)cols, (long long)most);
+  // one workgroup for 64 x 64 values or 16384 of them, numbered in 31 bits
+  if (batch * (((rows + 63) / 64 + 1) * ((cols + 63) / 64 + 1)) >= (1ll << 31) || batch >= (1ll << 31)) return set_error("a stack of %lld matrices of %lld x %lld is too large", (long long)batch, (long long)rows, (long long)cols);
+  return 0;
+}
+
+int tgg_newton_schulz_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int64_t* bytes) {
+  if (!bytes) return set_error("null pointer");
+  if (int e = newton_schulz_check(batch, rows, cols)) return e;
+  *bytes = batch ? newton_schulz_workspace(batch, (int)rows, (int)cols) : 0;
+  return 0;
+}
+
+static int newton_schulz_operands(const void* x, int x_dtype, const void* out, int out_dtype, int64_t batch, int64_t rows, int64_t cols, int steps, const void* workspace, int64_t workspace_bytes) {
+  if (int e = newton_schulz_check(batch, rows, cols)) return e;
+  if (x_dtype < 0 || x_dtype > 2 || out_dtype < 0 || out_dtype > 2) return set_error("type codes %d and %d not supported", x_dtype, out_dtype);
+  if (steps < 0 || steps > 100) return set_error("steps=%d outside [0, 100]", steps);
+  if (batch == 0) return 0;
+  if (!x || !out || !workspace) return set_error("null pointer");
+  if (((uintptr_t)x & (x_dtype == 2 ? 3 : 1)) || ((uintptr_t)out & (out_dtype == 2 ? 3 : 1))) return set_error("matrices must be aligned to their type");
+  if ((uintptr_t)workspace & 255) return set_error("the workspace must be 256-byte aligned");
+  const int64_t need = newton_schulz_workspace(batch, (int)rows, (int)cols);
+  if (workspace_bytes < need) return set_error("workspace of %lld bytes is too small (need %lld)", (long long)workspace_bytes, (long long)need);
+  return 0;
+}
+
+int tgg_newton_schulz(const void* x, void* out, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c, float eps, int dtype, void* workspace, int64_t workspace_bytes,
+                      void* stream) {
+  if (int e = newton_schulz_operands(x, dtype, out, dtype, batch, rows, cols, steps, workspace, workspace_bytes)) return e;
+  if (batch == 0) return 0;
+  return launch_newton_schulz(x, dtype, nullptr, 0.f, 0, out, dtype, 0, 0.f, 0.f, batch, (int)rows, (int)cols, steps, a, b, c, eps, workspace, (hipStream_t)stream);
+}
+
+int tgg_muon_update(void* weight, int weight_dtype, const void* grad, int grad_dtype, float* momentum, int64_t batch, int64_t rows, int64_t cols, float keep, float step, float beta, int nesterov,
+                    int steps, float a, float b, float c, float eps, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int e = newton_schulz_operands(grad, grad_dtype, weight, weight_dtype, batch, rows, cols, steps, workspace, workspace_bytes)) return e;
+  if (batch == 0) return 0;
+  if (!momentum) return set_error("null pointer");
+  if ((uintptr_t)momentum & 3) return set_error("matrices must be aligned to their type");
+  return launch_newton_schulz(grad, grad_dtype, momentum, beta, nesterov != 0, weight, weight_dtype, 1, keep, step, batch, (int)rows, (int)cols, steps, a, b, c, eps, workspace, (hipStream_t)stream);
+}
+
 int tgg_debug_tile_order(const int64_t* sizes, int G, int mode, int64_t m_total, int64_t aux, int N, int tile,
                          int grid, int split, int64_t* out, int64_t capacity, int64_t* num_tiles) {
   if (!sizes || !out || !num_tiles) return set_error("null pointer");

@@ -44,4 +44,9 @@ int launch_moe_router(const void* logits, int64_t row_bytes, int64_t tokens, int
 int launch_moe_router_bwd(const void* logits, int64_t row_bytes, const float* probs, const int32_t* indices, const float* grad, int64_t tokens,
                           int E, int k, int scoring, int renorm, int dt, void* dlogits, hipStream_t s);
 
+// Newton-Schulz orthogonalisation (newton_schulz.hip); types 0 = bf16, 1 = fp16, 2 = fp32
+int64_t newton_schulz_workspace(int64_t batch, int rows, int cols);
+int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, int nesterov, void* out, int out_dt, int weight, float keep, float step, int64_t batch, int rows, int cols, int steps,
+                         float ca, float cb, float cc, float eps, void* workspace, hipStream_t s);
+
 }  // namespace tgg

@@ -1,0 +1,212 @@
+// Main loop of the 16-bit products of newton_schulz.hip and lora.hip: a workgroup's tiles as one uninterrupted stream of 64-deep slabs.
+//
+// The scheme is that of the eight-wave kernels (gemm_fast.hip): eight waves, two slab buffers in LDS filled by direct copies that run two slabs
+// ahead across tile boundaries, fragment reads a K step ahead across the one barrier a slab, copies issued between multiplies.  What differs is
+// who says what a slab is: a problem P hands out slabs one after another, so a tile may add up products of several pairs of operands
+// (a matrix's two planes, a row's shared projection and its adapters), and takes a tile's sums.  P has
+//
+//   int tile_at(int pos)                  id of the workgroup's pos-th tile, -1 past the last one
+//   int slabs(int id)                     slabs of a tile, at least one
+//   void seek(int id)                     the next slab is the tile's first one; id -1: no more slabs
+//   void next(StreamSlab& s)              descriptors of the next slab; past a tile's last one it seeks the following tile by itself
+//   int a_offset(s, k), b_offset(s, k)    source offset of the lane's part of the wave's k-th copy of the slab's A or B operand, or kNoFetch
+//   void epilogue(id, acc, stage)         the tile's sums: acc[i][j][e] is row wm0 + 16 i + l16, column wn0 + 16 j + 4 lg + e
+//
+// A [rows, K] is K-contiguous; B is K-contiguous rows [columns, K] (B_KMAJOR) or token rows [K, columns].
+#pragma once
+#include "fast_common.hpp"
+
+namespace tgg {
+
+template <int BM_, int BN_, int WM_, int WN_> struct StreamCfg {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int NWAVES = WM * WN, THREADS = NWAVES * 64;
+  static constexpr int A_BYTES = BM * kSlabRowBytes, B_BYTES = BN * kSlabRowBytes, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int CA = A_BYTES / 1024 / NWAVES, CB = B_BYTES / 1024 / NWAVES, NC = CA + CB;  // copies of a wave and slab
+  static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+  static constexpr int EPI_OFF = 2 * STAGE_BYTES;
+  static_assert(CA * NWAVES * 1024 == A_BYTES && CB * NWAVES * 1024 == B_BYTES, "copies must divide evenly over waves");
+  static_assert(NWAVES == 8, "a wave keeps one swizzle pattern for all its copies");
+  static_assert(NC % 2 == 0 && TM % 2 == 0 && (TM * TN / 2) % (NC / 2) == 0, "a slab's copies are spread over the multiplies of two half K steps");
+};
+
+struct StreamSlab {
+  i32x4_t ra, rb;
+  int kind;  // the problem's
+};
+
+// where a wave's block of the tile begins, and a lane's place in a 16 x 16 block
+template <class C> struct StreamPlace {
+  int lane, wave, wm0, wn0, l16, lg;
+  TGG_DEV StreamPlace() {
+    lane = lane_id();
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    wm0 = (wave / C::WN) * (C::BM / C::WM);
+    wn0 = (wave % C::WN) * (C::BN / C::WN);
+    l16 = lane & 15;
+    lg = lane >> 4;
+  }
+};
+
+// Which tiles a workgroup takes: workgroups are dealt round robin to the XCDs, and each XCD takes a contiguous range of ids, so that what
+// runs together in front of one L2 shares operands.
+struct StreamWalk {
+  int first, stride, end;
+  TGG_DEV explicit StreamWalk(int tiles) {
+    const int grid = gridDim.x, id = blockIdx.x;
+    if ((grid & 7) || tiles <= grid) {
+      first = id;
+      stride = grid;
+      end = tiles;
+    } else {
+      const int xcd = id & 7;
+      first = (int)((int64_t)tiles * xcd / 8) + (id >> 3);
+      stride = grid >> 3;
+      end = (int)((int64_t)tiles * (xcd + 1) / 8);
+    }
+  }
+  TGG_DEV int at(int pos) const {
+    const int64_t id = first + (int64_t)pos * stride;
+    return id < end ? (int)id : -1;
+  }
+};
+
+template <int DT> TGG_DEV f32x4_t stream_mma(const i32x4_t& w, const i32x4_t& x, const f32x4_t& c) {
+  if constexpr (DT == DT_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), __builtin_bit_cast(bf16x8_t, x), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w), __builtin_bit_cast(f16x8_t, x), c, 0, 0, 0);
+}
+
+// A copy must not follow the vector instruction that wrote a scalar of its descriptor too closely, and the compiler does not look inside the copies.
+template <class P> TGG_DEV void stream_next(P& prob, StreamSlab& s) {
+  prob.next(s);
+  asm volatile("s_nop 4" : "+s"(s.ra), "+s"(s.rb));
+}
+
+template <class C, int DT, bool B_KMAJOR, class P> TGG_DEV void stream_gemm(P& prob, char* smem) {
+  const StreamPlace<C> at;
+  const uint32_t smem_addr = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
+  const int l16 = at.l16, lg = at.lg;
+
+  // a lane's LDS offsets of the fragment reads, relative to the operand's slab (see gemm_fast.hip)
+  int a_rd[2], b_rd[B_KMAJOR ? 2 : C::TN];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) a_rd[ks] = (at.wm0 + l16) * 128 + (((4 * ks + lg) ^ ((l16 / 2) % 8)) << 4);
+  if (B_KMAJOR) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) b_rd[ks] = (at.wn0 + l16) * 128 + (((4 * ks + lg) ^ ((l16 / 2) % 8)) << 4);
+  } else {
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      const int e = l16 >> 2, c = l16 & 3;
+      const int chunk = ((at.wn0 + 16 * j) / 8 + (c >> 1)) ^ Operand<C::BN, false>::token_swizzle(8 * (lg & 1) + e);
+      b_rd[j] = (lg * 8 + e) * (C::BN * 2) + chunk * 16 + (c & 1) * 8;
+    }
+  }
+  auto load_a = [&](const char* s, int ks, int i) -> i32x4_t { return *(const i32x4_t*)(s + a_rd[ks] + i * 16 * 128); };
+  auto load_b = [&](const char* s, int ks, int j) -> i32x4_t {
+    if (B_KMAJOR) return *(const i32x4_t*)(s + b_rd[ks] + j * 16 * 128);
+    const char* q = s + b_rd[B_KMAJOR ? 0 : j] + ks * 32 * (C::BN * 2);
+    const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr_t)q);
+    // four token rows on: their swizzle is the same (it goes by k % 4 and k / 8, or, in rows of 128 bytes, by k / 2 % 2 and k / 8)
+    const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr_t)(q + 4 * (C::BN * 2)));
+    return __builtin_bit_cast(i32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  constexpr int SP2 = (C::TM * C::TN / 2) / (C::NC / 2), SP1 = 1;  // multiplies between copies, behind the barrier and in the half step after that
+  StreamSlab sc, sc_next;
+  uint32_t sc_base = 0, sc_next_base = 0;
+  auto copy_k = [&](int k) {
+    if (k < C::CA) {
+      copy_b128_to_lds(sc.ra, sc_base + (at.wave + k * C::NWAVES) * 1024, prob.a_offset(sc, k));
+    } else {
+      copy_b128_to_lds(sc.rb, sc_base + C::A_BYTES + (at.wave + (k - C::CA) * C::NWAVES) * 1024, prob.b_offset(sc, k - C::CA));
+    }
+  };
+
+  prob.seek(prob.tile_at(0));
+  stream_next(prob, sc);
+  sc_base = smem_addr;
+#pragma unroll
+  for (int k = 0; k < C::NC; ++k) copy_k(k);
+  wait_vmcnt<0>();
+  __syncthreads();
+  stream_next(prob, sc);
+  sc_base = smem_addr + C::STAGE_BYTES;
+#pragma unroll
+  for (int k = 0; k < C::NC / 2; ++k) copy_k(k);
+  i32x4_t fa[C::TM - 1], fa_last[2], fb[2][C::TN];
+#pragma unroll
+  for (int i = 0; i < C::TM - 1; ++i) fa[i] = load_a(smem, 0, i);
+  fa_last[0] = load_a(smem, 0, C::TM - 1);
+#pragma unroll
+  for (int j = 0; j < C::TN; ++j) fb[0][j] = load_b(smem + C::A_BYTES, 0, j);
+  int ring = 0;
+
+  f32x4_t acc[C::TM][C::TN];
+  for (int pos = 0, id; (id = prob.tile_at(pos)) >= 0; ++pos) {
+    const int slabs = __builtin_amdgcn_readfirstlane(prob.slabs(id));
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    enum { READ_EARLY, READ_ROLL, READ_NONE, READ_CATCH_UP };  // as in gemm_fast.hip
+    auto half = [&](int cur, int h, const char* s, int ks, int mode, int k0, bool prepare = false) {
+      constexpr int HM = C::TM / 2;
+#pragma unroll
+      for (int ii = 0; ii < HM; ++ii) {
+        const int i = h * HM + ii;
+        const i32x4_t a = i == C::TM - 1 ? fa_last[cur] : fa[i < C::TM - 1 ? i : 0];
+#pragma unroll
+        for (int jj = 0; jj < C::TN; ++jj) {
+          const int j = (i & 1) ? C::TN - 1 - jj : jj;
+          acc[i][j] = stream_mma<DT>(fb[cur][j], a, acc[i][j]);
+          const int n = ii * C::TN + jj;
+          if (n == 0 && (mode == READ_EARLY || mode == READ_CATCH_UP)) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j2 = 0; j2 < C::TN; ++j2) fb[cur ^ 1][j2] = load_b(s + C::A_BYTES, ks, j2);
+            fa_last[cur ^ 1] = load_a(s, ks, C::TM - 1);
+            if (mode == READ_CATCH_UP) {
+#pragma unroll
+              for (int i2 = 0; i2 < HM; ++i2) fa[i2] = load_a(s, ks, i2);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (prepare && n == 1) {  // scalar work, under the multiplies just issued
+            stream_next(prob, sc_next);
+            sc_next_base = smem_addr + (ring & 1) * C::STAGE_BYTES;
+          }
+          const int sp = k0 == 0 ? SP1 : SP2;
+          if (k0 >= 0 && (n + 1) % sp == 0 && (n + 1) / sp <= C::NC / 2) {
+            __builtin_amdgcn_sched_barrier(0);
+            copy_k(k0 + (n + 1) / sp - 1);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        if (mode != READ_NONE && i < C::TM - 1) {
+          __builtin_amdgcn_sched_barrier(0);
+          fa[i < C::TM - 1 ? i : 0] = load_a(s, ks, i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    for (int kt = 0; kt < slabs; ++kt) {
+      const char* s = smem + (ring & 1) * C::STAGE_BYTES;
+      const char* sn = smem + ((ring + 1) & 1) * C::STAGE_BYTES;
+      half(0, 0, s, 1, READ_EARLY, C::NC / 2);
+      half(0, 1, s, 1, READ_ROLL, -1, true);
+      half(1, 0, sn, 0, READ_NONE, -1);
+      wait_vmcnt<0>();
+      __syncthreads();
+      sc = sc_next;
+      sc_base = sc_next_base;
+      half(1, 1, sn, 0, READ_CATCH_UP, 0);
+      ++ring;
+    }
+    prob.epilogue(id, acc, at, smem + C::EPI_OFF);
+  }
+  wait_vmcnt<0>();  // the trailing copies, which fetch nothing, still write LDS
+}
+
+}  // namespace tgg
