@@ -265,6 +265,21 @@ int tgg_moe_router(const void* logits, int64_t row_stride, int64_t num_tokens, i
 int tgg_moe_router_bwd(const void* logits, int64_t row_stride, const float* probs, const int32_t* indices, const float* grad, int64_t num_tokens, int num_experts,
                        int topk, int scoring, int renormalize, int dtype, void* dlogits, void* stream);
 
+/* Low-rank adapters of many requests beside a shared projection (dtype TGG_BF16 or TGG_F16):
+ *   out[m] = W x[m] + scales[l] B_l (A_l x[m]),  l = adapters[m];  rows whose entry is outside [0, L) have no adapter
+ * x [M, K], w [N, K], a [L, R, K], b [L, N, R], adapters [M] int32 or int64, scales [L] fp32 or null (1), out [M, N]; rows in any order.  One rounding, at the
+ * end.  N and K multiples of 8 up to 65536, R a multiple of 8 up to 128, L up to 1024.  h [M, R] fp32 (or null) receives scales[l] A_l x[m], zeros without an
+ * adapter, which the backward pass takes.
+ * _bwd: dx [M, K] = W^T g + A_l^T dh, da [L, R, K] = sum of dh[m] x[m]^T, db [L, N, R] = sum of g[m] h[m]^T over each adapter's rows, with
+ * dh[m] = scales[l] B_l^T g[m]; any of the three may be null (x is read for da, w for dx, h for db).  Adapters without rows get zeros.
+ * Sums have a fixed order: equal calls give equal bits.  The workspace (256-byte aligned; size from tgg_lora_workspace_bytes) is in use until
+ * the call's kernels are done.  The reference has no adapters. */
+int tgg_lora_workspace_bytes(int backward, int64_t M, int N, int K, int R, int L, int64_t* bytes);
+int tgg_lora_linear(const void* x, const void* w, const void* a, const void* b, const void* adapters, int adapters_i64, const float* scales, void* out, float* h, int64_t M, int N,
+                    int K, int R, int L, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int tgg_lora_linear_bwd(const void* grad, const void* x, const void* w, const void* a, const void* b, const void* adapters, int adapters_i64, const float* scales, const float* h,
+                        void* dx, void* da, void* db, int64_t M, int N, int K, int R, int L, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Newton-Schulz orthogonalisation of every matrix of a stack [batch, rows, cols] (contiguous; dtype TGG_BF16, TGG_F16 or 2 = fp32):
  *   X = x / (|x|_F + eps), then `steps` times  G = X X^T, X = a X + (b G + c G^2) X   (of the transposed matrix where rows > cols: the same matrix),
  * out in x's type.  Held in 22 bits or more throughout; results in fp16 and fp32 are as good as fp32 products, those in bf16

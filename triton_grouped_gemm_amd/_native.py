@@ -58,6 +58,9 @@ SIGNATURES = {
     "tgg_moe_unpermute_bwd": [_P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _P],
     "tgg_moe_router": [_P, _L, _L, _I, _I, _I, _I, _I, _P, _P, _P],
     "tgg_moe_router_bwd": [_P, _L, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P, _P],
+    "tgg_lora_workspace_bytes": [_I, _L, _I, _I, _I, _I, _P],
+    "tgg_lora_linear": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P, _L, _P],
+    "tgg_lora_linear_bwd": [_P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P, _L, _P],
     "tgg_newton_schulz_workspace_bytes": [_L, _L, _L, _P],
     "tgg_newton_schulz": [_P, _P, _L, _L, _L, _I, _F, _F, _F, _F, _I, _P, _L, _P],
     "tgg_muon_update": [_P, _I, _P, _I, _P, _L, _L, _L, _F, _F, _F, _I, _I, _F, _F, _F, _F, _P, _L, _P],

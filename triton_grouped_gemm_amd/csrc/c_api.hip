@@ -795,6 +795,57 @@ int tgg_moe_router_bwd(const void* logits, int64_t row_stride, const float* prob
                                (hipStream_t)stream);
 }
 
+// ---- low-rank adapters ------------------------------------------------------------------------------------------
+static int lora_check(int64_t M, int64_t N, int64_t K, int R, int L) {
+  if (M < 0 || M >= (1ll << 31)) return set_error("M=%lld outside [0, 2^31)", (long long)M);
+  if (N < 8 || K < 8 || (N & 7) || (K & 7)) return set_error("N and K must be positive multiples of 8, got N=%lld K=%lld", (long long)N, (long long)K);
+  if (N > 65536 || K > 65536) return set_error("N=%lld or K=%lld: at most 65536 is supported", (long long)N, (long long)K);
+  if (R < 8 || R > 128 || (R & 7)) return set_error("the rank must be a multiple of 8 in [8, 128], got %d", R);
+  if (L < 1 || L > TGG_MAX_GROUPS) return set_error("L=%d adapters outside [1, %d]", L, TGG_MAX_GROUPS);
+  // output tiles are numbered in 31 bits
+  if (((M + 127) / 128) * ((max(N, K) + 127) / 128) >= (1ll << 30)) return set_error("M=%lld, N=%lld, K=%lld: too large", (long long)M, (long long)N, (long long)K);
+  return 0;
+}
+
+int tgg_lora_workspace_bytes(int backward, int64_t M, int N, int K, int R, int L, int64_t* bytes) {
+  if (!bytes) return set_error("null pointer");
+  if (int e = lora_check(M, N, K, R, L)) return e;
+  *bytes = M ? lora_workspace(backward, M, N, K, R, L) : 0;
+  return 0;
+}
+
+static int lora_operands(int backward, const void* ids, int ids_i64, const float* scales, int64_t M, int N, int K, int R, int L, int dtype, const void* ws, int64_t ws_bytes) {
+  if (dtype != TGG_BF16 && dtype != TGG_F16) return set_error("data type code %d not supported", dtype);
+  if ((uintptr_t)ids & (ids_i64 ? 7 : 3)) return set_error("adapters must be aligned to their type");
+  if ((uintptr_t)scales & 3) return set_error("scales must be aligned to their type");
+  if (!ids || !ws) return set_error("null pointer");
+  if ((uintptr_t)ws & 255) return set_error("the workspace must be 256-byte aligned");
+  const int64_t need = lora_workspace(backward, M, N, K, R, L);
+  if (ws_bytes < need) return set_error("workspace of %lld bytes is too small (need %lld)", (long long)ws_bytes, (long long)need);
+  return 0;
+}
+
+int tgg_lora_linear(const void* x, const void* w, const void* a, const void* b, const void* adapters, int adapters_i64, const float* scales, void* out, float* h, int64_t M, int N, int K, int R, int L,
+                    int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int e = lora_check(M, N, K, R, L)) return e;
+  if (M == 0) return 0;
+  if (!x || !w || !a || !b || !out) return set_error("null pointer");
+  if (!aligned16(x) || !aligned16(w) || !aligned16(a) || !aligned16(b) || !aligned16(out) || !aligned16(h)) return set_error("operand pointers must be 16-byte aligned");
+  if (int e = lora_operands(0, adapters, adapters_i64, scales, M, N, K, R, L, dtype, workspace, workspace_bytes)) return e;
+  return launch_lora(x, w, a, b, adapters, adapters_i64 != 0, scales, out, h, M, N, K, R, L, dtype, workspace, (hipStream_t)stream);
+}
+
+int tgg_lora_linear_bwd(const void* grad, const void* x, const void* w, const void* a, const void* b, const void* adapters, int adapters_i64, const float* scales, const float* h, void* dx, void* da,
+                        void* db, int64_t M, int N, int K, int R, int L, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int e = lora_check(M, N, K, R, L)) return e;
+  if (M == 0) return 0;
+  if (!grad || !a || !b || (dx && !w) || (da && !x) || (db && !h)) return set_error("null pointer");
+  if (!aligned16(grad) || !aligned16(x) || !aligned16(w) || !aligned16(a) || !aligned16(b) || !aligned16(h) || !aligned16(dx) || !aligned16(da) || !aligned16(db))
+    return set_error("operand pointers must be 16-byte aligned");
+  if (int e = lora_operands(1, adapters, adapters_i64, scales, M, N, K, R, L, dtype, workspace, workspace_bytes)) return e;
+  return launch_lora_bwd(grad, x, w, a, b, adapters, adapters_i64 != 0, scales, h, dx, da, db, M, N, K, R, L, dtype, workspace, (hipStream_t)stream);
+}
+
 // ---- Newton-Schulz orthogonalisation --------------------------------------------------------------------------
 static int newton_schulz_check(int64_t batch, int64_t rows, int64_t cols) {
   constexpr int64_t most = 1 << 16;

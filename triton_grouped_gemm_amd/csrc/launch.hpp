@@ -44,6 +44,13 @@ int launch_moe_router(const void* logits, int64_t row_bytes, int64_t tokens, int
 int launch_moe_router_bwd(const void* logits, int64_t row_bytes, const float* probs, const int32_t* indices, const float* grad, int64_t tokens,
                           int E, int k, int scoring, int renorm, int dt, void* dlogits, hipStream_t s);
 
+// Low-rank adapters beside a shared projection (lora.hip)
+int64_t lora_workspace(int backward, int64_t M, int N, int K, int R, int L);
+int launch_lora(const void* x, const void* w, const void* a, const void* b, const void* ids, int ids_i64, const float* scales, void* out, float* h, int64_t M, int N, int K, int R, int L, int dt,
+                void* ws, hipStream_t s);
+int launch_lora_bwd(const void* grad, const void* x, const void* w, const void* a, const void* b, const void* ids, int ids_i64, const float* scales, const float* h, void* dx, void* da, void* db,
+                    int64_t M, int N, int K, int R, int L, int dt, void* ws, hipStream_t s);
+
 // Newton-Schulz orthogonalisation (newton_schulz.hip); types 0 = bf16, 1 = fp16, 2 = fp32
 int64_t newton_schulz_workspace(int64_t batch, int rows, int cols);
 int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, int nesterov, void* out, int out_dt, int weight, float keep, float step, int64_t batch, int rows, int cols, int steps,

@@ -1,0 +1,967 @@
+// Low-rank adapters of many requests beside a shared projection:
+//   y[m] = W x[m] + s_l B_l (A_l x[m]),   l = the row's adapter, no second term where it has none
+// with W [N, K], A [L, R, K], B [L, N, R], and the gradients of x, A and B:
+//   h[m] = s_l A_l x[m],   dh[m] = s_l B_l^T g[m],   dx = W^T g + A_l^T dh,   dA_l = sum of dh[m] x[m]^T over l's rows,   dB_l = sum of g[m] h[m]^T
+//
+// Three kinds of kernel:
+//   lora_down   h (or dh, from B transposed): few outputs, long sums.  A workgroup has 16 to 64 rows, its waves share the sum's length; the rows' distinct adapters
+//               are taken in turn (rows of a request follow one another, so that is mostly one), and a row keeps the sums of its own.
+//   lora_gemm   y and dx: the shared product, with R more values of depth for every adapter of a tile's rows: slabs of h, in which the rows of other adapters
+//               read as zeros, against slabs of B_l (A_l).  So the adapters enter the fp32 sums and there is one rounding.  h is fp32 and enters as two
+//               planes of the operands' type, high and low.  Half precision's range would cut them off: there each row is scaled to a power of two of its own, and
+//               the adapters' slabs come first, so that the sums are scaled back before the shared product is added.
+//   lora_outer  dA and dB: sums over an adapter's rows, which are gathered from wherever they stand.
+// and lora_few, which streams W for the few rows of a decode step.
+#include <type_traits>
+
+#include "launch.hpp"
+#include "stream_gemm.hpp"
+
+namespace tgg {
+
+namespace {
+
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+TGG_DEV rsrc_t window(const void* base, int64_t bytes) {
+  bytes = bytes < 0 ? 0 : (bytes > 0x7fffffff ? 0x7fffffff : bytes);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)uniform64((uint64_t)base), 0, __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
+}
+constexpr int kNowhere = 0x7ffffff0;  // beyond every window
+
+struct Ids {
+  const void* p;
+  int i64, L;
+  // the row's adapter, -1 where it has none
+  TGG_DEV int at(int64_t row) const {
+    const int64_t v = i64 ? ((const int64_t*)p)[row] : ((const int32_t*)p)[row];
+    return v >= 0 && v < L ? (int)v : -1;
+  }
+};
+
+template <int DT> TGG_DEV float from_bits(uint16_t h) {
+  if (DT == DT_BF16) return __builtin_bit_cast(float, (uint32_t)h << 16);
+  return (float)__builtin_bit_cast(_Float16, h);
+}
+// two 16-bit values that add up to v but for 2^-17 (bf16) or 2^-22 of it
+template <int DT> TGG_DEV void split2(float v, uint16_t& hi, uint16_t& lo) {
+  hi = Out16<DT>::cvt(v);
+  const float rest = v - from_bits<DT>(hi);
+  lo = Out16<DT>::cvt(__builtin_isfinite(rest) ? rest : 0.f);  // an infinity stays one
+}
+// 2^e with |v| 2^e in [2^10, 2^11); 1 for zeros and what is not finite
+TGG_DEV float row_scale(float v) {
+  if (!(v > 0.f) || !__builtin_isfinite(v)) return 1.f;
+  int e = (int)(__builtin_bit_cast(uint32_t, v) >> 23) - 127;
+  e = 10 - (e < -110 ? -110 : e);
+  return __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+}
+
+constexpr int kDownThreads = 512, kDownWaves = 8;
+
+struct DownParams {
+  const void* x;     // [M, depth]
+  const void* a;     // [L, R, depth]
+  const float* scales;
+  Ids ids;
+  float* h;          // [parts, M, R]: the sums, part by part of the depth
+  uint16_t* planes;  // [M, 2, R], or null
+  float* back;       // fp16 planes: what a row's planes are multiplied with, [M]
+  int32_t *counts, *lists;  // of each tile of `tile` rows, how many adapters it has and which; or null
+  int64_t M;
+  int R, depth, parts, tile, row_blocks;
+};
+
+constexpr int kMixed = 1 << 16;  // of a tile's count: its rows do not all have the one adapter
+
+// the adapters of a tile's rows, each once, in the order of their first rows
+TGG_DEV void tile_list(const DownParams& p, int t, char* smem) {
+  int32_t* const ids = (int32_t*)smem;
+  int32_t* const waves = ids + 256;
+  const int64_t row = (int64_t)t * p.tile + threadIdx.x;
+  const bool mine = threadIdx.x < p.tile && row < p.M;
+  const int id = mine ? p.ids.at(row) : -1;
+  if (threadIdx.x < 256) ids[threadIdx.x] = id;
+  __syncthreads();
+  bool first = id >= 0;
+  for (int i = 0; i < 256; ++i) first = first && !(i < threadIdx.x && ids[i] == id);
+  const uint64_t found = __ballot(first);
+  const int wave = threadIdx.x >> 6;
+  if (lane_id() == 0) waves[wave] = __popcll(found);
+  __syncthreads();
+  int at = 0, all = 0;
+  for (int w = 0; w < kDownWaves; ++w) {
+    if (w < wave) at += waves[w];
+    all += waves[w];
+  }
+  if (first) p.lists[(int64_t)t * p.tile + at + __popcll(found & ((1ull << lane_id()) - 1))] = id;
+  const uint64_t without = __ballot(mine && id < 0);
+  __syncthreads();
+  if (lane_id() == 0) waves[wave] = without != 0;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    bool mixed = all > 1;
+    for (int w = 0; w < kDownWaves; ++w) mixed = mixed || (all && waves[w]);
+    p.counts[t] = all | (mixed ? kMixed : 0);
+  }
+}
+
+// RB: blocks of 16 rows, RC: blocks of 16 of R (RC * 16 >= R).  blockIdx.x: rows, then tiles whose lists are made; y: adapters in turn; z: part of the depth.
+template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) void lora_down_kernel(const DownParams p) {
+  constexpr int COLS = RC * 16;
+  __shared__ __attribute__((aligned(16))) float sums[kDownWaves * 16 * COLS];
+  if ((int)blockIdx.x >= p.row_blocks) {
+    if (blockIdx.y == 0 && blockIdx.z == 0) tile_list(p, blockIdx.x - p.row_blocks, (char*)sums);
+    return;
+  }
+  const int lane = lane_id(), l16 = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row0 = (int64_t)blockIdx.x * (16 * RB);
+  const int rows = (int)min((int64_t)(16 * RB), p.M - row0);
+  const int id = lane < rows ? p.ids.at(row0 + lane) : -1;
+  // lanes whose row is the first of its adapter
+  uint64_t firsts = 0;
+#pragma unroll
+  for (int i = 0; i < 16 * RB; ++i) {
+    const int other = __builtin_amdgcn_readlane(id, i);
+    const uint64_t same = __ballot(id == other);
+    if (other >= 0 && (same & ((1ull << i) - 1)) == 0) firsts |= 1ull << i;
+  }
+  // this part's steps of 64 values
+  const int steps = (p.depth + 63) / 64, first_step = (int)((int64_t)steps * blockIdx.z / p.parts), end_step = (int)((int64_t)steps * (blockIdx.z + 1) / p.parts);
+  const rsrc_t xw = window((const uint16_t*)p.x + row0 * p.depth, (int64_t)rows * p.depth * 2);
+  float* const h = p.h + (int64_t)blockIdx.z * p.M * p.R;
+  if (blockIdx.y == 0) {  // rows without an adapter
+    for (int i = threadIdx.x; i < rows * p.R; i += kDownThreads) {
+      const int r = i / p.R, c = i - r * p.R;
+      if (p.ids.at(row0 + r) < 0) {
+        h[(row0 + r) * p.R + c] = 0.f;
+        if (p.planes) p.planes[((row0 + r) * 2) * p.R + c] = p.planes[((row0 + r) * 2 + 1) * p.R + c] = 0;
+        if (DT == DT_F16 && p.back && c == 0) p.back[row0 + r] = 1.f;
+      }
+    }
+  }
+  uint64_t left = firsts;
+  for (int turn = 0; left; ++turn, left &= left - 1) {
+    if (turn % (int)gridDim.y != (int)blockIdx.y) continue;
+    const int l = __builtin_amdgcn_readlane(id, __ffsll((unsigned long long)left) - 1);
+    const uint64_t keep = __ballot(id == l);
+    const rsrc_t aw = window((const uint16_t*)p.a + (int64_t)l * p.R * p.depth, (int64_t)p.R * p.depth * 2);
+    f32x4_t acc[RB][RC];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int c = 0; c < RC; ++c) acc[b][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    auto load = [&](i32x4_t (&x)[2][RB], i32x4_t (&a)[2][RC], int s) __attribute__((always_inline)) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const int k = s * 64 + ks * 32 + lg * 8;
+        const int at = s < end_step && k < p.depth ? (l16 * p.depth + k) * 2 : kNowhere;
+#pragma unroll
+        for (int b = 0; b < RB; ++b) x[ks][b] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xw, at == kNowhere ? kNowhere : at + b * 16 * p.depth * 2, 0, 0));
+#pragma unroll
+        for (int c = 0; c < RC; ++c) a[ks][c] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(aw, at == kNowhere ? kNowhere : at + c * 16 * p.depth * 2, 0, 0));
+      }
+    };
+    auto multiply = [&](const i32x4_t (&x)[2][RB], const i32x4_t (&a)[2][RC]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+          for (int c = 0; c < RC; ++c) acc[b][c] = stream_mma<DT>(a[ks][c], x[ks][b], acc[b][c]);  // lane: row l16, columns 4 lg + (0..3)
+    };
+    i32x4_t x0[2][RB], a0[2][RC], x1[2][RB], a1[2][RC];
+    load(x0, a0, first_step + wave);
+    for (int s = first_step + wave; s < end_step; s += 2 * kDownWaves) {
+      load(x1, a1, s + kDownWaves);
+      multiply(x0, a0);
+      load(x0, a0, s + 2 * kDownWaves);
+      multiply(x1, a1);
+    }
+    const float scale = p.scales ? p.scales[l] : 1.f;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < RC; ++c) *(f32x4_t*)&sums[(wave * 16 + l16) * COLS + 16 * c + 4 * lg] = acc[b][c];
+      __syncthreads();
+      // 32 threads a row
+      const int r = threadIdx.x >> 5, row = b * 16 + r;
+      constexpr int PER = (COLS + 31) / 32;
+      float v[PER], top = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int c = (threadIdx.x & 31) + 32 * i;
+        v[i] = 0.f;
+        if (c < COLS) {
+#pragma unroll
+          for (int w = 0; w < kDownWaves; ++w) v[i] += sums[(w * 16 + r) * COLS + c];
+          v[i] *= scale;
+        }
+        top = fmaxf(top, fabsf(v[i]));
+      }
+      const bool mine = row < rows && (keep >> row & 1);
+      float up = 1.f;
+      if (DT == DT_F16 && p.planes) {
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+        up = row_scale(top);
+        if (mine && (threadIdx.x & 31) == 0) p.back[row0 + row] = 1.f / up;
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int c = (threadIdx.x & 31) + 32 * i;
+        if (mine && c < p.R) {
+          h[(row0 + row) * p.R + c] = v[i];
+          if (p.planes) {
+            uint16_t hi, lo;
+            split2<DT>(v[i] * up, hi, lo);
+            p.planes[((row0 + row) * 2) * p.R + c] = hi;
+            p.planes[((row0 + row) * 2 + 1) * p.R + c] = lo;
+          }
+        }
+      }
+    }
+  }
+}
+
+// [L, N, R] -> [L, R, N]
+__global__ __launch_bounds__(256) void lora_transpose_kernel(const uint16_t* in, uint16_t* out, int N, int R, int tiles_n, int tiles_r) {
+  __shared__ uint16_t tile[64][66];
+  const int per = tiles_n * tiles_r, l = blockIdx.x / per, t = blockIdx.x % per, n0 = t / tiles_r * 64, r0 = t % tiles_r * 64, x = threadIdx.x & 63;
+  for (int y = threadIdx.x >> 6; y < 64; y += 4)
+    if (n0 + y < N && r0 + x < R) tile[y][x] = in[((int64_t)l * N + n0 + y) * R + r0 + x];
+  __syncthreads();
+  for (int y = threadIdx.x >> 6; y < 64; y += 4)
+    if (r0 + y < R && n0 + x < N) out[((int64_t)l * R + r0 + y) * N + n0 + x] = tile[x][y];
+}
+
+// ---- the shared product with the adapters' depth added ---------------------------------------------------------------------
+
+struct LoraGemm {
+  const void* x;        // [M, depth]
+  const void* w;        // NT [cols, depth], NN [depth, cols]
+  const void* pair;     // NT B [L, cols, R], NN A [L, R, cols]
+  const uint16_t* planes;  // [M, 2, R]
+  const float* back;    // fp16: [M]
+  Ids ids;
+  const int32_t *counts, *lists;
+  void* out;            // [M, cols]
+  int64_t M;
+  int cols, depth, R, tiles_m, tiles_n;
+};
+
+template <class C, int DT, bool NT> struct LoraProblem {
+  typedef Operand<C::BM, true> OpA;
+  typedef Operand<C::BN, NT> OpB;
+  static constexpr bool SCALED = DT == DT_F16, INSPECTS = true;
+  static constexpr int PITCH = C::TN * 32 + 16, STAGE_WAVE = 16 * PITCH;
+  static constexpr int FLAGS_OFF = C::NWAVES * STAGE_WAVE;  // of the epilogue's part: per parity of a tile's position, the tile (+ 1) whose adapters are not all finite
+  static constexpr int SMEM_BYTES = C::EPI_OFF + FLAGS_OFF + 16;
+  static constexpr int CHUNK = 8;  // column tiles that are taken together
+
+  const LoraGemm& p;
+  StreamWalk walk;
+  int a_voff, b_voff, a_tail, b_tail, kt, tail;
+  int lane_row, a_chunk, b_chunk;  // the lane's row within a copy, the chunk of a row that it fetches
+  int ext_slabs;                   // slabs of one adapter: 64 values of R at a time, high and low
+  int pos, issued, slabs_left, a_len, b_len;
+  int ext_left, ext_part, ext_adapter, ext_next, ext_at, ext_mixed;
+  int id_[C::CA];
+  uint64_t a_base, b_base;
+  int row0_, col0_, rows_;
+  bool live;
+
+  TGG_DEV explicit LoraProblem(const LoraGemm& q) : p(q), walk(q.tiles_m * q.tiles_n) {
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    a_voff = OpA::lane_voff(lane, wave % OpA::NPAT, p.depth * 2);
+    b_voff = OpB::lane_voff(lane, wave % OpB::NPAT, (NT ? p.depth : p.cols) * 2);
+    kt = (p.depth + 63) / 64;
+    const int chunks = (p.depth / 8) % 8;
+    tail = chunks != 0;
+    lane_row = lane / 8;
+    a_chunk = OpA::lane_chunk(lane, wave % OpA::NPAT);
+    b_chunk = NT ? OpB::lane_chunk(lane, wave % OpB::NPAT) : 0;
+    a_tail = a_chunk >= chunks ? kNoFetch : a_voff;
+    b_tail = NT && b_chunk >= chunks ? kNoFetch : b_voff;
+    ext_slabs = 2 * ((p.R + 63) / 64);
+    pos = -1;
+    live = false;
+  }
+  TGG_DEV int tile_at(int q) const { return walk.at(q); }
+  // chunks of column tiles, in them row tiles, in them columns: the workgroups of an XCD share rows and columns
+  TGG_DEV void locate(int id, int& tm, int& tn) const {
+    const int full = p.tiles_n / CHUNK * CHUNK, first = CHUNK * p.tiles_m;
+    const int c = id / first, in = id - c * first, width = c * CHUNK < full ? CHUNK : p.tiles_n - full;
+    tm = __builtin_amdgcn_readfirstlane(in / width);
+    tn = __builtin_amdgcn_readfirstlane(c * CHUNK + in % width);
+  }
+  TGG_DEV int ext_of(int tm) const { return (__builtin_amdgcn_readfirstlane(p.counts[tm]) & (kMixed - 1)) * ext_slabs; }
+  TGG_DEV int slabs(int id) const {
+    int tm, tn;
+    locate(id, tm, tn);
+    return kt + ext_of(tm);
+  }
+  TGG_DEV void seek(int id) {
+    ++pos;
+    live = id >= 0;
+    issued = 0;
+    ext_left = 0;
+    ext_part = 0;
+    if (!live) {
+      a_base = b_base = (uint64_t)p.x;
+      a_len = b_len = row0_ = col0_ = rows_ = 0;
+      return;
+    }
+    int tm, tn;
+    locate(id, tm, tn);
+    row0_ = tm * C::BM;
+    col0_ = tn * C::BN;
+    rows_ = __builtin_amdgcn_readfirstlane((int)min((int64_t)C::BM, p.M - row0_));
+    a_base = uniform64((uint64_t)p.x + (int64_t)row0_ * p.depth * 2);
+    a_len = __builtin_amdgcn_readfirstlane(rows_ * p.depth * 2);
+    b_base = uniform64((uint64_t)p.w + (NT ? (int64_t)col0_ * p.depth : (int64_t)col0_) * 2);
+    b_len = __builtin_amdgcn_readfirstlane(NT ? min(C::BN, p.cols - col0_) * p.depth * 2 : 0);
+    const int count = __builtin_amdgcn_readfirstlane(p.counts[tm]);
+    ext_left = (count & (kMixed - 1)) * ext_slabs;
+    ext_mixed = count & kMixed;
+    ext_at = tm * C::BM;
+    if (ext_left) {
+      ext_next = __builtin_amdgcn_readfirstlane(p.lists[ext_at]);
+#pragma unroll
+      for (int k = 0; k < C::CA; ++k) {
+        const int row = ((int)(threadIdx.x >> 6) + k * C::NWAVES) * 8 + lane_row;
+        id_[k] = row < rows_ ? p.ids.at(row0_ + row) : -1;
+      }
+    }
+  }
+  // kind: 0 a slab of the shared product, 1 its last, cut short, 2 + part of an adapter's (and kMixed)
+  TGG_DEV void next(StreamSlab& s) {
+    if (ext_left) {
+      if (ext_part == 0) {
+        ext_adapter = ext_next;
+        ++ext_at;
+        if (ext_left > ext_slabs) ext_next = __builtin_amdgcn_readfirstlane(p.lists[ext_at]);
+      }
+      const int r0 = (ext_part >> 1) * 64;
+      s.ra = make_rsrc32((uint64_t)p.planes + (int64_t)row0_ * p.R * 4, rows_ * p.R * 4);
+      if (NT) {
+        s.rb = make_rsrc32((uint64_t)p.pair + ((int64_t)ext_adapter * p.cols + col0_) * p.R * 2, min(C::BN, p.cols - col0_) * p.R * 2);
+      } else {
+        s.rb = make_rsrc32((uint64_t)p.pair + (((int64_t)ext_adapter * p.R + r0) * p.cols + col0_) * 2, min(64, p.R - r0) * p.cols * 2 - col0_ * 2);
+      }
+      s.kind = (2 + ext_part) | ext_mixed;
+      --ext_left;
+      if (++ext_part == ext_slabs) ext_part = 0;
+      return;
+    }
+    const int left = issued * 128;
+    s.ra = make_rsrc32(a_base + left, live ? a_len - left : 0);
+    if (NT) {
+      s.rb = make_rsrc32(b_base + left, live ? b_len - left : 0);
+    } else {
+      s.rb = make_rsrc32(b_base + (uint64_t)issued * 64 * p.cols * 2, live ? min(64, p.depth - issued * 64) * p.cols * 2 - col0_ * 2 : 0);
+    }
+    s.kind = tail && issued + 1 == kt ? 1 : 0;
+    if (live && ++issued == kt) seek(tile_at(pos + 1));
+  }
+  TGG_DEV int a_offset(const StreamSlab& s, int k) const {
+    const int idx = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + k * C::NWAVES;
+    if (s.kind < 2) return (s.kind ? a_tail : a_voff) + idx * OpA::RPI * p.depth * 2;
+    const int part = (s.kind & (kMixed - 1)) - 2, r = (part >> 1) * 64 + a_chunk * 8;
+    return r < p.R && id_[k] == ext_adapter ? (idx * 8 + lane_row) * p.R * 4 + (part & 1) * p.R * 2 + r * 2 : kNoFetch;
+  }
+  TGG_DEV int b_offset(const StreamSlab& s, int k) const {
+    const int idx = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + k * C::NWAVES;
+    if (s.kind < 2 || !NT) return (s.kind == 1 ? b_tail : b_voff) + idx * OpB::RPI * (NT ? p.depth : p.cols) * 2;
+    const int part = (s.kind & (kMixed - 1)) - 2, r = (part >> 1) * 64 + b_chunk * 8;
+    return r < p.R ? (idx * 8 + lane_row) * p.R * 2 + r * 2 : kNoFetch;
+  }
+
+  // A tile's rows of other adapters are zeros in an adapter's slab, and zero times infinity or NaN is NaN: where the rows do not all have the adapter, what is
+  // not finite is taken out of the slab, and the epilogue adds it to the rows that it belongs to.
+  static constexpr uint32_t EXPONENT = DT == DT_BF16 ? 0x7f80u : 0x7c00u;
+  TGG_DEV void inspect(const StreamSlab& s, char* b, int id, int q, char* stage) const {
+    if (!(s.kind & kMixed)) return;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < C::B_BYTES / (C::THREADS * 16); ++i) {
+      i32x4_t* const at = (i32x4_t*)(b + (i * C::THREADS + threadIdx.x) * 16);
+      i32x4_t v = *at;
+      bool here = false;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t x = (uint32_t)v[w];
+        const bool lo = (x & EXPONENT) == EXPONENT, hi = (x >> 16 & EXPONENT) == EXPONENT;
+        x = (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
+        v[w] = (int)x;
+        here = here || lo || hi;
+      }
+      if (here) *at = v;
+      bad = bad || here;
+    }
+    if (bad) ((int*)(stage + FLAGS_OFF))[q & 1] = id + 1;
+    __syncthreads();
+  }
+
+  // between the adapters' slabs and the shared product's: the planes' scales out of the sums
+  TGG_DEV void after_slab(int id, int done, int all, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at) const {
+    if (!SCALED || done != all - kt || done == 0) return;
+    int tm, tn;
+    locate(id, tm, tn);
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) {
+      const int64_t row = (int64_t)tm * C::BM + at.wm0 + 16 * i + at.l16;
+      const float back = row < p.M ? p.back[row] : 0.f;
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] *= back;
+    }
+  }
+
+  // what inspect() has taken out, for the lane's outputs
+  TGG_DEV void add_infinite(int tm, int tn, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at) const {
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) {
+      const int64_t row = (int64_t)tm * C::BM + at.wm0 + 16 * i + at.l16;
+      const int l = row < p.M ? p.ids.at(row) : -1;
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int col = tn * C::BN + at.wn0 + 16 * j + 4 * at.lg + e;
+          float add = 0.f;
+          if (l >= 0 && col < p.cols) {
+            for (int r = 0; r < p.R; ++r) {
+              const uint16_t b = ((const uint16_t*)p.pair)[NT ? ((int64_t)l * p.cols + col) * p.R + r : ((int64_t)l * p.R + r) * p.cols + col];
+              if ((b & EXPONENT) == EXPONENT) add += from_bits<DT>(b) * (from_bits<DT>(p.planes[row * 2 * p.R + r]) + from_bits<DT>(p.planes[(row * 2 + 1) * p.R + r]));
+            }
+          }
+          acc[i][j][e] += add;
+        }
+    }
+  }
+
+  TGG_DEV void epilogue(int id, int q, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at, char* stage) const {
+    int el = at.lane;
+    asm volatile("" : "+v"(el));
+    const int l16 = el & 15, lg = el >> 4;
+    int tm, tn;
+    locate(id, tm, tn);
+    if (__builtin_expect(((volatile int*)(stage + FLAGS_OFF))[q & 1] == id + 1, 0)) add_infinite(tm, tn, acc, at);
+    char* const mine = stage + at.wave * STAGE_WAVE;
+    const int cbase = tn * C::BN + at.wn0;
+    const int64_t rbase = (int64_t)tm * C::BM + at.wm0;
+    constexpr int CPS = 2 * C::TN, PASSES = 16 * CPS / 64;  // 16-byte pieces of a staged row, wave-wide reads of a strip
+    static_assert(PASSES * 64 == 16 * CPS, "a strip is read back by whole waves");
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) *(uint2*)(mine + l16 * PITCH + (16 * j + 4 * lg) * 2) = pack4<DT>(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+      asm volatile("" : : : "memory");
+#pragma unroll
+      for (int it = 0; it < PASSES; ++it) {
+        const int idx = it * 64 + el, r = idx / CPS, ch = idx % CPS;
+        const i32x4_t v = *(const i32x4_t*)(mine + r * PITCH + ch * 16);
+        const int64_t row = rbase + 16 * i + r;
+        if (row < p.M && cbase + ch * 8 < p.cols) store_c((i32x4_t*)((uint16_t*)p.out + row * p.cols + cbase + ch * 8), v, 1);
+      }
+      asm volatile("" : : : "memory");
+    }
+  }
+};
+
+template <class C, int DT, bool NT> __global__ __launch_bounds__(C::THREADS) void lora_gemm_kernel(const LoraGemm p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  LoraProblem<C, DT, NT> prob(p);
+  if (threadIdx.x < 2) ((int*)(smem + C::EPI_OFF + LoraProblem<C, DT, NT>::FLAGS_OFF))[threadIdx.x] = 0;
+  stream_gemm<C, DT, NT>(prob, smem);
+}
+
+// ---- few rows ---------------------------------------------------------------------------------------------------------------
+
+constexpr int kFewThreads = 512, kFewWaves = 8;
+
+struct FewParams {
+  const void *x, *w, *b;
+  const float* h;  // [parts, M, R]
+  Ids ids;
+  void* out;
+  int64_t M;
+  int N, K, R, parts;
+};
+
+// RB blocks of 16 rows x CB blocks of 16 columns; the waves share the depth.
+template <int DT, int RB, int CB> __global__ __launch_bounds__(kFewThreads) void lora_few_kernel(const FewParams p) {
+  constexpr int ROWS = RB * 16, COLS = CB * 16, QUADS = ROWS * COLS / 4, PER = (QUADS + kFewThreads - 1) / kFewThreads;
+  __shared__ __attribute__((aligned(16))) float sums[kFewWaves * ROWS * COLS];
+  const int lane = lane_id(), l16 = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * COLS;
+  const int64_t row0 = (int64_t)blockIdx.y * ROWS;
+  const int rows = (int)min((int64_t)ROWS, p.M - row0);
+  const rsrc_t xw = window((const uint16_t*)p.x + row0 * p.K, (int64_t)rows * p.K * 2);
+  const rsrc_t ww = window((const uint16_t*)p.w + (int64_t)n0 * p.K, (int64_t)min(COLS, p.N - n0) * p.K * 2);
+  const int steps = (p.K + 63) / 64;
+  auto load = [&](i32x4_t (&x)[2][RB], i32x4_t (&w)[2][CB], int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const int k = s * 64 + ks * 32 + lg * 8;
+      const int at = s < steps && k < p.K ? (l16 * p.K + k) * 2 : kNowhere;
+#pragma unroll
+      for (int c = 0; c < CB; ++c) w[ks][c] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ww, at == kNowhere ? kNowhere : at + c * 16 * p.K * 2, 0, 0));
+#pragma unroll
+      for (int b = 0; b < RB; ++b) x[ks][b] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xw, at == kNowhere ? kNowhere : at + b * 16 * p.K * 2, 0, 0));
+    }
+  };
+  f32x4_t acc[RB][CB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int c = 0; c < CB; ++c) acc[b][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](const i32x4_t (&x)[2][RB], const i32x4_t (&w)[2][CB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int c = 0; c < CB; ++c) acc[b][c] = stream_mma<DT>(w[ks][c], x[ks][b], acc[b][c]);
+  };
+  i32x4_t x0[2][RB], w0[2][CB], x1[2][RB], w1[2][CB];
+  load(x0, w0, wave);
+  load(x1, w1, wave + kFewWaves);
+  // the adapters' part of the thread's outputs, four columns of one row each, while the first weights arrive
+  float own[PER][4];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int q = threadIdx.x + i * kFewThreads, r = q / (COLS / 4), n = n0 + q % (COLS / 4) * 4;
+    own[i][0] = own[i][1] = own[i][2] = own[i][3] = 0.f;
+    if (r < rows && n < p.N) {
+      const int id = p.ids.at(row0 + r);
+      if (id >= 0) {
+        const uint16_t* const b = (const uint16_t*)p.b + ((int64_t)id * p.N + n) * p.R;
+        for (int c = 0; c < p.R; c += 8) {
+          float h[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          for (int part = 0; part < p.parts; ++part) {
+            const float* const hp = p.h + ((int64_t)part * p.M + row0 + r) * p.R + c;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] += hp[e];
+          }
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const i32x4_t v = *(const i32x4_t*)(b + (int64_t)y * p.R + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) own[i][y] = __builtin_fmaf(h[e], from_bits<DT>((uint16_t)((uint32_t)v[e / 2] >> (16 * (e & 1)))), own[i][y]);
+          }
+        }
+      }
+    }
+  }
+  for (int s = wave; s < steps; s += 2 * kFewWaves) {
+    multiply(x0, w0);
+    load(x0, w0, s + 2 * kFewWaves);
+    multiply(x1, w1);
+    load(x1, w1, s + 3 * kFewWaves);
+  }
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int c = 0; c < CB; ++c) *(f32x4_t*)&sums[(wave * ROWS + 16 * b + l16) * COLS + 16 * c + 4 * lg] = acc[b][c];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int q = threadIdx.x + i * kFewThreads, r = q / (COLS / 4), c = q % (COLS / 4) * 4;
+    if (r < rows && n0 + c < p.N) {
+      f32x4_t v = {own[i][0], own[i][1], own[i][2], own[i][3]};
+#pragma unroll
+      for (int w = 0; w < kFewWaves; ++w) {
+        const f32x4_t s = *(const f32x4_t*)&sums[(w * ROWS + r) * COLS + c];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += s[e];
+      }
+      *(uint2*)((uint16_t*)p.out + (row0 + r) * p.N + n0 + c) = pack4<DT>(v[0], v[1], v[2], v[3]);
+    }
+  }
+}
+
+// ---- gradients of the adapters ------------------------------------------------------------------------------------------
+
+constexpr int kOuterThreads = 256, kOuterWaves = 4, kOuterCols = 128, kOuterRows = 64, kOuterWindow = 4096;
+
+struct OuterParams {
+  const void *x, *g;       // [M, K], [M, N]
+  const float *dh, *h;     // [M, R]
+  Ids ids;
+  void *da, *db;           // [L, R, K], [L, N, R]; either may be null
+  float *part_a, *part_b;  // [parts, L, ...] where there are several parts
+  int32_t* rows;           // [parts, L]: rows of each part
+  int64_t M;
+  int K, N, R, L, parts, blocks_a;
+};
+
+// blockIdx.x: 128 columns of K (dA), then of N (dB); y: adapter; z: part of the rows.  RC blocks of 16 of R.
+template <int DT, int RC> __global__ __launch_bounds__(kOuterThreads) void lora_outer_kernel(const OuterParams p) {
+  typedef Operand<kOuterCols, false> OpZ;
+  constexpr int Z_BYTES = OpZ::SLAB_BYTES, PP = RC * 32 + 16, P_BYTES = kOuterRows * PP;  // a plane of the P tile: 64 rows of RC * 16 values
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  char* const zbuf = smem;                   // two tiles of 64 rows x 128 columns
+  char* const pbuf = smem + 2 * Z_BYTES;     // high and low plane
+  uint16_t* const list = (uint16_t*)(pbuf + 2 * P_BYTES);
+  int32_t* const scan = (int32_t*)(list + kOuterWindow);
+  float* const tops = (float*)(scan + kOuterWaves);
+  const int lane = lane_id(), l16 = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool is_a = (int)blockIdx.x < p.blocks_a;
+  const int l = blockIdx.y, cols = is_a ? p.K : p.N, col0 = (is_a ? blockIdx.x : blockIdx.x - p.blocks_a) * kOuterCols;
+  const uint16_t* const z = (const uint16_t*)(is_a ? p.x : p.g);
+  const float* const src = is_a ? p.dh : p.h;
+  const int64_t begin = p.M * blockIdx.z / p.parts, end = p.M * (blockIdx.z + 1) / p.parts;
+  const uint32_t smem_addr = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
+
+  f32x4_t acc[RC][2];
+#pragma unroll
+  for (int c = 0; c < RC; ++c) acc[c][0] = acc[c][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float unit = 0.f;  // fp16: what P is multiplied with, acc's values too (0: nothing so far)
+  int total = 0;
+  // the lane's place in a copy of four rows, and its chunk of the row
+  const int z_row = lane / OpZ::CPR, z_chunk = (lane % OpZ::CPR) ^ OpZ::token_swizzle(wave * OpZ::RPI + z_row);
+  const bool z_there = col0 + z_chunk * 8 < cols;
+
+  for (int64_t w0 = begin; w0 < end; w0 += kOuterWindow) {
+    // the window's rows of this adapter, in order
+    constexpr int PER = kOuterWindow / kOuterThreads;
+    const int n = (int)min((int64_t)kOuterWindow, end - w0);
+    int count = 0;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = threadIdx.x * PER + i;
+      if (r < n && p.ids.at(w0 + r) == l) {
+        mine |= 1u << i;
+        ++count;
+      }
+    }
+    int incl = count;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += o;
+    }
+    __syncthreads();  // the list and the scan of the window before have been read
+    if (lane == 63) scan[wave] = incl;
+    __syncthreads();
+    int at = incl - count, all = 0;
+    for (int w = 0; w < kOuterWaves; ++w) {
+      if (w < wave) at += scan[w];
+      all += scan[w];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (mine >> i & 1) list[at++] = (uint16_t)(threadIdx.x * PER + i);
+    __syncthreads();
+    all = __builtin_amdgcn_readfirstlane(all);
+    if (!all) continue;
+    total += all;
+    const i32x4_t zr = make_rsrc((uint64_t)z + (uint64_t)(w0 * cols + col0) * 2, (n * (int64_t)cols - col0) * 2);
+    auto copy = [&](int c, int buf) {
+#pragma unroll
+      for (int k = 0; k < OpZ::NI / kOuterWaves; ++k) {
+        const int idx = wave + k * kOuterWaves, r = c * kOuterRows + idx * OpZ::RPI + z_row;
+        const int voff = r < all && z_there ? (int)list[r < all ? r : 0] * cols * 2 + z_chunk * 16 : kNoFetch;
+        copy_b128_to_lds(zr, __builtin_amdgcn_readfirstlane(smem_addr + buf * Z_BYTES + idx * 1024), voff);
+      }
+    };
+    const int chunks = (all + kOuterRows - 1) / kOuterRows;
+    copy(0, 0);
+    for (int c = 0; c < chunks; ++c) {
+      // P: 64 rows of R values in fp32, four threads a row
+      constexpr int VALUES = RC * 4;
+      const int pr = threadIdx.x >> 2, pc = (threadIdx.x & 3) * VALUES, r = c * kOuterRows + pr;
+      float v[VALUES], top = 0.f;
+      const float* const row = src + (w0 + list[r < all ? r : 0]) * p.R;
+#pragma unroll
+      for (int i = 0; i < VALUES; ++i) {
+        v[i] = r < all && pc + i < p.R ? row[pc + i] : 0.f;
+        top = fmaxf(top, fabsf(v[i]));
+      }
+      if (DT == DT_F16) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+        if (lane == 0) tops[wave] = top;
+      }
+      wait_vmcnt<0>();
+      __syncthreads();  // this chunk's Z is there, the planes of the chunk before have been read
+      if (DT == DT_F16) {
+        top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        const float want = row_scale(top);
+        if (top > 0.f && (unit == 0.f || want < unit)) {  // larger values than before: the sums move to their scale
+          const float by = unit == 0.f ? 0.f : want / unit;
+#pragma unroll
+          for (int q = 0; q < RC; ++q)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[q][b][e] = unit == 0.f ? acc[q][b][e] : acc[q][b][e] * by;
+          unit = want;
+        }
+      }
+      const float by = DT == DT_F16 && unit != 0.f ? unit : 1.f;
+#pragma unroll
+      for (int i = 0; i < VALUES; i += 4) {
+        uint16_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split2<DT>(v[i + e] * by, hi[e], lo[e]);
+        *(uint2*)(pbuf + pr * PP + (pc + i) * 2) = {(uint32_t)hi[0] | (uint32_t)hi[1] << 16, (uint32_t)hi[2] | (uint32_t)hi[3] << 16};
+        *(uint2*)(pbuf + P_BYTES + pr * PP + (pc + i) * 2) = {(uint32_t)lo[0] | (uint32_t)lo[1] << 16, (uint32_t)lo[2] | (uint32_t)lo[3] << 16};
+      }
+      __syncthreads();
+      if (c + 1 < chunks) copy(c + 1, (c + 1) & 1);
+      const char* const zs = zbuf + (c & 1) * Z_BYTES;
+      const int e4 = l16 >> 2, c4 = l16 & 3;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        i32x4_t zf[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int chunk = ((wave * 32 + 16 * b) / 8 + (c4 >> 1)) ^ OpZ::token_swizzle(8 * (lg & 1) + e4);
+          const char* const q = zs + (ks * 32 + lg * 8 + e4) * OpZ::ROW_BYTES + chunk * 16 + (c4 & 1) * 8;
+          const i16x4_t lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr_t)q);
+          const i16x4_t hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr_t)(q + 4 * OpZ::ROW_BYTES));
+          zf[b] = __builtin_bit_cast(i32x4_t, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+#pragma unroll
+        for (int plane = 0; plane < 2; ++plane)
+#pragma unroll
+          for (int q = 0; q < RC; ++q) {
+            const char* const s = pbuf + plane * P_BYTES + (ks * 32 + lg * 8 + e4) * PP + q * 32 + c4 * 8;
+            const i16x4_t lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr_t)s);
+            const i16x4_t hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr_t)(s + 4 * PP));
+            const i32x4_t pf = __builtin_bit_cast(i32x4_t, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+            for (int b = 0; b < 2; ++b) acc[q][b] = is_a ? stream_mma<DT>(zf[b], pf, acc[q][b]) : stream_mma<DT>(pf, zf[b], acc[q][b]);
+          }
+      }
+    }
+  }
+  if (p.parts > 1 && blockIdx.x == 0 && threadIdx.x == 0) p.rows[blockIdx.z * p.L + l] = total;
+  if (p.parts > 1 && !total) return;
+  const float back = DT == DT_F16 && unit != 0.f ? 1.f / unit : 1.f;
+  // dA: lane has row 16 q + l16 of R, columns 16 b + 4 lg + (0..3); dB: row 16 b + l16 of N, columns 16 q + 4 lg + (0..3) of R
+#pragma unroll
+  for (int q = 0; q < RC; ++q)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int zc = col0 + wave * 32 + 16 * b, r = 16 * q + (is_a ? l16 : 4 * lg), c = zc + (is_a ? 4 * lg : l16);
+      if (r >= p.R || c >= cols) continue;
+      const f32x4_t v = {acc[q][b][0] * back, acc[q][b][1] * back, acc[q][b][2] * back, acc[q][b][3] * back};
+      const int64_t o = is_a ? ((int64_t)l * p.R + r) * p.K + c : ((int64_t)l * p.N + c) * p.R + r;
+      if (p.parts > 1) {
+        float* const part = is_a ? p.part_a + (int64_t)blockIdx.z * p.L * p.R * p.K : p.part_b + (int64_t)blockIdx.z * p.L * p.R * p.N;
+        *(f32x4_t*)(part + o) = v;
+      } else {
+        *(uint2*)((uint16_t*)(is_a ? p.da : p.db) + o) = pack4<DT>(v[0], v[1], v[2], v[3]);
+      }
+    }
+}
+
+// The parts' sums, in order.  Four values a thread; dA's values and then dB's.
+template <int DT> __global__ __launch_bounds__(256) void lora_join_kernel(const OuterParams p) {
+  const int64_t per_a = (int64_t)p.R * p.K, per_b = (int64_t)p.R * p.N, quads_a = p.da ? p.L * per_a / 4 : 0, quads_b = p.db ? p.L * per_b / 4 : 0;
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= quads_a + quads_b) return;
+  const bool is_a = i < quads_a;
+  if (!is_a) i -= quads_a;
+  const int64_t per = is_a ? per_a : per_b, o = i * 4;
+  const int l = (int)(o / per);
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.parts; ++s) {
+    if (!p.rows[s * p.L + l]) continue;
+    const f32x4_t t = *(const f32x4_t*)((is_a ? p.part_a : p.part_b) + s * p.L * per + o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += t[e];
+  }
+  *(uint2*)((uint16_t*)(is_a ? p.da : p.db) + o) = pack4<DT>(v[0], v[1], v[2], v[3]);
+}
+
+// ---- launches ---------------------------------------------------------------------------------------------------------------
+
+int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
+
+template <int DT, int RB> int down_rc(const DownParams& p, dim3 grid, hipStream_t s) {
+  const int rc = (p.R + 15) / 16;
+  if (rc <= 1) lora_down_kernel<DT, RB, 1><<<grid, dim3(kDownThreads), 0, s>>>(p);
+  else if (rc <= 2) lora_down_kernel<DT, RB, 2><<<grid, dim3(kDownThreads), 0, s>>>(p);
+  else if (rc <= 4) lora_down_kernel<DT, RB, 4><<<grid, dim3(kDownThreads), 0, s>>>(p);
+  else lora_down_kernel<DT, RB, 8><<<grid, dim3(kDownThreads), 0, s>>>(p);
+  return check_launch("lora_down");
+}
+
+template <int DT> int launch_down(DownParams p, hipStream_t s) {
+  const bool tall = p.M >= 8192;  // 32 rows a workgroup, else 16
+  const int rows = tall ? 32 : 16;
+  p.row_blocks = (int)((p.M + rows - 1) / rows);
+  const int lists = p.counts ? (int)((p.M + p.tile - 1) / p.tile) : 0;
+  // few rows: their adapters side by side
+  const int turns = p.row_blocks >= 1024 ? 1 : min(16, 1024 / p.row_blocks);
+  const dim3 grid(p.row_blocks + lists, tall ? 1 : turns, p.parts);
+  return tall ? down_rc<DT, 2>(p, grid, s) : down_rc<DT, 1>(p, grid, s);
+}
+
+typedef StreamCfg<256, 256, 2, 4> LoraWide;
+typedef StreamCfg<128, 128, 2, 4> LoraNarrow;
+
+template <class C, int DT, bool NT> int gemm_launch(const LoraGemm& p, hipStream_t s) {
+  typedef LoraProblem<C, DT, NT> P;
+  static bool attr_done = false;
+  if (!attr_done) {
+    if (hipFuncSetAttribute((const void*)lora_gemm_kernel<C, DT, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, P::SMEM_BYTES) != hipSuccess) return check_launch("hipFuncSetAttribute(lora_gemm)");
+    attr_done = true;
+  }
+  const int tiles = p.tiles_m * p.tiles_n, slots = num_cus() * (C::BM == 128 ? 2 : 1);
+  lora_gemm_kernel<C, DT, NT><<<dim3(tiles < slots ? tiles : slots), dim3(C::THREADS), P::SMEM_BYTES, s>>>(p);
+  return check_launch("lora_gemm");
+}
+
+template <int DT, bool NT> int launch_gemm(LoraGemm p, int tile, hipStream_t s) {
+  p.tiles_m = (int)((p.M + tile - 1) / tile);
+  p.tiles_n = (p.cols + tile - 1) / tile;
+  return tile == 256 ? gemm_launch<LoraWide, DT, NT>(p, s) : gemm_launch<LoraNarrow, DT, NT>(p, s);
+}
+
+// Tiles of 256 or of 128 for M x cols outputs: as for newton_schulz.hip's products
+int tile_of(int64_t M, int cols) {
+  auto tiles = [&](int b) { return (M + b - 1) / b * ((cols + b - 1) / b); };
+  const int64_t cus = num_cus();
+  return (tiles(256) + cus - 1) / cus * 3 <= (tiles(128) + 2 * cus - 1) / (2 * cus) * 2 ? 256 : 128;
+}
+
+bool few_rows(int64_t M) { return M <= 64; }
+int few_parts(int64_t M) { return M <= 16 ? 4 : 2; }  // parts of the depth in lora_down: more workgroups for few rows
+
+template <int DT> int launch_few(const FewParams& p, hipStream_t s) {
+  const dim3 threads(kFewThreads);
+  if (p.M <= 16) lora_few_kernel<DT, 1, 1><<<dim3((p.N + 15) / 16, 1), threads, 0, s>>>(p);
+  else if (p.M <= 32) lora_few_kernel<DT, 2, 1><<<dim3((p.N + 15) / 16, 1), threads, 0, s>>>(p);
+  else lora_few_kernel<DT, 4, 1><<<dim3((p.N + 15) / 16, (unsigned)((p.M + 63) / 64)), threads, 0, s>>>(p);
+  return check_launch("lora_few");
+}
+
+template <int DT, int RC> int outer_launch(const OuterParams& p, dim3 grid, hipStream_t s) {
+  constexpr int smem = 2 * kOuterRows * kOuterCols * 2 + 2 * kOuterRows * (RC * 32 + 16) + kOuterWindow * 2 + kOuterWaves * 8;
+  static bool attr_done = false;
+  if (!attr_done) {
+    if (hipFuncSetAttribute((const void*)lora_outer_kernel<DT, RC>, hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess) return check_launch("hipFuncSetAttribute(lora_outer)");
+    attr_done = true;
+  }
+  lora_outer_kernel<DT, RC><<<grid, dim3(kOuterThreads), smem, s>>>(p);
+  return check_launch("lora_outer");
+}
+
+// parts of the rows: enough workgroups for the chip, none of fewer than 1024 rows
+int outer_parts(int64_t M, int N, int K, int L) {
+  const int64_t groups = (int64_t)L * ((N + kOuterCols - 1) / kOuterCols + (K + kOuterCols - 1) / kOuterCols);
+  int64_t parts = (4 * num_cus() + groups - 1) / groups;
+  parts = min(parts, (M + 1023) / 1024);
+  return (int)max((int64_t)1, min(parts, (int64_t)64));
+}
+
+struct LoraPlan {
+  int tile, parts;
+  int64_t h, planes, back, counts, lists, bt, rows, part_a, part_b, bytes;
+};
+LoraPlan lora_plan(bool backward, int64_t M, int N, int K, int R, int L) {
+  LoraPlan q = {};
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) { const int64_t here = at; at += align256(bytes); return here; };
+  q.tile = tile_of(M, backward ? K : N);
+  const int64_t tiles = (M + q.tile - 1) / q.tile;
+  q.h = take((backward ? 1 : 4) * M * R * 4);
+  q.planes = take(M * R * 4);
+  q.back = take(M * 4);
+  q.counts = take(tiles * 4);
+  q.lists = take(tiles * q.tile * 4);
+  if (backward) {
+    q.parts = outer_parts(M, N, K, L);
+    q.bt = take((int64_t)L * N * R * 2);
+    q.rows = take((int64_t)q.parts * L * 4);
+    if (q.parts > 1) {
+      q.part_a = take((int64_t)q.parts * L * R * K * 4);
+      q.part_b = take((int64_t)q.parts * L * R * N * 4);
+    }
+  }
+  q.bytes = at;
+  return q;
+}
+
+template <int DT> int forward(const void* x, const void* w, const void* a, const void* b, const Ids& ids, const float* scales, void* out, float* h, int64_t M, int N, int K, int R, char* ws, hipStream_t s) {
+  const LoraPlan q = lora_plan(false, M, N, K, R, ids.L);
+  const bool few = few_rows(M);
+  DownParams d = {};
+  d.x = x; d.a = a; d.scales = scales; d.ids = ids; d.M = M; d.R = R; d.depth = K;
+  d.parts = few && !h ? few_parts(M) : 1;  // (what is kept for the backward pass is one sum)
+  d.h = h ? h : (float*)(ws + q.h);
+  if (!few) {
+    d.planes = (uint16_t*)(ws + q.planes); d.back = (float*)(ws + q.back);
+    d.counts = (int32_t*)(ws + q.counts); d.lists = (int32_t*)(ws + q.lists); d.tile = q.tile;
+  }
+  if (int e = launch_down<DT>(d, s)) return e;
+  if (few) return launch_few<DT>({x, w, b, d.h, ids, out, M, N, K, R, d.parts}, s);
+  LoraGemm g = {};
+  g.x = x; g.w = w; g.pair = b; g.planes = d.planes; g.back = d.back; g.ids = ids; g.counts = d.counts; g.lists = d.lists; g.out = out;
+  g.M = M; g.cols = N; g.depth = K; g.R = R;
+  return launch_gemm<DT, true>(g, q.tile, s);
+}
+
+template <int DT> int backward(const void* grad, const void* x, const void* w, const void* a, const void* b, const Ids& ids, const float* scales, const float* h, void* dx, void* da, void* db, int64_t M, int N,
+                               int K, int R, char* ws, hipStream_t s) {
+  const LoraPlan q = lora_plan(true, M, N, K, R, ids.L);
+  if (dx || da) {
+    const int tn = (N + 63) / 64, tr = (R + 63) / 64;
+    lora_transpose_kernel<<<dim3((unsigned)(ids.L * tn * tr)), dim3(256), 0, s>>>((const uint16_t*)b, (uint16_t*)(ws + q.bt), N, R, tn, tr);
+    if (int e = check_launch("lora_transpose")) return e;
+    DownParams d = {};
+    d.x = grad; d.a = ws + q.bt; d.scales = scales; d.ids = ids; d.M = M; d.R = R; d.depth = N; d.parts = 1;
+    d.h = (float*)(ws + q.h);
+    if (dx) {
+      d.planes = (uint16_t*)(ws + q.planes); d.back = (float*)(ws + q.back);
+      d.counts = (int32_t*)(ws + q.counts); d.lists = (int32_t*)(ws + q.lists); d.tile = q.tile;
+    }
+    if (int e = launch_down<DT>(d, s)) return e;
+    if (dx) {
+      LoraGemm g = {};
+      g.x = grad; g.w = w; g.pair = a; g.planes = d.planes; g.back = d.back; g.ids = ids; g.counts = d.counts; g.lists = d.lists; g.out = dx;
+      g.M = M; g.cols = K; g.depth = N; g.R = R;
+      if (int e = launch_gemm<DT, false>(g, q.tile, s)) return e;
+    }
+  }
+  if (!da && !db) return 0;
+  OuterParams o = {};
+  o.x = x; o.g = grad; o.dh = (const float*)(ws + q.h); o.h = h; o.ids = ids; o.da = da; o.db = db;
+  o.part_a = (float*)(ws + q.part_a); o.part_b = (float*)(ws + q.part_b); o.rows = (int32_t*)(ws + q.rows);
+  o.M = M; o.K = K; o.N = N; o.R = R; o.L = ids.L; o.parts = q.parts;
+  o.blocks_a = da ? (K + kOuterCols - 1) / kOuterCols : 0;
+  const dim3 grid(o.blocks_a + (db ? (N + kOuterCols - 1) / kOuterCols : 0), ids.L, q.parts);
+  const int rc = (R + 15) / 16;
+  if (int e = rc <= 1 ? outer_launch<DT, 1>(o, grid, s) : rc <= 2 ? outer_launch<DT, 2>(o, grid, s) : rc <= 4 ? outer_launch<DT, 4>(o, grid, s) : outer_launch<DT, 8>(o, grid, s)) return e;
+  if (q.parts == 1) return 0;
+  const int64_t quads = ((da ? (int64_t)ids.L * R * K : 0) + (db ? (int64_t)ids.L * R * N : 0)) / 4;
+  lora_join_kernel<DT><<<dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s>>>(o);
+  return check_launch("lora_join");
+}
+
+}  // namespace
+
+int64_t lora_workspace(int backward, int64_t M, int N, int K, int R, int L) { return lora_plan(backward != 0, M, N, K, R, L).bytes; }
+
+int launch_lora(const void* x, const void* w, const void* a, const void* b, const void* ids, int ids_i64, const float* scales, void* out, float* h, int64_t M, int N, int K, int R, int L, int dt,
+                void* ws, hipStream_t s) {
+  const Ids i = {ids, ids_i64, L};
+  return dt == DT_BF16 ? forward<DT_BF16>(x, w, a, b, i, scales, out, h, M, N, K, R, (char*)ws, s) : forward<DT_F16>(x, w, a, b, i, scales, out, h, M, N, K, R, (char*)ws, s);
+}
+
+int launch_lora_bwd(const void* grad, const void* x, const void* w, const void* a, const void* b, const void* ids, int ids_i64, const float* scales, const float* h, void* dx, void* da, void* db,
+                    int64_t M, int N, int K, int R, int L, int dt, void* ws, hipStream_t s) {
+  const Ids i = {ids, ids_i64, L};
+  return dt == DT_BF16 ? backward<DT_BF16>(grad, x, w, a, b, i, scales, h, dx, da, db, M, N, K, R, (char*)ws, s)
+                       : backward<DT_F16>(grad, x, w, a, b, i, scales, h, dx, da, db, M, N, K, R, (char*)ws, s);
+}
+
+}  // namespace tgg

@@ -61,7 +61,7 @@ TGG_DEV float ns_sum(const float* p, int n) {
 }
 
 template <class C, int MODE, bool PRECISE> struct NsProblem {
-  static constexpr bool B_KMAJOR = MODE != NS_UPDATE, SYM = MODE != NS_UPDATE;
+  static constexpr bool B_KMAJOR = MODE != NS_UPDATE, SYM = MODE != NS_UPDATE, SCALED = false, INSPECTS = false;
   typedef Operand<C::BM, true> OpA;
   typedef Operand<C::BN, B_KMAJOR> OpB;
   static_assert(!SYM || C::BM == C::BN, "symmetric results have square tiles");
@@ -166,7 +166,7 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
     return (s.kind ? b_tail : b_voff) + idx * OpB::RPI * p.ldb * 2;
   }
 
-  TGG_DEV void epilogue(int id, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at, char* stage) const {
+  TGG_DEV void epilogue(int id, int, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at, char* stage) const {
     int el = at.lane;
     asm volatile("" : "+v"(el));  // (addresses are made afresh per tile instead of living across the multiplies)
     const int l16 = el & 15, lg = el >> 4;

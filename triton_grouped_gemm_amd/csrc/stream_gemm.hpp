@@ -10,7 +10,9 @@
 //   void seek(int id)                     the next slab is the tile's first one; id -1: no more slabs
 //   void next(StreamSlab& s)              descriptors of the next slab; past a tile's last one it seeks the following tile by itself
 //   int a_offset(s, k), b_offset(s, k)    source offset of the lane's part of the wave's k-th copy of the slab's A or B operand, or kNoFetch
-//   void epilogue(id, acc, stage)         the tile's sums: acc[i][j][e] is row wm0 + 16 i + l16, column wn0 + 16 j + 4 lg + e
+//   void after_slab(id, n, slabs, acc, at)  where P::SCALED: the tile's sums after its first n slabs
+//   void inspect(s, b, id, pos, stage)    where P::INSPECTS: a slab of the pos-th tile id has landed, its B operand at b; ends with a barrier if it changes anything
+//   void epilogue(id, pos, acc, at, stage)  the tile's sums: acc[i][j][e] is row wm0 + 16 i + l16, column wn0 + 16 j + 4 lg + e
 //
 // A [rows, K] is K-contiguous; B is K-contiguous rows [columns, K] (B_KMAJOR) or token rows [K, columns].
 #pragma once
@@ -130,6 +132,7 @@ template <class C, int DT, bool B_KMAJOR, class P> TGG_DEV void stream_gemm(P& p
   for (int k = 0; k < C::NC; ++k) copy_k(k);
   wait_vmcnt<0>();
   __syncthreads();
+  if constexpr (P::INSPECTS) prob.inspect(sc, smem + C::A_BYTES, prob.tile_at(0), 0, smem + C::EPI_OFF);
   stream_next(prob, sc);
   sc_base = smem_addr + C::STAGE_BYTES;
 #pragma unroll
@@ -193,18 +196,23 @@ template <class C, int DT, bool B_KMAJOR, class P> TGG_DEV void stream_gemm(P& p
     };
     for (int kt = 0; kt < slabs; ++kt) {
       const char* s = smem + (ring & 1) * C::STAGE_BYTES;
-      const char* sn = smem + ((ring + 1) & 1) * C::STAGE_BYTES;
+      char* const sn = smem + ((ring + 1) & 1) * C::STAGE_BYTES;
       half(0, 0, s, 1, READ_EARLY, C::NC / 2);
       half(0, 1, s, 1, READ_ROLL, -1, true);
       half(1, 0, sn, 0, READ_NONE, -1);
       wait_vmcnt<0>();
       __syncthreads();
+      if constexpr (P::INSPECTS) {
+        const bool same = kt + 1 < slabs;
+        prob.inspect(sc, sn + C::A_BYTES, same ? id : prob.tile_at(pos + 1), same ? pos : pos + 1, smem + C::EPI_OFF);
+      }
       sc = sc_next;
       sc_base = sc_next_base;
       half(1, 1, sn, 0, READ_CATCH_UP, 0);
       ++ring;
+      if constexpr (P::SCALED) prob.after_slab(id, kt + 1, slabs, acc, at);
     }
-    prob.epilogue(id, acc, at, smem + C::EPI_OFF);
+    prob.epilogue(id, pos, acc, at, smem + C::EPI_OFF);
   }
   wait_vmcnt<0>();  // the trailing copies, which fetch nothing, still write LDS
 }

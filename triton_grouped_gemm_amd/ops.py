@@ -20,6 +20,7 @@ from ._native import require_gpu
 from .gemm.BF16.k_grouped_gemm import k_grouped_gemm
 from .gemm.BF16.m_grouped_gemm import m_grouped_gemm
 from .gemm.gated import gated_backward, m_grouped_gated_gemm, m_grouped_gated_gemm_projections
+from .lora import lora_linear  # noqa: F401
 from .newton_schulz import muon_update, orthogonalize  # noqa: F401
 
 
