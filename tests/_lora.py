@@ -1,12 +1,12 @@
 """The adapter operators' oracle: the formulas in 64 bits, and the bounds of the kernels' errors.
 
 A sum of n products in fp32 is off by at most (n + 16) 2^-24 of the sum of their magnitudes.  The hidden values h and dh are such sums; they enter the second
-product in two planes that leave out at most 2^-16 of a value (bf16; fp16 2^-21, and 2^-34 of the largest value that they share a scale with).  With |.| taken of every
-entry, e_h = c_K s |x||A|^T and e_dh = c_N s |g||B|, the results are off by at most
+product in two planes: of bfloat16 in out and dx (whatever the operands' type), which leave out at most 2^-8 of 2^-8 of a value, 2^-16; of the operands' type in dA and
+dB, in fp16 2^-21 and 2^-34 of the largest value that they share a scale with.  With |.| taken of every entry, e_h = c_K s |x||A|^T and e_dh = c_N s |g||B|, the results are off by at most
 
-    out  c_K |x||W|^T + (2^-16 + c_R) |h||B|^T + e_h |B|^T
-    dx   c_N |g||W|   + (2^-16 + c_R) |dh||A|  + e_dh |A|
-    dA   ((2^-16 + c_M) |dh| + e_dh)^T |x|          dB   |g|^T ((2^-16 + c_M) |h| + e_h)
+    out  c_K |x||W|^T + (2^-16 + c_4R) |h||B|^T + e_h |B|^T
+    dx   c_N |g||W|   + (2^-16 + c_4R) |dh||A|  + e_dh |A|
+    dA   ((2^-16 + c_M) |dh| + e_dh)^T |x|          dB   |g|^T ((2^-16 + c_M) |h| + e_h)      (fp16: 2^-21)
 
 before their one rounding, which adds half a step.
 """
@@ -64,9 +64,9 @@ def reference(x, w, a, b, g, adapters, s, dtype):
         h[at], e_hid[at] = hl, e_h + 2.0 ** -23 * hl.abs()
         shared = lambda v: 0.0 if dtype == torch.bfloat16 else 2.0 ** -34 * v.abs().max()
         out[at] += hl @ b[l].t()
-        e_out[at] += ((plane + c(2 * r)) * hl.abs() + shared(hl) + e_h) @ b[l].abs().t()
+        e_out[at] += ((2.0 ** -16 + c(4 * r)) * hl.abs() + e_h) @ b[l].abs().t()
         dx[at] += dhl @ a[l]
-        e_dx[at] += ((plane + c(2 * r)) * dhl.abs() + shared(dhl) + e_dh) @ a[l].abs()
+        e_dx[at] += ((2.0 ** -16 + c(4 * r)) * dhl.abs() + e_dh) @ a[l].abs()
         rows = 2 * len(at)
         da[l], e_da[l] = dhl.t() @ xl, ((plane + c(rows)) * dhl.abs() + shared(dhl) + e_dh).t() @ xl.abs()
         db[l], e_db[l] = gl.t() @ hl, gl.abs().t() @ ((plane + c(rows)) * hl.abs() + shared(hl) + e_h)

@@ -6,10 +6,10 @@
 // Three kinds of kernel:
 //   lora_down   h (or dh, from B transposed): few outputs, long sums.  A workgroup has 16 to 64 rows, its waves share the sum's length; the rows' distinct adapters
 //               are taken in turn (rows of a request follow one another, so that is mostly one), and a row keeps the sums of its own.
-//   lora_gemm   y and dx: the shared product, with R more values of depth for every adapter of a tile's rows: slabs of h, in which the rows of other adapters
-//               read as zeros, against slabs of B_l (A_l).  So the adapters enter the fp32 sums and there is one rounding.  h is fp32 and enters as two
-//               planes of the operands' type, high and low.  Half precision's range would cut them off: there each row is scaled to a power of two of its own, and
-//               the adapters' slabs come first, so that the sums are scaled back before the shared product is added.
+//   lora_gemm   y and dx: the shared product, whose sums begin with the adapters' part: for every adapter of a wave's rows, R more values of depth, h (the rows
+//               of other adapters as zeros) against B_l (A_l transposed), from memory to registers.  So the adapters enter the fp32 sums and there is one rounding.
+//               h is fp32 and enters as two planes of bfloat16, high and low, 16 bits with fp32's range; against them half-precision adapters are split into two bfloat16
+//               values without loss.
 //   lora_outer  dA and dB: sums over an adapter's rows, which are gathered from wherever they stand.
 // and lora_few, which streams W for the few rows of a decode step.
 #include <type_traits>
@@ -42,7 +42,7 @@ template <int DT> TGG_DEV float from_bits(uint16_t h) {
   if (DT == DT_BF16) return __builtin_bit_cast(float, (uint32_t)h << 16);
   return (float)__builtin_bit_cast(_Float16, h);
 }
-// two 16-bit values that add up to v but for 2^-17 (bf16) or 2^-22 of it
+// two 16-bit values that add up to v but for 2^-17 (bf16) or 2^-22 of it (and what half precision's range cuts off)
 template <int DT> TGG_DEV void split2(float v, uint16_t& hi, uint16_t& lo) {
   hi = Out16<DT>::cvt(v);
   const float rest = v - from_bits<DT>(hi);
@@ -64,55 +64,15 @@ struct DownParams {
   const float* scales;
   Ids ids;
   float* h;          // [parts, M, R]: the sums, part by part of the depth
-  uint16_t* planes;  // [M, 2, R], or null
-  float* back;       // fp16 planes: what a row's planes are multiplied with, [M]
-  int32_t *counts, *lists;  // of each tile of `tile` rows, how many adapters it has and which; or null
+  uint16_t* planes;  // [M, 2, R] bfloat16, or null
   int64_t M;
-  int R, depth, parts, tile, row_blocks;
+  int R, depth, parts;
 };
 
-constexpr int kMixed = 1 << 16;  // of a tile's count: its rows do not all have the one adapter
-
-// the adapters of a tile's rows, each once, in the order of their first rows
-TGG_DEV void tile_list(const DownParams& p, int t, char* smem) {
-  int32_t* const ids = (int32_t*)smem;
-  int32_t* const waves = ids + 256;
-  const int64_t row = (int64_t)t * p.tile + threadIdx.x;
-  const bool mine = threadIdx.x < p.tile && row < p.M;
-  const int id = mine ? p.ids.at(row) : -1;
-  if (threadIdx.x < 256) ids[threadIdx.x] = id;
-  __syncthreads();
-  bool first = id >= 0;
-  for (int i = 0; i < 256; ++i) first = first && !(i < threadIdx.x && ids[i] == id);
-  const uint64_t found = __ballot(first);
-  const int wave = threadIdx.x >> 6;
-  if (lane_id() == 0) waves[wave] = __popcll(found);
-  __syncthreads();
-  int at = 0, all = 0;
-  for (int w = 0; w < kDownWaves; ++w) {
-    if (w < wave) at += waves[w];
-    all += waves[w];
-  }
-  if (first) p.lists[(int64_t)t * p.tile + at + __popcll(found & ((1ull << lane_id()) - 1))] = id;
-  const uint64_t without = __ballot(mine && id < 0);
-  __syncthreads();
-  if (lane_id() == 0) waves[wave] = without != 0;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    bool mixed = all > 1;
-    for (int w = 0; w < kDownWaves; ++w) mixed = mixed || (all && waves[w]);
-    p.counts[t] = all | (mixed ? kMixed : 0);
-  }
-}
-
-// RB: blocks of 16 rows, RC: blocks of 16 of R (RC * 16 >= R).  blockIdx.x: rows, then tiles whose lists are made; y: adapters in turn; z: part of the depth.
+// RB: blocks of 16 rows, RC: blocks of 16 of R (RC * 16 >= R).  blockIdx.x: rows; y: adapters in turn; z: part of the depth.
 template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) void lora_down_kernel(const DownParams p) {
   constexpr int COLS = RC * 16;
   __shared__ __attribute__((aligned(16))) float sums[kDownWaves * 16 * COLS];
-  if ((int)blockIdx.x >= p.row_blocks) {
-    if (blockIdx.y == 0 && blockIdx.z == 0) tile_list(p, blockIdx.x - p.row_blocks, (char*)sums);
-    return;
-  }
   const int lane = lane_id(), l16 = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row0 = (int64_t)blockIdx.x * (16 * RB);
   const int rows = (int)min((int64_t)(16 * RB), p.M - row0);
@@ -135,7 +95,6 @@ template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) voi
       if (p.ids.at(row0 + r) < 0) {
         h[(row0 + r) * p.R + c] = 0.f;
         if (p.planes) p.planes[((row0 + r) * 2) * p.R + c] = p.planes[((row0 + r) * 2 + 1) * p.R + c] = 0;
-        if (DT == DT_F16 && p.back && c == 0) p.back[row0 + r] = 1.f;
       }
     }
   }
@@ -187,7 +146,7 @@ template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) voi
       // 32 threads a row
       const int r = threadIdx.x >> 5, row = b * 16 + r;
       constexpr int PER = (COLS + 31) / 32;
-      float v[PER], top = 0.f;
+      float v[PER];
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int c = (threadIdx.x & 31) + 32 * i;
@@ -197,16 +156,8 @@ template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) voi
           for (int w = 0; w < kDownWaves; ++w) v[i] += sums[(w * 16 + r) * COLS + c];
           v[i] *= scale;
         }
-        top = fmaxf(top, fabsf(v[i]));
       }
       const bool mine = row < rows && (keep >> row & 1);
-      float up = 1.f;
-      if (DT == DT_F16 && p.planes) {
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-        up = row_scale(top);
-        if (mine && (threadIdx.x & 31) == 0) p.back[row0 + row] = 1.f / up;
-      }
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int c = (threadIdx.x & 31) + 32 * i;
@@ -214,7 +165,7 @@ template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) voi
           h[(row0 + row) * p.R + c] = v[i];
           if (p.planes) {
             uint16_t hi, lo;
-            split2<DT>(v[i] * up, hi, lo);
+            split2<DT_BF16>(v[i], hi, lo);
             p.planes[((row0 + row) * 2) * p.R + c] = hi;
             p.planes[((row0 + row) * 2 + 1) * p.R + c] = lo;
           }
@@ -224,10 +175,19 @@ template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) voi
   }
 }
 
-// [L, N, R] -> [L, R, N]
-__global__ __launch_bounds__(256) void lora_transpose_kernel(const uint16_t* in, uint16_t* out, int N, int R, int tiles_n, int tiles_r) {
+// Two stacks of L matrices, transposed: [L, rows, cols] -> [L, cols, rows]
+struct TransposeParams {
+  struct { const uint16_t* in; uint16_t* out; int rows, cols, tiles_r, tiles_c; } s[2];
+  int first;  // workgroups of the first stack
+};
+__global__ __launch_bounds__(256) void lora_transpose_kernel(const TransposeParams p) {
   __shared__ uint16_t tile[64][66];
-  const int per = tiles_n * tiles_r, l = blockIdx.x / per, t = blockIdx.x % per, n0 = t / tiles_r * 64, r0 = t % tiles_r * 64, x = threadIdx.x & 63;
+  const int second = (int)blockIdx.x >= p.first, id = second ? blockIdx.x - p.first : blockIdx.x;
+  const auto& q = p.s[second];
+  const uint16_t* const in = q.in;
+  uint16_t* const out = q.out;
+  const int N = q.rows, R = q.cols;
+  const int per = q.tiles_r * q.tiles_c, l = id / per, t = id % per, n0 = t / q.tiles_c * 64, r0 = t % q.tiles_c * 64, x = threadIdx.x & 63;
   for (int y = threadIdx.x >> 6; y < 64; y += 4)
     if (n0 + y < N && r0 + x < R) tile[y][x] = in[((int64_t)l * N + n0 + y) * R + r0 + x];
   __syncthreads();
@@ -240,218 +200,148 @@ __global__ __launch_bounds__(256) void lora_transpose_kernel(const uint16_t* in,
 struct LoraGemm {
   const void* x;        // [M, depth]
   const void* w;        // NT [cols, depth], NN [depth, cols]
-  const void* pair;     // NT B [L, cols, R], NN A [L, R, cols]
-  const uint16_t* planes;  // [M, 2, R]
-  const float* back;    // fp16: [M]
+  const uint16_t* pair;    // [L, cols, R]: B, or A transposed
+  const uint16_t* planes;  // [M, 2, R] bfloat16
   Ids ids;
-  const int32_t *counts, *lists;
   void* out;            // [M, cols]
   int64_t M;
   int cols, depth, R, tiles_m, tiles_n;
 };
 
 template <class C, int DT, bool NT> struct LoraProblem {
-  typedef Operand<C::BM, true> OpA;
-  typedef Operand<C::BN, NT> OpB;
-  static constexpr bool SCALED = DT == DT_F16, INSPECTS = true;
   static constexpr int PITCH = C::TN * 32 + 16, STAGE_WAVE = 16 * PITCH;
-  static constexpr int FLAGS_OFF = C::NWAVES * STAGE_WAVE;  // of the epilogue's part: per parity of a tile's position, the tile (+ 1) whose adapters are not all finite
-  static constexpr int SMEM_BYTES = C::EPI_OFF + FLAGS_OFF + 16;
+  static constexpr int SMEM_BYTES = C::EPI_OFF + C::NWAVES * STAGE_WAVE;
   static constexpr int CHUNK = 8;  // column tiles that are taken together
+  static constexpr uint32_t EXPONENT = DT == DT_BF16 ? 0x7f80u : 0x7c00u;
 
   const LoraGemm& p;
   StreamWalk walk;
-  int a_voff, b_voff, a_tail, b_tail, kt, tail;
-  int lane_row, a_chunk, b_chunk;  // the lane's row within a copy, the chunk of a row that it fetches
-  int ext_slabs;                   // slabs of one adapter: 64 values of R at a time, high and low
-  int pos, issued, slabs_left, a_len, b_len;
-  int ext_left, ext_part, ext_adapter, ext_next, ext_at, ext_mixed;
-  int id_[C::CA];
-  uint64_t a_base, b_base;
-  int row0_, col0_, rows_;
-  bool live;
+  StreamCursor<C, NT> cur;
+  int pos;
+  bool infinite;  // begin() has left something out
 
-  TGG_DEV explicit LoraProblem(const LoraGemm& q) : p(q), walk(q.tiles_m * q.tiles_n) {
-    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    a_voff = OpA::lane_voff(lane, wave % OpA::NPAT, p.depth * 2);
-    b_voff = OpB::lane_voff(lane, wave % OpB::NPAT, (NT ? p.depth : p.cols) * 2);
-    kt = (p.depth + 63) / 64;
-    const int chunks = (p.depth / 8) % 8;
-    tail = chunks != 0;
-    lane_row = lane / 8;
-    a_chunk = OpA::lane_chunk(lane, wave % OpA::NPAT);
-    b_chunk = NT ? OpB::lane_chunk(lane, wave % OpB::NPAT) : 0;
-    a_tail = a_chunk >= chunks ? kNoFetch : a_voff;
-    b_tail = NT && b_chunk >= chunks ? kNoFetch : b_voff;
-    ext_slabs = 2 * ((p.R + 63) / 64);
-    pos = -1;
-    live = false;
-  }
+  TGG_DEV explicit LoraProblem(const LoraGemm& q) : p(q), walk(q.tiles_m * q.tiles_n), cur(q.depth * 2, (NT ? q.depth : q.cols) * 2, q.depth) { pos = -1; }
   TGG_DEV int tile_at(int q) const { return walk.at(q); }
+  TGG_DEV int slabs(int) const { return cur.kt; }
   // chunks of column tiles, in them row tiles, in them columns: the workgroups of an XCD share rows and columns
-  TGG_DEV void locate(int id, int& tm, int& tn) const {
+  struct Place { int tm, tn; };
+  TGG_DEV Place locate(int id) const {
     const int full = p.tiles_n / CHUNK * CHUNK, first = CHUNK * p.tiles_m;
     const int c = id / first, in = id - c * first, width = c * CHUNK < full ? CHUNK : p.tiles_n - full;
-    tm = __builtin_amdgcn_readfirstlane(in / width);
-    tn = __builtin_amdgcn_readfirstlane(c * CHUNK + in % width);
-  }
-  TGG_DEV int ext_of(int tm) const { return (__builtin_amdgcn_readfirstlane(p.counts[tm]) & (kMixed - 1)) * ext_slabs; }
-  TGG_DEV int slabs(int id) const {
-    int tm, tn;
-    locate(id, tm, tn);
-    return kt + ext_of(tm);
+    const int tm = in / width;
+    return {__builtin_amdgcn_readfirstlane(tm), __builtin_amdgcn_readfirstlane(c * CHUNK + in - tm * width)};
   }
   TGG_DEV void seek(int id) {
     ++pos;
-    live = id >= 0;
-    issued = 0;
-    ext_left = 0;
-    ext_part = 0;
-    if (!live) {
-      a_base = b_base = (uint64_t)p.x;
-      a_len = b_len = row0_ = col0_ = rows_ = 0;
-      return;
-    }
-    int tm, tn;
-    locate(id, tm, tn);
-    row0_ = tm * C::BM;
-    col0_ = tn * C::BN;
-    rows_ = __builtin_amdgcn_readfirstlane((int)min((int64_t)C::BM, p.M - row0_));
-    a_base = uniform64((uint64_t)p.x + (int64_t)row0_ * p.depth * 2);
-    a_len = __builtin_amdgcn_readfirstlane(rows_ * p.depth * 2);
-    b_base = uniform64((uint64_t)p.w + (NT ? (int64_t)col0_ * p.depth : (int64_t)col0_) * 2);
-    b_len = __builtin_amdgcn_readfirstlane(NT ? min(C::BN, p.cols - col0_) * p.depth * 2 : 0);
-    const int count = __builtin_amdgcn_readfirstlane(p.counts[tm]);
-    ext_left = (count & (kMixed - 1)) * ext_slabs;
-    ext_mixed = count & kMixed;
-    ext_at = tm * C::BM;
-    if (ext_left) {
-      ext_next = __builtin_amdgcn_readfirstlane(p.lists[ext_at]);
-#pragma unroll
-      for (int k = 0; k < C::CA; ++k) {
-        const int row = ((int)(threadIdx.x >> 6) + k * C::NWAVES) * 8 + lane_row;
-        id_[k] = row < rows_ ? p.ids.at(row0_ + row) : -1;
-      }
-    }
+    const bool live = id >= 0;
+    const Place at = locate(live ? id : 0);
+    const int64_t row0 = (int64_t)at.tm * C::BM, col0 = (int64_t)at.tn * C::BN;
+    cur.begin(live, (uint64_t)p.x + row0 * p.depth * 2, (uint64_t)p.w + (NT ? col0 * p.depth : col0) * 2, (int)min((int64_t)C::BM, p.M - row0), NT ? min(C::BN, p.cols - (int)col0) : p.depth, (int)col0 * 2);
   }
-  // kind: 0 a slab of the shared product, 1 its last, cut short, 2 + part of an adapter's (and kMixed)
-  TGG_DEV void next(StreamSlab& s) {
-    if (ext_left) {
-      if (ext_part == 0) {
-        ext_adapter = ext_next;
-        ++ext_at;
-        if (ext_left > ext_slabs) ext_next = __builtin_amdgcn_readfirstlane(p.lists[ext_at]);
-      }
-      const int r0 = (ext_part >> 1) * 64;
-      s.ra = make_rsrc32((uint64_t)p.planes + (int64_t)row0_ * p.R * 4, rows_ * p.R * 4);
-      if (NT) {
-        s.rb = make_rsrc32((uint64_t)p.pair + ((int64_t)ext_adapter * p.cols + col0_) * p.R * 2, min(C::BN, p.cols - col0_) * p.R * 2);
-      } else {
-        s.rb = make_rsrc32((uint64_t)p.pair + (((int64_t)ext_adapter * p.R + r0) * p.cols + col0_) * 2, min(64, p.R - r0) * p.cols * 2 - col0_ * 2);
-      }
-      s.kind = (2 + ext_part) | ext_mixed;
-      --ext_left;
-      if (++ext_part == ext_slabs) ext_part = 0;
-      return;
-    }
-    const int left = issued * 128;
-    s.ra = make_rsrc32(a_base + left, live ? a_len - left : 0);
-    if (NT) {
-      s.rb = make_rsrc32(b_base + left, live ? b_len - left : 0);
-    } else {
-      s.rb = make_rsrc32(b_base + (uint64_t)issued * 64 * p.cols * 2, live ? min(64, p.depth - issued * 64) * p.cols * 2 - col0_ * 2 : 0);
-    }
-    s.kind = tail && issued + 1 == kt ? 1 : 0;
-    if (live && ++issued == kt) seek(tile_at(pos + 1));
-  }
-  TGG_DEV int a_offset(const StreamSlab& s, int k) const {
-    const int idx = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + k * C::NWAVES;
-    if (s.kind < 2) return (s.kind ? a_tail : a_voff) + idx * OpA::RPI * p.depth * 2;
-    const int part = (s.kind & (kMixed - 1)) - 2, r = (part >> 1) * 64 + a_chunk * 8;
-    return r < p.R && id_[k] == ext_adapter ? (idx * 8 + lane_row) * p.R * 4 + (part & 1) * p.R * 2 + r * 2 : kNoFetch;
-  }
-  TGG_DEV int b_offset(const StreamSlab& s, int k) const {
-    const int idx = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + k * C::NWAVES;
-    if (s.kind < 2 || !NT) return (s.kind == 1 ? b_tail : b_voff) + idx * OpB::RPI * (NT ? p.depth : p.cols) * 2;
-    const int part = (s.kind & (kMixed - 1)) - 2, r = (part >> 1) * 64 + b_chunk * 8;
-    return r < p.R ? (idx * 8 + lane_row) * p.R * 2 + r * 2 : kNoFetch;
-  }
+  TGG_DEV void turn() { seek(tile_at(pos + 1)); }
 
-  // A tile's rows of other adapters are zeros in an adapter's slab, and zero times infinity or NaN is NaN: where the rows do not all have the adapter, what is
-  // not finite is taken out of the slab, and the epilogue adds it to the rows that it belongs to.
-  static constexpr uint32_t EXPONENT = DT == DT_BF16 ? 0x7f80u : 0x7c00u;
-  TGG_DEV void inspect(const StreamSlab& s, char* b, int id, int q, char* stage) const {
-    if (!(s.kind & kMixed)) return;
-    bool bad = false;
+  // The adapters' part.  Rows of other adapters are zeros against an adapter, and zero times infinity or NaN is NaN: where a wave's rows do not all have the
+  // adapter, what is not finite is taken out of it, and add_infinite() adds it to the rows that it belongs to.
+  TGG_DEV void begin(int id, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at) {
+    const Place tile = locate(id);
+    int el = at.lane;
+    asm volatile("" : "+v"(el));  // (addresses are made afresh per tile instead of living across the multiplies)
+    const int l16 = el & 15, lg = el >> 4;
+    const int64_t row0 = (int64_t)tile.tm * C::BM + at.wm0;
+    const int rows = (int)min((int64_t)(C::BM / C::WM), p.M - row0), col0 = tile.tn * C::BN + at.wn0;  // (rows may be negative)
+    infinite = false;
+    if (rows <= 0) return;
+    int ids[C::TM];
 #pragma unroll
-    for (int i = 0; i < C::B_BYTES / (C::THREADS * 16); ++i) {
-      i32x4_t* const at = (i32x4_t*)(b + (i * C::THREADS + threadIdx.x) * 16);
-      i32x4_t v = *at;
-      bool here = false;
+    for (int i = 0; i < C::TM; ++i) ids[i] = 16 * i + l16 < rows ? p.ids.at(row0 + 16 * i + l16) : -1;
+    const rsrc_t hw = window(p.planes + row0 * 2 * p.R, (int64_t)rows * p.R * 4);
+    for (int l = -1;;) {
+      // the wave's next adapter, in the order of their numbers
+      uint32_t lowest = 0xffffffffu;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t x = (uint32_t)v[w];
-        const bool lo = (x & EXPONENT) == EXPONENT, hi = (x >> 16 & EXPONENT) == EXPONENT;
-        x = (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
-        v[w] = (int)x;
-        here = here || lo || hi;
-      }
-      if (here) *at = v;
-      bad = bad || here;
-    }
-    if (bad) ((int*)(stage + FLAGS_OFF))[q & 1] = id + 1;
-    __syncthreads();
-  }
-
-  // between the adapters' slabs and the shared product's: the planes' scales out of the sums
-  TGG_DEV void after_slab(int id, int done, int all, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at) const {
-    if (!SCALED || done != all - kt || done == 0) return;
-    int tm, tn;
-    locate(id, tm, tn);
+      for (int i = 0; i < C::TM; ++i) lowest = ids[i] > l ? min(lowest, (uint32_t)ids[i]) : lowest;
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i) {
-      const int64_t row = (int64_t)tm * C::BM + at.wm0 + 16 * i + at.l16;
-      const float back = row < p.M ? p.back[row] : 0.f;
+      for (int d = 1; d < 16; d <<= 1) lowest = min(lowest, (uint32_t)__shfl_xor((int)lowest, d, 64));  // (all four groups of lanes hold the same rows)
+      l = __builtin_amdgcn_readfirstlane((int)lowest);
+      if (l < 0) break;
+      bool all = true;
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j)
+      for (int i = 0; i < C::TM; ++i) all = all && (ids[i] == l || 16 * i + l16 >= rows);
+      const bool mixed = __ballot(!all) != 0;
+      const rsrc_t bw = window(p.pair + ((int64_t)l * p.cols + col0) * p.R, (int64_t)min(C::BN / C::WN, p.cols - col0) * p.R * 2);
+#pragma unroll 1
+      for (int k0 = 0; k0 < 2 * p.R; k0 += 32) {  // depth: the high plane, then the low one
+        const int k = k0 + 8 * lg, r = k < p.R ? k : k - p.R;
+        i32x4_t b[C::TN];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] *= back;
-    }
-  }
-
-  // what inspect() has taken out, for the lane's outputs
-  TGG_DEV void add_infinite(int tm, int tn, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at) const {
+        for (int j = 0; j < C::TN; ++j) b[j] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(bw, k < 2 * p.R ? ((16 * j + l16) * p.R + r) * 2 : kNowhere, 0, 0));
+        if (mixed) {
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i) {
-      const int64_t row = (int64_t)tm * C::BM + at.wm0 + 16 * i + at.l16;
-      const int l = row < p.M ? p.ids.at(row) : -1;
+          for (int j = 0; j < C::TN; ++j) {
+            uint32_t out = 0;
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int col = tn * C::BN + at.wn0 + 16 * j + 4 * at.lg + e;
-          float add = 0.f;
-          if (l >= 0 && col < p.cols) {
-            for (int r = 0; r < p.R; ++r) {
-              const uint16_t b = ((const uint16_t*)p.pair)[NT ? ((int64_t)l * p.cols + col) * p.R + r : ((int64_t)l * p.R + r) * p.cols + col];
-              if ((b & EXPONENT) == EXPONENT) add += from_bits<DT>(b) * (from_bits<DT>(p.planes[row * 2 * p.R + r]) + from_bits<DT>(p.planes[(row * 2 + 1) * p.R + r]));
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t x = (uint32_t)b[j][w], bad = ((x & EXPONENT) == EXPONENT ? 0xffffu : 0u) | ((x >> 16 & EXPONENT) == EXPONENT ? 0xffff0000u : 0u);
+              b[j][w] = (int)(x & ~bad);
+              out |= bad;
             }
+            infinite = infinite || __ballot(out != 0) != 0;
           }
-          acc[i][j][e] += add;
         }
+        i32x4_t rest[C::TN];
+        if (DT == DT_F16) {
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const float v0 = from_bits<DT_F16>((uint16_t)b[j][w]), v1 = from_bits<DT_F16>((uint16_t)((uint32_t)b[j][w] >> 16));
+              const uint32_t high = pack2<DT_BF16>(v0, v1);
+              const float r0 = v0 - from_bits<DT_BF16>((uint16_t)high), r1 = v1 - from_bits<DT_BF16>((uint16_t)(high >> 16));
+              b[j][w] = (int)high;
+              rest[j][w] = (int)pack2<DT_BF16>(__builtin_isfinite(r0) ? r0 : 0.f, __builtin_isfinite(r1) ? r1 : 0.f);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) {
+          if (__ballot(ids[i] == l) == 0) continue;
+          const i32x4_t a = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(hw, ids[i] == l && k < 2 * p.R ? ((16 * i + l16) * 2 * p.R + k) * 2 : kNowhere, 0, 0));
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j) acc[i][j] = stream_mma<DT_BF16>(b[j], a, acc[i][j]);
+          if (DT == DT_F16) {
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j) acc[i][j] = stream_mma<DT_BF16>(rest[j], a, acc[i][j]);
+          }
+        }
+      }
+    }
+  }
+  // What begin() has taken out: an infinity or a NaN, whatever it is added to, so it may as well be added to the stored outputs.
+  TGG_DEV void add_infinite(int64_t row0, int col0, int lane) const {
+    wait_vmcnt<0>();  // (the wave's own stores)
+    const int col = col0 + lane;
+    if (lane >= C::BN / C::WN || col >= p.cols) return;
+#pragma unroll 1
+    for (int64_t row = row0; row < min(row0 + C::BM / C::WM, p.M); ++row) {
+      const int l = p.ids.at(row);
+      if (l < 0) continue;
+      const uint16_t* const b = p.pair + ((int64_t)l * p.cols + col) * p.R;
+      float add = 0.f;
+#pragma unroll 1
+      for (int r = 0; r < p.R; ++r)
+        if ((b[r] & EXPONENT) == EXPONENT) add += from_bits<DT>(b[r]) * (from_bits<DT_BF16>(p.planes[row * 2 * p.R + r]) + from_bits<DT_BF16>(p.planes[(row * 2 + 1) * p.R + r]));
+      volatile uint16_t* const o = (volatile uint16_t*)p.out + row * p.cols + col;
+      if (add != 0.f) *o = Out16<DT>::cvt(from_bits<DT>(*o) + add);
     }
   }
 
-  TGG_DEV void epilogue(int id, int q, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at, char* stage) const {
+  TGG_DEV void epilogue(int id, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at, char* stage) const {
     int el = at.lane;
     asm volatile("" : "+v"(el));
     const int l16 = el & 15, lg = el >> 4;
-    int tm, tn;
-    locate(id, tm, tn);
-    if (__builtin_expect(((volatile int*)(stage + FLAGS_OFF))[q & 1] == id + 1, 0)) add_infinite(tm, tn, acc, at);
+    const Place tile = locate(id);
     char* const mine = stage + at.wave * STAGE_WAVE;
-    const int cbase = tn * C::BN + at.wn0;
-    const int64_t rbase = (int64_t)tm * C::BM + at.wm0;
+    const int cbase = tile.tn * C::BN + at.wn0;
+    const int64_t rbase = (int64_t)tile.tm * C::BM + at.wm0;
     constexpr int CPS = 2 * C::TN, PASSES = 16 * CPS / 64;  // 16-byte pieces of a staged row, wave-wide reads of a strip
     static_assert(PASSES * 64 == 16 * CPS, "a strip is read back by whole waves");
 #pragma unroll
@@ -468,13 +358,13 @@ template <class C, int DT, bool NT> struct LoraProblem {
       }
       asm volatile("" : : : "memory");
     }
+    if (__builtin_expect(infinite, 0)) add_infinite(rbase, cbase, el);
   }
 };
 
 template <class C, int DT, bool NT> __global__ __launch_bounds__(C::THREADS) void lora_gemm_kernel(const LoraGemm p) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   LoraProblem<C, DT, NT> prob(p);
-  if (threadIdx.x < 2) ((int*)(smem + C::EPI_OFF + LoraProblem<C, DT, NT>::FLAGS_OFF))[threadIdx.x] = 0;
   stream_gemm<C, DT, NT>(prob, smem);
 }
 
@@ -794,14 +684,13 @@ template <int DT, int RB> int down_rc(const DownParams& p, dim3 grid, hipStream_
   return check_launch("lora_down");
 }
 
-template <int DT> int launch_down(DownParams p, hipStream_t s) {
+template <int DT> int launch_down(const DownParams& p, hipStream_t s) {
   const bool tall = p.M >= 8192;  // 32 rows a workgroup, else 16
   const int rows = tall ? 32 : 16;
-  p.row_blocks = (int)((p.M + rows - 1) / rows);
-  const int lists = p.counts ? (int)((p.M + p.tile - 1) / p.tile) : 0;
+  const int blocks = (int)((p.M + rows - 1) / rows);
   // few rows: their adapters side by side
-  const int turns = p.row_blocks >= 1024 ? 1 : min(16, 1024 / p.row_blocks);
-  const dim3 grid(p.row_blocks + lists, tall ? 1 : turns, p.parts);
+  const int turns = blocks >= 1024 ? 1 : min(16, 1024 / blocks);
+  const dim3 grid(blocks, tall ? 1 : turns, p.parts);
   return tall ? down_rc<DT, 2>(p, grid, s) : down_rc<DT, 1>(p, grid, s);
 }
 
@@ -865,21 +754,18 @@ int outer_parts(int64_t M, int N, int K, int L) {
 
 struct LoraPlan {
   int tile, parts;
-  int64_t h, planes, back, counts, lists, bt, rows, part_a, part_b, bytes;
+  int64_t h, planes, at, bt, rows, part_a, part_b, bytes;
 };
 LoraPlan lora_plan(bool backward, int64_t M, int N, int K, int R, int L) {
   LoraPlan q = {};
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t here = at; at += align256(bytes); return here; };
   q.tile = tile_of(M, backward ? K : N);
-  const int64_t tiles = (M + q.tile - 1) / q.tile;
   q.h = take((backward ? 1 : 4) * M * R * 4);
   q.planes = take(M * R * 4);
-  q.back = take(M * 4);
-  q.counts = take(tiles * 4);
-  q.lists = take(tiles * q.tile * 4);
   if (backward) {
     q.parts = outer_parts(M, N, K, L);
+    q.at = take((int64_t)L * K * R * 2);
     q.bt = take((int64_t)L * N * R * 2);
     q.rows = take((int64_t)q.parts * L * 4);
     if (q.parts > 1) {
@@ -898,14 +784,11 @@ template <int DT> int forward(const void* x, const void* w, const void* a, const
   d.x = x; d.a = a; d.scales = scales; d.ids = ids; d.M = M; d.R = R; d.depth = K;
   d.parts = few && !h ? few_parts(M) : 1;  // (what is kept for the backward pass is one sum)
   d.h = h ? h : (float*)(ws + q.h);
-  if (!few) {
-    d.planes = (uint16_t*)(ws + q.planes); d.back = (float*)(ws + q.back);
-    d.counts = (int32_t*)(ws + q.counts); d.lists = (int32_t*)(ws + q.lists); d.tile = q.tile;
-  }
+  if (!few) d.planes = (uint16_t*)(ws + q.planes);
   if (int e = launch_down<DT>(d, s)) return e;
   if (few) return launch_few<DT>({x, w, b, d.h, ids, out, M, N, K, R, d.parts}, s);
   LoraGemm g = {};
-  g.x = x; g.w = w; g.pair = b; g.planes = d.planes; g.back = d.back; g.ids = ids; g.counts = d.counts; g.lists = d.lists; g.out = out;
+  g.x = x; g.w = w; g.pair = (const uint16_t*)b; g.planes = d.planes; g.ids = ids; g.out = out;
   g.M = M; g.cols = N; g.depth = K; g.R = R;
   return launch_gemm<DT, true>(g, q.tile, s);
 }
@@ -914,20 +797,23 @@ template <int DT> int backward(const void* grad, const void* x, const void* w, c
                                int K, int R, char* ws, hipStream_t s) {
   const LoraPlan q = lora_plan(true, M, N, K, R, ids.L);
   if (dx || da) {
-    const int tn = (N + 63) / 64, tr = (R + 63) / 64;
-    lora_transpose_kernel<<<dim3((unsigned)(ids.L * tn * tr)), dim3(256), 0, s>>>((const uint16_t*)b, (uint16_t*)(ws + q.bt), N, R, tn, tr);
+    TransposeParams t = {};
+    const int tr = (R + 63) / 64, tn = (N + 63) / 64, tk = dx ? (K + 63) / 64 : 0;
+    t.s[0] = {(const uint16_t*)b, (uint16_t*)(ws + q.bt), N, R, tn, tr};
+    t.s[1] = {(const uint16_t*)a, (uint16_t*)(ws + q.at), R, K, tr, tk};
+    t.first = ids.L * tn * tr;
+    lora_transpose_kernel<<<dim3((unsigned)(t.first + ids.L * tk * tr)), dim3(256), 0, s>>>(t);
     if (int e = check_launch("lora_transpose")) return e;
     DownParams d = {};
     d.x = grad; d.a = ws + q.bt; d.scales = scales; d.ids = ids; d.M = M; d.R = R; d.depth = N; d.parts = 1;
     d.h = (float*)(ws + q.h);
     if (dx) {
-      d.planes = (uint16_t*)(ws + q.planes); d.back = (float*)(ws + q.back);
-      d.counts = (int32_t*)(ws + q.counts); d.lists = (int32_t*)(ws + q.lists); d.tile = q.tile;
-    }
+      d.planes = (uint16_t*)(ws + q.planes);
+      }
     if (int e = launch_down<DT>(d, s)) return e;
     if (dx) {
       LoraGemm g = {};
-      g.x = grad; g.w = w; g.pair = a; g.planes = d.planes; g.back = d.back; g.ids = ids; g.counts = d.counts; g.lists = d.lists; g.out = dx;
+      g.x = grad; g.w = w; g.pair = (const uint16_t*)(ws + q.at); g.planes = d.planes; g.ids = ids; g.out = dx;
       g.M = M; g.cols = K; g.depth = N; g.R = R;
       if (int e = launch_gemm<DT, false>(g, q.tile, s)) return e;
     }

@@ -61,9 +61,7 @@ TGG_DEV float ns_sum(const float* p, int n) {
 }
 
 template <class C, int MODE, bool PRECISE> struct NsProblem {
-  static constexpr bool B_KMAJOR = MODE != NS_UPDATE, SYM = MODE != NS_UPDATE, SCALED = false, INSPECTS = false;
-  typedef Operand<C::BM, true> OpA;
-  typedef Operand<C::BN, B_KMAJOR> OpB;
+  static constexpr bool B_KMAJOR = MODE != NS_UPDATE, SYM = MODE != NS_UPDATE;
   static_assert(!SYM || C::BM == C::BN, "symmetric results have square tiles");
   static constexpr int PITCH = C::TN * 32 + 16;  // staged strip of 16 rows: bytes between rows
   static constexpr int STAGE_WAVE = 16 * PITCH;
@@ -72,106 +70,71 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
 
   const NsProduct& p;
   StreamWalk walk;
-  int tiles_m, tiles_n, per_matrix;
-  int a_voff, b_voff, a_tail, b_tail;  // the lane's offsets in a whole slab, and in one that the depth cuts short
-  int kt, tail;
-  // the cursor
-  uint64_t a_hi, a_lo, b_hi, b_lo;  // the tile's first bytes in the planes
-  int pos, issued, pass, a_len, b_len, b_rows;
+  StreamCursor<C, B_KMAJOR> cur;
+  int tiles_m, tiles_n, per_matrix, pos, pass;
+  int64_t a_tile, b_tile;  // the tile's first bytes in the planes
+  int a_rows, b_rows, b_skip;
   bool live;
-  int row0_, col0_, m_;
 
-  TGG_DEV NsProblem(const NsProduct& q, int tiles_m_, int tiles_n_) : p(q), walk(q.batch * (SYM ? tiles_m_ * (tiles_m_ + 1) / 2 : tiles_m_ * tiles_n_)) {
+  TGG_DEV NsProblem(const NsProduct& q, int tiles_m_, int tiles_n_)
+      : p(q), walk(q.batch * (SYM ? tiles_m_ * (tiles_m_ + 1) / 2 : tiles_m_ * tiles_n_)), cur(q.lda * 2, q.ldb * 2, q.depth) {  // (planes are zero between the depth and the next multiple of 8)
     tiles_m = tiles_m_;
     tiles_n = tiles_n_;
     per_matrix = SYM ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n;
-    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    a_voff = OpA::lane_voff(lane, wave % OpA::NPAT, p.lda * 2);
-    b_voff = OpB::lane_voff(lane, wave % OpB::NPAT, p.ldb * 2);
-    kt = (p.depth + 63) / 64;
-    const int chunks = ((p.depth + 7) / 8) % 8;  // (planes are zero between the depth and the next multiple of 8)
-    tail = chunks != 0;
-    a_tail = OpA::lane_chunk(lane, wave % OpA::NPAT) >= chunks ? kNoFetch : a_voff;
-    b_tail = B_KMAJOR && OpB::lane_chunk(lane, wave % OpB::NPAT) >= chunks ? kNoFetch : b_voff;
     pos = -1;
-    live = false;
   }
   TGG_DEV int tile_at(int q) const { return walk.at(q); }
-  TGG_DEV int slabs(int) const { return PRECISE ? 3 * kt : kt; }
+  TGG_DEV int slabs(int) const { return PRECISE ? 3 * cur.kt : cur.kt; }
   // id -> matrix, first row, first column
-  TGG_DEV void locate(int id, int& m, int& row0, int& col0) const {
-    m = id / per_matrix;
-    const int t = id - m * per_matrix;
+  struct Place { int m, row0, col0; };
+  TGG_DEV Place locate(int id) const {
+    const int m = id / per_matrix, t = id - m * per_matrix;
     int i, j;
     if (SYM) {
-      i = (int)((__builtin_sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-      while (i * (i + 1) / 2 > t) --i;
-      while ((i + 1) * (i + 2) / 2 <= t) ++i;
+      i = (int)((__builtin_sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);  // (within one: t is exact)
+      i -= i * (i + 1) / 2 > t;
+      i += (i + 1) * (i + 2) / 2 <= t;
       j = t - i * (i + 1) / 2;
     } else {
       i = t / tiles_n;
       j = t - i * tiles_n;
     }
-    m = __builtin_amdgcn_readfirstlane(m);
-    row0 = __builtin_amdgcn_readfirstlane(i * C::BM);
-    col0 = __builtin_amdgcn_readfirstlane(j * C::BN);
+    return {__builtin_amdgcn_readfirstlane(m), __builtin_amdgcn_readfirstlane(i * C::BM), __builtin_amdgcn_readfirstlane(j * C::BN)};
+  }
+  // passes: high x high planes, high x low, low x high
+  TGG_DEV void begin_pass() {
+    const uint16_t* const a = PRECISE && pass == 2 ? p.a_lo : p.a_hi;
+    const uint16_t* const b = PRECISE && pass == 1 ? p.b_lo : p.b_hi;
+    cur.begin(live, (uint64_t)a + a_tile, (uint64_t)b + b_tile, a_rows, b_rows, b_skip);
   }
   TGG_DEV void seek(int id) {
     ++pos;
+    pass = 0;
     live = id >= 0;
-    issued = pass = 0;
-    if (!live) {
-      a_hi = a_lo = b_hi = b_lo = (uint64_t)p.a_hi;
-      a_len = b_len = b_rows = 0;
-      return;
-    }
-    locate(id, m_, row0_, col0_);
-    const int64_t a_at = (m_ * p.a_stride + (int64_t)row0_ * p.lda) * 2;
-    const int64_t b_at = (m_ * p.b_stride + (B_KMAJOR ? (int64_t)col0_ * p.ldb : (int64_t)col0_)) * 2;
-    a_hi = uniform64((uint64_t)p.a_hi + a_at);
-    b_hi = uniform64((uint64_t)p.b_hi + b_at);
-    if (PRECISE) {
-      a_lo = uniform64((uint64_t)p.a_lo + a_at);
-      b_lo = uniform64((uint64_t)p.b_lo + b_at);
-    }
-    const int rows = min(C::BM, p.rows - row0_);
-    a_len = __builtin_amdgcn_readfirstlane(rows * p.lda * 2);
-    if (B_KMAJOR) b_len = __builtin_amdgcn_readfirstlane(min(C::BN, p.cols - col0_) * p.ldb * 2);
-    b_rows = p.depth;
+    const Place at = locate(live ? id : 0);
+    a_tile = (at.m * p.a_stride + (int64_t)at.row0 * p.lda) * 2;
+    b_tile = (at.m * p.b_stride + (B_KMAJOR ? (int64_t)at.col0 * p.ldb : (int64_t)at.col0)) * 2;
+    a_rows = min(C::BM, p.rows - at.row0);
+    b_rows = B_KMAJOR ? min(C::BN, p.cols - at.col0) : p.depth;
+    b_skip = at.col0 * 2;
+    begin_pass();
   }
-  TGG_DEV void next(StreamSlab& s) {
-    const int left = issued * 128;
-    // passes: high x high, high x low, low x high
-    const uint64_t a = PRECISE && pass == 2 ? a_lo : a_hi, b = PRECISE && pass == 1 ? b_lo : b_hi;
-    s.ra = make_rsrc32(a + left, live ? a_len - left : 0);
-    if (B_KMAJOR) {
-      s.rb = make_rsrc32(b + left, live ? b_len - left : 0);
-    } else {  // token rows issued * 64 ... of the matrix
-      const int rows = min(64, b_rows - issued * 64);
-      s.rb = make_rsrc32(b + (uint64_t)issued * 64 * p.ldb * 2, live ? rows * p.ldb * 2 - col0_ * 2 : 0);
-    }
-    s.kind = tail && issued + 1 == kt;
-    if (!live) return;
-    if (++issued == kt) {
-      issued = 0;
-      if (!PRECISE || ++pass == 3) seek(tile_at(pos + 1));
+  TGG_DEV void turn() {
+    if (PRECISE && pass < 2) {
+      ++pass;
+      begin_pass();
+    } else {
+      seek(tile_at(pos + 1));
     }
   }
-  TGG_DEV int a_offset(const StreamSlab& s, int k) const {
-    const int idx = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + k * C::NWAVES;
-    return (s.kind ? a_tail : a_voff) + idx * OpA::RPI * p.lda * 2;
-  }
-  TGG_DEV int b_offset(const StreamSlab& s, int k) const {
-    const int idx = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + k * C::NWAVES;
-    return (s.kind ? b_tail : b_voff) + idx * OpB::RPI * p.ldb * 2;
-  }
+  TGG_DEV void begin(int, f32x4_t (&)[C::TM][C::TN], const StreamPlace<C>&) const {}
 
-  TGG_DEV void epilogue(int id, int, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at, char* stage) const {
+  TGG_DEV void epilogue(int id, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at, char* stage) const {
     int el = at.lane;
     asm volatile("" : "+v"(el));  // (addresses are made afresh per tile instead of living across the multiplies)
     const int l16 = el & 15, lg = el >> 4;
-    int m, row0, col0;
-    locate(id, m, row0, col0);
+    const Place tile = locate(id);
+    const int m = tile.m, row0 = tile.row0, col0 = tile.col0;
     const float inv_rows = 1.f / (float)p.rows;
     const float d = p.x_tiles ? ns_sum(p.x_sums + (int64_t)m * p.x_tiles, p.x_tiles) * inv_rows : inv_rows;
     const float e = MODE == NS_GRAM ? 0.f : ns_sum(p.a_sums + (int64_t)m * p.a_tiles, p.a_tiles) * inv_rows;

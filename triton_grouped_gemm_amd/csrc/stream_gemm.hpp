@@ -5,14 +5,13 @@
 // who says what a slab is: a problem P hands out slabs one after another, so a tile may add up products of several pairs of operands
 // (a matrix's two planes, a row's shared projection and its adapters), and takes a tile's sums.  P has
 //
+//   StreamCursor<C, B_KMAJOR> cur         where the copies are
 //   int tile_at(int pos)                  id of the workgroup's pos-th tile, -1 past the last one
 //   int slabs(int id)                     slabs of a tile, at least one
-//   void seek(int id)                     the next slab is the tile's first one; id -1: no more slabs
-//   void next(StreamSlab& s)              descriptors of the next slab; past a tile's last one it seeks the following tile by itself
-//   int a_offset(s, k), b_offset(s, k)    source offset of the lane's part of the wave's k-th copy of the slab's A or B operand, or kNoFetch
-//   void after_slab(id, n, slabs, acc, at)  where P::SCALED: the tile's sums after its first n slabs
-//   void inspect(s, b, id, pos, stage)    where P::INSPECTS: a slab of the pos-th tile id has landed, its B operand at b; ends with a barrier if it changes anything
-//   void epilogue(id, pos, acc, at, stage)  the tile's sums: acc[i][j][e] is row wm0 + 16 i + l16, column wn0 + 16 j + 4 lg + e
+//   void seek(int id)                     begins the tile's slabs in `cur`; id -1: no more slabs
+//   void turn()                           the slabs begun last have all been handed out: begins the tile's next ones, or seeks the next tile
+//   void begin(id, acc, at)               the tile's sums before its first slab (they are zero)
+//   void epilogue(id, acc, at, stage)     the tile's sums: acc[i][j][e] is row wm0 + 16 i + l16, column wn0 + 16 j + 4 lg + e
 //
 // A [rows, K] is K-contiguous; B is K-contiguous rows [columns, K] (B_KMAJOR) or token rows [K, columns].
 #pragma once
@@ -34,7 +33,60 @@ template <int BM_, int BN_, int WM_, int WN_> struct StreamCfg {
 
 struct StreamSlab {
   i32x4_t ra, rb;
-  int kind;  // the problem's
+};
+
+// The slabs of one pair of operands: descriptors that move on by 64 values of depth, and the lane's source offsets in the wave's copies, which stay the same but
+// for a last slab that the depth cuts short.  32-bit bookkeeping keeps the scalar work per slab short (eight waves share the scalar unit).
+template <class C, bool B_KMAJOR> struct StreamCursor {
+  typedef Operand<C::BM, true> OpA;
+  typedef Operand<C::BN, B_KMAJOR> OpB;
+  int va[C::CA], vb[C::CB];
+  int lda, ldb;            // bytes between rows
+  int a_voff, b_voff;
+  bool a_there, b_there;   // whether the lane fetches in a slab that is cut short
+  int kt, tail;            // slabs; whether the last one is cut short
+  uint64_t a_at, b_at;     // the next slab
+  int a_rem, b_rem, b_skip;  // bytes left of the tile's rows; of token rows, how many are left, and the bytes in front of the tile's columns
+  int run;                 // slabs until something changes
+  bool in_tail;
+
+  TGG_DEV StreamCursor(int lda_, int ldb_, int depth) : lda(lda_), ldb(ldb_) {
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    a_voff = OpA::lane_voff(lane, wave % OpA::NPAT, lda) + wave * OpA::RPI * lda;
+    b_voff = OpB::lane_voff(lane, wave % OpB::NPAT, ldb) + wave * OpB::RPI * ldb;
+    kt = (depth + 63) / 64;
+    const int chunks = ((depth + 7) / 8) % 8;  // 16-byte pieces of a K-contiguous row in a slab that is cut short
+    tail = chunks != 0;
+    a_there = OpA::lane_chunk(lane, wave % OpA::NPAT) < chunks;
+    b_there = !B_KMAJOR || OpB::lane_chunk(lane, wave % OpB::NPAT) < chunks;
+  }
+  TGG_DEV void offsets(bool whole) {
+#pragma unroll
+    for (int k = 0; k < C::CA; ++k) va[k] = whole || a_there ? a_voff + k * C::NWAVES * OpA::RPI * lda : kNoFetch;
+#pragma unroll
+    for (int k = 0; k < C::CB; ++k) vb[k] = whole || b_there ? b_voff + k * C::NWAVES * OpB::RPI * ldb : kNoFetch;
+    in_tail = !whole;
+    run = whole ? kt - tail : 1;
+  }
+  // a, b: the tile's first bytes; rows of A, and of B its columns' rows or (token rows) the depth.  live false: nothing, for good
+  TGG_DEV void begin(bool live, uint64_t a, uint64_t b, int a_rows, int b_rows, int skip) {
+    a_at = uniform64(a);
+    b_at = uniform64(b);
+    a_rem = __builtin_amdgcn_readfirstlane(live ? a_rows * lda : 0);
+    b_rem = __builtin_amdgcn_readfirstlane(live ? (B_KMAJOR ? b_rows * ldb : b_rows) : 0);
+    b_skip = skip;
+    offsets(kt > tail);
+    run = live ? run : 0x7fffffff;
+  }
+  TGG_DEV void next(StreamSlab& s) {
+    s.ra = make_rsrc32(a_at, a_rem);
+    s.rb = make_rsrc32(b_at, B_KMAJOR ? b_rem : min(64, b_rem) * ldb - b_skip);
+    a_at += 128;
+    a_rem -= 128;
+    b_at += B_KMAJOR ? 128 : (uint64_t)(64 * ldb);
+    b_rem -= B_KMAJOR ? 128 : 64;
+    --run;
+  }
 };
 
 // where a wave's block of the tile begins, and a lane's place in a 16 x 16 block
@@ -78,9 +130,13 @@ template <int DT> TGG_DEV f32x4_t stream_mma(const i32x4_t& w, const i32x4_t& x,
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w), __builtin_bit_cast(f16x8_t, x), c, 0, 0, 0);
 }
 
-// A copy must not follow the vector instruction that wrote a scalar of its descriptor too closely, and the compiler does not look inside the copies.
+// The next slab.  All copies of the one before have been issued: offsets may change.  (A copy must not follow the vector instruction that wrote a scalar of its
+// descriptor too closely, and the compiler does not look inside the copies.)
 template <class P> TGG_DEV void stream_next(P& prob, StreamSlab& s) {
-  prob.next(s);
+  if (__builtin_expect(prob.cur.run == 0, 0)) {
+    if (prob.cur.tail && !prob.cur.in_tail) prob.cur.offsets(false); else prob.turn();
+  }
+  prob.cur.next(s);
   asm volatile("s_nop 4" : "+s"(s.ra), "+s"(s.rb));
 }
 
@@ -104,8 +160,8 @@ template <class C, int DT, bool B_KMAJOR, class P> TGG_DEV void stream_gemm(P& p
       b_rd[j] = (lg * 8 + e) * (C::BN * 2) + chunk * 16 + (c & 1) * 8;
     }
   }
-  auto load_a = [&](const char* s, int ks, int i) -> i32x4_t { return *(const i32x4_t*)(s + a_rd[ks] + i * 16 * 128); };
-  auto load_b = [&](const char* s, int ks, int j) -> i32x4_t {
+  auto load_a = [&](const char* s, int ks, int i) __attribute__((always_inline)) -> i32x4_t { return *(const i32x4_t*)(s + a_rd[ks] + i * 16 * 128); };
+  auto load_b = [&](const char* s, int ks, int j) __attribute__((always_inline)) -> i32x4_t {
     if (B_KMAJOR) return *(const i32x4_t*)(s + b_rd[ks] + j * 16 * 128);
     const char* q = s + b_rd[B_KMAJOR ? 0 : j] + ks * 32 * (C::BN * 2);
     const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr_t)q);
@@ -117,11 +173,11 @@ template <class C, int DT, bool B_KMAJOR, class P> TGG_DEV void stream_gemm(P& p
   constexpr int SP2 = (C::TM * C::TN / 2) / (C::NC / 2), SP1 = 1;  // multiplies between copies, behind the barrier and in the half step after that
   StreamSlab sc, sc_next;
   uint32_t sc_base = 0, sc_next_base = 0;
-  auto copy_k = [&](int k) {
+  auto copy_k = [&](int k) __attribute__((always_inline)) {
     if (k < C::CA) {
-      copy_b128_to_lds(sc.ra, sc_base + (at.wave + k * C::NWAVES) * 1024, prob.a_offset(sc, k));
+      copy_b128_to_lds(sc.ra, sc_base + (at.wave + k * C::NWAVES) * 1024, prob.cur.va[k]);
     } else {
-      copy_b128_to_lds(sc.rb, sc_base + C::A_BYTES + (at.wave + (k - C::CA) * C::NWAVES) * 1024, prob.b_offset(sc, k - C::CA));
+      copy_b128_to_lds(sc.rb, sc_base + C::A_BYTES + (at.wave + (k - C::CA) * C::NWAVES) * 1024, prob.cur.vb[k - C::CA]);
     }
   };
 
@@ -132,17 +188,11 @@ template <class C, int DT, bool B_KMAJOR, class P> TGG_DEV void stream_gemm(P& p
   for (int k = 0; k < C::NC; ++k) copy_k(k);
   wait_vmcnt<0>();
   __syncthreads();
-  if constexpr (P::INSPECTS) prob.inspect(sc, smem + C::A_BYTES, prob.tile_at(0), 0, smem + C::EPI_OFF);
   stream_next(prob, sc);
   sc_base = smem_addr + C::STAGE_BYTES;
 #pragma unroll
   for (int k = 0; k < C::NC / 2; ++k) copy_k(k);
   i32x4_t fa[C::TM - 1], fa_last[2], fb[2][C::TN];
-#pragma unroll
-  for (int i = 0; i < C::TM - 1; ++i) fa[i] = load_a(smem, 0, i);
-  fa_last[0] = load_a(smem, 0, C::TM - 1);
-#pragma unroll
-  for (int j = 0; j < C::TN; ++j) fb[0][j] = load_b(smem + C::A_BYTES, 0, j);
   int ring = 0;
 
   f32x4_t acc[C::TM][C::TN];
@@ -152,8 +202,20 @@ template <class C, int DT, bool B_KMAJOR, class P> TGG_DEV void stream_gemm(P& p
     for (int i = 0; i < C::TM; ++i)
 #pragma unroll
       for (int j = 0; j < C::TN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    prob.begin(id, acc, at);
+    // The first slab's first fragments.  (The slab before has read them already, if this is not the first tile: read again, their registers are free for begin() and epilogue().)
+    {
+      const char* s = smem + (ring & 1) * C::STAGE_BYTES;
+#pragma unroll
+      for (int i = 0; i < C::TM - 1; ++i) fa[i] = load_a(s, 0, i);
+      fa_last[0] = load_a(s, 0, C::TM - 1);
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) fb[0][j] = load_b(s + C::A_BYTES, 0, j);
+    }
     enum { READ_EARLY, READ_ROLL, READ_NONE, READ_CATCH_UP };  // as in gemm_fast.hip
-    auto half = [&](int cur, int h, const char* s, int ks, int mode, int k0, bool prepare = false) {
+    // (inlined before anything else: a lambda that is simplified by itself turns stores to the problem's members into stores through selected pointers, and the
+    // members stay in memory)
+    auto half = [&](int cur, int h, const char* s, int ks, int mode, int k0, bool prepare = false) __attribute__((always_inline)) {
       constexpr int HM = C::TM / 2;
 #pragma unroll
       for (int ii = 0; ii < HM; ++ii) {
@@ -196,23 +258,18 @@ template <class C, int DT, bool B_KMAJOR, class P> TGG_DEV void stream_gemm(P& p
     };
     for (int kt = 0; kt < slabs; ++kt) {
       const char* s = smem + (ring & 1) * C::STAGE_BYTES;
-      char* const sn = smem + ((ring + 1) & 1) * C::STAGE_BYTES;
+      const char* sn = smem + ((ring + 1) & 1) * C::STAGE_BYTES;
       half(0, 0, s, 1, READ_EARLY, C::NC / 2);
       half(0, 1, s, 1, READ_ROLL, -1, true);
       half(1, 0, sn, 0, READ_NONE, -1);
       wait_vmcnt<0>();
       __syncthreads();
-      if constexpr (P::INSPECTS) {
-        const bool same = kt + 1 < slabs;
-        prob.inspect(sc, sn + C::A_BYTES, same ? id : prob.tile_at(pos + 1), same ? pos : pos + 1, smem + C::EPI_OFF);
-      }
       sc = sc_next;
       sc_base = sc_next_base;
       half(1, 1, sn, 0, READ_CATCH_UP, 0);
       ++ring;
-      if constexpr (P::SCALED) prob.after_slab(id, kt + 1, slabs, acc, at);
     }
-    prob.epilogue(id, pos, acc, at, smem + C::EPI_OFF);
+    prob.epilogue(id, acc, at, smem + C::EPI_OFF);
   }
   wait_vmcnt<0>();  // the trailing copies, which fetch nothing, still write LDS
 }
