@@ -803,7 +803,7 @@ static int lora_check(int64_t M, int64_t N, int64_t K, int R, int L) {
   if (R < 8 || R > 128 || (R & 7)) return set_error("the rank must be a multiple of 8 in [8, 128], got %d", R);
   if (L < 1 || L > TGG_MAX_GROUPS) return set_error("L=%d adapters outside [1, %d]", L, TGG_MAX_GROUPS);
   // output tiles are numbered in 31 bits
-  if (((M + 127) / 128) * ((max(N, K) + 127) / 128) >= (1ll << 30)) return set_error("M=%lld, N=%lld, K=%lld: too large", (long long)M, (long long)N, (long long)K);
+  if (((M + 127) / 128) * (((N > K ? N : K) + 127) / 128) >= (1ll << 30)) return set_error("M=%lld, N=%lld, K=%lld: too large", (long long)M, (long long)N, (long long)K);
   return 0;
 }
 

@@ -75,7 +75,7 @@ template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) voi
   __shared__ __attribute__((aligned(16))) float sums[kDownWaves * 16 * COLS];
   const int lane = lane_id(), l16 = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row0 = (int64_t)blockIdx.x * (16 * RB);
-  const int rows = (int)min((int64_t)(16 * RB), p.M - row0);
+  const int rows = (int)lesser(16 * RB, p.M - row0);
   const int id = lane < rows ? p.ids.at(row0 + lane) : -1;
   // lanes whose row is the first of its adapter
   uint64_t firsts = 0;
@@ -236,7 +236,7 @@ template <class C, int DT, bool NT> struct LoraProblem {
     const bool live = id >= 0;
     const Place at = locate(live ? id : 0);
     const int64_t row0 = (int64_t)at.tm * C::BM, col0 = (int64_t)at.tn * C::BN;
-    cur.begin(live, (uint64_t)p.x + row0 * p.depth * 2, (uint64_t)p.w + (NT ? col0 * p.depth : col0) * 2, (int)min((int64_t)C::BM, p.M - row0), NT ? min(C::BN, p.cols - (int)col0) : p.depth, (int)col0 * 2);
+    cur.begin(live, (uint64_t)p.x + row0 * p.depth * 2, (uint64_t)p.w + (NT ? col0 * p.depth : col0) * 2, (int)lesser(C::BM, p.M - row0), NT ? min(C::BN, p.cols - (int)col0) : p.depth, (int)col0 * 2);
   }
   TGG_DEV void turn() { seek(tile_at(pos + 1)); }
 
@@ -248,7 +248,7 @@ template <class C, int DT, bool NT> struct LoraProblem {
     asm volatile("" : "+v"(el));  // (addresses are made afresh per tile instead of living across the multiplies)
     const int l16 = el & 15, lg = el >> 4;
     const int64_t row0 = (int64_t)tile.tm * C::BM + at.wm0;
-    const int rows = (int)min((int64_t)(C::BM / C::WM), p.M - row0), col0 = tile.tn * C::BN + at.wn0;  // (rows may be negative)
+    const int rows = (int)lesser(C::BM / C::WM, p.M - row0), col0 = tile.tn * C::BN + at.wn0;  // (rows may be negative)
     infinite = false;
     if (rows <= 0) return;
     int ids[C::TM];
@@ -321,7 +321,7 @@ template <class C, int DT, bool NT> struct LoraProblem {
     const int col = col0 + lane;
     if (lane >= C::BN / C::WN || col >= p.cols) return;
 #pragma unroll 1
-    for (int64_t row = row0; row < min(row0 + C::BM / C::WM, p.M); ++row) {
+    for (int64_t row = row0; row < lesser(row0 + C::BM / C::WM, p.M); ++row) {
       const int l = p.ids.at(row);
       if (l < 0) continue;
       const uint16_t* const b = p.pair + ((int64_t)l * p.cols + col) * p.R;
@@ -388,7 +388,7 @@ template <int DT, int RB, int CB> __global__ __launch_bounds__(kFewThreads) void
   const int lane = lane_id(), l16 = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = blockIdx.x * COLS;
   const int64_t row0 = (int64_t)blockIdx.y * ROWS;
-  const int rows = (int)min((int64_t)ROWS, p.M - row0);
+  const int rows = (int)lesser(ROWS, p.M - row0);
   const rsrc_t xw = window((const uint16_t*)p.x + row0 * p.K, (int64_t)rows * p.K * 2);
   const rsrc_t ww = window((const uint16_t*)p.w + (int64_t)n0 * p.K, (int64_t)min(COLS, p.N - n0) * p.K * 2);
   const int steps = (p.K + 63) / 64;
@@ -518,7 +518,7 @@ template <int DT, int RC> __global__ __launch_bounds__(kOuterThreads) void lora_
   for (int64_t w0 = begin; w0 < end; w0 += kOuterWindow) {
     // the window's rows of this adapter, in order
     constexpr int PER = kOuterWindow / kOuterThreads;
-    const int n = (int)min((int64_t)kOuterWindow, end - w0);
+    const int n = (int)lesser(kOuterWindow, end - w0);
     int count = 0;
     uint32_t mine = 0;
 #pragma unroll
@@ -689,7 +689,7 @@ template <int DT> int launch_down(const DownParams& p, hipStream_t s) {
   const int rows = tall ? 32 : 16;
   const int blocks = (int)((p.M + rows - 1) / rows);
   // few rows: their adapters side by side
-  const int turns = blocks >= 1024 ? 1 : min(16, 1024 / blocks);
+  const int turns = blocks >= 1024 ? 1 : (int)lesser(16, 1024 / blocks);
   const dim3 grid(blocks, tall ? 1 : turns, p.parts);
   return tall ? down_rc<DT, 2>(p, grid, s) : down_rc<DT, 1>(p, grid, s);
 }
@@ -748,8 +748,8 @@ template <int DT, int RC> int outer_launch(const OuterParams& p, dim3 grid, hipS
 int outer_parts(int64_t M, int N, int K, int L) {
   const int64_t groups = (int64_t)L * ((N + kOuterCols - 1) / kOuterCols + (K + kOuterCols - 1) / kOuterCols);
   int64_t parts = (4 * num_cus() + groups - 1) / groups;
-  parts = min(parts, (M + 1023) / 1024);
-  return (int)max((int64_t)1, min(parts, (int64_t)64));
+  parts = lesser(parts, (M + 1023) / 1024);
+  return (int)larger(1, lesser(parts, 64));
 }
 
 struct LoraPlan {

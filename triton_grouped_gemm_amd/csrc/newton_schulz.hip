@@ -15,16 +15,22 @@
 //
 // G and G^2 are symmetric: only tiles on and below the diagonal are computed, and stored twice.  No sum depends on the order of arrival: norms are
 // summed per tile and the tiles' sums in order.
-#include <type_traits>
 
 #include "launch.hpp"
 #include "stream_gemm.hpp"
 
 namespace tgg {
 
-enum : int { NS_GRAM = 0, NS_POLY = 1, NS_UPDATE = 2 };
+enum : int { NS_GRAM = 0, NS_POLY = 1, NS_UPDATE = 2, NS_LAST = 3 };  // NS_LAST: the last step's update, straight to the result
 
 constexpr float kNsScale = 1024.f, kNsInv2 = 1.f / (1024.f * 1024.f);
+
+// Where results go: out = v, or with `weight` out = keep out - step v.
+struct NsTarget {
+  void* out;
+  int dt, weight;  // dt 0 bf16, 1 fp16, 2 fp32
+  float keep, step;
+};
 
 // One product for all matrices.  Planes: element (m, i, j) at m * stride + i * ld + j.
 struct NsProduct {
@@ -39,6 +45,8 @@ struct NsProduct {
   const float *x_sums, *a_sums;               // |X|^2 and |A|^2 by tile, x_tiles and a_tiles a matrix
   float* o_sums;                              // the result's (GRAM, UPDATE)
   int x_tiles, a_tiles;                       // x_tiles 0: the first step, d = 1 / M
+  NsTarget target;                            // LAST
+  int tall;                                   // LAST: the result is the transposed matrix
 };
 
 namespace {
@@ -51,6 +59,9 @@ TGG_DEV NsSplit ns_split(float v) {
 }
 TGG_DEV float ns_f16(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
 
+TGG_DEV float ns_from16(uint16_t x, int dt) { return dt == 0 ? __builtin_bit_cast(float, (uint32_t)x << 16) : ns_f16(x); }
+TGG_DEV uint16_t ns_to16(float x, int dt) { return dt == 0 ? Out16<DT_BF16>::cvt(x) : Out16<DT_F16>::cvt(x); }
+
 // the n sums of a matrix, added by a wave: every lane gets the same bits, and every workgroup
 TGG_DEV float ns_sum(const float* p, int n) {
   float s = 0.f;
@@ -60,13 +71,75 @@ TGG_DEV float ns_sum(const float* p, int n) {
   return s;
 }
 
+// n (up to 8) neighbouring values as fp32; VEC: all eight, in 16-byte loads
+template <bool VEC> TGG_DEV void ns_load8(float (&v)[8], const void* p, int64_t i, int dt, int n) {
+  if (VEC) {
+    if (dt == 2) {
+      const f32x4_t a = *(const f32x4_t*)((const float*)p + i), b = *(const f32x4_t*)((const float*)p + i + 4);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        v[x] = a[x];
+        v[4 + x] = b[x];
+      }
+    } else {
+      const i32x4_t a = *(const i32x4_t*)((const uint16_t*)p + i);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[x] = ns_from16((uint16_t)((uint32_t)a[x / 2] >> (16 * (x & 1))), dt);
+    }
+  } else {
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] = x >= n ? 0.f : dt == 2 ? ((const float*)p)[i + x] : ns_from16(((const uint16_t*)p)[i + x], dt);
+  }
+}
+template <bool VEC> TGG_DEV void ns_store8(void* p, int64_t i, int dt, const float (&v)[8], int n) {
+  if (VEC) {
+    if (dt == 2) {
+      *(f32x4_t*)((float*)p + i) = f32x4_t{v[0], v[1], v[2], v[3]};
+      *(f32x4_t*)((float*)p + i + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+    } else {
+      i32x4_t a;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) a[x] = (int)(dt == 0 ? pack2<DT_BF16>(v[2 * x], v[2 * x + 1]) : pack2<DT_F16>(v[2 * x], v[2 * x + 1]));
+      *(i32x4_t*)((uint16_t*)p + i) = a;
+    }
+  } else {
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      if (x < n) {
+        if (dt == 2) ((float*)p)[i + x] = v[x]; else ((uint16_t*)p)[i + x] = ns_to16(v[x], dt);
+      }
+  }
+}
+// n (up to 8) neighbouring results at element o; v in the planes' scale.  whole: all eight, aligned
+TGG_DEV void ns_store_result(const NsTarget& t, int64_t o, float (&v)[8], int n, bool whole) {
+  if (whole) {
+    float old[8];
+    if (t.weight) ns_load8<true>(old, t.out, o, t.dt, 8);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] = t.weight ? t.keep * old[x] - t.step * (v[x] * (1.f / kNsScale)) : v[x] * (1.f / kNsScale);
+    ns_store8<true>(t.out, o, t.dt, v, 8);
+  } else {
+    float old[8];
+    if (t.weight) ns_load8<false>(old, t.out, o, t.dt, n);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] = t.weight ? t.keep * old[x] - t.step * (v[x] * (1.f / kNsScale)) : v[x] * (1.f / kNsScale);
+    ns_store8<false>(t.out, o, t.dt, v, n);
+  }
+}
+
 template <class C, int MODE, bool PRECISE> struct NsProblem {
-  static constexpr bool B_KMAJOR = MODE != NS_UPDATE, SYM = MODE != NS_UPDATE;
+  static constexpr bool SYM = MODE <= NS_POLY, B_KMAJOR = SYM;
   static_assert(!SYM || C::BM == C::BN, "symmetric results have square tiles");
-  static constexpr int PITCH = C::TN * 32 + 16;  // staged strip of 16 rows: bytes between rows
-  static constexpr int STAGE_WAVE = 16 * PITCH;
-  static constexpr int SUMS_OFF = C::NWAVES * STAGE_WAVE;
-  static constexpr int SMEM_BYTES = C::EPI_OFF + SUMS_OFF + C::NWAVES * 4;
+  // The epilogue takes pieces of 16 rows x HC columns of the wave's block through the wave's staging: a multiply leaves a lane four columns of one row, and
+  // neighbouring lanes in different rows, of which every one is an access of its own (64 cycles an instruction; 256-row tiles spent 36 us there).  Staged, a lane has eight columns and
+  // four lanes 64 bytes of a row.
+  static constexpr int HC = C::TN >= 2 ? 32 : 16, PIECES = C::TN * 16 / HC, LPR = HC / 8;
+  // Bytes between rows: fp32 (16-byte pieces swizzled by the row, no padding: two workgroups of 128-row tiles have to fit a compute unit), 16 bits, 16 bits transposed.
+  static constexpr int PITCH = HC * 4, PITCH16 = HC * 2 + 16, PITCH_T = 48;
+  static constexpr int STAGE_WAVE = 16 * PITCH > HC * PITCH_T ? 16 * PITCH : HC * PITCH_T;
+  static constexpr int SMEM_BYTES = C::EPI_OFF + C::NWAVES * STAGE_WAVE;
+  static_assert(STAGE_WAVE >= 16 * PITCH16 && (C::BM != 128 || 2 * SMEM_BYTES <= 160 * 1024), "the staging's size");
+  static TGG_DEV int staged(int row, int piece) { return row * PITCH + ((piece ^ (row % (HC / 4))) << 4); }
 
   const NsProduct& p;
   StreamWalk walk;
@@ -129,103 +202,143 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
   }
   TGG_DEV void begin(int, f32x4_t (&)[C::TM][C::TN], const StreamPlace<C>&) const {}
 
+  // A piece of 16-bit values, eight columns of a row a lane, to out with rows and columns exchanged; row, col: the piece's first, `pitch` values between out's rows.  The
+  // transposing read hands a lane four rows of a column; through LDS again, two lanes have a column's 16 rows.
+  TGG_DEV void store_transposed(char* mine, const i32x4_t& v, uint16_t* out, int64_t pitch, int row, int col, int rows_end, int cols_end, int el) const {
+    const int l16 = el & 15, lg = el >> 4;
+    if (el < 16 * LPR) *(i32x4_t*)(mine + el / LPR * PITCH16 + el % LPR * 16) = v;
+    asm volatile("" : : : "memory");  // read as another type, by other lanes of the wave; its LDS operations complete in order
+    i16x4_t t[HC / 16];
+#pragma unroll
+    for (int j = 0; j < HC / 16; ++j) t[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr_t)(mine + (4 * lg + (l16 >> 2)) * PITCH16 + (16 * j + 4 * (l16 & 3)) * 2));
+    asm volatile("" : : : "memory");
+#pragma unroll
+    for (int j = 0; j < HC / 16; ++j) *(i16x4_t*)(mine + (16 * j + l16) * PITCH_T + lg * 8) = t[j];
+    asm volatile("" : : : "memory");
+    const int c = el >> 1, r = (el & 1) * 8;
+    if (c < HC && col + c < cols_end && row + r < rows_end) *(i32x4_t*)(out + (int64_t)(col + c) * pitch + row + r) = *(const i32x4_t*)(mine + c * PITCH_T + r * 2);
+    asm volatile("" : : : "memory");
+  }
+
+  TGG_DEV void store_planes(int64_t o, const uint32_t (&w)[8]) const {
+    i32x4_t hi, lo;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      hi[x] = (int)((w[2 * x] & 0xffffu) | w[2 * x + 1] << 16);
+      lo[x] = (int)(w[2 * x] >> 16 | (w[2 * x + 1] & 0xffff0000u));
+    }
+    *(i32x4_t*)(p.o_hi + o) = hi;
+    if (p.o_lo) *(i32x4_t*)(p.o_lo + o) = lo;
+  }
+
   TGG_DEV void epilogue(int id, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at, char* stage) const {
     int el = at.lane;
     asm volatile("" : "+v"(el));  // (addresses are made afresh per tile instead of living across the multiplies)
     const int l16 = el & 15, lg = el >> 4;
     const Place tile = locate(id);
-    const int m = tile.m, row0 = tile.row0, col0 = tile.col0;
+    const int m = tile.m;
+    const int64_t base = m * p.o_stride;
+    const int rbase = tile.row0 + at.wm0, cbase = tile.col0 + at.wn0;
+    const int rl = el / LPR, cl = el % LPR * 8;  // the lane's row and first column of a piece
+    // what the result adds to, some pieces ahead of its use: a wait for it is one for the stores before it too
+    constexpr int AHEAD = C::BM == 256 ? 4 : 2;
+    i32x4_t c_hi[AHEAD], c_lo[AHEAD];
+    auto fetch = [&](int q, int n) __attribute__((always_inline)) {
+      const int row = rbase + n / PIECES * 16 + rl, col = cbase + n % PIECES * HC + cl;
+      c_hi[q] = c_lo[q] = i32x4_t{0, 0, 0, 0};
+      if (el < 16 * LPR && row < p.rows && col < p.ldo) {
+        const int64_t o = base + (int64_t)row * p.ldo + col;
+        c_hi[q] = *(const i32x4_t*)(p.c_hi + o);
+        c_lo[q] = *(const i32x4_t*)(p.c_lo + o);
+      }
+    };
+    if (MODE != NS_GRAM) {
+#pragma unroll
+      for (int n = 0; n < AHEAD && n < C::TM * PIECES; ++n) fetch(n, n);
+    }
     const float inv_rows = 1.f / (float)p.rows;
     const float d = p.x_tiles ? ns_sum(p.x_sums + (int64_t)m * p.x_tiles, p.x_tiles) * inv_rows : inv_rows;
     const float e = MODE == NS_GRAM ? 0.f : ns_sum(p.a_sums + (int64_t)m * p.a_tiles, p.a_tiles) * inv_rows;
     // the result is f acc + g C, less h on the diagonal, all times kNsScale
-    const float f = (MODE == NS_POLY ? p.cc : 1.f) * kNsInv2;
-    const float g = MODE == NS_POLY ? p.cb + 2.f * p.cc * d : MODE == NS_UPDATE ? p.ca + p.cb * d + p.cc * d * d + p.cc * e : 0.f;
-    const float h = MODE == NS_GRAM ? d : MODE == NS_POLY ? p.cc * e : 0.f;
-    const int64_t base = m * p.o_stride;
-    const int rbase = row0 + at.wm0, cbase = col0 + at.wn0;
-    const bool mirror = SYM && row0 != col0;
+    const float f = (MODE == NS_POLY ? p.cc : 1.f) * kNsInv2 * kNsScale;
+    const float g = MODE == NS_POLY ? p.cb + 2.f * p.cc * d : !SYM ? p.ca + p.cb * d + p.cc * d * d + p.cc * e : 0.f;
+    const float h = (MODE == NS_GRAM ? d : MODE == NS_POLY ? p.cc * e : 0.f) * kNsScale;
+    const bool mirror = SYM && tile.row0 != tile.col0;
     char* const mine = stage + at.wave * STAGE_WAVE;
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i) {
-      const int row = rbase + 16 * i + l16;
-      uint2 hi[C::TN], lo[C::TN];
+    for (int n = 0; n < C::TM * PIECES; ++n) {
+      const int i = n / PIECES, half = n % PIECES;
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j) {
-        const int col = cbase + 16 * j + 4 * lg;
-        const bool there = row < p.rows && col < p.ldo;
-        const int64_t o = base + (int64_t)row * p.ldo + col;
-        uint2 ch = {0, 0}, cl = {0, 0};
-        if (MODE != NS_GRAM && there) {
-          ch = *(const uint2*)(p.c_hi + o);
-          cl = *(const uint2*)(p.c_lo + o);
-        }
-        float v[4];
+      for (int j = 0; j < HC / 16; ++j) *(f32x4_t*)(mine + staged(l16, 4 * j + lg)) = acc[i][half * (HC / 16) + j];
+      asm volatile("" : : : "memory");
+      const int row = rbase + 16 * i + rl, col = cbase + half * HC + cl;
+      float v[8];
+      {
+        const f32x4_t a = *(const f32x4_t*)(mine + staged(rl % 16, cl / 4)), b = *(const f32x4_t*)(mine + staged(rl % 16, cl / 4 + 1));
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          float c = 0.f;
-          if (MODE != NS_GRAM) {
-            const uint32_t wh = x < 2 ? ch.x : ch.y, wl = x < 2 ? cl.x : cl.y;
-            c = ns_f16((uint16_t)(wh >> (16 * (x & 1)))) + ns_f16((uint16_t)(wl >> (16 * (x & 1))));
-          }
-          const float r = f * kNsScale * acc[i][j][x] + g * c - (SYM && row == col + x ? h * kNsScale : 0.f);
-          v[x] = row < p.rows && col + x < p.cols ? r : 0.f;  // (what lies beyond is a sum of whatever the operands' next rows hold)
-          sum += v[x] * v[x];
-        }
-        uint16_t a[4], b[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const NsSplit s = ns_split(v[x]);
-          a[x] = s.hi;
-          b[x] = s.lo;
-        }
-        hi[j] = {(uint32_t)a[0] | (uint32_t)a[1] << 16, (uint32_t)a[2] | (uint32_t)a[3] << 16};
-        lo[j] = {(uint32_t)b[0] | (uint32_t)b[1] << 16, (uint32_t)b[2] | (uint32_t)b[3] << 16};
-        if (there) {
-          *(uint2*)(p.o_hi + o) = hi[j];
-          if (p.o_lo) *(uint2*)(p.o_lo + o) = lo[j];
+          v[x] = f * a[x];
+          v[4 + x] = f * b[x];
         }
       }
-      if (SYM && mirror) {
-        // transposed through LDS: rows of the mirrored tile are this strip's columns, 16 values of each
+      asm volatile("" : : : "memory");
+      const bool mine_too = LPR == 4 || el < 16 * LPR;
 #pragma unroll
-        for (int plane = 0; plane < 2; ++plane) {
-          uint16_t* const out = plane ? p.o_lo : p.o_hi;
-          if (out) {
+      for (int x = 0; x < 8; ++x) {
+        if (MODE != NS_GRAM) {
+          const uint32_t wh = (uint32_t)c_hi[n % AHEAD][x / 2] >> (16 * (x & 1)), wl = (uint32_t)c_lo[n % AHEAD][x / 2] >> (16 * (x & 1));
+          v[x] = __builtin_fmaf(g, ns_f16((uint16_t)wh) + ns_f16((uint16_t)wl), v[x]);
+        }
+        if (SYM && row == col + x) v[x] -= h;
+        v[x] = mine_too && row < p.rows && col + x < p.cols ? v[x] : 0.f;  // (what lies beyond is a sum of whatever the operands' next rows hold)
+        sum = __builtin_fmaf(v[x], v[x], sum);
+      }
+      if (MODE != NS_GRAM && n + AHEAD < C::TM * PIECES) fetch(n % AHEAD, n + AHEAD);
+      if constexpr (MODE == NS_LAST) {
+        const float by = 1.f / kNsScale;
+        if (p.tall) {  // 16-bit results only
+          i32x4_t w;
 #pragma unroll
-            for (int j = 0; j < C::TN; ++j) *(uint2*)(mine + l16 * PITCH + (16 * j + 4 * lg) * 2) = plane ? lo[j] : hi[j];
-            asm volatile("" : : : "memory");  // read as another type, by other lanes of the wave; its LDS operations complete in order
+          for (int x = 0; x < 4; ++x) w[x] = (int)(p.target.dt == 0 ? pack2<DT_BF16>(v[2 * x] * by, v[2 * x + 1] * by) : pack2<DT_F16>(v[2 * x] * by, v[2 * x + 1] * by));
+          store_transposed(mine, w, (uint16_t*)p.target.out + (int64_t)m * p.rows * p.cols, p.rows, rbase + 16 * i, cbase + half * HC, p.rows, p.cols, el);
+        } else if (mine_too && row < p.rows && col < p.cols) {
+          ns_store_result(p.target, ((int64_t)m * p.rows + row) * p.cols + col, v, min(8, p.cols - col), (p.cols & 7) == 0);
+        }
+      } else {
+        uint32_t w[8];  // both planes of a value
 #pragma unroll
-            for (int it = 0; it < (C::TN * 32 + 63) / 64; ++it) {
-              const int idx = it * 64 + el, c = idx >> 1, r0 = (idx & 1) * 8;  // 8 rows of column c
-              uint32_t w[4];
-#pragma unroll
-              for (int x = 0; x < 4; ++x)
-                w[x] = (uint32_t)*(const uint16_t*)(mine + (r0 + 2 * x) * PITCH + c * 2) | (uint32_t)*(const uint16_t*)(mine + (r0 + 2 * x + 1) * PITCH + c * 2) << 16;
-              const int orow = cbase + c, ocol = rbase + 16 * i + r0;
-              if (orow < p.cols && ocol < p.ldo) {
-                const i32x4_t q = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
-                *(i32x4_t*)(out + base + (int64_t)orow * p.ldo + ocol) = q;
-              }
-            }
-            asm volatile("" : : : "memory");
+        for (int x = 0; x < 8; ++x) {
+          const NsSplit q = ns_split(v[x]);
+          w[x] = (uint32_t)q.hi | (uint32_t)q.lo << 16;
+        }
+        if (mine_too && row < p.rows && col < p.ldo) store_planes(base + (int64_t)row * p.ldo + col, w);
+        if (SYM && mirror) {  // the same with rows and columns exchanged: a lane has eight rows of a column
+          if (mine_too) {
+            *(i32x4_t*)(mine + staged(rl, cl / 4)) = i32x4_t{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+            *(i32x4_t*)(mine + staged(rl, cl / 4 + 1)) = i32x4_t{(int)w[4], (int)w[5], (int)w[6], (int)w[7]};
           }
+          asm volatile("" : : : "memory");
+          const int c = el >> 1, r0 = (el & 1) * 8;
+          if (c < HC) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) w[x] = *(const uint32_t*)(mine + staged(r0 + x, c >> 2) + (c & 3) * 4);
+            if (cbase + half * HC + c < p.cols && rbase + 16 * i + r0 < p.ldo) store_planes(base + (int64_t)(cbase + half * HC + c) * p.ldo + rbase + 16 * i + r0, w);
+          }
+          asm volatile("" : : : "memory");
         }
       }
     }
-    if (MODE != NS_POLY) {
+    if (MODE == NS_GRAM || MODE == NS_UPDATE) {
       if (mirror) sum *= 2.f;
 #pragma unroll
       for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x, 64);
-      float* const sums = (float*)(stage + SUMS_OFF);
-      __syncthreads();  // the sums of the tile before have been read
-      if (el == 0) sums[at.wave] = sum;
+      if (el == 0) *(float*)mine = sum;  // (read before the next tile's epilogue: its slabs have barriers)
       __syncthreads();
       if (threadIdx.x == 0) {
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < C::NWAVES; ++w) s += sums[w];
+        for (int w = 0; w < C::NWAVES; ++w) s += *(const float*)(stage + w * STAGE_WAVE);
         p.o_sums[id] = s * kNsInv2;
       }
     }
@@ -242,10 +355,16 @@ template <class C, int MODE, bool PRECISE> __global__ __launch_bounds__(C::THREA
 
 constexpr int kNsThreads = 256, kNsChunk = 16384;  // values of a workgroup's sum of squares
 
-TGG_DEV float ns_load(const void* p, int64_t i, int dt) {  // dt 0 bf16, 1 fp16, 2 fp32
-  if (dt == 2) return ((const float*)p)[i];
-  const uint16_t h = ((const uint16_t*)p)[i];
-  return dt == 0 ? __builtin_bit_cast(float, (uint32_t)h << 16) : ns_f16(h);
+TGG_DEV void ns_store_planes(uint16_t* hi, uint16_t* lo, int64_t o, const float (&v)[8]) {
+  i32x4_t a, b;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const NsSplit s0 = ns_split(v[2 * x]), s1 = ns_split(v[2 * x + 1]);
+    a[x] = (int)((uint32_t)s0.hi | (uint32_t)s1.hi << 16);
+    b[x] = (int)((uint32_t)s0.lo | (uint32_t)s1.lo << 16);
+  }
+  *(i32x4_t*)(hi + o) = a;
+  *(i32x4_t*)(lo + o) = b;
 }
 
 // What is orthogonalised: x, or, with momentum, the momentum's value after this step and with Nesterov's look ahead.
@@ -255,25 +374,32 @@ struct NsSource {
   float beta, keep;  // keep = 1 - beta
   int nesterov, dt;
 };
-TGG_DEV float ns_direction(const NsSource& s, int64_t i, float m) {
-  const float x = ns_load(s.x, i, s.dt);
-  if (!s.momentum) return x;
-  return s.nesterov ? s.beta * m + s.keep * x : m;
+// eight values of the direction; `step`: the momentum takes its step
+template <bool VEC> TGG_DEV void ns_direction(float (&v)[8], const NsSource& s, int64_t i, int n, bool step) {
+  ns_load8<VEC>(v, s.x, i, s.dt, n);
+  if (!s.momentum) return;
+  float m[8];
+  ns_load8<VEC>(m, s.momentum, i, 2, n);
+  if (step) {
+#pragma unroll
+    for (int x = 0; x < 8; ++x) m[x] = s.beta * m[x] + s.keep * v[x];
+    ns_store8<VEC>(s.momentum, i, 2, m, n);
+  }
+#pragma unroll
+  for (int x = 0; x < 8; ++x) v[x] = s.nesterov ? s.beta * m[x] + s.keep * v[x] : m[x];
 }
 
-// Sums of squares of a matrix's chunks; with momentum, its step.
-__global__ __launch_bounds__(kNsThreads) void ns_norm_kernel(const NsSource s, int64_t values, int chunks, double* sums) {
+// Sums of squares of a matrix's chunks, in 64 bits (values far from 1 have no squares in fp32); with momentum, its step.  VEC: matrices are multiples of eight values.
+template <bool VEC> __global__ __launch_bounds__(kNsThreads) void ns_norm_kernel(const NsSource s, int64_t values, int chunks, double* sums) {
   const int m = blockIdx.x / chunks, c = blockIdx.x % chunks;
-  const int64_t first = m * values + (int64_t)c * kNsChunk, end = min(first + kNsChunk, (m + 1) * values);
+  const int64_t first = m * values + (int64_t)c * kNsChunk, end = lesser(first + kNsChunk, (m + 1) * values);
   double sum = 0.0;
-  for (int64_t i = first + threadIdx.x; i < end; i += kNsThreads) {
-    float mom = 0.f;
-    if (s.momentum) {
-      mom = s.beta * s.momentum[i] + s.keep * ns_load(s.x, i, s.dt);
-      s.momentum[i] = mom;
-    }
-    const double v = ns_direction(s, i, mom);
-    sum += v * v;
+#pragma unroll 2
+  for (int64_t i = first + threadIdx.x * 8; i < end; i += kNsThreads * 8) {
+    float v[8];
+    ns_direction<VEC>(v, s, i, (int)lesser(8, end - i), true);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) sum = __builtin_fma((double)v[x], (double)v[x], sum);
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
@@ -287,13 +413,22 @@ __global__ __launch_bounds__(kNsThreads) void ns_norm_kernel(const NsSource s, i
   }
 }
 
-// Tiles of 64 x 64 into the planes, transposed where the matrix is tall.
-__global__ __launch_bounds__(kNsThreads) void ns_load_kernel(const NsSource s, int rows, int cols, int tall, int chunks, const double* sums, float eps, uint16_t* hi, uint16_t* lo, int64_t stride,
-                                                             int ld, int tiles_r, int tiles_c) {
+// Tiles of 64 x 64 into the planes, transposed where the matrix is tall.  VEC: rows are multiples of eight values.
+template <bool VEC> __global__ __launch_bounds__(kNsThreads) void ns_load_kernel(const NsSource s, int rows, int cols, int tall, int chunks, const double* sums, float eps, uint16_t* hi, uint16_t* lo, int64_t stride,
+                                                                                 int ld, int tiles_r, int tiles_c) {
   __shared__ float tile[64][65];
   __shared__ double waves[kNsThreads / 64];
   const int per = tiles_r * tiles_c, m = blockIdx.x / per, t = blockIdx.x % per;
   const int r0 = t / tiles_c * 64, c0 = t % tiles_c * 64;
+  const int y0 = threadIdx.x >> 3, x0 = (threadIdx.x & 7) * 8;  // two rows of 32 apart, eight values each
+  float v[2][8];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int r = r0 + y0 + 32 * q, n = r < rows ? min(8, cols - c0 - x0) : 0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[q][x] = 0.f;
+    if (n > 0) ns_direction<VEC>(v[q], s, ((int64_t)m * rows + r) * cols + c0 + x0, n, false);
+  }
   double sum = 0.0;
   for (int i = threadIdx.x; i < chunks; i += kNsThreads) sum += sums[(int64_t)m * chunks + i];
 #pragma unroll
@@ -303,60 +438,78 @@ __global__ __launch_bounds__(kNsThreads) void ns_load_kernel(const NsSource s, i
   sum = 0.0;
   for (int w = 0; w < kNsThreads / 64; ++w) sum += waves[w];
   const float inv = (float)((double)kNsScale / (sqrt(sum) + (double)eps));
-  const int x = threadIdx.x & 63;
-  for (int y = threadIdx.x >> 6; y < 64; y += kNsThreads / 64) {
-    float v = 0.f;
-    if (r0 + y < rows && c0 + x < cols) {
-      const int64_t i = ((int64_t)m * rows + r0 + y) * cols + c0 + x;
-      v = ns_direction(s, i, s.momentum ? s.momentum[i] : 0.f) * inv;
-    }
-    tile[y][x] = v;
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[q][x] *= inv;
+  if (!tall) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (r0 + y0 + 32 * q < rows && c0 + x0 < ld) ns_store_planes(hi, lo, m * stride + (int64_t)(r0 + y0 + 32 * q) * ld + c0 + x0, v[q]);
+    return;
   }
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) tile[y0 + 32 * q][x0 + x] = v[q][x];
   __syncthreads();
-  const int o_rows = tall ? cols : rows, or0 = tall ? c0 : r0, oc0 = tall ? r0 : c0;
-  for (int y = threadIdx.x >> 6; y < 64; y += kNsThreads / 64) {
-    if (or0 + y < o_rows && oc0 + x < ld) {
-      const NsSplit v = ns_split(tall ? tile[x][y] : tile[y][x]);
-      const int64_t o = m * stride + (int64_t)(or0 + y) * ld + oc0 + x;
-      hi[o] = v.hi;
-      lo[o] = v.lo;
-    }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int r = c0 + y0 + 32 * q, c = r0 + x0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[q][x] = tile[x0 + x][y0 + 32 * q];
+    if (r < cols && c < ld) ns_store_planes(hi, lo, m * stride + (int64_t)r * ld + c, v[q]);
   }
 }
 
-// Out of the planes: out = v, or with `weight` out = keep out - step v.
-struct NsTarget {
-  void* out;
-  int dt, weight;
-  float keep, step;
-};
-__global__ __launch_bounds__(kNsThreads) void ns_store_kernel(const NsTarget o, int rows, int cols, int tall, const uint16_t* hi, const uint16_t* lo, int64_t stride, int ld, int tiles_r, int tiles_c) {
+// Out of the planes where the last step's update cannot: transposed results of more than 16 bits or with weights, odd ones, and those of no steps at all.
+template <bool VEC> __global__ __launch_bounds__(kNsThreads) void ns_store_kernel(const NsTarget o, int rows, int cols, int tall, const uint16_t* hi, const uint16_t* lo, int64_t stride, int ld, int tiles_r, int tiles_c) {
   __shared__ float tile[64][65];
   const int per = tiles_r * tiles_c, m = blockIdx.x / per, t = blockIdx.x % per;
   const int r0 = t / tiles_c * 64, c0 = t % tiles_c * 64;  // of the result
-  const int p_rows = tall ? cols : rows, p_cols = tall ? rows : cols, pr0 = tall ? c0 : r0, pc0 = tall ? r0 : c0;
-  const int x = threadIdx.x & 63;
-  for (int y = threadIdx.x >> 6; y < 64; y += kNsThreads / 64) {
-    float v = 0.f;
-    if (pr0 + y < p_rows && pc0 + x < p_cols) {
-      const int64_t i = m * stride + (int64_t)(pr0 + y) * ld + pc0 + x;
-      v = (ns_f16(hi[i]) + ns_f16(lo[i])) * (1.f / kNsScale);
+  const int p_rows = tall ? cols : rows, pr0 = tall ? c0 : r0, pc0 = tall ? r0 : c0;
+  const int y0 = threadIdx.x >> 3, x0 = (threadIdx.x & 7) * 8;
+  float v[2][8];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    i32x4_t a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+    if (pr0 + y0 + 32 * q < p_rows && pc0 + x0 < ld) {
+      const int64_t i = m * stride + (int64_t)(pr0 + y0 + 32 * q) * ld + pc0 + x0;
+      a = *(const i32x4_t*)(hi + i);
+      b = *(const i32x4_t*)(lo + i);
     }
-    if (tall) tile[x][y] = v; else tile[y][x] = v;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[q][x] = (ns_f16((uint16_t)((uint32_t)a[x / 2] >> (16 * (x & 1)))) + ns_f16((uint16_t)((uint32_t)b[x / 2] >> (16 * (x & 1))))) * (1.f / kNsScale);
   }
-  __syncthreads();
-  for (int y = threadIdx.x >> 6; y < 64; y += kNsThreads / 64) {
-    if (r0 + y >= rows || c0 + x >= cols) continue;
-    const int64_t i = ((int64_t)m * rows + r0 + y) * cols + c0 + x;
-    float v = tile[y][x];
-    if (o.weight) v = o.keep * ns_load(o.out, i, o.dt) - o.step * v;
-    if (o.dt == 2) ((float*)o.out)[i] = v;
-    else ((uint16_t*)o.out)[i] = o.dt == 0 ? Out16<DT_BF16>::cvt(v) : Out16<DT_F16>::cvt(v);
+  if (tall) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int x = 0; x < 8; ++x) tile[y0 + 32 * q][x0 + x] = v[q][x];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[q][x] = tile[x0 + x][y0 + 32 * q];
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int r = r0 + y0 + 32 * q, n = r < rows ? min(8, cols - c0 - x0) : 0;
+    if (n <= 0) continue;
+    const int64_t i = ((int64_t)m * rows + r) * cols + c0 + x0;
+    if (o.weight) {
+      float old[8];
+      ns_load8<VEC>(old, o.out, i, o.dt, n);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[q][x] = o.keep * old[x] - o.step * v[q][x];
+    }
+    ns_store8<VEC>(o.out, i, o.dt, v[q], n);
   }
 }
 
 typedef StreamCfg<256, 256, 2, 4> NsWide;
 typedef StreamCfg<128, 128, 2, 4> NsNarrow;
+typedef StreamCfg<64, 64, 2, 4, 8> NsSmall;
 
 template <class C, int MODE, bool PRECISE> int ns_launch(const NsProduct& p, hipStream_t s) {
   typedef NsProblem<C, MODE, PRECISE> P;
@@ -367,36 +520,44 @@ template <class C, int MODE, bool PRECISE> int ns_launch(const NsProduct& p, hip
   }
   const int tm = (p.rows + C::BM - 1) / C::BM, tn = (p.cols + C::BN - 1) / C::BN;
   const int64_t tiles = (int64_t)p.batch * (P::SYM ? tm * (tm + 1) / 2 : tm * tn);
-  const int slots = num_cus() * (C::BM == 128 ? 2 : 1);
+  const int slots = num_cus() * (int)(160 * 1024 / P::SMEM_BYTES);
   ns_product_kernel<C, MODE, PRECISE><<<dim3((unsigned)(tiles < slots ? tiles : slots)), dim3(C::THREADS), P::SMEM_BYTES, s>>>(p, tm, tn);
   return check_launch("ns_product");
 }
 
-template <int MODE> int ns_product(const NsProduct& p, bool wide, bool precise, hipStream_t s) {
-  if (wide) return precise ? ns_launch<NsWide, MODE, true>(p, s) : ns_launch<NsWide, MODE, false>(p, s);
+template <int MODE> int ns_product(const NsProduct& p, int tile, bool precise, hipStream_t s) {
+  if (tile == 64) return precise ? ns_launch<NsSmall, MODE, true>(p, s) : ns_launch<NsSmall, MODE, false>(p, s);
+  if (tile == 256) return precise ? ns_launch<NsWide, MODE, true>(p, s) : ns_launch<NsWide, MODE, false>(p, s);
   return precise ? ns_launch<NsNarrow, MODE, true>(p, s) : ns_launch<NsNarrow, MODE, false>(p, s);
 }
 
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 int64_t ns_align(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
 // Where everything is in the workspace, and how the products are tiled.
 struct NsPlan {
   int m, n, ldm, ldn, chunks;
-  bool tall, wide_gram, wide_poly, wide_update;
+  bool tall;
+  int gram_tile, poly_tile, update_tile;
   int gram_tiles, update_tiles;
   int64_t x_plane, g_plane;  // elements of a plane of all matrices
   int64_t off_x, off_a, off_b, off_sums, off_xs[2], off_as, bytes;
 };
 
-// Tiles of 256 or of 128: rounds of the compute units (two workgroups of the narrow tiles share one).  A quarter of a wide tile's work takes a narrow one about a third of its time.
-bool ns_wide(int64_t batch, int rows, int cols, bool sym) {
+// Tiles of 64, 128 or 256 for a product of `slabs` slabs of depth a tile: the estimated time in microseconds, from the rounds of workgroups and what a tile took.  A round of 256-row
+// tiles: 1.65 a slab and 24 for results and start; of two 128-row tiles a compute unit 1.2 and 10, of one 0.8 and 8; of one 64-row tile, with eight slabs in flight, 0.38 and 1.  Measured for stacks of
+// 1 to 64 matrices of 128 to 2048 rows, the choice was the fastest or within 3 % of it; the other tiles took 1.1 to 2.7 times as long (512 x 512: 136, 186 and 384 us in
+// tiles of 64, 128 and 256; 64 of 1536 x 2048: 22.7, 9.3 and 8.2 ms).
+int ns_tile(int64_t batch, int rows, int cols, bool sym, int64_t slabs) {
   auto tiles = [&](int b) { const int64_t tm = (rows + b - 1) / b, tn = (cols + b - 1) / b; return batch * (sym ? tm * (tm + 1) / 2 : tm * tn); };
-  const int64_t cus = num_cus();
-  const int64_t wide = (tiles(256) + cus - 1) / cus * 3, narrow = (tiles(128) + 2 * cus - 1) / (2 * cus) * 2;
-  return wide <= narrow;
+  const int64_t cus = num_cus(), full = tiles(128) / (2 * cus), rest = tiles(128) % (2 * cus);
+  const double pair = 1.2 * slabs + 10;
+  const double small = (tiles(64) + cus - 1) / cus * (0.38 * slabs + 1), wide = (tiles(256) + cus - 1) / cus * (1.65 * slabs + 24);
+  const double narrow = full * pair + (rest == 0 ? 0 : rest <= cus ? 0.8 * slabs + 8 : pair);
+  return small <= narrow && small <= wide ? 64 : narrow <= wide ? 128 : 256;
 }
 
-NsPlan ns_plan(int64_t batch, int rows, int cols) {
+NsPlan ns_plan(int64_t batch, int rows, int cols, bool precise) {
   NsPlan q;
   q.tall = rows > cols;
   q.m = q.tall ? cols : rows;
@@ -404,9 +565,11 @@ NsPlan ns_plan(int64_t batch, int rows, int cols) {
   q.ldm = (q.m + 7) & ~7;
   q.ldn = (q.n + 7) & ~7;
   q.chunks = (int)(((int64_t)rows * cols + kNsChunk - 1) / kNsChunk);
-  q.wide_gram = q.wide_poly = ns_wide(batch, q.m, q.m, true);
-  q.wide_update = ns_wide(batch, q.m, q.n, false);
-  const int bg = q.wide_gram ? 256 : 128, bu = q.wide_update ? 256 : 128;
+  const int passes = precise ? 3 : 1, deep = (q.n + 63) / 64 * passes, shallow = (q.m + 63) / 64 * passes;
+  q.gram_tile = ns_tile(batch, q.m, q.m, true, deep);
+  q.poly_tile = ns_tile(batch, q.m, q.m, true, shallow);
+  q.update_tile = ns_tile(batch, q.m, q.n, false, shallow);
+  const int bg = q.gram_tile, bu = q.update_tile;
   const int tg = (q.m + bg - 1) / bg;
   q.gram_tiles = tg * (tg + 1) / 2;
   q.update_tiles = ((q.m + bu - 1) / bu) * ((q.n + bu - 1) / bu);
@@ -428,12 +591,13 @@ NsPlan ns_plan(int64_t batch, int rows, int cols) {
 
 }  // namespace
 
-int64_t newton_schulz_workspace(int64_t batch, int rows, int cols) { return ns_plan(batch, rows, cols).bytes; }
+int64_t newton_schulz_workspace(int64_t batch, int rows, int cols) { return larger(ns_plan(batch, rows, cols, false).bytes, ns_plan(batch, rows, cols, true).bytes); }
 
 // x -> out, or with momentum the weights' step on out.  dt: 0 bf16, 1 fp16, 2 fp32
 int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, int nesterov, void* out, int out_dt, int weight, float keep, float step, int64_t batch, int rows, int cols, int steps,
                          float ca, float cb, float cc, float eps, void* workspace, hipStream_t s) {
-  const NsPlan q = ns_plan(batch, rows, cols);
+  const bool precise = out_dt != 0;  // results of more than 8 bits
+  const NsPlan q = ns_plan(batch, rows, cols, precise);
   char* const ws = (char*)workspace;
   const int64_t xp = ns_align(q.x_plane * 2), gp = ns_align(q.g_plane * 2);
   uint16_t* xs[2][2] = {{(uint16_t*)(ws + q.off_x), (uint16_t*)(ws + q.off_x + xp)}, {(uint16_t*)(ws + q.off_x + 2 * xp), (uint16_t*)(ws + q.off_x + 3 * xp)}};
@@ -441,14 +605,21 @@ int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, i
   double* sums = (double*)(ws + q.off_sums);
   float* const x_sums[2] = {(float*)(ws + q.off_xs[0]), (float*)(ws + q.off_xs[1])};
   float* const a_sums = (float*)(ws + q.off_as);
-  const bool precise = out_dt != 0;  // results of more than 8 bits
   const NsSource src = {x, momentum, beta, 1.f - beta, nesterov, x_dt};
-  ns_norm_kernel<<<dim3((unsigned)(batch * q.chunks)), dim3(kNsThreads), 0, s>>>(src, (int64_t)rows * cols, q.chunks, sums);
+  const bool vec_in = ((int64_t)rows * cols & 7) == 0 && aligned16(x) && aligned16(momentum), vec_rows = (cols & 7) == 0;
+  const dim3 threads(kNsThreads), norm_grid((unsigned)(batch * q.chunks));
+  if (vec_in) ns_norm_kernel<true><<<norm_grid, threads, 0, s>>>(src, (int64_t)rows * cols, q.chunks, sums);
+  else ns_norm_kernel<false><<<norm_grid, threads, 0, s>>>(src, (int64_t)rows * cols, q.chunks, sums);
   if (int e = check_launch("ns_norm")) return e;
   // tiles cover the planes' padding too: columns up to a multiple of 8
   const int tr = ((q.tall ? q.ldn : rows) + 63) / 64, tc = ((q.tall ? cols : q.ldn) + 63) / 64;
-  ns_load_kernel<<<dim3((unsigned)(batch * tr * tc)), dim3(kNsThreads), 0, s>>>(src, rows, cols, q.tall, q.chunks, sums, eps, xs[0][0], xs[0][1], (int64_t)q.m * q.ldn, q.ldn, tr, tc);
+  const dim3 load_grid((unsigned)(batch * tr * tc));
+  if (vec_in && vec_rows) ns_load_kernel<true><<<load_grid, threads, 0, s>>>(src, rows, cols, q.tall, q.chunks, sums, eps, xs[0][0], xs[0][1], (int64_t)q.m * q.ldn, q.ldn, tr, tc);
+  else ns_load_kernel<false><<<load_grid, threads, 0, s>>>(src, rows, cols, q.tall, q.chunks, sums, eps, xs[0][0], xs[0][1], (int64_t)q.m * q.ldn, q.ldn, tr, tc);
   if (int e = check_launch("ns_load")) return e;
+  const NsTarget dst = {out, out_dt, weight, keep, step};
+  // the last step's update writes rows of the result; transposed ones if they are plain 16-bit values in whole eights
+  const bool direct = steps > 0 && (q.tall ? !weight && out_dt != 2 && (q.m & 7) == 0 && aligned16(out) : aligned16(out));
   const int64_t xstride = (int64_t)q.m * q.ldn, gstride = (int64_t)q.m * q.ldm;
   for (int i = 0; i < steps; ++i) {
     uint16_t **from = xs[i & 1], **to = xs[(i + 1) & 1];
@@ -463,21 +634,25 @@ int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, i
     p.a_hi = p.b_hi = from[0]; p.a_lo = p.b_lo = from[1];
     p.lda = p.ldb = q.ldn; p.a_stride = p.b_stride = xstride;
     p.o_hi = a_hi; p.o_lo = a_lo; p.ldo = q.ldm; p.o_stride = gstride; p.o_sums = a_sums;
-    if (int e = ns_product<NS_GRAM>(p, q.wide_gram, precise, s)) return e;
+    if (int e = ns_product<NS_GRAM>(p, q.gram_tile, precise, s)) return e;
     p.depth = q.m;
     p.a_hi = p.b_hi = p.c_hi = a_hi; p.a_lo = p.b_lo = p.c_lo = a_lo;
     p.lda = p.ldb = q.ldm; p.a_stride = p.b_stride = gstride;
     p.o_hi = b_hi; p.o_lo = precise ? b_lo : nullptr; p.o_sums = nullptr;
-    if (int e = ns_product<NS_POLY>(p, q.wide_poly, precise, s)) return e;
+    if (int e = ns_product<NS_POLY>(p, q.poly_tile, precise, s)) return e;
     p.cols = q.n;
     p.a_hi = b_hi; p.a_lo = b_lo;
     p.b_hi = p.c_hi = from[0]; p.b_lo = p.c_lo = from[1]; p.ldb = q.ldn; p.b_stride = xstride;
     p.o_hi = to[0]; p.o_lo = to[1]; p.ldo = q.ldn; p.o_stride = xstride; p.o_sums = x_sums[(i + 1) & 1];
-    if (int e = ns_product<NS_UPDATE>(p, q.wide_update, precise, s)) return e;
+    p.target = dst;
+    p.tall = q.tall;
+    if (direct && i == steps - 1) return ns_product<NS_LAST>(p, q.update_tile, precise, s);
+    if (int e = ns_product<NS_UPDATE>(p, q.update_tile, precise, s)) return e;
   }
-  const NsTarget dst = {out, out_dt, weight, keep, step};
   const int sr = (rows + 63) / 64, sc = (cols + 63) / 64;
-  ns_store_kernel<<<dim3((unsigned)(batch * sr * sc)), dim3(kNsThreads), 0, s>>>(dst, rows, cols, q.tall, xs[steps & 1][0], xs[steps & 1][1], xstride, q.ldn, sr, sc);
+  const dim3 store_grid((unsigned)(batch * sr * sc));
+  if (vec_rows && aligned16(out)) ns_store_kernel<true><<<store_grid, threads, 0, s>>>(dst, rows, cols, q.tall, xs[steps & 1][0], xs[steps & 1][1], xstride, q.ldn, sr, sc);
+  else ns_store_kernel<false><<<store_grid, threads, 0, s>>>(dst, rows, cols, q.tall, xs[steps & 1][0], xs[steps & 1][1], xstride, q.ldn, sr, sc);
   return check_launch("ns_store");
 }
 

@@ -1,7 +1,7 @@
 // Main loop of the 16-bit products of newton_schulz.hip and lora.hip: a workgroup's tiles as one uninterrupted stream of 64-deep slabs.
 //
-// The scheme is that of the eight-wave kernels (gemm_fast.hip): eight waves, two slab buffers in LDS filled by direct copies that run two slabs
-// ahead across tile boundaries, fragment reads a K step ahead across the one barrier a slab, copies issued between multiplies.  What differs is
+// The scheme is that of the eight-wave kernels (gemm_fast.hip): eight waves, a ring of slab buffers in LDS (two, more for small tiles, whose slabs take less time than
+// their copies) filled by direct copies that run that many slabs ahead across tile boundaries, fragment reads a K step ahead across the one barrier a slab, copies issued between multiplies.  What differs is
 // who says what a slab is: a problem P hands out slabs one after another, so a tile may add up products of several pairs of operands
 // (a matrix's two planes, a row's shared projection and its adapters), and takes a tile's sums.  P has
 //
@@ -19,13 +19,18 @@
 
 namespace tgg {
 
-template <int BM_, int BN_, int WM_, int WN_> struct StreamCfg {
+// (min and max of two 64-bit numbers: the runtime's own are for 32-bit ones in host code and cut them off)
+__host__ __device__ constexpr int64_t lesser(int64_t a, int64_t b) { return a < b ? a : b; }
+__host__ __device__ constexpr int64_t larger(int64_t a, int64_t b) { return a < b ? b : a; }
+
+template <int BM_, int BN_, int WM_, int WN_, int RING_ = 2> struct StreamCfg {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int RING = RING_;
   static constexpr int NWAVES = WM * WN, THREADS = NWAVES * 64;
   static constexpr int A_BYTES = BM * kSlabRowBytes, B_BYTES = BN * kSlabRowBytes, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int CA = A_BYTES / 1024 / NWAVES, CB = B_BYTES / 1024 / NWAVES, NC = CA + CB;  // copies of a wave and slab
   static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-  static constexpr int EPI_OFF = 2 * STAGE_BYTES;
+  static constexpr int EPI_OFF = RING * STAGE_BYTES;
   static_assert(CA * NWAVES * 1024 == A_BYTES && CB * NWAVES * 1024 == B_BYTES, "copies must divide evenly over waves");
   static_assert(NWAVES == 8, "a wave keeps one swizzle pattern for all its copies");
   static_assert(NC % 2 == 0 && TM % 2 == 0 && (TM * TN / 2) % (NC / 2) == 0, "a slab's copies are spread over the multiplies of two half K steps");
@@ -175,25 +180,28 @@ template <class C, int DT, bool B_KMAJOR, class P> TGG_DEV void stream_gemm(P& p
   uint32_t sc_base = 0, sc_next_base = 0;
   auto copy_k = [&](int k) __attribute__((always_inline)) {
     if (k < C::CA) {
-      copy_b128_to_lds(sc.ra, sc_base + (at.wave + k * C::NWAVES) * 1024, prob.cur.va[k]);
+      copy_b128_to_lds(sc.ra, __builtin_amdgcn_readfirstlane(sc_base + (at.wave + k * C::NWAVES) * 1024), prob.cur.va[k]);
     } else {
-      copy_b128_to_lds(sc.rb, sc_base + C::A_BYTES + (at.wave + (k - C::CA) * C::NWAVES) * 1024, prob.cur.vb[k - C::CA]);
+      copy_b128_to_lds(sc.rb, __builtin_amdgcn_readfirstlane(sc_base + C::A_BYTES + (at.wave + (k - C::CA) * C::NWAVES) * 1024), prob.cur.vb[k - C::CA]);
     }
   };
 
   prob.seek(prob.tile_at(0));
-  stream_next(prob, sc);
-  sc_base = smem_addr;
 #pragma unroll
-  for (int k = 0; k < C::NC; ++k) copy_k(k);
-  wait_vmcnt<0>();
+  for (int q = 0; q < C::RING - 1; ++q) {
+    stream_next(prob, sc);
+    sc_base = smem_addr + q * C::STAGE_BYTES;
+#pragma unroll
+    for (int k = 0; k < C::NC; ++k) copy_k(k);
+  }
+  wait_vmcnt<(C::RING - 2) * C::NC>();
   __syncthreads();
   stream_next(prob, sc);
-  sc_base = smem_addr + C::STAGE_BYTES;
+  sc_base = smem_addr + (C::RING - 1) * C::STAGE_BYTES;
 #pragma unroll
   for (int k = 0; k < C::NC / 2; ++k) copy_k(k);
   i32x4_t fa[C::TM - 1], fa_last[2], fb[2][C::TN];
-  int ring = 0;
+  int ring = 0;  // the buffer of the slab that is multiplied
 
   f32x4_t acc[C::TM][C::TN];
   for (int pos = 0, id; (id = prob.tile_at(pos)) >= 0; ++pos) {
@@ -205,7 +213,7 @@ template <class C, int DT, bool B_KMAJOR, class P> TGG_DEV void stream_gemm(P& p
     prob.begin(id, acc, at);
     // The first slab's first fragments.  (The slab before has read them already, if this is not the first tile: read again, their registers are free for begin() and epilogue().)
     {
-      const char* s = smem + (ring & 1) * C::STAGE_BYTES;
+      const char* s = smem + ring * C::STAGE_BYTES;
 #pragma unroll
       for (int i = 0; i < C::TM - 1; ++i) fa[i] = load_a(s, 0, i);
       fa_last[0] = load_a(s, 0, C::TM - 1);
@@ -237,9 +245,9 @@ template <class C, int DT, bool B_KMAJOR, class P> TGG_DEV void stream_gemm(P& p
             }
             __builtin_amdgcn_sched_barrier(0);
           }
-          if (prepare && n == 1) {  // scalar work, under the multiplies just issued
+          if (prepare && n == (HM * C::TN > 1 ? 1 : 0)) {  // scalar work, under the multiplies just issued
             stream_next(prob, sc_next);
-            sc_next_base = smem_addr + (ring & 1) * C::STAGE_BYTES;
+            sc_next_base = smem_addr + ring * C::STAGE_BYTES;
           }
           const int sp = k0 == 0 ? SP1 : SP2;
           if (k0 >= 0 && (n + 1) % sp == 0 && (n + 1) / sp <= C::NC / 2) {
@@ -257,17 +265,18 @@ template <class C, int DT, bool B_KMAJOR, class P> TGG_DEV void stream_gemm(P& p
       __builtin_amdgcn_sched_barrier(0);
     };
     for (int kt = 0; kt < slabs; ++kt) {
-      const char* s = smem + (ring & 1) * C::STAGE_BYTES;
-      const char* sn = smem + ((ring + 1) & 1) * C::STAGE_BYTES;
+      const char* s = smem + ring * C::STAGE_BYTES;
+      const int next = ring + 1 == C::RING ? 0 : ring + 1;
+      const char* sn = smem + next * C::STAGE_BYTES;
       half(0, 0, s, 1, READ_EARLY, C::NC / 2);
       half(0, 1, s, 1, READ_ROLL, -1, true);
       half(1, 0, sn, 0, READ_NONE, -1);
-      wait_vmcnt<0>();
+      wait_vmcnt<(C::RING - 2) * C::NC>();  // the next slab is there; those behind it may be on their way
       __syncthreads();
       sc = sc_next;
       sc_base = sc_next_base;
       half(1, 1, sn, 0, READ_CATCH_UP, 0);
-      ++ring;
+      ring = next;
     }
     prob.epilogue(id, acc, at, smem + C::EPI_OFF);
   }
