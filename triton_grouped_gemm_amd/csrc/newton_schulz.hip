@@ -127,8 +127,17 @@ TGG_DEV void ns_store_result(const NsTarget& t, int64_t o, float (&v)[8], int n,
   }
 }
 
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
+TGG_DEV rsrc_t ns_window(const void* base, int64_t bytes) {
+  bytes = bytes < 0 ? 0 : (bytes > 0x3fffffff ? 0x3fffffff : bytes);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)uniform64((uint64_t)base), 0, __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
+}
+constexpr int kNowhere = 0x40000000;  // beyond every window, also with a tile's rows added
+
 template <class C, int MODE, bool PRECISE> struct NsProblem {
   static constexpr bool SYM = MODE <= NS_POLY, B_KMAJOR = SYM;
+  static constexpr bool C_LO = MODE >= NS_UPDATE || PRECISE, O_LO = MODE == NS_UPDATE || PRECISE;  // whether what is added, and the result, have a low plane
   static_assert(!SYM || C::BM == C::BN, "symmetric results have square tiles");
   // The epilogue takes pieces of 16 rows x HC columns of the wave's block through the wave's staging: a multiply leaves a lane four columns of one row, and
   // neighbouring lanes in different rows, of which every one is an access of its own (64 cycles an instruction; 256-row tiles spent 36 us there).  Staged, a lane has eight columns and
@@ -220,17 +229,6 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
     asm volatile("" : : : "memory");
   }
 
-  TGG_DEV void store_planes(int64_t o, const uint32_t (&w)[8]) const {
-    i32x4_t hi, lo;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      hi[x] = (int)((w[2 * x] & 0xffffu) | w[2 * x + 1] << 16);
-      lo[x] = (int)(w[2 * x] >> 16 | (w[2 * x + 1] & 0xffff0000u));
-    }
-    *(i32x4_t*)(p.o_hi + o) = hi;
-    if (p.o_lo) *(i32x4_t*)(p.o_lo + o) = lo;
-  }
-
   TGG_DEV void epilogue(int id, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at, char* stage) const {
     int el = at.lane;
     asm volatile("" : "+v"(el));  // (addresses are made afresh per tile instead of living across the multiplies)
@@ -240,21 +238,26 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
     const int64_t base = m * p.o_stride;
     const int rbase = tile.row0 + at.wm0, cbase = tile.col0 + at.wn0;
     const int rl = el / LPR, cl = el % LPR * 8;  // the lane's row and first column of a piece
+    const bool mine_too = LPR == 4 || el < 16 * LPR;
+    // Planes are reached through windows that begin at the tile's first row (the mirrored tile's: its first column) and end with the matrix's last: what lies below reads as zeros and is not
+    // written.  Columns to the right of a row are nowhere.
+    auto rows_of = [&](const uint16_t* plane, int first, int rows) __attribute__((always_inline)) { return ns_window(plane + base + (int64_t)first * p.ldo, (int64_t)lesser(rows, p.rows - first) * p.ldo * 2); };
+    const rsrc_t o_hi = rows_of(p.o_hi, tile.row0, C::BM), o_lo = rows_of(p.o_lo, tile.row0, O_LO ? C::BM : 0);
+    const rsrc_t c_hi_w = rows_of(p.c_hi, tile.row0, MODE != NS_GRAM ? C::BM : 0), c_lo_w = rows_of(p.c_lo, tile.row0, MODE != NS_GRAM && C_LO ? C::BM : 0);
+    const int pitch = p.ldo * 2;
+    int lane_at[PIECES];
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) lane_at[q] = mine_too && cbase + q * HC + cl < p.ldo ? (at.wm0 + rl) * pitch + (cbase + q * HC + cl) * 2 : kNowhere;
     // what the result adds to, some pieces ahead of its use: a wait for it is one for the stores before it too
     constexpr int AHEAD = C::BM == 256 ? 4 : 2;
     i32x4_t c_hi[AHEAD], c_lo[AHEAD];
-    auto fetch = [&](int q, int n) __attribute__((always_inline)) {
-      const int row = rbase + n / PIECES * 16 + rl, col = cbase + n % PIECES * HC + cl;
-      c_hi[q] = c_lo[q] = i32x4_t{0, 0, 0, 0};
-      if (el < 16 * LPR && row < p.rows && col < p.ldo) {
-        const int64_t o = base + (int64_t)row * p.ldo + col;
-        c_hi[q] = *(const i32x4_t*)(p.c_hi + o);
-        c_lo[q] = *(const i32x4_t*)(p.c_lo + o);
-      }
+    auto fetch = [&](int n) __attribute__((always_inline)) {
+      c_hi[n % AHEAD] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(c_hi_w, lane_at[n % PIECES] + n / PIECES * 16 * pitch, 0, 0));
+      if (C_LO) c_lo[n % AHEAD] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(c_lo_w, lane_at[n % PIECES] + n / PIECES * 16 * pitch, 0, 0));
     };
     if (MODE != NS_GRAM) {
 #pragma unroll
-      for (int n = 0; n < AHEAD && n < C::TM * PIECES; ++n) fetch(n, n);
+      for (int n = 0; n < AHEAD && n < C::TM * PIECES; ++n) fetch(n);
     }
     const float inv_rows = 1.f / (float)p.rows;
     const float d = p.x_tiles ? ns_sum(p.x_sums + (int64_t)m * p.x_tiles, p.x_tiles) * inv_rows : inv_rows;
@@ -263,7 +266,10 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
     const float f = (MODE == NS_POLY ? p.cc : 1.f) * kNsInv2 * kNsScale;
     const float g = MODE == NS_POLY ? p.cb + 2.f * p.cc * d : !SYM ? p.ca + p.cb * d + p.cc * d * d + p.cc * e : 0.f;
     const float h = (MODE == NS_GRAM ? d : MODE == NS_POLY ? p.cc * e : 0.f) * kNsScale;
-    const bool mirror = SYM && tile.row0 != tile.col0;
+    const bool diagonal = SYM && tile.row0 == tile.col0, edge = tile.row0 + C::BM > p.rows || tile.col0 + C::BN > p.cols || LPR != 4;
+    const rsrc_t m_hi = rows_of(p.o_hi, tile.col0, SYM ? C::BN : 0), m_lo = rows_of(p.o_lo, tile.col0, SYM && O_LO ? C::BN : 0);
+    const int c_row = el >> 1, r0 = (el & 1) * 8;  // of the mirrored piece
+    const int mirror_at = c_row < HC ? (at.wn0 + c_row) * pitch + (rbase + r0) * 2 : kNowhere;
     char* const mine = stage + at.wave * STAGE_WAVE;
     float sum = 0.f;
 #pragma unroll
@@ -283,18 +289,28 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
         }
       }
       asm volatile("" : : : "memory");
-      const bool mine_too = LPR == 4 || el < 16 * LPR;
+      if (MODE != NS_GRAM) {
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        if (MODE != NS_GRAM) {
-          const uint32_t wh = (uint32_t)c_hi[n % AHEAD][x / 2] >> (16 * (x & 1)), wl = (uint32_t)c_lo[n % AHEAD][x / 2] >> (16 * (x & 1));
-          v[x] = __builtin_fmaf(g, ns_f16((uint16_t)wh) + ns_f16((uint16_t)wl), v[x]);
+        for (int x = 0; x < 8; ++x) {
+          const int h2 = c_hi[n % AHEAD][x / 2], l2 = C_LO ? c_lo[n % AHEAD][x / 2] : 0;  // (a bit cast of a vector's element takes the first one)
+          const f16x2_t hi = __builtin_bit_cast(f16x2_t, h2), lo = __builtin_bit_cast(f16x2_t, l2);
+          if (C_LO) v[x] = __builtin_fmaf((float)lo[x & 1], g, v[x]);
+          v[x] = __builtin_fmaf((float)hi[x & 1], g, v[x]);
         }
-        if (SYM && row == col + x) v[x] -= h;
-        v[x] = mine_too && row < p.rows && col + x < p.cols ? v[x] : 0.f;  // (what lies beyond is a sum of whatever the operands' next rows hold)
-        sum = __builtin_fmaf(v[x], v[x], sum);
+        if (n + AHEAD < C::TM * PIECES) fetch(n + AHEAD);
       }
-      if (MODE != NS_GRAM && n + AHEAD < C::TM * PIECES) fetch(n % AHEAD, n + AHEAD);
+      if (diagonal) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] -= row == col + x ? h : 0.f;
+      }
+      if (edge) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = mine_too && row < p.rows && col + x < p.cols ? v[x] : 0.f;  // (what lies beyond is a sum of whatever the operands' next rows hold)
+      }
+      if (MODE == NS_GRAM || MODE == NS_UPDATE) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) sum = __builtin_fmaf(v[x], v[x], sum);
+      }
       if constexpr (MODE == NS_LAST) {
         const float by = 1.f / kNsScale;
         if (p.tall) {  // 16-bit results only
@@ -303,34 +319,47 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
           for (int x = 0; x < 4; ++x) w[x] = (int)(p.target.dt == 0 ? pack2<DT_BF16>(v[2 * x] * by, v[2 * x + 1] * by) : pack2<DT_F16>(v[2 * x] * by, v[2 * x + 1] * by));
           store_transposed(mine, w, (uint16_t*)p.target.out + (int64_t)m * p.rows * p.cols, p.rows, rbase + 16 * i, cbase + half * HC, p.rows, p.cols, el);
         } else if (mine_too && row < p.rows && col < p.cols) {
-          ns_store_result(p.target, ((int64_t)m * p.rows + row) * p.cols + col, v, min(8, p.cols - col), (p.cols & 7) == 0);
+          ns_store_result(p.target, ((int64_t)m * p.rows + row) * p.cols + col, v, (int)lesser(8, p.cols - col), (p.cols & 7) == 0);
         }
       } else {
-        uint32_t w[8];  // both planes of a value
+        i32x4_t hi, lo;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const NsSplit q = ns_split(v[x]);
-          w[x] = (uint32_t)q.hi | (uint32_t)q.lo << 16;
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t q = pack2<DT_F16>(v[2 * x], v[2 * x + 1]);
+          const f16x2_t r = __builtin_bit_cast(f16x2_t, q);
+          hi[x] = (int)q;
+          lo[x] = (int)pack2<DT_F16>(v[2 * x] - (float)r[0], v[2 * x + 1] - (float)r[1]);
         }
-        if (mine_too && row < p.rows && col < p.ldo) store_planes(base + (int64_t)row * p.ldo + col, w);
-        if (SYM && mirror) {  // the same with rows and columns exchanged: a lane has eight rows of a column
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, hi), o_hi, lane_at[half] + i * 16 * pitch, 0, 0);
+        if (O_LO) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, lo), o_lo, lane_at[half] + i * 16 * pitch, 0, 0);
+        if (SYM && !diagonal) {  // the same with rows and columns exchanged: both planes of a value in a word, a lane reads eight rows of a column
+          uint32_t w[8];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            w[2 * x] = ((uint32_t)hi[x] & 0xffffu) | (uint32_t)lo[x] << 16;
+            w[2 * x + 1] = (uint32_t)hi[x] >> 16 | ((uint32_t)lo[x] & 0xffff0000u);
+          }
           if (mine_too) {
             *(i32x4_t*)(mine + staged(rl, cl / 4)) = i32x4_t{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
             *(i32x4_t*)(mine + staged(rl, cl / 4 + 1)) = i32x4_t{(int)w[4], (int)w[5], (int)w[6], (int)w[7]};
           }
           asm volatile("" : : : "memory");
-          const int c = el >> 1, r0 = (el & 1) * 8;
-          if (c < HC) {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) w[x] = *(const uint32_t*)(mine + staged(r0 + x, c >> 2) + (c & 3) * 4);
-            if (cbase + half * HC + c < p.cols && rbase + 16 * i + r0 < p.ldo) store_planes(base + (int64_t)(cbase + half * HC + c) * p.ldo + rbase + 16 * i + r0, w);
+          for (int x = 0; x < 8; ++x) w[x] = *(const uint32_t*)(mine + staged(r0 + x, c_row % HC >> 2) + (c_row & 3) * 4);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            hi[x] = (int)((w[2 * x] & 0xffffu) | w[2 * x + 1] << 16);
+            lo[x] = (int)(w[2 * x] >> 16 | (w[2 * x + 1] & 0xffff0000u));
           }
+          const int o = rbase + 16 * i + r0 < p.ldo ? mirror_at + half * HC * pitch + i * 32 : kNowhere;
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, hi), m_hi, o, 0, 0);
+          if (O_LO) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, lo), m_lo, o, 0, 0);
           asm volatile("" : : : "memory");
         }
       }
     }
     if (MODE == NS_GRAM || MODE == NS_UPDATE) {
-      if (mirror) sum *= 2.f;
+      if (SYM && !diagonal) sum *= 2.f;
 #pragma unroll
       for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x, 64);
       if (el == 0) *(float*)mine = sum;  // (read before the next tile's epilogue: its slabs have barriers)
@@ -633,7 +662,7 @@ int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, i
     p.depth = q.n;
     p.a_hi = p.b_hi = from[0]; p.a_lo = p.b_lo = from[1];
     p.lda = p.ldb = q.ldn; p.a_stride = p.b_stride = xstride;
-    p.o_hi = a_hi; p.o_lo = a_lo; p.ldo = q.ldm; p.o_stride = gstride; p.o_sums = a_sums;
+    p.o_hi = a_hi; p.o_lo = precise ? a_lo : nullptr; p.ldo = q.ldm; p.o_stride = gstride; p.o_sums = a_sums;
     if (int e = ns_product<NS_GRAM>(p, q.gram_tile, precise, s)) return e;
     p.depth = q.m;
     p.a_hi = p.b_hi = p.c_hi = a_hi; p.a_lo = p.b_lo = p.c_lo = a_lo;
