@@ -239,6 +239,46 @@ PyObject* m_grouped_gemm_int4(PyObject*, PyObject* const* args, Py_ssize_t nargs
   END_HANDLE_TH_ERRORS
 }
 
+// (x, weight, lora_a, lora_b, adapters, scales or None) -> out
+PyObject* lora_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TGG_ARGS(6);
+  TGG_TENSOR(x, 0);
+  TGG_TENSOR(w, 1);
+  TGG_TENSOR(a, 2);
+  TGG_TENSOR(b, 3);
+  TGG_TENSOR(ids, 4);
+  const at::Tensor* scales = nullptr;
+  if (args[5] != Py_None) {
+    scales = plain(args[5], device);
+    if (!scales) Py_RETURN_NONE;
+  }
+  if (x.dim() != 2 || w.dim() != 2 || a.dim() != 3 || b.dim() != 3 || records(x) || records(w) || records(a) || records(b) || (scales && records(*scales))) Py_RETURN_NONE;
+  const int64_t m = x.size(0), k = x.size(1), n = w.size(0), l = a.size(0), r = a.size(1);
+  const int dt = code16(x);
+  if (dt < 0 || w.scalar_type() != x.scalar_type() || a.scalar_type() != x.scalar_type() || b.scalar_type() != x.scalar_type() || m == 0 || w.size(1) != k || a.size(2) != k ||
+      b.size(0) != l || b.size(1) != n || b.size(2) != r || n < 8 || k < 8 || (n & 7) || (k & 7) || n > 65536 || k > 65536 || r < 8 || r > 128 || (r & 7) || l < 1 || l > kMaxGroups ||
+      !sizes_ok(ids, m) || !x.is_contiguous() || !w.is_contiguous() || !a.is_contiguous() || !b.is_contiguous() ||
+      (scales && (scales->scalar_type() != at::kFloat || scales->dim() != 1 || scales->size(0) != l || !scales->is_contiguous())))
+    Py_RETURN_NONE;
+  static const c10::OperatorName op("moe::lora_linear", "");
+  if (replaced(op)) Py_RETURN_NONE;
+  int64_t bytes;
+  if (tgg_lora_workspace_bytes(0, m, (int)n, (int)k, (int)r, (int)l, &bytes) != 0) Py_RETURN_NONE;
+  RECORD_FUNCTION(op.name, std::vector<c10::IValue>({x, w, a, b, ids}));
+  at::Tensor out, ws;
+  int rc;
+  {
+    const Unlocked unlocked;
+    out = at::empty({m, n}, x.options());
+    ws = at::empty({bytes}, x.options().dtype(at::kByte));
+    rc = tgg_lora_linear(x.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(), is64(ids), scales ? scales->data_ptr<float>() : nullptr, out.data_ptr(), nullptr, m, (int)n, (int)k,
+                         (int)r, (int)l, dt, ws.data_ptr(), bytes, stream());
+  }
+  return done("tgg_lora_linear", rc, out);
+  END_HANDLE_TH_ERRORS
+}
+
 // (grad, h, activation) -> dh
 PyObject* gated_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -702,6 +742,7 @@ PyMethodDef methods[] = {
     {"m_grouped_gemm", (PyCFunction)(void*)m_grouped_gemm, METH_FASTCALL, nullptr},
     {"m_grouped_gated_gemm", (PyCFunction)(void*)m_grouped_gated_gemm, METH_FASTCALL, nullptr},
     {"m_grouped_gemm_int4", (PyCFunction)(void*)m_grouped_gemm_int4, METH_FASTCALL, nullptr},
+    {"lora_linear", (PyCFunction)(void*)lora_linear, METH_FASTCALL, nullptr},
     {"gated_backward", (PyCFunction)(void*)gated_backward, METH_FASTCALL, nullptr},
     {"m_grouped_gemm_masked", (PyCFunction)(void*)m_grouped_gemm_masked, METH_FASTCALL, nullptr},
     {"k_grouped_gemm", (PyCFunction)(void*)k_grouped_gemm, METH_FASTCALL, nullptr},

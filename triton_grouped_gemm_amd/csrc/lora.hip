@@ -56,6 +56,62 @@ TGG_DEV float row_scale(float v) {
   return __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
 }
 
+// Chunks of 256 values of depth of a few rows of two K-contiguous operands, through a ring in LDS; the eight waves share a chunk's depth, 32 values each.  (Fragments read
+// straight from memory have every lane in another row than its neighbours, which takes the address unit 64 cycles instead of 16: 64 rows of x and 16 columns
+// of W a workgroup, 4096 x 4096: 23 us.)  Rows of 512 bytes, 16-byte pieces swizzled by the row.
+template <int XB, int WB, int STAGES> struct ChunkRing {
+  static constexpr int X_BYTES = XB * 16 * 512, STAGE_BYTES = X_BYTES + WB * 16 * 512, BYTES = STAGES * STAGE_BYTES, NC = XB + WB;  // NC: a wave's copies of a chunk
+  static_assert(BYTES <= 160 * 1024 && (STAGES - 1) * NC < 64, "LDS, and copies that a wait can count");
+  i32x4_t xr, wr;
+  int voff, piece, pitch, depth, step, end;  // the lane's offset in a copy; chunks step ... end - 1
+  uint32_t at;
+  char* smem;
+
+  TGG_DEV ChunkRing(char* smem_, const void* x, int64_t x_bytes, const void* w, int64_t w_bytes, int depth_, int first, int end_) : depth(depth_), step(first), end(end_), smem(smem_) {
+    xr = make_rsrc((uint64_t)x, x_bytes);
+    wr = make_rsrc((uint64_t)w, w_bytes);
+    at = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
+    const int lane = lane_id(), wave = threadIdx.x >> 6, row = 2 * wave + (lane >> 5);  // of 16
+    pitch = depth * 2;
+    piece = (lane & 31) ^ row;
+    voff = row * pitch + piece * 16;
+  }
+  TGG_DEV void copy(int chunk) {
+    const bool there = chunk < end && chunk * 256 + piece * 8 < depth;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t to = at + chunk_buffer(chunk) * STAGE_BYTES + wave * 1024;
+    asm volatile("s_nop 4" : "+s"(xr), "+s"(wr));
+#pragma unroll
+    for (int i = 0; i < XB; ++i) copy_b128_to_lds(xr, __builtin_amdgcn_readfirstlane(to + i * 8192), there ? voff + chunk * 512 + i * 16 * pitch : kNoFetch);
+#pragma unroll
+    for (int i = 0; i < WB; ++i) copy_b128_to_lds(wr, __builtin_amdgcn_readfirstlane(to + X_BYTES + i * 8192), there ? voff + chunk * 512 + i * 16 * pitch : kNoFetch);
+  }
+  TGG_DEV int chunk_buffer(int chunk) const { return (chunk - step) % STAGES; }
+  // run(x fragments, w fragments) for every chunk, on the wave's 32 values of it
+  template <class F> TGG_DEV void run(F&& f) {
+    const int lane = lane_id(), l16 = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int frag = l16 * 512 + (((4 * wave + lg) ^ l16) << 4);
+    for (int c = step; c < end; ++c) {
+      wait_vmcnt<(STAGES - 2) * NC>();
+      __syncthreads();  // the chunk is there, and the buffer of the one before has been read
+      copy(c + STAGES - 1);
+      const char* const s = smem + chunk_buffer(c) * STAGE_BYTES + frag;
+      i32x4_t x[XB], w[WB];
+#pragma unroll
+      for (int i = 0; i < XB; ++i) x[i] = *(const i32x4_t*)(s + i * 8192);
+#pragma unroll
+      for (int i = 0; i < WB; ++i) w[i] = *(const i32x4_t*)(s + X_BYTES + i * 8192);
+      f(x, w);
+    }
+    wait_vmcnt<0>();  // (the copies behind the last chunk fetch nothing, but write)
+    __syncthreads();
+  }
+  TGG_DEV void start() {
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) copy(step + i);
+  }
+};
+
 constexpr int kDownThreads = 512, kDownWaves = 8;
 
 struct DownParams {
@@ -71,8 +127,11 @@ struct DownParams {
 
 // RB: blocks of 16 rows, RC: blocks of 16 of R (RC * 16 >= R).  blockIdx.x: rows; y: adapters in turn; z: part of the depth.
 template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) void lora_down_kernel(const DownParams p) {
-  constexpr int COLS = RC * 16;
-  __shared__ __attribute__((aligned(16))) float sums[kDownWaves * 16 * COLS];
+  constexpr int COLS = RC * 16, STAGES = RB + RC <= 3 ? 4 : RB + RC <= 6 ? 3 : 2;
+  typedef ChunkRing<RB, RC, STAGES> Ring;
+  static_assert(kDownWaves * 16 * COLS * 4 <= Ring::BYTES, "the waves' sums reuse the ring");
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  float* const sums = (float*)smem;
   const int lane = lane_id(), l16 = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row0 = (int64_t)blockIdx.x * (16 * RB);
   const int rows = (int)lesser(16 * RB, p.M - row0);
@@ -85,9 +144,7 @@ template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) voi
     const uint64_t same = __ballot(id == other);
     if (other >= 0 && (same & ((1ull << i) - 1)) == 0) firsts |= 1ull << i;
   }
-  // this part's steps of 64 values
-  const int steps = (p.depth + 63) / 64, first_step = (int)((int64_t)steps * blockIdx.z / p.parts), end_step = (int)((int64_t)steps * (blockIdx.z + 1) / p.parts);
-  const rsrc_t xw = window((const uint16_t*)p.x + row0 * p.depth, (int64_t)rows * p.depth * 2);
+  const int chunks = (p.depth + 255) / 256, first_chunk = (int)((int64_t)chunks * blockIdx.z / p.parts), end_chunk = (int)((int64_t)chunks * (blockIdx.z + 1) / p.parts);
   float* const h = p.h + (int64_t)blockIdx.z * p.M * p.R;
   if (blockIdx.y == 0) {  // rows without an adapter
     for (int i = threadIdx.x; i < rows * p.R; i += kDownThreads) {
@@ -103,75 +160,48 @@ template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) voi
     if (turn % (int)gridDim.y != (int)blockIdx.y) continue;
     const int l = __builtin_amdgcn_readlane(id, __ffsll((unsigned long long)left) - 1);
     const uint64_t keep = __ballot(id == l);
-    const rsrc_t aw = window((const uint16_t*)p.a + (int64_t)l * p.R * p.depth, (int64_t)p.R * p.depth * 2);
+    Ring ring(smem, (const uint16_t*)p.x + row0 * p.depth, (int64_t)rows * p.depth * 2, (const uint16_t*)p.a + (int64_t)l * p.R * p.depth, (int64_t)p.R * p.depth * 2, p.depth, first_chunk, end_chunk);
     f32x4_t acc[RB][RC];
 #pragma unroll
     for (int b = 0; b < RB; ++b)
 #pragma unroll
       for (int c = 0; c < RC; ++c) acc[b][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    auto load = [&](i32x4_t (&x)[2][RB], i32x4_t (&a)[2][RC], int s) __attribute__((always_inline)) {
+    ring.start();
+    ring.run([&](const i32x4_t (&x)[RB], const i32x4_t (&a)[RC]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const int k = s * 64 + ks * 32 + lg * 8;
-        const int at = s < end_step && k < p.depth ? (l16 * p.depth + k) * 2 : kNowhere;
+      for (int b = 0; b < RB; ++b)
 #pragma unroll
-        for (int b = 0; b < RB; ++b) x[ks][b] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xw, at == kNowhere ? kNowhere : at + b * 16 * p.depth * 2, 0, 0));
-#pragma unroll
-        for (int c = 0; c < RC; ++c) a[ks][c] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(aw, at == kNowhere ? kNowhere : at + c * 16 * p.depth * 2, 0, 0));
-      }
-    };
-    auto multiply = [&](const i32x4_t (&x)[2][RB], const i32x4_t (&a)[2][RC]) __attribute__((always_inline)) {
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int b = 0; b < RB; ++b)
-#pragma unroll
-          for (int c = 0; c < RC; ++c) acc[b][c] = stream_mma<DT>(a[ks][c], x[ks][b], acc[b][c]);  // lane: row l16, columns 4 lg + (0..3)
-    };
-    i32x4_t x0[2][RB], a0[2][RC], x1[2][RB], a1[2][RC];
-    load(x0, a0, first_step + wave);
-    for (int s = first_step + wave; s < end_step; s += 2 * kDownWaves) {
-      load(x1, a1, s + kDownWaves);
-      multiply(x0, a0);
-      load(x0, a0, s + 2 * kDownWaves);
-      multiply(x1, a1);
-    }
+        for (int c = 0; c < RC; ++c) acc[b][c] = stream_mma<DT>(a[c], x[b], acc[b][c]);  // lane: row l16, columns 4 lg + (0..3)
+    });
     const float scale = p.scales ? p.scales[l] : 1.f;
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
-      __syncthreads();
+      if (b) __syncthreads();
 #pragma unroll
       for (int c = 0; c < RC; ++c) *(f32x4_t*)&sums[(wave * 16 + l16) * COLS + 16 * c + 4 * lg] = acc[b][c];
       __syncthreads();
       // 32 threads a row
       const int r = threadIdx.x >> 5, row = b * 16 + r;
-      constexpr int PER = (COLS + 31) / 32;
-      float v[PER];
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int c = (threadIdx.x & 31) + 32 * i;
-        v[i] = 0.f;
-        if (c < COLS) {
-#pragma unroll
-          for (int w = 0; w < kDownWaves; ++w) v[i] += sums[(w * 16 + r) * COLS + c];
-          v[i] *= scale;
-        }
-      }
       const bool mine = row < rows && (keep >> row & 1);
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
+      for (int i = 0; i < (COLS + 31) / 32; ++i) {
         const int c = (threadIdx.x & 31) + 32 * i;
         if (mine && c < p.R) {
-          h[(row0 + row) * p.R + c] = v[i];
+          float v = 0.f;
+#pragma unroll
+          for (int w = 0; w < kDownWaves; ++w) v += sums[(w * 16 + r) * COLS + c];
+          v *= scale;
+          h[(row0 + row) * p.R + c] = v;
           if (p.planes) {
             uint16_t hi, lo;
-            split2<DT_BF16>(v[i], hi, lo);
+            split2<DT_BF16>(v, hi, lo);
             p.planes[((row0 + row) * 2) * p.R + c] = hi;
             p.planes[((row0 + row) * 2 + 1) * p.R + c] = lo;
           }
         }
       }
     }
+    __syncthreads();  // the sums have been read: the ring's again
   }
 }
 
@@ -381,95 +411,65 @@ struct FewParams {
   int N, K, R, parts;
 };
 
-// RB blocks of 16 rows x CB blocks of 16 columns; the waves share the depth.
-template <int DT, int RB, int CB> __global__ __launch_bounds__(kFewThreads) void lora_few_kernel(const FewParams p) {
-  constexpr int ROWS = RB * 16, COLS = CB * 16, QUADS = ROWS * COLS / 4, PER = (QUADS + kFewThreads - 1) / kFewThreads;
-  __shared__ __attribute__((aligned(16))) float sums[kFewWaves * ROWS * COLS];
+// RB blocks of 16 rows x 16 columns; the waves share the depth.
+template <int DT, int RB> __global__ __launch_bounds__(kFewThreads) void lora_few_kernel(const FewParams p) {
+  constexpr int ROWS = RB * 16, COLS = 16, QUADS = ROWS * COLS / 4;
+  typedef ChunkRing<RB, 1, RB == 1 ? 6 : RB == 2 ? 5 : 3> Ring;
+  static_assert(QUADS <= kFewThreads && kFewWaves * ROWS * COLS * 4 <= Ring::BYTES, "a thread has four outputs; the waves' sums reuse the ring");
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  float* const sums = (float*)smem;
   const int lane = lane_id(), l16 = lane & 15, lg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = blockIdx.x * COLS;
   const int64_t row0 = (int64_t)blockIdx.y * ROWS;
   const int rows = (int)lesser(ROWS, p.M - row0);
-  const rsrc_t xw = window((const uint16_t*)p.x + row0 * p.K, (int64_t)rows * p.K * 2);
-  const rsrc_t ww = window((const uint16_t*)p.w + (int64_t)n0 * p.K, (int64_t)min(COLS, p.N - n0) * p.K * 2);
-  const int steps = (p.K + 63) / 64;
-  auto load = [&](i32x4_t (&x)[2][RB], i32x4_t (&w)[2][CB], int s) __attribute__((always_inline)) {
+  Ring ring(smem, (const uint16_t*)p.x + row0 * p.K, (int64_t)rows * p.K * 2, (const uint16_t*)p.w + (int64_t)n0 * p.K, (int64_t)lesser(COLS, p.N - n0) * p.K * 2, p.K, 0, (p.K + 255) / 256);
+  ring.start();
+  // the adapters' part of the thread's outputs, four columns of one row, while the first weights arrive
+  float own[4] = {0.f, 0.f, 0.f, 0.f};
+  const int r = threadIdx.x / (COLS / 4), c = threadIdx.x % (COLS / 4) * 4;
+  const bool mine = r < rows && n0 + c < p.N;
+  if (mine) {
+    const int id = p.ids.at(row0 + r);
+    if (id >= 0) {
+      const uint16_t* const b = (const uint16_t*)p.b + ((int64_t)id * p.N + n0 + c) * p.R;
+      for (int k = 0; k < p.R; k += 8) {
+        float h[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int part = 0; part < p.parts; ++part) {
+          const f32x4_t* const hp = (const f32x4_t*)(p.h + ((int64_t)part * p.M + row0 + r) * p.R + k);
+          const f32x4_t h0 = hp[0], h1 = hp[1];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const int k = s * 64 + ks * 32 + lg * 8;
-      const int at = s < steps && k < p.K ? (l16 * p.K + k) * 2 : kNowhere;
-#pragma unroll
-      for (int c = 0; c < CB; ++c) w[ks][c] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ww, at == kNowhere ? kNowhere : at + c * 16 * p.K * 2, 0, 0));
-#pragma unroll
-      for (int b = 0; b < RB; ++b) x[ks][b] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xw, at == kNowhere ? kNowhere : at + b * 16 * p.K * 2, 0, 0));
-    }
-  };
-  f32x4_t acc[RB][CB];
-#pragma unroll
-  for (int b = 0; b < RB; ++b)
-#pragma unroll
-    for (int c = 0; c < CB; ++c) acc[b][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](const i32x4_t (&x)[2][RB], const i32x4_t (&w)[2][CB]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int b = 0; b < RB; ++b)
-#pragma unroll
-        for (int c = 0; c < CB; ++c) acc[b][c] = stream_mma<DT>(w[ks][c], x[ks][b], acc[b][c]);
-  };
-  i32x4_t x0[2][RB], w0[2][CB], x1[2][RB], w1[2][CB];
-  load(x0, w0, wave);
-  load(x1, w1, wave + kFewWaves);
-  // the adapters' part of the thread's outputs, four columns of one row each, while the first weights arrive
-  float own[PER][4];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int q = threadIdx.x + i * kFewThreads, r = q / (COLS / 4), n = n0 + q % (COLS / 4) * 4;
-    own[i][0] = own[i][1] = own[i][2] = own[i][3] = 0.f;
-    if (r < rows && n < p.N) {
-      const int id = p.ids.at(row0 + r);
-      if (id >= 0) {
-        const uint16_t* const b = (const uint16_t*)p.b + ((int64_t)id * p.N + n) * p.R;
-        for (int c = 0; c < p.R; c += 8) {
-          float h[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          for (int part = 0; part < p.parts; ++part) {
-            const float* const hp = p.h + ((int64_t)part * p.M + row0 + r) * p.R + c;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] += hp[e];
+          for (int e = 0; e < 4; ++e) {
+            h[e] += h0[e];
+            h[4 + e] += h1[e];
           }
+        }
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const i32x4_t v = *(const i32x4_t*)(b + (int64_t)y * p.R + c);
+        for (int y = 0; y < 4; ++y) {
+          const i32x4_t v = *(const i32x4_t*)(b + (int64_t)y * p.R + k);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) own[i][y] = __builtin_fmaf(h[e], from_bits<DT>((uint16_t)((uint32_t)v[e / 2] >> (16 * (e & 1)))), own[i][y]);
-          }
+          for (int e = 0; e < 8; ++e) own[y] = __builtin_fmaf(h[e], from_bits<DT>((uint16_t)((uint32_t)v[e / 2] >> (16 * (e & 1)))), own[y]);
         }
       }
     }
   }
-  for (int s = wave; s < steps; s += 2 * kFewWaves) {
-    multiply(x0, w0);
-    load(x0, w0, s + 2 * kFewWaves);
-    multiply(x1, w1);
-    load(x1, w1, s + 3 * kFewWaves);
-  }
+  f32x4_t acc[RB];
 #pragma unroll
-  for (int b = 0; b < RB; ++b)
+  for (int b = 0; b < RB; ++b) acc[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  ring.run([&](const i32x4_t (&x)[RB], const i32x4_t (&w)[1]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < CB; ++c) *(f32x4_t*)&sums[(wave * ROWS + 16 * b + l16) * COLS + 16 * c + 4 * lg] = acc[b][c];
+    for (int b = 0; b < RB; ++b) acc[b] = stream_mma<DT>(w[0], x[b], acc[b]);
+  });
+#pragma unroll
+  for (int b = 0; b < RB; ++b) *(f32x4_t*)&sums[(wave * ROWS + 16 * b + l16) * COLS + 4 * lg] = acc[b];
   __syncthreads();
+  if (mine) {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int q = threadIdx.x + i * kFewThreads, r = q / (COLS / 4), c = q % (COLS / 4) * 4;
-    if (r < rows && n0 + c < p.N) {
-      f32x4_t v = {own[i][0], own[i][1], own[i][2], own[i][3]};
+    for (int w = 0; w < kFewWaves; ++w) {
+      const f32x4_t t = *(const f32x4_t*)&sums[(w * ROWS + r) * COLS + c];
 #pragma unroll
-      for (int w = 0; w < kFewWaves; ++w) {
-        const f32x4_t s = *(const f32x4_t*)&sums[(w * ROWS + r) * COLS + c];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += s[e];
-      }
-      *(uint2*)((uint16_t*)p.out + (row0 + r) * p.N + n0 + c) = pack4<DT>(v[0], v[1], v[2], v[3]);
+      for (int e = 0; e < 4; ++e) own[e] += t[e];
     }
+    *(uint2*)((uint16_t*)p.out + (row0 + r) * p.N + n0 + c) = pack4<DT>(own[0], own[1], own[2], own[3]);
   }
 }
 
@@ -675,23 +675,29 @@ template <int DT> __global__ __launch_bounds__(256) void lora_join_kernel(const 
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
-template <int DT, int RB> int down_rc(const DownParams& p, dim3 grid, hipStream_t s) {
-  const int rc = (p.R + 15) / 16;
-  if (rc <= 1) lora_down_kernel<DT, RB, 1><<<grid, dim3(kDownThreads), 0, s>>>(p);
-  else if (rc <= 2) lora_down_kernel<DT, RB, 2><<<grid, dim3(kDownThreads), 0, s>>>(p);
-  else if (rc <= 4) lora_down_kernel<DT, RB, 4><<<grid, dim3(kDownThreads), 0, s>>>(p);
-  else lora_down_kernel<DT, RB, 8><<<grid, dim3(kDownThreads), 0, s>>>(p);
-  return check_launch("lora_down");
+template <class Kern, class P> int launch_smem(Kern kern, int smem, bool& attr_done, dim3 grid, int threads, const P& p, hipStream_t s, const char* what) {
+  if (!attr_done) {
+    if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess) return check_launch("hipFuncSetAttribute(lora)");
+    attr_done = true;
+  }
+  kern<<<grid, dim3(threads), smem, s>>>(p);
+  return check_launch(what);
+}
+
+template <int DT, int RB, int RC> int down_launch(const DownParams& p, hipStream_t s) {
+  static bool attr_done = false;
+  constexpr int smem = ChunkRing<RB, RC, (RB + RC <= 3 ? 4 : RB + RC <= 6 ? 3 : 2)>::BYTES;
+  const int64_t blocks = (p.M + 16 * RB - 1) / (16 * RB);
+  // few rows: their adapters side by side
+  const int turns = RB > 1 || blocks >= 1024 ? 1 : (int)lesser(16, 1024 / blocks);
+  return launch_smem(lora_down_kernel<DT, RB, RC>, smem, attr_done, dim3((unsigned)blocks, turns, p.parts), kDownThreads, p, s, "lora_down");
 }
 
 template <int DT> int launch_down(const DownParams& p, hipStream_t s) {
-  const bool tall = p.M >= 8192;  // 32 rows a workgroup, else 16
-  const int rows = tall ? 32 : 16;
-  const int blocks = (int)((p.M + rows - 1) / rows);
-  // few rows: their adapters side by side
-  const int turns = blocks >= 1024 ? 1 : (int)lesser(16, 1024 / blocks);
-  const dim3 grid(blocks, tall ? 1 : turns, p.parts);
-  return tall ? down_rc<DT, 2>(p, grid, s) : down_rc<DT, 1>(p, grid, s);
+  const int rc = (p.R + 15) / 16;
+  if (rc > 4) return down_launch<DT, 1, 8>(p, s);
+  if (p.M >= 4096) return rc <= 1 ? down_launch<DT, 2, 1>(p, s) : rc <= 2 ? down_launch<DT, 2, 2>(p, s) : down_launch<DT, 2, 4>(p, s);  // 32 rows a workgroup read the adapter half as often
+  return rc <= 1 ? down_launch<DT, 1, 1>(p, s) : rc <= 2 ? down_launch<DT, 1, 2>(p, s) : down_launch<DT, 1, 4>(p, s);
 }
 
 typedef StreamCfg<256, 256, 2, 4> LoraWide;
@@ -700,13 +706,8 @@ typedef StreamCfg<128, 128, 2, 4> LoraNarrow;
 template <class C, int DT, bool NT> int gemm_launch(const LoraGemm& p, hipStream_t s) {
   typedef LoraProblem<C, DT, NT> P;
   static bool attr_done = false;
-  if (!attr_done) {
-    if (hipFuncSetAttribute((const void*)lora_gemm_kernel<C, DT, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, P::SMEM_BYTES) != hipSuccess) return check_launch("hipFuncSetAttribute(lora_gemm)");
-    attr_done = true;
-  }
   const int tiles = p.tiles_m * p.tiles_n, slots = num_cus() * (C::BM == 128 ? 2 : 1);
-  lora_gemm_kernel<C, DT, NT><<<dim3(tiles < slots ? tiles : slots), dim3(C::THREADS), P::SMEM_BYTES, s>>>(p);
-  return check_launch("lora_gemm");
+  return launch_smem(lora_gemm_kernel<C, DT, NT>, P::SMEM_BYTES, attr_done, dim3(tiles < slots ? tiles : slots), C::THREADS, p, s, "lora_gemm");
 }
 
 template <int DT, bool NT> int launch_gemm(LoraGemm p, int tile, hipStream_t s) {
@@ -725,23 +726,17 @@ int tile_of(int64_t M, int cols) {
 bool few_rows(int64_t M) { return M <= 64; }
 int few_parts(int64_t M) { return M <= 16 ? 4 : 2; }  // parts of the depth in lora_down: more workgroups for few rows
 
-template <int DT> int launch_few(const FewParams& p, hipStream_t s) {
-  const dim3 threads(kFewThreads);
-  if (p.M <= 16) lora_few_kernel<DT, 1, 1><<<dim3((p.N + 15) / 16, 1), threads, 0, s>>>(p);
-  else if (p.M <= 32) lora_few_kernel<DT, 2, 1><<<dim3((p.N + 15) / 16, 1), threads, 0, s>>>(p);
-  else lora_few_kernel<DT, 4, 1><<<dim3((p.N + 15) / 16, (unsigned)((p.M + 63) / 64)), threads, 0, s>>>(p);
-  return check_launch("lora_few");
+template <int DT, int RB> int few_launch(const FewParams& p, hipStream_t s) {
+  static bool attr_done = false;
+  constexpr int smem = ChunkRing<RB, 1, (RB == 1 ? 6 : RB == 2 ? 5 : 3)>::BYTES;
+  return launch_smem(lora_few_kernel<DT, RB>, smem, attr_done, dim3((p.N + 15) / 16, (unsigned)((p.M + 16 * RB - 1) / (16 * RB))), kFewThreads, p, s, "lora_few");
 }
+template <int DT> int launch_few(const FewParams& p, hipStream_t s) { return p.M <= 16 ? few_launch<DT, 1>(p, s) : p.M <= 32 ? few_launch<DT, 2>(p, s) : few_launch<DT, 4>(p, s); }
 
 template <int DT, int RC> int outer_launch(const OuterParams& p, dim3 grid, hipStream_t s) {
   constexpr int smem = 2 * kOuterRows * kOuterCols * 2 + 2 * kOuterRows * (RC * 32 + 16) + kOuterWindow * 2 + kOuterWaves * 8;
   static bool attr_done = false;
-  if (!attr_done) {
-    if (hipFuncSetAttribute((const void*)lora_outer_kernel<DT, RC>, hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess) return check_launch("hipFuncSetAttribute(lora_outer)");
-    attr_done = true;
-  }
-  lora_outer_kernel<DT, RC><<<grid, dim3(kOuterThreads), smem, s>>>(p);
-  return check_launch("lora_outer");
+  return launch_smem(lora_outer_kernel<DT, RC>, smem, attr_done, grid, kOuterThreads, p, s, "lora_outer");
 }
 
 // parts of the rows: enough workgroups for the chip, none of fewer than 1024 rows

@@ -126,6 +126,10 @@ def _(grad, x, weight, lora_a, lora_b, adapters, scales, h, want_x, want_a, want
     return tuple(t.new_empty(t.shape if want else (0,)) for t, want in ((x, want_x), (lora_a, want_a), (lora_b, want_b)))
 
 
+# (what is registered for them runs in ``lora_linear`` too: see EagerOp)
+_lora_linear.__class__ = _lora_linear_hidden.__class__ = _lora_linear_backward.__class__ = _native.EagerOp
+
+
 class LoraLinear(torch.autograd.Function):
     """``lora_linear`` with the gradients of activations, adapters and, where it is asked for, of the shared weights (the K-grouped product of all
     rows).  ``scales`` has none."""
@@ -160,6 +164,10 @@ def lora_linear(x: Tensor, weight: Tensor, lora_a: Tensor, lora_b: Tensor, adapt
     8 up to 128, L up to 1024); ``adapters`` ``[M]`` int32 or int64 on the GPU, in any order: a row whose entry is outside ``[0, L)``
     (-1, say) has no adapter; ``scales`` ``[L]`` fp32, 1 unless given.  fp32 to the one rounding at the end.  Differentiable in ``x``, ``weight``,
     ``lora_a`` and ``lora_b``; adapters without rows get zero gradients."""
+    if not (_lora_linear.replaced or torch.compiler.is_compiling()):
+        out = (_native._host or _native.host()).lora_linear(x, weight, lora_a, lora_b, adapters, scales)
+        if out is not None:
+            return out
     _check(x, weight, lora_a, lora_b, adapters, scales)
     if scales is not None and scales.requires_grad and torch.is_grad_enabled():
         raise ValueError("scales is not differentiable: detach it")
