@@ -239,43 +239,96 @@ PyObject* m_grouped_gemm_int4(PyObject*, PyObject* const* args, Py_ssize_t nargs
   END_HANDLE_TH_ERRORS
 }
 
-// (x, weight, lora_a, lora_b, adapters, scales or None) -> out
+// What the adapter calls have in common: plain operands in the kernels' form, nothing to record.
+struct LoraArgs {
+  const at::Tensor *x, *w, *a, *b, *ids, *scales;
+  int64_t m, k, n, l, r;
+  int dt;
+};
+bool lora_args(PyObject* const* args, c10::DeviceIndex& device, LoraArgs& q) {
+  const at::Tensor** const to[5] = {&q.x, &q.w, &q.a, &q.b, &q.ids};
+  for (int i = 0; i < 5; ++i)
+    if (!(*to[i] = plain(args[i], device))) return false;
+  q.scales = nullptr;
+  if (args[5] != Py_None && !(q.scales = plain(args[5], device))) return false;
+  const at::Tensor &x = *q.x, &w = *q.w, &a = *q.a, &b = *q.b;
+  if (x.dim() != 2 || w.dim() != 2 || a.dim() != 3 || b.dim() != 3 || records(x) || records(w) || records(a) || records(b) || (q.scales && records(*q.scales))) return false;
+  q.m = x.size(0), q.k = x.size(1), q.n = w.size(0), q.l = a.size(0), q.r = a.size(1), q.dt = code16(x);
+  const at::ScalarType type = x.scalar_type();
+  return q.dt >= 0 && w.scalar_type() == type && a.scalar_type() == type && b.scalar_type() == type && q.m > 0 && w.size(1) == q.k && a.size(2) == q.k && b.size(0) == q.l && b.size(1) == q.n &&
+         b.size(2) == q.r && q.n >= 8 && q.k >= 8 && !(q.n & 7) && !(q.k & 7) && q.n <= 65536 && q.k <= 65536 && q.r >= 8 && q.r <= 128 && !(q.r & 7) && q.l >= 1 && q.l <= kMaxGroups &&
+         sizes_ok(*q.ids, q.m) && x.is_contiguous() && w.is_contiguous() && a.is_contiguous() && b.is_contiguous() &&
+         (!q.scales || (q.scales->scalar_type() == at::kFloat && q.scales->dim() == 1 && q.scales->size(0) == q.l && q.scales->is_contiguous()));
+}
+
+// (x, weight, lora_a, lora_b, adapters, scales or None, hidden) -> out, or (out, h)
 PyObject* lora_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  TGG_ARGS(6);
-  TGG_TENSOR(x, 0);
-  TGG_TENSOR(w, 1);
-  TGG_TENSOR(a, 2);
-  TGG_TENSOR(b, 3);
-  TGG_TENSOR(ids, 4);
-  const at::Tensor* scales = nullptr;
-  if (args[5] != Py_None) {
-    scales = plain(args[5], device);
-    if (!scales) Py_RETURN_NONE;
-  }
-  if (x.dim() != 2 || w.dim() != 2 || a.dim() != 3 || b.dim() != 3 || records(x) || records(w) || records(a) || records(b) || (scales && records(*scales))) Py_RETURN_NONE;
-  const int64_t m = x.size(0), k = x.size(1), n = w.size(0), l = a.size(0), r = a.size(1);
-  const int dt = code16(x);
-  if (dt < 0 || w.scalar_type() != x.scalar_type() || a.scalar_type() != x.scalar_type() || b.scalar_type() != x.scalar_type() || m == 0 || w.size(1) != k || a.size(2) != k ||
-      b.size(0) != l || b.size(1) != n || b.size(2) != r || n < 8 || k < 8 || (n & 7) || (k & 7) || n > 65536 || k > 65536 || r < 8 || r > 128 || (r & 7) || l < 1 || l > kMaxGroups ||
-      !sizes_ok(ids, m) || !x.is_contiguous() || !w.is_contiguous() || !a.is_contiguous() || !b.is_contiguous() ||
-      (scales && (scales->scalar_type() != at::kFloat || scales->dim() != 1 || scales->size(0) != l || !scales->is_contiguous())))
-    Py_RETURN_NONE;
-  static const c10::OperatorName op("moe::lora_linear", "");
+  TGG_ARGS(7);
+  TGG_TRUTH(hidden, 6);
+  LoraArgs q;
+  if (!lora_args(args, device, q)) Py_RETURN_NONE;
+  static const c10::OperatorName plain_op("moe::lora_linear", ""), hidden_op("moe::lora_linear_hidden", "");
+  const c10::OperatorName& op = hidden ? hidden_op : plain_op;
   if (replaced(op)) Py_RETURN_NONE;
   int64_t bytes;
-  if (tgg_lora_workspace_bytes(0, m, (int)n, (int)k, (int)r, (int)l, &bytes) != 0) Py_RETURN_NONE;
-  RECORD_FUNCTION(op.name, std::vector<c10::IValue>({x, w, a, b, ids}));
-  at::Tensor out, ws;
+  if (tgg_lora_workspace_bytes(0, q.m, (int)q.n, (int)q.k, (int)q.r, (int)q.l, &bytes) != 0) Py_RETURN_NONE;
+  RECORD_FUNCTION(op.name, std::vector<c10::IValue>({*q.x, *q.w, *q.a, *q.b, *q.ids}));
+  at::Tensor out, h, ws;
   int rc;
   {
     const Unlocked unlocked;
-    out = at::empty({m, n}, x.options());
-    ws = at::empty({bytes}, x.options().dtype(at::kByte));
-    rc = tgg_lora_linear(x.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(), is64(ids), scales ? scales->data_ptr<float>() : nullptr, out.data_ptr(), nullptr, m, (int)n, (int)k,
-                         (int)r, (int)l, dt, ws.data_ptr(), bytes, stream());
+    out = at::empty({q.m, q.n}, q.x->options());
+    if (hidden) h = at::empty({q.m, q.r}, q.x->options().dtype(at::kFloat));
+    ws = at::empty({bytes}, q.x->options().dtype(at::kByte));
+    rc = tgg_lora_linear(q.x->data_ptr(), q.w->data_ptr(), q.a->data_ptr(), q.b->data_ptr(), q.ids->data_ptr(), is64(*q.ids), q.scales ? q.scales->data_ptr<float>() : nullptr, out.data_ptr(),
+                         hidden ? h.data_ptr<float>() : nullptr, q.m, (int)q.n, (int)q.k, (int)q.r, (int)q.l, q.dt, ws.data_ptr(), bytes, stream());
   }
-  return done("tgg_lora_linear", rc, out);
+  return rc == 0 && hidden ? pair(out, h) : done("tgg_lora_linear", rc, out);
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, weight, lora_a, lora_b, adapters, scales or None, grad, h, want_x, want_a, want_b) -> (dx, da, db), None where not wanted
+PyObject* lora_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TGG_ARGS(11);
+  TGG_TRUTH(want_x, 8);
+  TGG_TRUTH(want_a, 9);
+  TGG_TRUTH(want_b, 10);
+  LoraArgs q;
+  if (!lora_args(args, device, q)) Py_RETURN_NONE;
+  TGG_TENSOR(grad, 6);
+  TGG_TENSOR(h, 7);
+  if (grad.dim() != 2 || grad.size(0) != q.m || grad.size(1) != q.n || grad.scalar_type() != q.x->scalar_type() || !grad.is_contiguous() || records(grad) || h.dim() != 2 || h.size(0) != q.m ||
+      h.size(1) != q.r || h.scalar_type() != at::kFloat || !h.is_contiguous() || records(h))
+    Py_RETURN_NONE;
+  static const c10::OperatorName op("moe::lora_linear_backward", "");
+  if (replaced(op)) Py_RETURN_NONE;
+  int64_t bytes;
+  if (tgg_lora_workspace_bytes(1, q.m, (int)q.n, (int)q.k, (int)q.r, (int)q.l, &bytes) != 0) Py_RETURN_NONE;
+  RECORD_FUNCTION(op.name, std::vector<c10::IValue>({grad, *q.x, *q.w, *q.a, *q.b, *q.ids}));
+  at::Tensor dx, da, db, ws;
+  int rc;
+  {
+    const Unlocked unlocked;
+    if (want_x) dx = at::empty({q.m, q.k}, q.x->options());
+    if (want_a) da = at::empty({q.l, q.r, q.k}, q.x->options());
+    if (want_b) db = at::empty({q.l, q.n, q.r}, q.x->options());
+    ws = at::empty({bytes}, q.x->options().dtype(at::kByte));
+    rc = tgg_lora_linear_bwd(grad.data_ptr(), q.x->data_ptr(), q.w->data_ptr(), q.a->data_ptr(), q.b->data_ptr(), q.ids->data_ptr(), is64(*q.ids), q.scales ? q.scales->data_ptr<float>() : nullptr,
+                             h.data_ptr<float>(), want_x ? dx.data_ptr() : nullptr, want_a ? da.data_ptr() : nullptr, want_b ? db.data_ptr() : nullptr, q.m, (int)q.n, (int)q.k, (int)q.r, (int)q.l,
+                             q.dt, ws.data_ptr(), bytes, stream());
+  }
+  if (rc != 0) return done("tgg_lora_linear_bwd", rc, grad);
+  PyObject* const t = PyTuple_New(3);
+  if (!t) return nullptr;
+  const at::Tensor* const results[3] = {&dx, &da, &db};
+  for (int i = 0; i < 3; ++i) {
+    PyObject* o = Py_None;
+    if (results[i]->defined()) o = THPVariable_Wrap(*results[i]); else Py_INCREF(o);
+    PyTuple_SET_ITEM(t, i, o);
+  }
+  return t;
   END_HANDLE_TH_ERRORS
 }
 
@@ -743,6 +796,7 @@ PyMethodDef methods[] = {
     {"m_grouped_gated_gemm", (PyCFunction)(void*)m_grouped_gated_gemm, METH_FASTCALL, nullptr},
     {"m_grouped_gemm_int4", (PyCFunction)(void*)m_grouped_gemm_int4, METH_FASTCALL, nullptr},
     {"lora_linear", (PyCFunction)(void*)lora_linear, METH_FASTCALL, nullptr},
+    {"lora_linear_backward", (PyCFunction)(void*)lora_linear_backward, METH_FASTCALL, nullptr},
     {"gated_backward", (PyCFunction)(void*)gated_backward, METH_FASTCALL, nullptr},
     {"m_grouped_gemm_masked", (PyCFunction)(void*)m_grouped_gemm_masked, METH_FASTCALL, nullptr},
     {"k_grouped_gemm", (PyCFunction)(void*)k_grouped_gemm, METH_FASTCALL, nullptr},

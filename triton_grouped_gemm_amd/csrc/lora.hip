@@ -113,6 +113,8 @@ template <int XB, int WB, int STAGES> struct ChunkRing {
 };
 
 constexpr int kDownThreads = 512, kDownWaves = 8;
+// chunks of `blocks` blocks of 16 rows (8 KB each) in the ring: two workgroups a compute unit where three chunks of each fit
+constexpr int down_stages(int blocks) { return blocks <= 2 ? 5 : blocks <= 6 ? 3 : 2; }
 
 struct DownParams {
   const void* x;     // [M, depth]
@@ -127,7 +129,7 @@ struct DownParams {
 
 // RB: blocks of 16 rows, RC: blocks of 16 of R (RC * 16 >= R).  blockIdx.x: rows; y: adapters in turn; z: part of the depth.
 template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) void lora_down_kernel(const DownParams p) {
-  constexpr int COLS = RC * 16, STAGES = RB + RC <= 3 ? 4 : RB + RC <= 6 ? 3 : 2;
+  constexpr int COLS = RC * 16, STAGES = down_stages(RB + RC);
   typedef ChunkRing<RB, RC, STAGES> Ring;
   static_assert(kDownWaves * 16 * COLS * 4 <= Ring::BYTES, "the waves' sums reuse the ring");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -285,63 +287,98 @@ template <class C, int DT, bool NT> struct LoraProblem {
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) ids[i] = 16 * i + l16 < rows ? p.ids.at(row0 + 16 * i + l16) : -1;
     const rsrc_t hw = window(p.planes + row0 * 2 * p.R, (int64_t)rows * p.R * 4);
-    for (int l = -1;;) {
-      // the wave's next adapter, in the order of their numbers
+    // Steps of 32 values of depth (the high plane, then the low one) of every adapter, in the order of their numbers.  Of narrow tiles a step's operands are under way while the
+    // step before is multiplied (16 adapters in 64 rows, rank 32: the two steps of each took 1.25 us, the wait for memory).
+    struct Step {
+      int l, k0;
+      bool mixed;
+    };
+    auto next_adapter = [&](int after) __attribute__((always_inline)) {
       uint32_t lowest = 0xffffffffu;
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) lowest = ids[i] > l ? min(lowest, (uint32_t)ids[i]) : lowest;
+      for (int i = 0; i < C::TM; ++i) lowest = ids[i] > after && (uint32_t)ids[i] < lowest ? (uint32_t)ids[i] : lowest;
 #pragma unroll
-      for (int d = 1; d < 16; d <<= 1) lowest = min(lowest, (uint32_t)__shfl_xor((int)lowest, d, 64));  // (all four groups of lanes hold the same rows)
-      l = __builtin_amdgcn_readfirstlane((int)lowest);
-      if (l < 0) break;
+      for (int d = 1; d < 16; d <<= 1) {  // (all four groups of lanes hold the same rows)
+        const uint32_t other = (uint32_t)__shfl_xor((int)lowest, d, 64);
+        lowest = other < lowest ? other : lowest;
+      }
+      Step s;
+      s.l = __builtin_amdgcn_readfirstlane((int)lowest);
+      s.k0 = 0;
       bool all = true;
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) all = all && (ids[i] == l || 16 * i + l16 >= rows);
-      const bool mixed = __ballot(!all) != 0;
-      const rsrc_t bw = window(p.pair + ((int64_t)l * p.cols + col0) * p.R, (int64_t)min(C::BN / C::WN, p.cols - col0) * p.R * 2);
-#pragma unroll 1
-      for (int k0 = 0; k0 < 2 * p.R; k0 += 32) {  // depth: the high plane, then the low one
-        const int k = k0 + 8 * lg, r = k < p.R ? k : k - p.R;
-        i32x4_t b[C::TN];
+      for (int i = 0; i < C::TM; ++i) all = all && (ids[i] == s.l || 16 * i + l16 >= rows);
+      s.mixed = __ballot(!all) != 0;
+      return s;
+    };
+    auto advance = [&](const Step& s) __attribute__((always_inline)) {
+      if (s.k0 + 32 < 2 * p.R) return Step{s.l, s.k0 + 32, s.mixed};
+      return next_adapter(s.l);
+    };
+    auto load = [&](const Step& s, i32x4_t (&a)[C::TM], i32x4_t (&b)[C::TN]) __attribute__((always_inline)) {
+      const rsrc_t bw = window(p.pair + ((int64_t)s.l * p.cols + col0) * p.R, (int64_t)min(C::BN / C::WN, p.cols - col0) * p.R * 2);
+      const int k = s.k0 + 8 * lg, r = k < p.R ? k : k - p.R;
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j) b[j] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(bw, k < 2 * p.R ? ((16 * j + l16) * p.R + r) * 2 : kNowhere, 0, 0));
-        if (mixed) {
+      for (int j = 0; j < C::TN; ++j) b[j] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(bw, k < 2 * p.R ? ((16 * j + l16) * p.R + r) * 2 : kNowhere, 0, 0));
 #pragma unroll
-          for (int j = 0; j < C::TN; ++j) {
-            uint32_t out = 0;
+      for (int i = 0; i < C::TM; ++i) a[i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(hw, ids[i] == s.l && k < 2 * p.R ? ((16 * i + l16) * 2 * p.R + k) * 2 : kNowhere, 0, 0));
+    };
+    auto multiply = [&](const Step& s, const i32x4_t (&a)[C::TM], i32x4_t (&b)[C::TN]) __attribute__((always_inline)) {
+      if (s.mixed) {
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const uint32_t x = (uint32_t)b[j][w], bad = ((x & EXPONENT) == EXPONENT ? 0xffffu : 0u) | ((x >> 16 & EXPONENT) == EXPONENT ? 0xffff0000u : 0u);
-              b[j][w] = (int)(x & ~bad);
-              out |= bad;
-            }
-            infinite = infinite || __ballot(out != 0) != 0;
+        for (int j = 0; j < C::TN; ++j) {
+          uint32_t out = 0;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t x = (uint32_t)b[j][w], bad = ((x & EXPONENT) == EXPONENT ? 0xffffu : 0u) | ((x >> 16 & EXPONENT) == EXPONENT ? 0xffff0000u : 0u);
+            b[j][w] = (int)(x & ~bad);
+            out |= bad;
           }
+          infinite = infinite || __ballot(out != 0) != 0;
         }
-        i32x4_t rest[C::TN];
+      }
+      i32x4_t rest[C::TN];
+      if (DT == DT_F16) {
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float v0 = from_bits<DT_F16>((uint16_t)b[j][w]), v1 = from_bits<DT_F16>((uint16_t)((uint32_t)b[j][w] >> 16));
+            const uint32_t high = pack2<DT_BF16>(v0, v1);
+            const float r0 = v0 - from_bits<DT_BF16>((uint16_t)high), r1 = v1 - from_bits<DT_BF16>((uint16_t)(high >> 16));
+            b[j][w] = (int)high;
+            rest[j][w] = (int)pack2<DT_BF16>(__builtin_isfinite(r0) ? r0 : 0.f, __builtin_isfinite(r1) ? r1 : 0.f);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        if (__ballot(ids[i] == s.l) == 0) continue;
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) acc[i][j] = stream_mma<DT_BF16>(b[j], a[i], acc[i][j]);
         if (DT == DT_F16) {
 #pragma unroll
-          for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const float v0 = from_bits<DT_F16>((uint16_t)b[j][w]), v1 = from_bits<DT_F16>((uint16_t)((uint32_t)b[j][w] >> 16));
-              const uint32_t high = pack2<DT_BF16>(v0, v1);
-              const float r0 = v0 - from_bits<DT_BF16>((uint16_t)high), r1 = v1 - from_bits<DT_BF16>((uint16_t)(high >> 16));
-              b[j][w] = (int)high;
-              rest[j][w] = (int)pack2<DT_BF16>(__builtin_isfinite(r0) ? r0 : 0.f, __builtin_isfinite(r1) ? r1 : 0.f);
-            }
+          for (int j = 0; j < C::TN; ++j) acc[i][j] = stream_mma<DT_BF16>(rest[j], a[i], acc[i][j]);
         }
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i) {
-          if (__ballot(ids[i] == l) == 0) continue;
-          const i32x4_t a = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(hw, ids[i] == l && k < 2 * p.R ? ((16 * i + l16) * 2 * p.R + k) * 2 : kNowhere, 0, 0));
-#pragma unroll
-          for (int j = 0; j < C::TN; ++j) acc[i][j] = stream_mma<DT_BF16>(b[j], a, acc[i][j]);
-          if (DT == DT_F16) {
-#pragma unroll
-            for (int j = 0; j < C::TN; ++j) acc[i][j] = stream_mma<DT_BF16>(rest[j], a, acc[i][j]);
-          }
-        }
+      }
+    };
+    i32x4_t a0[C::TM], b0[C::TN];
+    if constexpr (C::TM == 4) {
+      i32x4_t a1[C::TM], b1[C::TN];
+      Step s = next_adapter(-1);
+      if (s.l >= 0) load(s, a0, b0);
+      while (s.l >= 0) {
+        const Step t = advance(s);
+        if (t.l >= 0) load(t, a1, b1);
+        multiply(s, a0, b0);
+        if (t.l < 0) break;
+        s = advance(t);
+        if (s.l >= 0) load(s, a0, b0);
+        multiply(t, a1, b1);
+      }
+    } else {
+      for (Step s = next_adapter(-1); s.l >= 0; s = advance(s)) {
+        load(s, a0, b0);
+        multiply(s, a0, b0);
       }
     }
   }
@@ -392,7 +429,7 @@ template <class C, int DT, bool NT> struct LoraProblem {
   }
 };
 
-template <class C, int DT, bool NT> __global__ __launch_bounds__(C::THREADS) void lora_gemm_kernel(const LoraGemm p) {
+template <class C, int DT, bool NT> __global__ __launch_bounds__(C::THREADS, C::BM == 128 ? 4 : 2) void lora_gemm_kernel(const LoraGemm p) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   LoraProblem<C, DT, NT> prob(p);
   stream_gemm<C, DT, NT>(prob, smem);
@@ -686,7 +723,7 @@ template <class Kern, class P> int launch_smem(Kern kern, int smem, bool& attr_d
 
 template <int DT, int RB, int RC> int down_launch(const DownParams& p, hipStream_t s) {
   static bool attr_done = false;
-  constexpr int smem = ChunkRing<RB, RC, (RB + RC <= 3 ? 4 : RB + RC <= 6 ? 3 : 2)>::BYTES;
+  constexpr int smem = ChunkRing<RB, RC, down_stages(RB + RC)>::BYTES;
   const int64_t blocks = (p.M + 16 * RB - 1) / (16 * RB);
   // few rows: their adapters side by side
   const int turns = RB > 1 || blocks >= 1024 ? 1 : (int)lesser(16, 1024 / blocks);

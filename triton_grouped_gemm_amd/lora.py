@@ -136,7 +136,10 @@ class LoraLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, lora_a, lora_b, adapters, scales):
-        out, h = _lora_linear_hidden(x, weight, lora_a, lora_b, adapters, scales)
+        result = None
+        if not (_lora_linear_hidden.replaced or torch.compiler.is_compiling()):
+            result = (_native._host or _native.host()).lora_linear(x, weight, lora_a, lora_b, adapters, scales, True)
+        out, h = result if result is not None else _lora_linear_hidden(x, weight, lora_a, lora_b, adapters, scales)
         ctx.save_for_backward(x, weight, lora_a, lora_b, adapters, scales, h)
         return out
 
@@ -145,7 +148,11 @@ class LoraLinear(torch.autograd.Function):
     def backward(ctx, grad):
         x, weight, lora_a, lora_b, adapters, scales, h = ctx.saved_tensors
         want = [ctx.needs_input_grad[0], ctx.needs_input_grad[2], ctx.needs_input_grad[3]]
-        grads = _lora_linear_backward(grad, x, weight, lora_a, lora_b, adapters, scales, h, *want)
+        grads = None
+        if any(want) and not (_lora_linear_backward.replaced or torch.compiler.is_compiling()):
+            grads = (_native._host or _native.host()).lora_linear_backward(x, weight, lora_a, lora_b, adapters, scales, grad.contiguous(), h, *want)
+        if grads is None:
+            grads = _lora_linear_backward(grad, x, weight, lora_a, lora_b, adapters, scales, h, *want)
         dx, da, db = (g if w else None for g, w in zip(grads, want))
         dw = None
         if ctx.needs_input_grad[1]:
@@ -165,7 +172,7 @@ def lora_linear(x: Tensor, weight: Tensor, lora_a: Tensor, lora_b: Tensor, adapt
     (-1, say) has no adapter; ``scales`` ``[L]`` fp32, 1 unless given.  fp32 to the one rounding at the end.  Differentiable in ``x``, ``weight``,
     ``lora_a`` and ``lora_b``; adapters without rows get zero gradients."""
     if not (_lora_linear.replaced or torch.compiler.is_compiling()):
-        out = (_native._host or _native.host()).lora_linear(x, weight, lora_a, lora_b, adapters, scales)
+        out = (_native._host or _native.host()).lora_linear(x, weight, lora_a, lora_b, adapters, scales, False)
         if out is not None:
             return out
     _check(x, weight, lora_a, lora_b, adapters, scales)
