@@ -145,10 +145,10 @@ def test_empty_batch_and_empty_adapters(dev):
     assert (da[0] == 0).all() and (da[2] == 0).all() and (db[0] == 0).all() and (db[2] == 0).all() and (da[1] != 0).any()
 
 
-@pytest.mark.parametrize("m", [40, 300])
-def test_rows_do_not_touch_each_other(dev, m):
+@pytest.mark.parametrize("m,dtype", [(40, BF16), (300, BF16), (300, F16)])
+def test_rows_do_not_touch_each_other(dev, m, dtype):
     """NaN in a row, or in another adapter, stays there; a row's bits do not depend on what stands beside it."""
-    x, w, a, b, g, adapters, s = make(m, 136, 72, 16, 5, BF16, 12, dev, "each")
+    x, w, a, b, g, adapters, s = make(m, 136, 72, 16, 5, dtype, 12, dev, "each")
     plain = ops.lora_linear(x, w, a, b, adapters, s)
     y = x.clone()
     y[7] = float("nan")
@@ -165,6 +165,59 @@ def test_rows_do_not_touch_each_other(dev, m):
     got = ops.lora_linear(x, w, a, bad, adapters, s)
     rest = adapters != 2
     assert torch.equal(got[rest], plain[rest]) and torch.isnan(got[~rest]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_broken_adapter_in_the_backward_pass(dev, dtype):
+    """Its own gradients, and those of its rows, are what the formulas say; nobody else's change."""
+    t = make(200, 136, 72, 16, 5, dtype, 18, dev, "each")
+    x, w, a, b, g, adapters, s = t
+    _, dx, da, db = run(*t)
+    bad = a.clone()
+    bad[1, 3, 5] = float("nan")
+    _, dx2, da2, db2 = run(x, w, bad, b, g, adapters, s)
+    others, rest = torch.arange(5, device=dev) != 1, adapters != 1
+    assert torch.equal(dx2[rest], dx[rest]) and torch.isnan(dx2[~rest][:, 5]).all()
+    assert torch.equal(da2, da)  # (dA reads B, x and the gradient)
+    assert torch.equal(db2[others], db[others]) and torch.isnan(db2[1][:, 3]).all()
+    bad = b.clone()
+    bad[4] = float("inf")
+    _, dx2, da2, db2 = run(x, w, a, bad, g, adapters, s)
+    others, rest = torch.arange(5, device=dev) != 4, adapters != 4
+    assert torch.equal(dx2[rest], dx[rest]) and not torch.isfinite(dx2[~rest]).any()
+    assert torch.equal(da2[others], da[others]) and torch.equal(db2, db)
+
+
+def test_another_stream_and_a_side_effect_free_call(dev):
+    x, w, a, b, g, adapters, s = make(120, 64, 64, 16, 3, BF16, 19, dev)
+    want = ops.lora_linear(x, w, a, b, adapters, s)
+    kept = [t.clone() for t in (x, w, a, b, adapters, s)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.lora_linear(x, w, a, b, adapters, s)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and all(torch.equal(p, q) for p, q in zip(kept, (x, w, a, b, adapters, s)))
+
+
+def test_compiled(dev):
+    x, w, a, b, g, adapters, s = make(90, 64, 72, 16, 3, BF16, 21, dev)
+    want = run(x, w, a, b, g, adapters, s)
+    call = torch.compile(lambda x, a, b: ops.lora_linear(x, w, a, b, adapters, s) * 1.0, fullgraph=True, backend="aot_eager")
+    leaves = [t.clone().requires_grad_(True) for t in (x, a, b)]
+    out = call(*leaves)
+    got = torch.autograd.grad(out, leaves, g)
+    assert all(torch.equal(p, q) for p, q in zip((out.detach(), *got), want))
+    with torch.no_grad():
+        assert torch.equal(call(x, a, b), want[0])
+
+
+def test_the_native_path_and_the_operator_agree(dev):
+    for m in (3, 200):
+        x, w, a, b, g, adapters, s = make(m, 64, 72, 16, 3, F16, 22, dev)
+        assert torch.equal(ops.lora_linear(x, w, a, b, adapters, s), torch.ops.moe.lora_linear(x, w, a, b, adapters, s))
+        _, h = torch.ops.moe.lora_linear_hidden(x, w, a, b, adapters, s)
+        assert all(torch.equal(p, q) for p, q in zip(run(x, w, a, b, g, adapters, s)[1:], torch.ops.moe.lora_linear_backward(g, x, w, a, b, adapters, s, h, True, True, True)))
 
 
 def test_strided_operands(dev):

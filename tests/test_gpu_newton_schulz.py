@@ -104,8 +104,8 @@ def test_one_step(dev, shape, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_one_step_of_wide_tiles(dev, dtype):
-    """Stacks large enough for 256 x 256 tiles, below and beside the diagonal, with tails."""
-    for shape in ((70, 300, 520), (40, 700, 264)):
+    """Stacks large enough for tiles of 128 and of 256, below and beside the diagonal, with tails."""
+    for shape in ((70, 300, 520), (40, 700, 264), (40, 1000, 1304), (24, 1800, 1100)):
         x = make(shape, "random", dtype, 5, dev)
         got = ops.orthogonalize(x, steps=1)
         pick = [0, shape[0] // 2, shape[0] - 1]
@@ -141,6 +141,36 @@ def test_strided_input(dev):
     x = make((3, 60, 100), "random", torch.bfloat16, 4, dev)
     assert torch.equal(ops.orthogonalize(x[:, ::2, 5:90]), ops.orthogonalize(x[:, ::2, 5:90].contiguous()))
     assert torch.equal(ops.orthogonalize(x.transpose(1, 2)), ops.orthogonalize(x.transpose(1, 2).contiguous()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_matrices_that_begin_anywhere(dev, dtype):
+    """Contiguous stacks that are not aligned to 16 bytes, as slices of a flat buffer are."""
+    for shape in ((2, 24, 40), (3, 40, 24), (2, 33, 17)):
+        flat = torch.zeros(shape[0] * shape[1] * shape[2] + 8, dtype=dtype, device=dev)
+        x = make(shape, "random", dtype, 8, dev)
+        part = flat[1:1 + x.numel()].view(shape)
+        part.copy_(x)
+        assert part.data_ptr() % 16 != 0
+        assert torch.equal(ops.orthogonalize(part), ops.orthogonalize(x))
+        whole, mom = x.clone(), torch.zeros(shape, device=dev)
+        ops.muon_update(whole, x, mom, 0.1)
+        odd = torch.zeros(x.numel() + 8, device=dev)[1:1 + x.numel()].view(shape)
+        w = flat.clone()[1:1 + x.numel()].view(shape)
+        ops.muon_update(w, part, odd, 0.1)
+        assert torch.equal(w, whole) and torch.equal(odd, mom)
+        assert (flat[0] == 0) and (flat[1 + x.numel():] == 0).all()
+
+
+def test_shared_memory_is_refused(dev):
+    w = make((2, 16, 16), "random", torch.float32, 9, dev)
+    m = torch.zeros_like(w)
+    for args in ((w, m, m), (w, w, m), (m, w, m)):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.muon_update(*args, 0.1)
+    both = torch.zeros(3, 16, 16, device=dev)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.muon_update(both[:2], w, both[1:], 0.1)
 
 
 def test_zeros_nan_and_infinity_stay_in_their_matrix(dev):

@@ -29,6 +29,7 @@ constexpr float kNsScale = 1024.f, kNsInv2 = 1.f / (1024.f * 1024.f);
 struct NsTarget {
   void* out;
   int dt, weight;  // dt 0 bf16, 1 fp16, 2 fp32
+  int whole;       // eight elements of a row are whole and aligned to 16 bytes
   float keep, step;
 };
 
@@ -110,21 +111,16 @@ template <bool VEC> TGG_DEV void ns_store8(void* p, int64_t i, int dt, const flo
       }
   }
 }
+// Fused operations of steps are written out here and in ns_mix: which product the compiler fuses may differ between variants, and an unaligned matrix has to
+// get an aligned one's bits.
+TGG_DEV float ns_stepped(const NsTarget& t, float old, float v) { return __builtin_fmaf(-t.step, v, t.keep * old); }
 // n (up to 8) neighbouring results at element o; v in the planes' scale.  whole: all eight, aligned
 TGG_DEV void ns_store_result(const NsTarget& t, int64_t o, float (&v)[8], int n, bool whole) {
-  if (whole) {
-    float old[8];
-    if (t.weight) ns_load8<true>(old, t.out, o, t.dt, 8);
+  float old[8];
+  if (t.weight) whole ? ns_load8<true>(old, t.out, o, t.dt, 8) : ns_load8<false>(old, t.out, o, t.dt, n);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) v[x] = t.weight ? t.keep * old[x] - t.step * (v[x] * (1.f / kNsScale)) : v[x] * (1.f / kNsScale);
-    ns_store8<true>(t.out, o, t.dt, v, 8);
-  } else {
-    float old[8];
-    if (t.weight) ns_load8<false>(old, t.out, o, t.dt, n);
-#pragma unroll
-    for (int x = 0; x < 8; ++x) v[x] = t.weight ? t.keep * old[x] - t.step * (v[x] * (1.f / kNsScale)) : v[x] * (1.f / kNsScale);
-    ns_store8<false>(t.out, o, t.dt, v, n);
-  }
+  for (int x = 0; x < 8; ++x) v[x] = t.weight ? ns_stepped(t, old[x], v[x] * (1.f / kNsScale)) : v[x] * (1.f / kNsScale);
+  whole ? ns_store8<true>(t.out, o, t.dt, v, 8) : ns_store8<false>(t.out, o, t.dt, v, n);
 }
 
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
@@ -319,7 +315,7 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
           for (int x = 0; x < 4; ++x) w[x] = (int)(p.target.dt == 0 ? pack2<DT_BF16>(v[2 * x] * by, v[2 * x + 1] * by) : pack2<DT_F16>(v[2 * x] * by, v[2 * x + 1] * by));
           store_transposed(mine, w, (uint16_t*)p.target.out + (int64_t)m * p.rows * p.cols, p.rows, rbase + 16 * i, cbase + half * HC, p.rows, p.cols, el);
         } else if (mine_too && row < p.rows && col < p.cols) {
-          ns_store_result(p.target, ((int64_t)m * p.rows + row) * p.cols + col, v, (int)lesser(8, p.cols - col), (p.cols & 7) == 0);
+          ns_store_result(p.target, ((int64_t)m * p.rows + row) * p.cols + col, v, (int)lesser(8, p.cols - col), p.target.whole);
         }
       } else {
         i32x4_t hi, lo;
@@ -403,6 +399,7 @@ struct NsSource {
   float beta, keep;  // keep = 1 - beta
   int nesterov, dt;
 };
+TGG_DEV float ns_mix(const NsSource& s, float m, float g) { return __builtin_fmaf(s.beta, m, s.keep * g); }
 // eight values of the direction; `step`: the momentum takes its step
 template <bool VEC> TGG_DEV void ns_direction(float (&v)[8], const NsSource& s, int64_t i, int n, bool step) {
   ns_load8<VEC>(v, s.x, i, s.dt, n);
@@ -411,11 +408,11 @@ template <bool VEC> TGG_DEV void ns_direction(float (&v)[8], const NsSource& s, 
   ns_load8<VEC>(m, s.momentum, i, 2, n);
   if (step) {
 #pragma unroll
-    for (int x = 0; x < 8; ++x) m[x] = s.beta * m[x] + s.keep * v[x];
+    for (int x = 0; x < 8; ++x) m[x] = ns_mix(s, m[x], v[x]);
     ns_store8<VEC>(s.momentum, i, 2, m, n);
   }
 #pragma unroll
-  for (int x = 0; x < 8; ++x) v[x] = s.nesterov ? s.beta * m[x] + s.keep * v[x] : m[x];
+  for (int x = 0; x < 8; ++x) v[x] = s.nesterov ? ns_mix(s, m[x], v[x]) : m[x];
 }
 
 // Sums of squares of a matrix's chunks, in 64 bits (values far from 1 have no squares in fp32); with momentum, its step.  VEC: matrices are multiples of eight values.
@@ -530,7 +527,7 @@ template <bool VEC> __global__ __launch_bounds__(kNsThreads) void ns_store_kerne
       float old[8];
       ns_load8<VEC>(old, o.out, i, o.dt, n);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) v[q][x] = o.keep * old[x] - o.step * v[q][x];
+      for (int x = 0; x < 8; ++x) v[q][x] = ns_stepped(o, old[x], v[q][x]);
     }
     ns_store8<VEC>(o.out, i, o.dt, v[q], n);
   }
@@ -646,9 +643,9 @@ int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, i
   if (vec_in && vec_rows) ns_load_kernel<true><<<load_grid, threads, 0, s>>>(src, rows, cols, q.tall, q.chunks, sums, eps, xs[0][0], xs[0][1], (int64_t)q.m * q.ldn, q.ldn, tr, tc);
   else ns_load_kernel<false><<<load_grid, threads, 0, s>>>(src, rows, cols, q.tall, q.chunks, sums, eps, xs[0][0], xs[0][1], (int64_t)q.m * q.ldn, q.ldn, tr, tc);
   if (int e = check_launch("ns_load")) return e;
-  const NsTarget dst = {out, out_dt, weight, keep, step};
+  const NsTarget dst = {out, out_dt, weight, vec_rows && aligned16(out), keep, step};
   // the last step's update writes rows of the result; transposed ones if they are plain 16-bit values in whole eights
-  const bool direct = steps > 0 && (q.tall ? !weight && out_dt != 2 && (q.m & 7) == 0 && aligned16(out) : aligned16(out));
+  const bool direct = steps > 0 && (q.tall ? !weight && out_dt != 2 && (q.m & 7) == 0 && aligned16(out) : true);
   const int64_t xstride = (int64_t)q.m * q.ldn, gstride = (int64_t)q.m * q.ldm;
   for (int i = 0; i < steps; ++i) {
     uint16_t **from = xs[i & 1], **to = xs[(i + 1) & 1];
@@ -680,7 +677,7 @@ int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, i
   }
   const int sr = (rows + 63) / 64, sc = (cols + 63) / 64;
   const dim3 store_grid((unsigned)(batch * sr * sc));
-  if (vec_rows && aligned16(out)) ns_store_kernel<true><<<store_grid, threads, 0, s>>>(dst, rows, cols, q.tall, xs[steps & 1][0], xs[steps & 1][1], xstride, q.ldn, sr, sc);
+  if (dst.whole) ns_store_kernel<true><<<store_grid, threads, 0, s>>>(dst, rows, cols, q.tall, xs[steps & 1][0], xs[steps & 1][1], xstride, q.ldn, sr, sc);
   else ns_store_kernel<false><<<store_grid, threads, 0, s>>>(dst, rows, cols, q.tall, xs[steps & 1][0], xs[steps & 1][1], xstride, q.ldn, sr, sc);
   return check_launch("ns_store");
 }

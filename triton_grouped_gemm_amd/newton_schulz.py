@@ -74,7 +74,7 @@ def orthogonalize(x: Tensor, steps: int = 5, coefficients: Sequence[float] = COE
     """Every matrix of ``x`` ``[..., rows, columns]`` (bf16, fp16 or fp32, any sizes up to 65536) after ``steps`` Newton-Schulz products, in its type.
 
     Results in fp16 and fp32 are as good as fp32 products; those in bf16 are multiplied in half precision (22 bits where values are carried
-    over), which stays below their own rounding.  A matrix of zeros stays one; one with a NaN or an infinity becomes
+    over), which stays below their own rounding.  A matrix of zeros stays one (unless ``eps`` is 0); one with a NaN or an infinity becomes
     NaN, and no other of the stack is touched by it.  ``coefficients`` have to keep singular values near 1 (entries below 64).  Not differentiable."""
     coefficients = tuple(float(v) for v in coefficients)
     steps, eps = int(steps), float(eps)
@@ -89,6 +89,8 @@ def _muon_update(weight: Tensor, grad: Tensor, momentum: Tensor, keep: float, st
     batch, rows, cols = _check_muon(weight, grad, momentum, steps, (a, b, c), eps)
     require_gpu(weight, grad, momentum)
     grad = grad.contiguous()
+    if any(_overlap(p, q) for p, q in ((weight, momentum), (grad, momentum), (weight, grad))):
+        raise ValueError("weight, grad and momentum must not share memory")
     if batch:
         with torch.cuda.device(weight.device):
             workspace, need = _workspace(batch, rows, cols, weight.device)
@@ -100,6 +102,11 @@ def _muon_update(weight: Tensor, grad: Tensor, momentum: Tensor, keep: float, st
 @_muon_update.register_fake
 def _(weight, grad, momentum, keep, step, beta, nesterov, steps, a, b, c, eps):
     return None
+
+
+def _overlap(p: Tensor, q: Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    return p.data_ptr() < q.data_ptr() + q.numel() * q.element_size() and q.data_ptr() < p.data_ptr() + p.numel() * p.element_size()
 
 
 def _check_muon(weight: Tensor, grad: Tensor, momentum: Tensor, steps: int, coefficients: Sequence[float], eps: float) -> Tuple[int, int, int]:
@@ -124,7 +131,7 @@ def muon_update(weight: Tensor, grad: Tensor, momentum: Tensor, lr: float, beta:
         u        = beta momentum + (1 - beta) grad   with ``nesterov``, else momentum
         weight   = (1 - lr weight_decay) weight - lr scale orthogonalize(u)
 
-    ``momentum`` is fp32; ``weight`` and ``grad`` are bf16, fp16 or fp32 each.  ``scale`` is ``sqrt(max(1, rows / columns))`` unless given.  The
+    ``momentum`` is fp32; ``weight`` and ``grad`` are bf16, fp16 or fp32 each.  ``scale`` is ``sqrt(max(1, rows / columns))`` unless given.  ``momentum``, ``weight`` and ``grad`` do not share memory.  The
     direction is as exact as ``weight``'s type asks for (see ``orthogonalize``) and the weights are rounded once."""
     coefficients = tuple(float(v) for v in coefficients)
     steps, eps, beta = int(steps), float(eps), float(beta)
