@@ -268,7 +268,7 @@ int tgg_moe_router_bwd(const void* logits, int64_t row_stride, const float* prob
 /* Low-rank adapters of many requests beside a shared projection (dtype TGG_BF16 or TGG_F16):
  *   out[m] = W x[m] + scales[l] B_l (A_l x[m]),  l = adapters[m];  rows whose entry is outside [0, L) have no adapter
  * x [M, K], w [N, K], a [L, R, K], b [L, N, R], adapters [M] int32 or int64, scales [L] fp32 or null (1), out [M, N]; rows in any order.  One rounding, at the
- * end.  N and K multiples of 8 up to 65536, R a multiple of 8 up to 128, L up to 1024.  h [M, R] fp32 (or null) receives scales[l] A_l x[m], zeros without an
+ * end.  N and K multiples of 8 up to 65536, R a multiple of 8 up to 128, L up to 1024, M below 2^27.  h [M, R] fp32 (or null) receives scales[l] A_l x[m], zeros without an
  * adapter, which the backward pass takes.
  * _bwd: dx [M, K] = W^T g + A_l^T dh, da [L, R, K] = sum of dh[m] x[m]^T, db [L, N, R] = sum of g[m] h[m]^T over each adapter's rows, with
  * dh[m] = scales[l] B_l^T g[m]; any of the three may be null (x is read for da, w for dx, h for db).  Adapters without rows get zeros.
@@ -282,13 +282,13 @@ int tgg_lora_linear_bwd(const void* grad, const void* x, const void* w, const vo
 
 /* Newton-Schulz orthogonalisation of every matrix of a stack [batch, rows, cols] (contiguous; dtype TGG_BF16, TGG_F16 or 2 = fp32):
  *   X = x / (|x|_F + eps), then `steps` times  G = X X^T, X = a X + (b G + c G^2) X   (of the transposed matrix where rows > cols: the same matrix),
- * out in x's type.  Held in 22 bits or more throughout; results in fp16 and fp32 are as good as fp32 products, those in bf16
- * are multiplied in half precision where that stays below their own rounding.  Values must keep |X| entries below 64 and those of the polynomial
+ * out in x's type (out may be x).  X is carried from step to step in 22 bits; results in fp16 and fp32 are as good as fp32 products, those in bf16
+ * are multiplied in half precision (11 bits), which stays below their own rounding.  Values must keep |X| entries below 64 and those of the polynomial
  * below 64 (any coefficients that keep singular values near 1 do); beyond, results are not finite.
  * tgg_muon_update: the optimiser's step, in place:
  *   momentum = beta momentum + (1 - beta) grad (fp32);  u = nesterov ? beta momentum + (1 - beta) grad : momentum;
  *   weight = keep weight - step X(u), rounded once to its type
- * grad and weight in types of their own.  Rows and columns up to 65536.  The workspace (256-byte aligned; size from
+ * grad and weight in types of their own; the three share no memory.  Rows and columns up to 65536, stacks of fewer than 2^24 blocks of 64 x 64 values.  The workspace (256-byte aligned; size from
  * tgg_newton_schulz_workspace_bytes) is in use until the call's kernels are done.  The reference has no optimiser. */
 int tgg_newton_schulz_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int64_t* bytes);
 int tgg_newton_schulz(const void* x, void* out, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c, float eps, int dtype, void* workspace,

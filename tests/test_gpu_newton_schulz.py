@@ -43,7 +43,7 @@ def one_step(x, ex, precise, coefficients):
     shift = g.diagonal().abs().max()
     gs = g.abs() + shift * eye
     p = b * g + c * (g @ g)
-    ep = abs(b) * eg + abs(c) * (gm * (gs @ gs) + 2 * g.abs() @ eg) + 2.0 ** -21 * (abs(b) + 2 * abs(c) * shift) * gs
+    ep = abs(b) * eg + abs(c) * (gm * (gs @ gs) + 2 * g.abs() @ eg) + h * (abs(b) + 2 * abs(c) * shift) * gs  # (the linear term takes A as the products do)
     ps = p.abs() + p.diagonal().abs().max() * eye
     out = a * x + p @ x
     eo = abs(a) * ex + gm * (ps @ ax) + ep @ ax + ps @ ex + 2.0 ** -21 * out.abs() + 2.0 ** -30

@@ -35,6 +35,7 @@ def test_c_abi_forward(p):
     call("L=1025", L=1025)
     call("M=-1", M=-1)
     call("M=2147483648", M=1 << 31)
+    call("M=134217728", M=1 << 27)  # 512 threads for 16 rows, and fewer than 2^32 in a launch
     call("not supported", dt=2)
     call("16-byte aligned", x=p + 8)
     call("16-byte aligned", h=p + 8)

@@ -38,6 +38,11 @@ def test_workspace_holds_the_planes():
         refused("bad stack", "tgg_newton_schulz_workspace_bytes", *shape, ctypes.addressof(need))
     refused("at most 65536", "tgg_newton_schulz_workspace_bytes", 1, 65537, 5, ctypes.addressof(need))
     refused("too large", "tgg_newton_schulz_workspace_bytes", 1 << 31, 8, 8, ctypes.addressof(need))
+    # launches of fewer than 2^32 threads, 256 for a block of 64 x 64 values; nothing of a call may run where a later launch of it cannot
+    refused("too large", "tgg_newton_schulz_workspace_bytes", 1 << 62, 65536, 65536, ctypes.addressof(need))
+    refused("too large", "tgg_newton_schulz_workspace_bytes", 1 << 24, 1, 1, ctypes.addressof(need))
+    refused("too large", "tgg_newton_schulz_workspace_bytes", 1 << 14, 65536, 1, ctypes.addressof(need))
+    assert workspace((1 << 24) - 1, 1, 1) > 0 and workspace(15, 65536, 65536) > 0
 
 
 def test_newton_schulz_c_abi(p):

@@ -797,7 +797,8 @@ int tgg_moe_router_bwd(const void* logits, int64_t row_stride, const float* prob
 
 // ---- low-rank adapters ------------------------------------------------------------------------------------------
 static int lora_check(int64_t M, int64_t N, int64_t K, int R, int L) {
-  if (M < 0 || M >= (1ll << 31)) return set_error("M=%lld outside [0, 2^31)", (long long)M);
+  // lora_down: a workgroup of 512 threads for 16 rows, and a launch has fewer than 2^32 threads
+  if (M < 0 || M >= (1ll << 27)) return set_error("M=%lld outside [0, 2^27)", (long long)M);
   if (N < 8 || K < 8 || (N & 7) || (K & 7)) return set_error("N and K must be positive multiples of 8, got N=%lld K=%lld", (long long)N, (long long)K);
   if (N > 65536 || K > 65536) return set_error("N=%lld or K=%lld: at most 65536 is supported", (long long)N, (long long)K);
   if (R < 8 || R > 128 || (R & 7)) return set_error("the rank must be a multiple of 8 in [8, 128], got %d", R);
@@ -851,8 +852,8 @@ static int newton_schulz_check(int64_t batch, int64_t rows, int64_t cols) {
   constexpr int64_t most = 1 << 16;
   if (batch < 0 || rows < 1 || cols < 1) return set_error("bad stack of %lld matrices of %lld x %lld", (long long)batch, (long long)rows, (long long)cols);
   if (rows > most || cols > most) return set_error("matrices of %lld x %lld: at most %lld rows and columns are supported", (long long)rows, (long long)cols, (long long)most);
-  // one workgroup for 64 x 64 values or 16384 of them, numbered in 31 bits
-  if (batch * (((rows + 63) / 64 + 1) * ((cols + 63) / 64 + 1)) >= (1ll << 31) || batch >= (1ll << 31)) return set_error("a stack of %lld matrices of %lld x %lld is too large", (long long)batch, (long long)rows, (long long)cols);
+  // a workgroup of 256 threads for 64 x 64 values (of rows padded to eights), and a launch has fewer than 2^32 threads
+  if (batch >= (1ll << 24) || batch * (((rows + 7 + 63) / 64) * ((cols + 7 + 63) / 64)) >= (1ll << 24)) return set_error("a stack of %lld matrices of %lld x %lld is too large", (long long)batch, (long long)rows, (long long)cols);
   return 0;
 }
 

@@ -712,22 +712,19 @@ template <int DT> __global__ __launch_bounds__(256) void lora_join_kernel(const 
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
-template <class Kern, class P> int launch_smem(Kern kern, int smem, bool& attr_done, dim3 grid, int threads, const P& p, hipStream_t s, const char* what) {
-  if (!attr_done) {
-    if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess) return check_launch("hipFuncSetAttribute(lora)");
-    attr_done = true;
-  }
+template <class Kern, class P> int launch_smem(Kern kern, int smem, bool (&attr_set)[64], dim3 grid, int threads, const P& p, hipStream_t s, const char* what) {
+  if (int e = stream_lds(kern, smem, attr_set)) return e;
   kern<<<grid, dim3(threads), smem, s>>>(p);
   return check_launch(what);
 }
 
 template <int DT, int RB, int RC> int down_launch(const DownParams& p, hipStream_t s) {
-  static bool attr_done = false;
+  static bool attr_set[64] = {false};
   constexpr int smem = ChunkRing<RB, RC, down_stages(RB + RC)>::BYTES;
   const int64_t blocks = (p.M + 16 * RB - 1) / (16 * RB);
   // few rows: their adapters side by side
   const int turns = RB > 1 || blocks >= 1024 ? 1 : (int)lesser(16, 1024 / blocks);
-  return launch_smem(lora_down_kernel<DT, RB, RC>, smem, attr_done, dim3((unsigned)blocks, turns, p.parts), kDownThreads, p, s, "lora_down");
+  return launch_smem(lora_down_kernel<DT, RB, RC>, smem, attr_set, dim3((unsigned)blocks, turns, p.parts), kDownThreads, p, s, "lora_down");
 }
 
 template <int DT> int launch_down(const DownParams& p, hipStream_t s) {
@@ -742,9 +739,9 @@ typedef StreamCfg<128, 128, 2, 4> LoraNarrow;
 
 template <class C, int DT, bool NT> int gemm_launch(const LoraGemm& p, hipStream_t s) {
   typedef LoraProblem<C, DT, NT> P;
-  static bool attr_done = false;
+  static bool attr_set[64] = {false};
   const int tiles = p.tiles_m * p.tiles_n, slots = num_cus() * (C::BM == 128 ? 2 : 1);
-  return launch_smem(lora_gemm_kernel<C, DT, NT>, P::SMEM_BYTES, attr_done, dim3(tiles < slots ? tiles : slots), C::THREADS, p, s, "lora_gemm");
+  return launch_smem(lora_gemm_kernel<C, DT, NT>, P::SMEM_BYTES, attr_set, dim3(tiles < slots ? tiles : slots), C::THREADS, p, s, "lora_gemm");
 }
 
 template <int DT, bool NT> int launch_gemm(LoraGemm p, int tile, hipStream_t s) {
@@ -764,16 +761,16 @@ bool few_rows(int64_t M) { return M <= 64; }
 int few_parts(int64_t M) { return M <= 16 ? 4 : 2; }  // parts of the depth in lora_down: more workgroups for few rows
 
 template <int DT, int RB> int few_launch(const FewParams& p, hipStream_t s) {
-  static bool attr_done = false;
+  static bool attr_set[64] = {false};
   constexpr int smem = ChunkRing<RB, 1, (RB == 1 ? 6 : RB == 2 ? 5 : 3)>::BYTES;
-  return launch_smem(lora_few_kernel<DT, RB>, smem, attr_done, dim3((p.N + 15) / 16, (unsigned)((p.M + 16 * RB - 1) / (16 * RB))), kFewThreads, p, s, "lora_few");
+  return launch_smem(lora_few_kernel<DT, RB>, smem, attr_set, dim3((p.N + 15) / 16, (unsigned)((p.M + 16 * RB - 1) / (16 * RB))), kFewThreads, p, s, "lora_few");
 }
 template <int DT> int launch_few(const FewParams& p, hipStream_t s) { return p.M <= 16 ? few_launch<DT, 1>(p, s) : p.M <= 32 ? few_launch<DT, 2>(p, s) : few_launch<DT, 4>(p, s); }
 
 template <int DT, int RC> int outer_launch(const OuterParams& p, dim3 grid, hipStream_t s) {
   constexpr int smem = 2 * kOuterRows * kOuterCols * 2 + 2 * kOuterRows * (RC * 32 + 16) + kOuterWindow * 2 + kOuterWaves * 8;
-  static bool attr_done = false;
-  return launch_smem(lora_outer_kernel<DT, RC>, smem, attr_done, grid, kOuterThreads, p, s, "lora_outer");
+  static bool attr_set[64] = {false};
+  return launch_smem(lora_outer_kernel<DT, RC>, smem, attr_set, grid, kOuterThreads, p, s, "lora_outer");
 }
 
 // parts of the rows: enough workgroups for the chip, none of fewer than 1024 rows
@@ -839,9 +836,7 @@ template <int DT> int backward(const void* grad, const void* x, const void* w, c
     DownParams d = {};
     d.x = grad; d.a = ws + q.bt; d.scales = scales; d.ids = ids; d.M = M; d.R = R; d.depth = N; d.parts = 1;
     d.h = (float*)(ws + q.h);
-    if (dx) {
-      d.planes = (uint16_t*)(ws + q.planes);
-      }
+    if (dx) d.planes = (uint16_t*)(ws + q.planes);
     if (int e = launch_down<DT>(d, s)) return e;
     if (dx) {
       LoraGemm g = {};

@@ -539,11 +539,8 @@ typedef StreamCfg<64, 64, 2, 4, 8> NsSmall;
 
 template <class C, int MODE, bool PRECISE> int ns_launch(const NsProduct& p, hipStream_t s) {
   typedef NsProblem<C, MODE, PRECISE> P;
-  static bool attr_done = false;
-  if (!attr_done) {
-    if (hipFuncSetAttribute((const void*)ns_product_kernel<C, MODE, PRECISE>, hipFuncAttributeMaxDynamicSharedMemorySize, P::SMEM_BYTES) != hipSuccess) return check_launch("hipFuncSetAttribute(ns_product)");
-    attr_done = true;
-  }
+  static bool attr_set[64] = {false};
+  if (int e = stream_lds(ns_product_kernel<C, MODE, PRECISE>, P::SMEM_BYTES, attr_set)) return e;
   const int tm = (p.rows + C::BM - 1) / C::BM, tn = (p.cols + C::BN - 1) / C::BN;
   const int64_t tiles = (int64_t)p.batch * (P::SYM ? tm * (tm + 1) / 2 : tm * tn);
   const int slots = num_cus() * (int)(160 * 1024 / P::SMEM_BYTES);

@@ -16,12 +16,24 @@
 // A [rows, K] is K-contiguous; B is K-contiguous rows [columns, K] (B_KMAJOR) or token rows [K, columns].
 #pragma once
 #include "fast_common.hpp"
+#include "launch.hpp"
 
 namespace tgg {
 
 // (min and max of two 64-bit numbers: the runtime's own are for 32-bit ones in host code and cut them off)
 __host__ __device__ constexpr int64_t lesser(int64_t a, int64_t b) { return a < b ? a : b; }
 __host__ __device__ constexpr int64_t larger(int64_t a, int64_t b) { return a < b ? b : a; }
+
+// a kernel's dynamic LDS beyond the default limit: once for each device
+template <class Kern> int stream_lds(Kern kern, int bytes, bool (&attr_set)[64]) {
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  const bool listed = dev >= 0 && dev < 64;
+  if (listed && attr_set[dev]) return 0;
+  if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return check_launch("hipFuncSetAttribute(stream)");
+  if (listed) attr_set[dev] = true;
+  return 0;
+}
 
 template <int BM_, int BN_, int WM_, int WN_, int RING_ = 2> struct StreamCfg {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;

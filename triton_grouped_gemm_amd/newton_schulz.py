@@ -73,8 +73,8 @@ def _(x, steps, a, b, c, eps):
 def orthogonalize(x: Tensor, steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS, eps: float = 1e-7) -> Tensor:
     """Every matrix of ``x`` ``[..., rows, columns]`` (bf16, fp16 or fp32, any sizes up to 65536) after ``steps`` Newton-Schulz products, in its type.
 
-    Results in fp16 and fp32 are as good as fp32 products; those in bf16 are multiplied in half precision (22 bits where values are carried
-    over), which stays below their own rounding.  A matrix of zeros stays one (unless ``eps`` is 0); one with a NaN or an infinity becomes
+    Results in fp16 and fp32 are as good as fp32 products; those in bf16 are multiplied in half precision (11 bits; 22 where values are carried
+    from step to step), which stays below their own rounding.  A matrix of zeros stays one (unless ``eps`` is 0); one with a NaN or an infinity becomes
     NaN, and no other of the stack is touched by it.  ``coefficients`` have to keep singular values near 1 (entries below 64).  Not differentiable."""
     coefficients = tuple(float(v) for v in coefficients)
     steps, eps = int(steps), float(eps)
