@@ -27,6 +27,11 @@ CASES = [
     (513, 1544, 8, 16, 200, BF16, "each", False),
     (1000, 136, 136, 24, 1024, F16, "each", True),
     (700, 128, 392, 72, 6, BF16, "none", False),
+    (127, 520, 264, 16, 100, BF16, "each", True),
+    (129, 520, 264, 16, 100, BF16, "each", True),
+    (140, 72, 64, 16, 4, F16, "mixed", True),
+    (8200, 136, 264, 40, 3, BF16, "mixed", True),
+    (8193, 72, 136, 64, 2, F16, "runs", False),
 ]
 
 
@@ -51,6 +56,15 @@ def test_forward_and_gradients(dev, m, n, k, r, count, dtype, ids, scales):
 def test_wide_tiles_and_parts_of_the_rows(dev, dtype, ids):
     """Enough tiles for the wide ones in both directions; the adapters' gradients are summed in parts."""
     t = make(6001, 2568, 4104, 16, 5, dtype, 2, dev, ids)
+    want = reference(*t, dtype)
+    for name, got in zip(("out", "dx", "da", "db"), run(*t)):
+        check(name, got, *want[name])
+
+
+@pytest.mark.parametrize("m,dtype,ids", [(6001, BF16, "mixed"), (6001, F16, "runs"), (1025, BF16, "runs"), (513, F16, "0")])
+def test_gradients_in_parts_of_the_rows(dev, m, dtype, ids):
+    """Few columns: the rows are shared out over many workgroups, of which some have no row of an adapter."""
+    t = make(m, 264, 392, 24, 2, dtype, 5, dev, ids)
     want = reference(*t, dtype)
     for name, got in zip(("out", "dx", "da", "db"), run(*t)):
         check(name, got, *want[name])

@@ -730,8 +730,10 @@ template <int DT, int RB, int RC> int down_launch(const DownParams& p, hipStream
 template <int DT> int launch_down(const DownParams& p, hipStream_t s) {
   const int rc = (p.R + 15) / 16;
   if (rc > 4) return down_launch<DT, 1, 8>(p, s);
-  if (p.M >= 4096) return rc <= 1 ? down_launch<DT, 2, 1>(p, s) : rc <= 2 ? down_launch<DT, 2, 2>(p, s) : down_launch<DT, 2, 4>(p, s);  // 32 rows a workgroup read the adapter half as often
-  return rc <= 1 ? down_launch<DT, 1, 1>(p, s) : rc <= 2 ? down_launch<DT, 1, 2>(p, s) : down_launch<DT, 1, 4>(p, s);
+  // 32 rows a workgroup read the adapter half as often, which pays where its chunks are the larger part and the chip is full anyway: depth 4096, rank 64, with the product behind it, 16384 rows
+  // 117 us (16 rows: 126), 4096 rows 88 (87); rank 16, 16384 rows 95 (92).
+  if (rc > 2) return p.M >= 8192 ? down_launch<DT, 2, 4>(p, s) : down_launch<DT, 1, 4>(p, s);
+  return rc <= 1 ? down_launch<DT, 1, 1>(p, s) : down_launch<DT, 1, 2>(p, s);
 }
 
 typedef StreamCfg<256, 256, 2, 4> LoraWide;
@@ -757,8 +759,10 @@ int tile_of(int64_t M, int cols) {
   return (tiles(256) + cus - 1) / cus * 3 <= (tiles(128) + 2 * cus - 1) / (2 * cus) * 2 ? 256 : 128;
 }
 
-bool few_rows(int64_t M) { return M <= 64; }
-int few_parts(int64_t M) { return M <= 16 ? 4 : 2; }  // parts of the depth in lora_down: more workgroups for few rows
+// lora_few up to 128 rows.  It reads W once for 64 rows, and rows of many adapters cost it little: 4096 x 4096, every row another adapter, 64 rows 26 us (lora_gemm: 124), 128 rows 39 (128), 256 rows
+// 65 (126); 2048 x 8192, one adapter, 64 rows 29 (42), 128 rows 45 (43).
+bool few_rows(int64_t M) { return M <= 128; }
+constexpr int kFewParts = 2;  // parts of the depth in lora_down for few rows: more workgroups, 64 rows of 4096 25.9 us in 2 parts, 26.7 in 1 and 26.4 in 4
 
 template <int DT, int RB> int few_launch(const FewParams& p, hipStream_t s) {
   static bool attr_set[64] = {false};
@@ -773,11 +777,11 @@ template <int DT, int RC> int outer_launch(const OuterParams& p, dim3 grid, hipS
   return launch_smem(lora_outer_kernel<DT, RC>, smem, attr_set, grid, kOuterThreads, p, s, "lora_outer");
 }
 
-// parts of the rows: enough workgroups for the chip, none of fewer than 1024 rows
+// Parts of the rows: two workgroups a compute unit at most, each looking through 512 rows at least; adding parts costs a pass over them.  Backward passes: 2048 rows of 16 adapters (448 workgroups a part)
+// 56 us in one part, 67 in two; 16384 rows of 8 (512) 117 and 134; 32768 rows of 4 (64) 112, 93, 103 and 112 in 4, 8, 16 and 32 parts; 4096 rows of 256 x 256, 2 adapters (8) 42, 34, 31 and 33 in 2, 4, 8 and 16.
 int outer_parts(int64_t M, int N, int K, int L) {
   const int64_t groups = (int64_t)L * ((N + kOuterCols - 1) / kOuterCols + (K + kOuterCols - 1) / kOuterCols);
-  int64_t parts = (4 * num_cus() + groups - 1) / groups;
-  parts = lesser(parts, (M + 1023) / 1024);
+  const int64_t parts = lesser(2 * num_cus() / groups, (M + 511) / 512);
   return (int)larger(1, lesser(parts, 64));
 }
 
@@ -790,7 +794,7 @@ LoraPlan lora_plan(bool backward, int64_t M, int N, int K, int R, int L) {
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t here = at; at += align256(bytes); return here; };
   q.tile = tile_of(M, backward ? K : N);
-  q.h = take((backward ? 1 : 4) * M * R * 4);
+  q.h = take((!backward && few_rows(M) ? kFewParts : 1) * M * R * 4);
   q.planes = take(M * R * 4);
   if (backward) {
     q.parts = outer_parts(M, N, K, L);
@@ -811,7 +815,7 @@ template <int DT> int forward(const void* x, const void* w, const void* a, const
   const bool few = few_rows(M);
   DownParams d = {};
   d.x = x; d.a = a; d.scales = scales; d.ids = ids; d.M = M; d.R = R; d.depth = K;
-  d.parts = few && !h ? few_parts(M) : 1;  // (what is kept for the backward pass is one sum)
+  d.parts = few && !h ? kFewParts : 1;  // (what is kept for the backward pass is one sum)
   d.h = h ? h : (float*)(ws + q.h);
   if (!few) d.planes = (uint16_t*)(ws + q.planes);
   if (int e = launch_down<DT>(d, s)) return e;
