@@ -61,7 +61,7 @@ def test_wide_tiles_and_parts_of_the_rows(dev, dtype, ids):
         check(name, got, *want[name])
 
 
-@pytest.mark.parametrize("m,dtype,ids", [(6001, BF16, "mixed"), (6001, F16, "runs"), (1025, BF16, "runs"), (513, F16, "0")])
+@pytest.mark.parametrize("m,dtype,ids", [(6001, BF16, "mixed"), (6001, F16, "runs"), (2050, BF16, "runs"), (1025, BF16, "runs"), (513, F16, "0")])
 def test_gradients_in_parts_of_the_rows(dev, m, dtype, ids):
     """Few columns: the rows are shared out over many workgroups, of which some have no row of an adapter."""
     t = make(m, 264, 392, 24, 2, dtype, 5, dev, ids)

@@ -777,12 +777,12 @@ template <int DT, int RC> int outer_launch(const OuterParams& p, dim3 grid, hipS
   return launch_smem(lora_outer_kernel<DT, RC>, smem, attr_set, grid, kOuterThreads, p, s, "lora_outer");
 }
 
-// Parts of the rows: two workgroups a compute unit at most, each looking through 512 rows at least; adding parts costs a pass over them.  Backward passes: 2048 rows of 16 adapters (448 workgroups a part)
-// 56 us in one part, 67 in two; 16384 rows of 8 (512) 117 and 134; 32768 rows of 4 (64) 112, 93, 103 and 112 in 4, 8, 16 and 32 parts; 4096 rows of 256 x 256, 2 adapters (8) 42, 34, 31 and 33 in 2, 4, 8 and 16.
+// Parts of the rows: 512 rows of an adapter a part on average, as adapters have unequal shares of the rows and the longest one's workgroups are waited for; adding the parts costs a pass
+// over them.  Forward and backward passes, rows in unequal requests: 16384 rows of 8 adapters, 4096 x 4096, 990, 932, 926 and 943 us in 1, 2, 4 and 8 parts; 32768 of 4, 1024 x 1024, 325, 270, 238 and
+// 241 in 4, 8, 16 and 32; 2047 of 16, 1536 x 2048, 179 and 191 in 1 and 2; 16384 of 32, 2048 x 2048, 337, 333 and 351 in 1, 2 and 8.
 int outer_parts(int64_t M, int N, int K, int L) {
   const int64_t groups = (int64_t)L * ((N + kOuterCols - 1) / kOuterCols + (K + kOuterCols - 1) / kOuterCols);
-  const int64_t parts = lesser(2 * num_cus() / groups, (M + 511) / 512);
-  return (int)larger(1, lesser(parts, 64));
+  return (int)larger(1, lesser(64, lesser(8 * num_cus() / groups, M / (512 * (int64_t)L))));
 }
 
 struct LoraPlan {
