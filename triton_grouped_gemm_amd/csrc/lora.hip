@@ -58,7 +58,7 @@ TGG_DEV float row_scale(float v) {
 
 // Chunks of 256 values of depth of a few rows of two K-contiguous operands, through a ring in LDS; the eight waves share a chunk's depth, 32 values each.  (Fragments read
 // straight from memory have every lane in another row than its neighbours, which takes the address unit 64 cycles instead of 16: 64 rows of x and 16 columns
-// of W a workgroup, 4096 x 4096: 23 us.)  Rows of 512 bytes, 16-byte pieces swizzled by the row.
+// of W a workgroup, 4096 x 4096: 23 us; through the ring 14.)  Rows of 512 bytes, 16-byte pieces swizzled by the row.
 template <int XB, int WB, int STAGES> struct ChunkRing {
   static constexpr int X_BYTES = XB * 16 * 512, STAGE_BYTES = X_BYTES + WB * 16 * 512, BYTES = STAGES * STAGE_BYTES, NC = XB + WB;  // NC: a wave's copies of a chunk
   static_assert(BYTES <= 160 * 1024 && (STAGES - 1) * NC < 64, "LDS, and copies that a wait can count");
@@ -127,7 +127,8 @@ struct DownParams {
   int R, depth, parts;
 };
 
-// RB: blocks of 16 rows, RC: blocks of 16 of R (RC * 16 >= R).  blockIdx.x: rows; y: adapters in turn; z: part of the depth.
+// RB: blocks of 16 rows, RC: blocks of 16 of R (RC * 16 >= R).  blockIdx.x: rows; y: adapters in turn; z: part of the depth.  Bound by reading the rows (16384 x 4096, rank 16: 31 us, 4.3 TB/s)
+// where they follow one another, by a ring's start for every adapter of 16 rows (and the adapters, from L2) where they are mixed: 2047 rows of 16 adapters, rank 32, depth 1536, 20 us.
 template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) void lora_down_kernel(const DownParams p) {
   constexpr int COLS = RC * 16, STAGES = down_stages(RB + RC);
   typedef ChunkRing<RB, RC, STAGES> Ring;
@@ -207,7 +208,7 @@ template <int DT, int RB, int RC> __global__ __launch_bounds__(kDownThreads) voi
   }
 }
 
-// Two stacks of L matrices, transposed: [L, rows, cols] -> [L, cols, rows]
+// Two stacks of L matrices, transposed, for the backward pass, whose sums run along the other sides (8 adapters of 4096 + 4096 columns, rank 16: 8 us): [L, rows, cols] -> [L, cols, rows]
 struct TransposeParams {
   struct { const uint16_t* in; uint16_t* out; int rows, cols, tiles_r, tiles_c; } s[2];
   int first;  // workgroups of the first stack
@@ -228,6 +229,9 @@ __global__ __launch_bounds__(256) void lora_transpose_kernel(const TransposePara
 }
 
 // ---- the shared product with the adapters' depth added ---------------------------------------------------------------------
+// 16384 rows, 4096 x 4096, rank 16: y 392 to 408 us, dx 402 to 411 (1.35 PFLOP/s, the matrix pipe 0.73 of the cycles; torch's library product of 8192 x 8192 x 8192 reaches 1.39).  Where a tile's rows are of many
+// adapters every one of them is R more values of depth in two planes (and again two for the parts of half-precision adapters): 2047 rows of 16 adapters, rank 32, 1536 x 2048, 57 and 63 us, of which the
+// adapters' part is more than half.
 
 struct LoraGemm {
   const void* x;        // [M, depth]
@@ -448,7 +452,8 @@ struct FewParams {
   int N, K, R, parts;
 };
 
-// RB blocks of 16 rows x 16 columns; the waves share the depth.
+// RB blocks of 16 rows x 16 columns; the waves share the depth.  Bound by W: 64 rows, 4096 x 4096, 14.2 us for 34 MB of W (2.4 TB/s, every compute unit reads x's 512 KB besides, from L2); one row,
+// 768 x 2048, 5.2 us, the latency of a ring's start, the adapters' part and the join of eight waves.
 template <int DT, int RB> __global__ __launch_bounds__(kFewThreads) void lora_few_kernel(const FewParams p) {
   constexpr int ROWS = RB * 16, COLS = 16, QUADS = ROWS * COLS / 4;
   typedef ChunkRing<RB, 1, RB == 1 ? 6 : RB == 2 ? 5 : 3> Ring;
@@ -525,7 +530,8 @@ struct OuterParams {
   int K, N, R, L, parts, blocks_a;
 };
 
-// blockIdx.x: 128 columns of K (dA), then of N (dB); y: adapter; z: part of the rows.  RC blocks of 16 of R.
+// blockIdx.x: 128 columns of K (dA), then of N (dB); y: adapter; z: part of the rows.  RC blocks of 16 of R.  Every workgroup lists its adapter's rows window by window, so that ids may stand in any
+// order, and sums them in the order of their numbers.  Bound by reading x and g once: 16384 rows of 8 adapters, 4096 + 4096 columns, 85 us for 268 MB (3.2 TB/s); 2047 rows of 16, 13.6 us.
 template <int DT, int RC> __global__ __launch_bounds__(kOuterThreads) void lora_outer_kernel(const OuterParams p) {
   typedef Operand<kOuterCols, false> OpZ;
   constexpr int Z_BYTES = OpZ::SLAB_BYTES, PP = RC * 32 + 16, P_BYTES = kOuterRows * PP;  // a plane of the P tile: 64 rows of RC * 16 values

@@ -2,16 +2,20 @@
 //
 //   X_0 = X / (|X|_F + eps);   G = X X^T,   X <- a X + (b G + c G^2) X      once a step
 //
-// X is taken as [M, N] with M <= N (a tall matrix is transposed on its way in and out: the iteration commutes with it).  Every X and G is held as two
+// X is taken as [M, N] with M <= N (a tall matrix is transposed on its way in and out: the iteration commutes with it).  X is carried as two
 // planes of half precision, high and low, 22 bits together, scaled by 2^10 so that the low plane keeps its bits: singular values
 // stay near or below 1, so entries do not overflow.
 //
 // Results in bfloat16 are multiplied from the high planes alone, 11 bits, with what the rounding would reach first taken out of the products:
-// the sum that carries X over, a X, and the linear term of the polynomial use both planes, and G and the polynomial enter the products less their mean diagonal, whose part is
+// the sum that carries X over, a X, uses both planes, and G and the polynomial enter products (and G the linear term), in one plane, less their mean diagonal, whose part is
 // exact:   A = G - d I,   B = (b + 2 c d) A + c (A^2 - e I),   X <- (a + b d + c d^2 + c e) X + B X,   d = |X|^2 / M,   e = |A|^2 / M.
 // The rounding of near-identity matrices is then that of what is left of them.  Errors against 64 bits, before the last rounding (random and low-rank matrices of 256 to 768 rows): 2e-4 to 1.1e-3, where
 // G and B with their diagonals give up to 2.6e-3 and bfloat16 operands 2e-2; the result's own rounding is 1.7e-3.  Results in half precision and fp32 add the products of
 // high and low planes, three multiplies for one, and are as good as fp32 products.
+//
+// A step of 64 matrices of 1536 x 2048 takes 343 us for G, 305 for the polynomial and 749 for the update; 7.2 ms in all, 0.80 PFLOP/s counting half of a symmetric product (the products alone 0.83).  The
+// matrix pipe is busy in 0.4 to 0.6 of the cycles: between tiles eight waves store results and read what they add to (25 us a tile of 256, of 1.4 us a slab of 64; without its stores an update takes 525 us),
+// and 64 x 21 triangular tiles are 5.25 rounds of the chip.  What is small is bound by latency: 512 x 512, three kernels of 8 us a step.
 //
 // G and G^2 are symmetric: only tiles on and below the diagonal are computed, and stored twice.  No sum depends on the order of arrival: norms are
 // summed per tile and the tiles' sums in order.
@@ -415,7 +419,7 @@ template <bool VEC> TGG_DEV void ns_direction(float (&v)[8], const NsSource& s, 
   for (int x = 0; x < 8; ++x) v[x] = s.nesterov ? ns_mix(s, m[x], v[x]) : m[x];
 }
 
-// Sums of squares of a matrix's chunks, in 64 bits (values far from 1 have no squares in fp32); with momentum, its step.  VEC: matrices are multiples of eight values.
+// Sums of squares of a matrix's chunks, in 64 bits (values far from 1 have no squares in fp32); with momentum, its step.  16 x 2048 x 768 with momentum 46 us for 252 MB, 64 x 1536 x 2048 76 us for 403 MB (5.3 TB/s).  VEC: matrices are multiples of eight values.
 template <bool VEC> __global__ __launch_bounds__(kNsThreads) void ns_norm_kernel(const NsSource s, int64_t values, int chunks, double* sums) {
   const int m = blockIdx.x / chunks, c = blockIdx.x % chunks;
   const int64_t first = m * values + (int64_t)c * kNsChunk, end = lesser(first + kNsChunk, (m + 1) * values);
@@ -439,7 +443,7 @@ template <bool VEC> __global__ __launch_bounds__(kNsThreads) void ns_norm_kernel
   }
 }
 
-// Tiles of 64 x 64 into the planes, transposed where the matrix is tall.  VEC: rows are multiples of eight values.
+// Tiles of 64 x 64 into the planes, transposed where the matrix is tall.  64 x 1536 x 2048: 221 us for 1.2 GB (5.5 TB/s).  VEC: rows are multiples of eight values.
 template <bool VEC> __global__ __launch_bounds__(kNsThreads) void ns_load_kernel(const NsSource s, int rows, int cols, int tall, int chunks, const double* sums, float eps, uint16_t* hi, uint16_t* lo, int64_t stride,
                                                                                  int ld, int tiles_r, int tiles_c) {
   __shared__ float tile[64][65];
@@ -570,7 +574,7 @@ struct NsPlan {
 // Tiles of 64, 128 or 256 for a product of `slabs` slabs of depth a tile: the estimated time in microseconds, from the rounds of workgroups and what a tile took.  A round of 256-row
 // tiles: 1.65 a slab and 24 for results and start; of two 128-row tiles a compute unit 1.2 and 10, of one 0.8 and 8; of one 64-row tile, with eight slabs in flight, 0.38 and 1.  Measured for stacks of
 // 1 to 64 matrices of 128 to 2048 rows, the choice was the fastest or within 3 % of it; the other tiles took 1.1 to 2.7 times as long (512 x 512: 136, 186 and 384 us in
-// tiles of 64, 128 and 256; 64 of 1536 x 2048: 22.7, 9.3 and 8.2 ms).
+// tiles of 64, 128 and 256; 64 of 1536 x 2048: 22.7, 9.3 and 8.2 ms, before the last changes to results' stores).
 int ns_tile(int64_t batch, int rows, int cols, bool sym, int64_t slabs) {
   auto tiles = [&](int b) { const int64_t tm = (rows + b - 1) / b, tn = (cols + b - 1) / b; return batch * (sym ? tm * (tm + 1) / 2 : tm * tn); };
   const int64_t cus = num_cus(), full = tiles(128) / (2 * cus), rest = tiles(128) % (2 * cus);
