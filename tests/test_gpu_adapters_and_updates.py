@@ -171,3 +171,32 @@ def test_operators_beyond_two_to_the_31_values(dev, memory_given_back):
     dh = torch.ones(1, n, dtype=torch.float64, device=dev) @ b[0].double()  # the same for every row of the adapter
     want_da = dh.t() @ x.detach()[adapters == 0].sum(0, keepdim=True, dtype=torch.float64)
     assert (da[0].double() - want_da).norm() <= 2.0 ** -7 * want_da.norm()
+
+
+def test_weights_beyond_four_gigabytes(dev, memory_given_back):
+    """The last rows and columns of shared weights and adapters at the sides' limit, in both directions."""
+    if torch.cuda.get_device_properties(dev).total_memory < 200 << 30:
+        pytest.skip("needs 200 GiB")
+    n, k, r = 65536, 65536, 16
+    gen = torch.Generator(device=dev).manual_seed(3)
+    w = torch.empty(n, k, dtype=torch.bfloat16, device=dev)
+    for i in range(0, n, 8192):
+        w[i:i + 8192] = torch.randn(8192, k, generator=gen, device=dev)
+    t = lambda *shape: torch.randn(*shape, generator=gen, device=dev).to(torch.bfloat16)
+    a, b = t(2, r, k) * 2.0 ** -4, t(2, n, r)
+    for m in (5, 150):
+        x, g = t(m, k), t(m, n)
+        adapters = (torch.arange(m, device=dev) % 3 - 1).to(torch.int32)
+        xl = x.clone().requires_grad_(True)
+        out = ops.lora_linear(xl, w, a, b, adapters)
+        dx, = torch.autograd.grad(out, xl, g)
+        has = (adapters >= 0)[:, None]
+        mine = adapters.clamp_min(0).long()
+        h = torch.stack([x[i].double() @ a[mine[i]].double().t() for i in range(m)]) * has
+        dh = torch.stack([g[i].double() @ b[mine[i]].double() for i in range(m)]) * has
+        for part in (slice(0, 64), slice(n - 64, n)):
+            want = x.double() @ w[part].double().t() + (b[:, part].double()[mine] * h[:, None, :]).sum(-1)
+            want_dx = g.double() @ w[:, part].double() + (a[:, :, part].double()[mine] * dh[:, :, None]).sum(1)
+            # one rounding to bf16, half a step of 2^-8, and sums in fp32: 65536 terms of like size give 2^-24 * 65536 = 2^-8 at the very most
+            assert (out[:, part].double() - want).norm() <= 2.0 ** -7 * want.norm()
+            assert (dx[:, part].double() - want_dx).norm() <= 2.0 ** -7 * want_dx.norm()
