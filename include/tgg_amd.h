@@ -282,8 +282,7 @@ int tgg_lora_linear_bwd(const void* grad, const void* x, const void* w, const vo
 
 /* Newton-Schulz orthogonalisation of every matrix of a stack [batch, rows, cols] (contiguous; dtype TGG_BF16, TGG_F16 or 2 = fp32):
  *   X = x / (|x|_F + eps), then `steps` times  G = X X^T, X = a X + (b G + c G^2) X   (of the transposed matrix where rows > cols: the same matrix),
- * out in x's type (out may be x).  X is carried from step to step in 22 bits; results in fp16 and fp32 are as good as fp32 products, those in bf16
- * are multiplied in half precision (11 bits), which stays below their own rounding.  Values must keep |X| entries below 64 and those of the polynomial
+ * out in x's type (out may be x).  Matrices are multiplied and carried from step to step in 22 bits with fp32 sums, whatever the type.  Values must keep |X| entries below 64 and those of the polynomial
  * below 64 (any coefficients that keep singular values near 1 do); beyond, results are not finite.
  * tgg_muon_update: the optimiser's step, in place:
  *   momentum = beta momentum + (1 - beta) grad (fp32);  u = nesterov ? beta momentum + (1 - beta) grad : momentum;

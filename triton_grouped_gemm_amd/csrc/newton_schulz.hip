@@ -6,16 +6,16 @@
 // planes of half precision, high and low, 22 bits together, scaled by 2^10 so that the low plane keeps its bits: singular values
 // stay near or below 1, so entries do not overflow.
 //
-// Results in bfloat16 are multiplied from the high planes alone, 11 bits, with what the rounding would reach first taken out of the products:
-// the sum that carries X over, a X, uses both planes, and G and the polynomial enter products (and G the linear term), in one plane, less their mean diagonal, whose part is
-// exact:   A = G - d I,   B = (b + 2 c d) A + c (A^2 - e I),   X <- (a + b d + c d^2 + c e) X + B X,   d = |X|^2 / M,   e = |A|^2 / M.
-// The rounding of near-identity matrices is then that of what is left of them.  Errors against 64 bits, before the last rounding (random and low-rank matrices of 256 to 768 rows): 2e-4 to 1.1e-3, where
-// G and B with their diagonals give up to 2.6e-3 and bfloat16 operands 2e-2; the result's own rounding is 1.7e-3.  Results in half precision and fp32 add the products of
-// high and low planes, three multiplies for one, and are as good as fp32 products.
+// Products add up high x high, high x low and low x high planes, three multiplies for one, whatever the result's type.  (High planes alone, 11 bits, do not do for bfloat16 results either.  What X's rounding
+// leaves out lands in weak directions too, and each of them grows by up to 3.4445 a step: in front of the last rounding, which is 1.7e-3 of the norm, emulated, 7e-4 for random matrices of 512 rows, but 8e-3 for
+// 8 x 4096 of rank 4 over 0.3 % noise, 3e-2 for exactly low-rank ones after eight steps.  Both planes of X alone: 3e-3 for 512 x 2048 of which four rows are not zero.  Both planes of everything: 3e-5 at most in
+// five steps.)
+// G and the polynomial enter products less their mean diagonal, whose part is exact, so that the rounding of near-identity matrices is that of what is left of them:
+//   A = G - d I,   B = (b + 2 c d) A + c (A^2 - e I),   X <- (a + b d + c d^2 + c e) X + B X,   d = |X|^2 / M,   e = |A|^2 / M.
 //
-// A step of 64 matrices of 1536 x 2048 takes 343 us for G, 305 for the polynomial and 749 for the update; 7.2 ms in all, 0.80 PFLOP/s counting half of a symmetric product (the products alone 0.83).  The
-// matrix pipe is busy in 0.4 to 0.6 of the cycles: between tiles eight waves store results and read what they add to (25 us a tile of 256, of 1.4 us a slab of 64; without its stores an update takes 525 us),
-// and 64 x 21 triangular tiles are 5.25 rounds of the chip.  What is small is bound by latency: 512 x 512, three kernels of 8 us a step.
+// A step of 64 matrices of 1536 x 2048 takes 1015 us for G, 843 for the polynomial and 1595 for the update; 17.5 ms in all, 1.0 PFLOP/s counting three products and half of a symmetric one.
+// Between tiles eight waves store results and read what they add to (25 us a tile of 256, of 1.4 us a slab of 64), and 64 x 21 triangular tiles are 5.25 rounds of the chip.  What is small is bound by
+// latency: 512 x 512, three kernels of 13.5 us a step.
 //
 // G and G^2 are symmetric: only tiles on and below the diagonal are computed, and stored twice.  No sum depends on the order of arrival: norms are
 // summed per tile and the tiles' sums in order.
@@ -40,7 +40,7 @@ struct NsTarget {
 // One product for all matrices.  Planes: element (m, i, j) at m * stride + i * ld + j.
 struct NsProduct {
   const uint16_t *a_hi, *a_lo, *b_hi, *b_lo;  // operands: GRAM X, X; POLY A, A; UPDATE B, X
-  uint16_t *o_hi, *o_lo;                      // result's planes; o_lo may be null
+  uint16_t *o_hi, *o_lo;                      // result's planes
   const uint16_t *c_hi, *c_lo;                // what the epilogue adds: POLY A, UPDATE X
   int64_t a_stride, b_stride, o_stride;       // per matrix, in elements
   int lda, ldb, ldo;
@@ -135,9 +135,8 @@ TGG_DEV rsrc_t ns_window(const void* base, int64_t bytes) {
 }
 constexpr int kNowhere = 0x40000000;  // beyond every window, also with a tile's rows added
 
-template <class C, int MODE, bool PRECISE> struct NsProblem {
+template <class C, int MODE> struct NsProblem {
   static constexpr bool SYM = MODE <= NS_POLY, B_KMAJOR = SYM;
-  static constexpr bool C_LO = MODE >= NS_UPDATE || PRECISE, O_LO = MODE == NS_UPDATE || PRECISE;  // whether what is added, and the result, have a low plane
   static_assert(!SYM || C::BM == C::BN, "symmetric results have square tiles");
   // The epilogue takes pieces of 16 rows x HC columns of the wave's block through the wave's staging: a multiply leaves a lane four columns of one row, and
   // neighbouring lanes in different rows, of which every one is an access of its own (64 cycles an instruction; 256-row tiles spent 36 us there).  Staged, a lane has eight columns and
@@ -166,7 +165,7 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
     pos = -1;
   }
   TGG_DEV int tile_at(int q) const { return walk.at(q); }
-  TGG_DEV int slabs(int) const { return PRECISE ? 3 * cur.kt : cur.kt; }
+  TGG_DEV int slabs(int) const { return 3 * cur.kt; }
   // id -> matrix, first row, first column
   struct Place { int m, row0, col0; };
   TGG_DEV Place locate(int id) const {
@@ -185,8 +184,8 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
   }
   // passes: high x high planes, high x low, low x high
   TGG_DEV void begin_pass() {
-    const uint16_t* const a = PRECISE && pass == 2 ? p.a_lo : p.a_hi;
-    const uint16_t* const b = PRECISE && pass == 1 ? p.b_lo : p.b_hi;
+    const uint16_t* const a = pass == 2 ? p.a_lo : p.a_hi;
+    const uint16_t* const b = pass == 1 ? p.b_lo : p.b_hi;
     cur.begin(live, (uint64_t)a + a_tile, (uint64_t)b + b_tile, a_rows, b_rows, b_skip);
   }
   TGG_DEV void seek(int id) {
@@ -202,7 +201,7 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
     begin_pass();
   }
   TGG_DEV void turn() {
-    if (PRECISE && pass < 2) {
+    if (pass < 2) {
       ++pass;
       begin_pass();
     } else {
@@ -242,8 +241,8 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
     // Planes are reached through windows that begin at the tile's first row (the mirrored tile's: its first column) and end with the matrix's last: what lies below reads as zeros and is not
     // written.  Columns to the right of a row are nowhere.
     auto rows_of = [&](const uint16_t* plane, int first, int rows) __attribute__((always_inline)) { return ns_window(plane + base + (int64_t)first * p.ldo, (int64_t)lesser(rows, p.rows - first) * p.ldo * 2); };
-    const rsrc_t o_hi = rows_of(p.o_hi, tile.row0, C::BM), o_lo = rows_of(p.o_lo, tile.row0, O_LO ? C::BM : 0);
-    const rsrc_t c_hi_w = rows_of(p.c_hi, tile.row0, MODE != NS_GRAM ? C::BM : 0), c_lo_w = rows_of(p.c_lo, tile.row0, MODE != NS_GRAM && C_LO ? C::BM : 0);
+    const rsrc_t o_hi = rows_of(p.o_hi, tile.row0, C::BM), o_lo = rows_of(p.o_lo, tile.row0, C::BM);
+    const rsrc_t c_hi_w = rows_of(p.c_hi, tile.row0, MODE != NS_GRAM ? C::BM : 0), c_lo_w = rows_of(p.c_lo, tile.row0, MODE != NS_GRAM ? C::BM : 0);
     const int pitch = p.ldo * 2;
     int lane_at[PIECES];
 #pragma unroll
@@ -253,7 +252,7 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
     i32x4_t c_hi[AHEAD], c_lo[AHEAD];
     auto fetch = [&](int n) __attribute__((always_inline)) {
       c_hi[n % AHEAD] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(c_hi_w, lane_at[n % PIECES] + n / PIECES * 16 * pitch, 0, 0));
-      if (C_LO) c_lo[n % AHEAD] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(c_lo_w, lane_at[n % PIECES] + n / PIECES * 16 * pitch, 0, 0));
+      c_lo[n % AHEAD] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(c_lo_w, lane_at[n % PIECES] + n / PIECES * 16 * pitch, 0, 0));
     };
     if (MODE != NS_GRAM) {
 #pragma unroll
@@ -267,7 +266,7 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
     const float g = MODE == NS_POLY ? p.cb + 2.f * p.cc * d : !SYM ? p.ca + p.cb * d + p.cc * d * d + p.cc * e : 0.f;
     const float h = (MODE == NS_GRAM ? d : MODE == NS_POLY ? p.cc * e : 0.f) * kNsScale;
     const bool diagonal = SYM && tile.row0 == tile.col0, edge = tile.row0 + C::BM > p.rows || tile.col0 + C::BN > p.cols || LPR != 4;
-    const rsrc_t m_hi = rows_of(p.o_hi, tile.col0, SYM ? C::BN : 0), m_lo = rows_of(p.o_lo, tile.col0, SYM && O_LO ? C::BN : 0);
+    const rsrc_t m_hi = rows_of(p.o_hi, tile.col0, SYM ? C::BN : 0), m_lo = rows_of(p.o_lo, tile.col0, SYM ? C::BN : 0);
     const int c_row = el >> 1, r0 = (el & 1) * 8;  // of the mirrored piece
     const int mirror_at = c_row < HC ? (at.wn0 + c_row) * pitch + (rbase + r0) * 2 : kNowhere;
     char* const mine = stage + at.wave * STAGE_WAVE;
@@ -292,9 +291,9 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
       if (MODE != NS_GRAM) {
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-          const int h2 = c_hi[n % AHEAD][x / 2], l2 = C_LO ? c_lo[n % AHEAD][x / 2] : 0;  // (a bit cast of a vector's element takes the first one)
+          const int h2 = c_hi[n % AHEAD][x / 2], l2 = c_lo[n % AHEAD][x / 2];  // (a bit cast of a vector's element takes the first one)
           const f16x2_t hi = __builtin_bit_cast(f16x2_t, h2), lo = __builtin_bit_cast(f16x2_t, l2);
-          if (C_LO) v[x] = __builtin_fmaf((float)lo[x & 1], g, v[x]);
+          v[x] = __builtin_fmaf((float)lo[x & 1], g, v[x]);
           v[x] = __builtin_fmaf((float)hi[x & 1], g, v[x]);
         }
         if (n + AHEAD < C::TM * PIECES) fetch(n + AHEAD);
@@ -331,7 +330,7 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
           lo[x] = (int)pack2<DT_F16>(v[2 * x] - (float)r[0], v[2 * x + 1] - (float)r[1]);
         }
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, hi), o_hi, lane_at[half] + i * 16 * pitch, 0, 0);
-        if (O_LO) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, lo), o_lo, lane_at[half] + i * 16 * pitch, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, lo), o_lo, lane_at[half] + i * 16 * pitch, 0, 0);
         if (SYM && !diagonal) {  // the same with rows and columns exchanged: both planes of a value in a word, a lane reads eight rows of a column
           uint32_t w[8];
 #pragma unroll
@@ -353,7 +352,7 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
           }
           const int o = rbase + 16 * i + r0 < p.ldo ? mirror_at + half * HC * pitch + i * 32 : kNowhere;
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, hi), m_hi, o, 0, 0);
-          if (O_LO) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, lo), m_lo, o, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, lo), m_lo, o, 0, 0);
           asm volatile("" : : : "memory");
         }
       }
@@ -374,10 +373,10 @@ template <class C, int MODE, bool PRECISE> struct NsProblem {
   }
 };
 
-template <class C, int MODE, bool PRECISE> __global__ __launch_bounds__(C::THREADS) void ns_product_kernel(const NsProduct p, int tiles_m, int tiles_n) {
+template <class C, int MODE> __global__ __launch_bounds__(C::THREADS) void ns_product_kernel(const NsProduct p, int tiles_m, int tiles_n) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  NsProblem<C, MODE, PRECISE> prob(p, tiles_m, tiles_n);
-  stream_gemm<C, DT_F16, NsProblem<C, MODE, PRECISE>::B_KMAJOR>(prob, smem);
+  NsProblem<C, MODE> prob(p, tiles_m, tiles_n);
+  stream_gemm<C, DT_F16, NsProblem<C, MODE>::B_KMAJOR>(prob, smem);
 }
 
 // ---- into the planes and out of them -------------------------------------------------------------------------------------
@@ -541,22 +540,18 @@ typedef StreamCfg<256, 256, 2, 4> NsWide;
 typedef StreamCfg<128, 128, 2, 4> NsNarrow;
 typedef StreamCfg<64, 64, 2, 4, 8> NsSmall;
 
-template <class C, int MODE, bool PRECISE> int ns_launch(const NsProduct& p, hipStream_t s) {
-  typedef NsProblem<C, MODE, PRECISE> P;
+template <class C, int MODE> int ns_launch(const NsProduct& p, hipStream_t s) {
+  typedef NsProblem<C, MODE> P;
   static bool attr_set[64] = {false};
-  if (int e = stream_lds(ns_product_kernel<C, MODE, PRECISE>, P::SMEM_BYTES, attr_set)) return e;
+  if (int e = stream_lds(ns_product_kernel<C, MODE>, P::SMEM_BYTES, attr_set)) return e;
   const int tm = (p.rows + C::BM - 1) / C::BM, tn = (p.cols + C::BN - 1) / C::BN;
   const int64_t tiles = (int64_t)p.batch * (P::SYM ? tm * (tm + 1) / 2 : tm * tn);
   const int slots = num_cus() * (int)(160 * 1024 / P::SMEM_BYTES);
-  ns_product_kernel<C, MODE, PRECISE><<<dim3((unsigned)(tiles < slots ? tiles : slots)), dim3(C::THREADS), P::SMEM_BYTES, s>>>(p, tm, tn);
+  ns_product_kernel<C, MODE><<<dim3((unsigned)(tiles < slots ? tiles : slots)), dim3(C::THREADS), P::SMEM_BYTES, s>>>(p, tm, tn);
   return check_launch("ns_product");
 }
 
-template <int MODE> int ns_product(const NsProduct& p, int tile, bool precise, hipStream_t s) {
-  if (tile == 64) return precise ? ns_launch<NsSmall, MODE, true>(p, s) : ns_launch<NsSmall, MODE, false>(p, s);
-  if (tile == 256) return precise ? ns_launch<NsWide, MODE, true>(p, s) : ns_launch<NsWide, MODE, false>(p, s);
-  return precise ? ns_launch<NsNarrow, MODE, true>(p, s) : ns_launch<NsNarrow, MODE, false>(p, s);
-}
+template <int MODE> int ns_product(const NsProduct& p, int tile, hipStream_t s) { return tile == 64 ? ns_launch<NsSmall, MODE>(p, s) : tile == 256 ? ns_launch<NsWide, MODE>(p, s) : ns_launch<NsNarrow, MODE>(p, s); }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 int64_t ns_align(int64_t x) { return (x + 255) & ~(int64_t)255; }
@@ -573,8 +568,8 @@ struct NsPlan {
 
 // Tiles of 64, 128 or 256 for a product of `slabs` slabs of depth a tile: the estimated time in microseconds, from the rounds of workgroups and what a tile took.  A round of 256-row
 // tiles: 1.65 a slab and 24 for results and start; of two 128-row tiles a compute unit 1.2 and 10, of one 0.8 and 8; of one 64-row tile, with eight slabs in flight, 0.38 and 1.  Measured for stacks of
-// 1 to 64 matrices of 128 to 2048 rows, the choice was the fastest or within 3 % of it; the other tiles took 1.1 to 2.7 times as long (512 x 512: 136, 186 and 384 us in
-// tiles of 64, 128 and 256; 64 of 1536 x 2048: 22.7, 9.3 and 8.2 ms, before the last changes to results' stores).
+// 1 to 64 matrices of 128 to 2048 rows, the choice was the fastest or within 3 % of it, but for 64 matrices of 256 x 512 and 512 x 512 (9 and 12 %); the other tiles took up to 3 times as long (five steps in tiles of 64, 128 and 256:
+// 512 x 512 215, 307 and 594 us; 8 of 768 x 2048 1604, 919 and 1256; 64 of 1536 x 2048 52.2, 21.1 and 17.5 ms).
 int ns_tile(int64_t batch, int rows, int cols, bool sym, int64_t slabs) {
   auto tiles = [&](int b) { const int64_t tm = (rows + b - 1) / b, tn = (cols + b - 1) / b; return batch * (sym ? tm * (tm + 1) / 2 : tm * tn); };
   const int64_t cus = num_cus(), full = tiles(128) / (2 * cus), rest = tiles(128) % (2 * cus);
@@ -584,7 +579,7 @@ int ns_tile(int64_t batch, int rows, int cols, bool sym, int64_t slabs) {
   return small <= narrow && small <= wide ? 64 : narrow <= wide ? 128 : 256;
 }
 
-NsPlan ns_plan(int64_t batch, int rows, int cols, bool precise) {
+NsPlan ns_plan(int64_t batch, int rows, int cols) {
   NsPlan q;
   q.tall = rows > cols;
   q.m = q.tall ? cols : rows;
@@ -592,7 +587,7 @@ NsPlan ns_plan(int64_t batch, int rows, int cols, bool precise) {
   q.ldm = (q.m + 7) & ~7;
   q.ldn = (q.n + 7) & ~7;
   q.chunks = (int)(((int64_t)rows * cols + kNsChunk - 1) / kNsChunk);
-  const int passes = precise ? 3 : 1, deep = (q.n + 63) / 64 * passes, shallow = (q.m + 63) / 64 * passes;
+  const int deep = (q.n + 63) / 64 * 3, shallow = (q.m + 63) / 64 * 3;
   q.gram_tile = ns_tile(batch, q.m, q.m, true, deep);
   q.poly_tile = ns_tile(batch, q.m, q.m, true, shallow);
   q.update_tile = ns_tile(batch, q.m, q.n, false, shallow);
@@ -618,13 +613,12 @@ NsPlan ns_plan(int64_t batch, int rows, int cols, bool precise) {
 
 }  // namespace
 
-int64_t newton_schulz_workspace(int64_t batch, int rows, int cols) { return larger(ns_plan(batch, rows, cols, false).bytes, ns_plan(batch, rows, cols, true).bytes); }
+int64_t newton_schulz_workspace(int64_t batch, int rows, int cols) { return ns_plan(batch, rows, cols).bytes; }
 
 // x -> out, or with momentum the weights' step on out.  dt: 0 bf16, 1 fp16, 2 fp32
 int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, int nesterov, void* out, int out_dt, int weight, float keep, float step, int64_t batch, int rows, int cols, int steps,
                          float ca, float cb, float cc, float eps, void* workspace, hipStream_t s) {
-  const bool precise = out_dt != 0;  // results of more than 8 bits
-  const NsPlan q = ns_plan(batch, rows, cols, precise);
+  const NsPlan q = ns_plan(batch, rows, cols);
   char* const ws = (char*)workspace;
   const int64_t xp = ns_align(q.x_plane * 2), gp = ns_align(q.g_plane * 2);
   uint16_t* xs[2][2] = {{(uint16_t*)(ws + q.off_x), (uint16_t*)(ws + q.off_x + xp)}, {(uint16_t*)(ws + q.off_x + 2 * xp), (uint16_t*)(ws + q.off_x + 3 * xp)}};
@@ -660,21 +654,21 @@ int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, i
     p.depth = q.n;
     p.a_hi = p.b_hi = from[0]; p.a_lo = p.b_lo = from[1];
     p.lda = p.ldb = q.ldn; p.a_stride = p.b_stride = xstride;
-    p.o_hi = a_hi; p.o_lo = precise ? a_lo : nullptr; p.ldo = q.ldm; p.o_stride = gstride; p.o_sums = a_sums;
-    if (int e = ns_product<NS_GRAM>(p, q.gram_tile, precise, s)) return e;
+    p.o_hi = a_hi; p.o_lo = a_lo; p.ldo = q.ldm; p.o_stride = gstride; p.o_sums = a_sums;
+    if (int e = ns_product<NS_GRAM>(p, q.gram_tile, s)) return e;
     p.depth = q.m;
     p.a_hi = p.b_hi = p.c_hi = a_hi; p.a_lo = p.b_lo = p.c_lo = a_lo;
     p.lda = p.ldb = q.ldm; p.a_stride = p.b_stride = gstride;
-    p.o_hi = b_hi; p.o_lo = precise ? b_lo : nullptr; p.o_sums = nullptr;
-    if (int e = ns_product<NS_POLY>(p, q.poly_tile, precise, s)) return e;
+    p.o_hi = b_hi; p.o_lo = b_lo; p.o_sums = nullptr;
+    if (int e = ns_product<NS_POLY>(p, q.poly_tile, s)) return e;
     p.cols = q.n;
     p.a_hi = b_hi; p.a_lo = b_lo;
     p.b_hi = p.c_hi = from[0]; p.b_lo = p.c_lo = from[1]; p.ldb = q.ldn; p.b_stride = xstride;
     p.o_hi = to[0]; p.o_lo = to[1]; p.ldo = q.ldn; p.o_stride = xstride; p.o_sums = x_sums[(i + 1) & 1];
     p.target = dst;
     p.tall = q.tall;
-    if (direct && i == steps - 1) return ns_product<NS_LAST>(p, q.update_tile, precise, s);
-    if (int e = ns_product<NS_UPDATE>(p, q.update_tile, precise, s)) return e;
+    if (direct && i == steps - 1) return ns_product<NS_LAST>(p, q.update_tile, s);
+    if (int e = ns_product<NS_UPDATE>(p, q.update_tile, s)) return e;
   }
   const int sr = (rows + 63) / 64, sc = (cols + 63) / 64;
   const dim3 store_grid((unsigned)(batch * sr * sc));

@@ -73,8 +73,7 @@ def _(x, steps, a, b, c, eps):
 def orthogonalize(x: Tensor, steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS, eps: float = 1e-7) -> Tensor:
     """Every matrix of ``x`` ``[..., rows, columns]`` (bf16, fp16 or fp32, any sizes up to 65536) after ``steps`` Newton-Schulz products, in its type.
 
-    Results in fp16 and fp32 are as good as fp32 products; those in bf16 are multiplied in half precision (11 bits; 22 where values are carried
-    from step to step), which stays below their own rounding.  A matrix of zeros stays one (unless ``eps`` is 0); one with a NaN or an infinity becomes
+    Multiplied and carried from step to step in 22 bits with fp32 sums, whatever the type, and rounded once at the end.  A matrix of zeros stays one (unless ``eps`` is 0); one with a NaN or an infinity becomes
     NaN, and no other of the stack is touched by it.  ``coefficients`` have to keep singular values near 1 (entries below 64).  Not differentiable."""
     coefficients = tuple(float(v) for v in coefficients)
     steps, eps = int(steps), float(eps)
@@ -132,7 +131,7 @@ def muon_update(weight: Tensor, grad: Tensor, momentum: Tensor, lr: float, beta:
         weight   = (1 - lr weight_decay) weight - lr scale orthogonalize(u)
 
     ``momentum`` is fp32; ``weight`` and ``grad`` are bf16, fp16 or fp32 each.  ``scale`` is ``sqrt(max(1, rows / columns))`` unless given.  ``momentum``, ``weight`` and ``grad`` do not share memory.  The
-    direction is as exact as ``weight``'s type asks for (see ``orthogonalize``) and the weights are rounded once."""
+    direction is multiplied as ``orthogonalize`` does it and the weights are rounded once."""
     coefficients = tuple(float(v) for v in coefficients)
     steps, eps, beta = int(steps), float(eps), float(beta)
     _, rows, cols = _check_muon(weight, grad, momentum, steps, coefficients, eps)
