@@ -11,6 +11,7 @@ from pathlib import Path
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "libtgg_amd.so"
 
@@ -117,6 +118,11 @@ class EagerOp(torch.library.CustomOpDef):
     def register_kernel(self, device_types, *rest):
         self.replaced = self.replaced or device_types is None
         return super().register_kernel(device_types, *rest)
+
+
+def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether one of them carries a forward-mode tangent, which an operator without a rule for it would drop."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def last_error() -> str:

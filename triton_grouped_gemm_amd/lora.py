@@ -152,6 +152,8 @@ class LoraLinear(torch.autograd.Function):
         if any(want) and not (_lora_linear_backward.replaced or torch.compiler.is_compiling()):
             grads = (_native._host or _native.host()).lora_linear_backward(x, weight, lora_a, lora_b, adapters, scales, grad.contiguous(), h, *want)
         if grads is None:
+            if not torch.compiler.is_compiling() and _native.has_tangent(grad):
+                raise RuntimeError("the gradients of lora_linear have no forward-mode derivative (no jvp): detach what they are multiplied with")
             grads = _lora_linear_backward(grad, x, weight, lora_a, lora_b, adapters, scales, h, *want)
         dx, da, db = (g if w else None for g, w in zip(grads, want))
         dw = None
@@ -170,7 +172,7 @@ def lora_linear(x: Tensor, weight: Tensor, lora_a: Tensor, lora_b: Tensor, adapt
     ``x`` ``[M, K]``, ``weight`` ``[N, K]``, ``lora_a`` ``[L, R, K]`` and ``lora_b`` ``[L, N, R]`` in bf16 or fp16 (N and K multiples of 8 up to 65536, R one of
     8 up to 128, L up to 1024, M below 2^27); ``adapters`` ``[M]`` int32 or int64 on the GPU, in any order: a row whose entry is outside ``[0, L)``
     (-1, say) has no adapter; ``scales`` ``[L]`` fp32, 1 unless given.  fp32 to the one rounding at the end.  Differentiable in ``x``, ``weight``,
-    ``lora_a`` and ``lora_b``; adapters without rows get zero gradients."""
+    ``lora_a`` and ``lora_b``, once and backwards (forward-mode tangents are refused); adapters without rows get zero gradients."""
     if not (_lora_linear.replaced or torch.compiler.is_compiling()):
         out = (_native._host or _native.host()).lora_linear(x, weight, lora_a, lora_b, adapters, scales, False)
         if out is not None:
@@ -179,6 +181,7 @@ def lora_linear(x: Tensor, weight: Tensor, lora_a: Tensor, lora_b: Tensor, adapt
     if scales is not None and scales.requires_grad and torch.is_grad_enabled():
         raise ValueError("scales is not differentiable: detach it")
     require_gpu(x)
-    if (torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, lora_a, lora_b))) or torch.compiler.is_compiling():
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, lora_a, lora_b))) or torch.compiler.is_compiling() \
+            or _native.has_tangent(x, weight, lora_a, lora_b, scales):  # (the function refuses a tangent)
         return LoraLinear.apply(x, weight, lora_a, lora_b, adapters, scales)
     return _lora_linear(x, weight, lora_a, lora_b, adapters, scales)

@@ -46,6 +46,11 @@ def _check(name: str, x: Tensor, steps: int, coefficients: Sequence[float], eps:
     return math.prod(x.shape[:-2]), rows, cols
 
 
+def _refuse_tangents(name: str, *tensors: Tensor) -> None:
+    if not torch.compiler.is_compiling() and _native.has_tangent(*tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative (no jvp): detach its operands")
+
+
 def _workspace(batch: int, rows: int, cols: int, device: torch.device):
     need = _workspace_bytes(batch, rows, cols, device.index)
     return torch.empty(need, dtype=torch.uint8, device=device), need
@@ -74,10 +79,11 @@ def orthogonalize(x: Tensor, steps: int = 5, coefficients: Sequence[float] = COE
     """Every matrix of ``x`` ``[..., rows, columns]`` (bf16, fp16 or fp32, any sizes up to 65536) after ``steps`` Newton-Schulz products, in its type.
 
     Multiplied and carried from step to step in 22 bits with fp32 sums, whatever the type, and rounded once at the end.  A matrix of zeros stays one (unless ``eps`` is 0); one with a NaN or an infinity becomes
-    NaN, and no other of the stack is touched by it.  ``coefficients`` have to keep singular values near 1 (entries below 64).  Not differentiable."""
+    NaN, and no other of the stack is touched by it.  ``coefficients`` have to keep singular values near 1 (entries below 64).  Not differentiable, in either mode."""
     coefficients = tuple(float(v) for v in coefficients)
     steps, eps = int(steps), float(eps)
     _check("x", x, steps, coefficients, eps)
+    _refuse_tangents("orthogonalize", x)
     require_gpu(x)
     return _orthogonalize(x, steps, *coefficients, eps)
 
@@ -139,5 +145,6 @@ def muon_update(weight: Tensor, grad: Tensor, momentum: Tensor, lr: float, beta:
     lr, weight_decay = float(lr), float(weight_decay)
     if not all(math.isfinite(v) for v in (lr, beta, weight_decay, scale)):
         raise ValueError(f"lr, beta, weight_decay and scale must be finite, got {lr}, {beta}, {weight_decay} and {scale}")
+    _refuse_tangents("muon_update", weight, grad, momentum)
     require_gpu(weight, grad, momentum)
     _muon_update(weight, grad, momentum, 1.0 - lr * weight_decay, lr * scale, beta, bool(nesterov), steps, *coefficients, eps)
