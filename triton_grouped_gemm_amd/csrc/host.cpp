@@ -240,6 +240,7 @@ PyObject* m_grouped_gemm_int4(PyObject*, PyObject* const* args, Py_ssize_t nargs
 }
 
 // What the adapter calls have in common: plain operands in the kernels' form, nothing to record.
+bool aligned16(const at::Tensor& t) { return ((uintptr_t)t.data_ptr() & 15) == 0; }
 struct LoraArgs {
   const at::Tensor *x, *w, *a, *b, *ids, *scales;
   int64_t m, k, n, l, r;
@@ -257,7 +258,7 @@ bool lora_args(PyObject* const* args, c10::DeviceIndex& device, LoraArgs& q) {
   const at::ScalarType type = x.scalar_type();
   return q.dt >= 0 && w.scalar_type() == type && a.scalar_type() == type && b.scalar_type() == type && q.m > 0 && w.size(1) == q.k && a.size(2) == q.k && b.size(0) == q.l && b.size(1) == q.n &&
          b.size(2) == q.r && q.n >= 8 && q.k >= 8 && !(q.n & 7) && !(q.k & 7) && q.n <= 65536 && q.k <= 65536 && q.r >= 8 && q.r <= 128 && !(q.r & 7) && q.l >= 1 && q.l <= kMaxGroups &&
-         sizes_ok(*q.ids, q.m) && x.is_contiguous() && w.is_contiguous() && a.is_contiguous() && b.is_contiguous() &&
+         sizes_ok(*q.ids, q.m) && x.is_contiguous() && w.is_contiguous() && a.is_contiguous() && b.is_contiguous() && aligned16(x) && aligned16(w) && aligned16(a) && aligned16(b) &&
          (!q.scales || (q.scales->scalar_type() == at::kFloat && q.scales->dim() == 1 && q.scales->size(0) == q.l && q.scales->is_contiguous()));
 }
 
@@ -300,7 +301,7 @@ PyObject* lora_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t narg
   TGG_TENSOR(grad, 6);
   TGG_TENSOR(h, 7);
   if (grad.dim() != 2 || grad.size(0) != q.m || grad.size(1) != q.n || grad.scalar_type() != q.x->scalar_type() || !grad.is_contiguous() || records(grad) || h.dim() != 2 || h.size(0) != q.m ||
-      h.size(1) != q.r || h.scalar_type() != at::kFloat || !h.is_contiguous() || records(h))
+      h.size(1) != q.r || h.scalar_type() != at::kFloat || !h.is_contiguous() || records(h) || !aligned16(grad) || !aligned16(h))
     Py_RETURN_NONE;
   static const c10::OperatorName op("moe::lora_linear_backward", "");
   if (replaced(op)) Py_RETURN_NONE;

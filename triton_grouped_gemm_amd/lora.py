@@ -52,11 +52,18 @@ def _check(x: Tensor, weight: Tensor, lora_a: Tensor, lora_b: Tensor, adapters: 
         raise ValueError("all operands must live on one GPU")
 
 
+def _aligned(t: Tensor) -> Tensor:
+    """``t`` as the kernels take it, contiguous and from a multiple of 16 bytes on: a slice of a flat buffer is copied, and so is a gradient that autograd hands back as one."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _launch(x, weight, lora_a, lora_b, adapters, scales, keep_h: bool):
     _check(x, weight, lora_a, lora_b, adapters, scales)
     require_gpu(x)
     (m, k), n, (count, r) = x.shape, weight.shape[0], lora_a.shape[:2]
-    x, weight, lora_a, lora_b, adapters = x.contiguous(), weight.contiguous(), lora_a.contiguous(), lora_b.contiguous(), adapters.contiguous()
+    x, weight, lora_a, lora_b = (_aligned(t) for t in (x, weight, lora_a, lora_b))
+    adapters = adapters.contiguous()
     scales = None if scales is None else scales.contiguous()
     out = x.new_empty(m, n)
     h = x.new_empty(m, r, dtype=torch.float32) if keep_h else None
@@ -104,7 +111,8 @@ def _lora_linear_backward(grad: Tensor, x: Tensor, weight: Tensor, lora_a: Tenso
     if not grad.device == h.device == x.device:
         raise ValueError("all operands must live on one GPU")
     require_gpu(x)
-    grad, x, weight, lora_a, lora_b, adapters, h = (t.contiguous() for t in (grad, x, weight, lora_a, lora_b, adapters, h))
+    grad, x, weight, lora_a, lora_b, h = (_aligned(t) for t in (grad, x, weight, lora_a, lora_b, h))
+    adapters = adapters.contiguous()
     scales = None if scales is None else scales.contiguous()
     dx = torch.empty_like(x) if want_x else x.new_empty(0)
     make = torch.empty_like if m else torch.zeros_like
@@ -160,7 +168,7 @@ class LoraLinear(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             if x.shape[0]:
                 rows = torch.full((1,), x.shape[0], dtype=torch.int32, device=x.device)
-                dw = k_grouped_gemm(grad.contiguous(), x.contiguous(), rows)[0]
+                dw = k_grouped_gemm(_aligned(grad), _aligned(x), rows)[0]
             else:
                 dw = torch.zeros_like(weight)
         return dx, dw, da, db, None, None
@@ -170,7 +178,7 @@ def lora_linear(x: Tensor, weight: Tensor, lora_a: Tensor, lora_b: Tensor, adapt
     """``out[m] = weight x[m] + scales[l] lora_b[l] (lora_a[l] x[m])`` with ``l = adapters[m]``, ``[M, N]``.
 
     ``x`` ``[M, K]``, ``weight`` ``[N, K]``, ``lora_a`` ``[L, R, K]`` and ``lora_b`` ``[L, N, R]`` in bf16 or fp16 (N and K multiples of 8 up to 65536, R one of
-    8 up to 128, L up to 1024, M below 2^27); ``adapters`` ``[M]`` int32 or int64 on the GPU, in any order: a row whose entry is outside ``[0, L)``
+    8 up to 128, L up to 1024, M below 2^27; operands that are not contiguous, or do not begin at a multiple of 16 bytes, are copied); ``adapters`` ``[M]`` int32 or int64 on the GPU, in any order: a row whose entry is outside ``[0, L)``
     (-1, say) has no adapter; ``scales`` ``[L]`` fp32, 1 unless given.  fp32 to the one rounding at the end.  Differentiable in ``x``, ``weight``,
     ``lora_a`` and ``lora_b``, once and backwards (forward-mode tangents are refused); adapters without rows get zero gradients."""
     if not (_lora_linear.replaced or torch.compiler.is_compiling()):
