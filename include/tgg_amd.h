@@ -268,7 +268,7 @@ int tgg_moe_router_bwd(const void* logits, int64_t row_stride, const float* prob
 /* Low-rank adapters of many requests beside a shared projection (dtype TGG_BF16 or TGG_F16):
  *   out[m] = W x[m] + scales[l] B_l (A_l x[m]),  l = adapters[m];  rows whose entry is outside [0, L) have no adapter
  * x [M, K], w [N, K], a [L, R, K], b [L, N, R], adapters [M] int32 or int64, scales [L] fp32 or null (1), out [M, N]; rows in any order.  One rounding, at the
- * end.  N and K multiples of 8 up to 65536, R a multiple of 8 up to 128, L up to 1024, M below 2^27.  h [M, R] fp32 (or null) receives scales[l] A_l x[m], zeros without an
+ * end.  N and K multiples of 8 up to 65536, R a multiple of 8 up to 128, L up to 1024, M up to 2^27 - 16.  h [M, R] fp32 (or null) receives scales[l] A_l x[m], zeros without an
  * adapter, which the backward pass takes.
  * _bwd: dx [M, K] = W^T g + A_l^T dh, da [L, R, K] = sum of dh[m] x[m]^T, db [L, N, R] = sum of g[m] h[m]^T over each adapter's rows, with
  * dh[m] = scales[l] B_l^T g[m]; any of the three may be null (x is read for da, w for dx, h for db).  Adapters without rows get zeros.

@@ -797,8 +797,8 @@ int tgg_moe_router_bwd(const void* logits, int64_t row_stride, const float* prob
 
 // ---- low-rank adapters ------------------------------------------------------------------------------------------
 static int lora_check(int64_t M, int64_t N, int64_t K, int R, int L) {
-  // lora_down: a workgroup of 512 threads for 16 rows, and a launch has fewer than 2^32 threads
-  if (M < 0 || M >= (1ll << 27)) return set_error("M=%lld outside [0, 2^27)", (long long)M);
+  // lora_down: a workgroup of 512 threads for 16 rows begun, and a launch has fewer than 2^32 threads
+  if (M < 0 || M > (1ll << 27) - 16) return set_error("M=%lld outside [0, 2^27 - 16]", (long long)M);
   if (N < 8 || K < 8 || (N & 7) || (K & 7)) return set_error("N and K must be positive multiples of 8, got N=%lld K=%lld", (long long)N, (long long)K);
   if (N > 65536 || K > 65536) return set_error("N=%lld or K=%lld: at most 65536 is supported", (long long)N, (long long)K);
   if (R < 8 || R > 128 || (R & 7)) return set_error("the rank must be a multiple of 8 in [8, 128], got %d", R);
