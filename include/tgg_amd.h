@@ -285,7 +285,7 @@ int tgg_lora_linear_bwd(const void* grad, const void* x, const void* w, const vo
  * out in x's type (out may be x).  Matrices are multiplied and carried from step to step in 22 bits with fp32 sums, whatever the type.  Values must keep |X| entries below 64 and those of the polynomial
  * below 64 (any coefficients that keep singular values near 1 do); beyond, results are not finite.
  * tgg_muon_update: the optimiser's step, in place:
- *   momentum = beta momentum + (1 - beta) grad (fp32);  u = nesterov ? beta momentum + (1 - beta) grad : momentum;
+ *   momentum = beta momentum + (1 - beta) grad (fp32; beta and 1 - beta are rounded from the double);  u = nesterov ? beta momentum + (1 - beta) grad : momentum;
  *   weight = keep weight - step X(u), rounded once to its type
  * grad and weight in types of their own; the three share no memory.  Rows and columns up to 65536, stacks of fewer than 2^24 blocks of 64 x 64 values.  The workspace (256-byte aligned; size from
  * tgg_newton_schulz_workspace_bytes) is in use until the call's kernels are done.  The reference has no optimiser. */
@@ -293,7 +293,7 @@ int tgg_newton_schulz_workspace_bytes(int64_t batch, int64_t rows, int64_t cols,
 int tgg_newton_schulz(const void* x, void* out, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c, float eps, int dtype, void* workspace,
                       int64_t workspace_bytes, void* stream);
 int tgg_muon_update(void* weight, int weight_dtype, const void* grad, int grad_dtype, float* momentum, int64_t batch, int64_t rows, int64_t cols, float keep, float step,
-                    float beta, int nesterov, int steps, float a, float b, float c, float eps, void* workspace, int64_t workspace_bytes, void* stream);
+                    double beta, int nesterov, int steps, float a, float b, float c, float eps, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Test hook, runs entirely on the host (no GPU needed): the order in which `grid` persistent workgroups walk
  * the output tiles of a launch, computed by the same scheduler functions the kernels execute.  It restates

@@ -6,7 +6,7 @@ caller gets an exception.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_void_p
 from pathlib import Path
 from typing import Optional
 
@@ -20,7 +20,7 @@ MAX_GROUPS = 1024  # TGG_MAX_GROUPS: plain 16-bit M-grouped and K-grouped GEMM
 MAX_GROUPS_OTHER = 512  # TGG_MAX_GROUPS_OTHER: every other GEMM entry point
 QUEUE_WORDS = 16  # TGG_QUEUE_WORDS: int32 words of the K-grouped kernels' work queue (zero before a launch, zero after)
 
-_P, _I, _L, _F = c_void_p, c_int, c_int64, c_float
+_P, _I, _L, _F, _D = c_void_p, c_int, c_int64, c_float, c_double
 
 # name -> argument types; every function returns int unless noted
 SIGNATURES = {
@@ -64,7 +64,7 @@ SIGNATURES = {
     "tgg_lora_linear_bwd": [_P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P, _L, _P],
     "tgg_newton_schulz_workspace_bytes": [_L, _L, _L, _P],
     "tgg_newton_schulz": [_P, _P, _L, _L, _L, _I, _F, _F, _F, _F, _I, _P, _L, _P],
-    "tgg_muon_update": [_P, _I, _P, _I, _P, _L, _L, _L, _F, _F, _F, _I, _I, _F, _F, _F, _F, _P, _L, _P],
+    "tgg_muon_update": [_P, _I, _P, _I, _P, _L, _L, _L, _F, _F, _D, _I, _I, _F, _F, _F, _F, _P, _L, _P],
     "tgg_debug_tile_order": [_P, _I, _I, _L, _L, _I, _I, _I, _I, _P, _L, _P],
     "tgg_debug_row_tiles": [_P, _I, _I, _L, _L, _I, _I, _P, _L, _P],
     "tgg_debug_queue_order": [_I, _I, _P],

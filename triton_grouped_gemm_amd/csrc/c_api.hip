@@ -881,10 +881,10 @@ int tgg_newton_schulz(const void* x, void* out, int64_t batch, int64_t rows, int
                       void* stream) {
   if (int e = newton_schulz_operands(x, dtype, out, dtype, batch, rows, cols, steps, workspace, workspace_bytes)) return e;
   if (batch == 0) return 0;
-  return launch_newton_schulz(x, dtype, nullptr, 0.f, 0, out, dtype, 0, 0.f, 0.f, batch, (int)rows, (int)cols, steps, a, b, c, eps, workspace, (hipStream_t)stream);
+  return launch_newton_schulz(x, dtype, nullptr, 0.0, 0, out, dtype, 0, 0.f, 0.f, batch, (int)rows, (int)cols, steps, a, b, c, eps, workspace, (hipStream_t)stream);
 }
 
-int tgg_muon_update(void* weight, int weight_dtype, const void* grad, int grad_dtype, float* momentum, int64_t batch, int64_t rows, int64_t cols, float keep, float step, float beta, int nesterov,
+int tgg_muon_update(void* weight, int weight_dtype, const void* grad, int grad_dtype, float* momentum, int64_t batch, int64_t rows, int64_t cols, float keep, float step, double beta, int nesterov,
                     int steps, float a, float b, float c, float eps, void* workspace, int64_t workspace_bytes, void* stream) {
   if (int e = newton_schulz_operands(grad, grad_dtype, weight, weight_dtype, batch, rows, cols, steps, workspace, workspace_bytes)) return e;
   if (batch == 0) return 0;

@@ -53,7 +53,7 @@ int launch_lora_bwd(const void* grad, const void* x, const void* w, const void* 
 
 // Newton-Schulz orthogonalisation (newton_schulz.hip); types 0 = bf16, 1 = fp16, 2 = fp32
 int64_t newton_schulz_workspace(int64_t batch, int rows, int cols);
-int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, int nesterov, void* out, int out_dt, int weight, float keep, float step, int64_t batch, int rows, int cols, int steps,
+int launch_newton_schulz(const void* x, int x_dt, float* momentum, double beta, int nesterov, void* out, int out_dt, int weight, float keep, float step, int64_t batch, int rows, int cols, int steps,
                          float ca, float cb, float cc, float eps, void* workspace, hipStream_t s);
 
 }  // namespace tgg

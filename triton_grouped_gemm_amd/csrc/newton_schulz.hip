@@ -399,7 +399,7 @@ TGG_DEV void ns_store_planes(uint16_t* hi, uint16_t* lo, int64_t o, const float 
 struct NsSource {
   const void* x;   // the input or the gradient
   float* momentum; // or null
-  float beta, keep;  // keep = 1 - beta
+  float beta, keep;  // keep = 1 - beta, in 64 bits before its rounding (1 - 0.999f is 1.3e-5 of itself off)
   int nesterov, dt;
 };
 TGG_DEV float ns_mix(const NsSource& s, float m, float g) { return __builtin_fmaf(s.beta, m, s.keep * g); }
@@ -616,7 +616,7 @@ NsPlan ns_plan(int64_t batch, int rows, int cols) {
 int64_t newton_schulz_workspace(int64_t batch, int rows, int cols) { return ns_plan(batch, rows, cols).bytes; }
 
 // x -> out, or with momentum the weights' step on out.  dt: 0 bf16, 1 fp16, 2 fp32
-int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, int nesterov, void* out, int out_dt, int weight, float keep, float step, int64_t batch, int rows, int cols, int steps,
+int launch_newton_schulz(const void* x, int x_dt, float* momentum, double beta, int nesterov, void* out, int out_dt, int weight, float keep, float step, int64_t batch, int rows, int cols, int steps,
                          float ca, float cb, float cc, float eps, void* workspace, hipStream_t s) {
   const NsPlan q = ns_plan(batch, rows, cols);
   char* const ws = (char*)workspace;
@@ -626,7 +626,7 @@ int launch_newton_schulz(const void* x, int x_dt, float* momentum, float beta, i
   double* sums = (double*)(ws + q.off_sums);
   float* const x_sums[2] = {(float*)(ws + q.off_xs[0]), (float*)(ws + q.off_xs[1])};
   float* const a_sums = (float*)(ws + q.off_as);
-  const NsSource src = {x, momentum, beta, 1.f - beta, nesterov, x_dt};
+  const NsSource src = {x, momentum, (float)beta, (float)(1.0 - beta), nesterov, x_dt};
   const bool vec_in = ((int64_t)rows * cols & 7) == 0 && aligned16(x) && aligned16(momentum), vec_rows = (cols & 7) == 0;
   const dim3 threads(kNsThreads), norm_grid((unsigned)(batch * q.chunks));
   if (vec_in) ns_norm_kernel<true><<<norm_grid, threads, 0, s>>>(src, (int64_t)rows * cols, q.chunks, sums);
