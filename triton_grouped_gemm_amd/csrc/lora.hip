@@ -613,7 +613,7 @@ template <int DT, int RC> __global__ __launch_bounds__(kOuterThreads) void lora_
 #pragma unroll
       for (int i = 0; i < VALUES; ++i) {
         v[i] = r < all && pc + i < p.R ? row[pc + i] : 0.f;
-        top = fmaxf(top, fabsf(v[i]));
+        top = fmaxf(top, __builtin_isfinite(v[i]) ? fabsf(v[i]) : 0.f);  // (an infinity needs no scale and must not set the others')
       }
       if (DT == DT_F16) {
 #pragma unroll
