@@ -9,7 +9,7 @@
 //   lora_gemm   y and dx: the shared product, whose sums begin with the adapters' part: for every adapter of a wave's rows, R more values of depth, h (the rows
 //               of other adapters as zeros) against B_l (A_l transposed), from memory to registers.  So the adapters enter the fp32 sums and there is one rounding.
 //               h is fp32 and enters as two planes of bfloat16, high and low, 16 bits with fp32's range; against them half-precision adapters are split into two bfloat16
-//               values without loss.
+//               values without loss.  Infinities come out as the formulas have them: no part of a value that is zero, or of the other sign, meets one.
 //   lora_outer  dA and dB: sums over an adapter's rows, which are gathered from wherever they stand.
 // and lora_few, which streams W for the few rows of a decode step.
 #include <type_traits>
@@ -43,8 +43,10 @@ template <int DT> TGG_DEV float from_bits(uint16_t h) {
   return (float)__builtin_bit_cast(_Float16, h);
 }
 // two 16-bit values that add up to v but for 2^-17 (bf16) or 2^-22 of it (and what half precision's range cuts off)
-template <int DT> TGG_DEV void split2(float v, uint16_t& hi, uint16_t& lo) {
+// keep: a value below half precision's smallest step becomes one in the high part (and is taken back in the low one): what is not zero has no zero for a high part
+template <int DT> TGG_DEV void split2(float v, uint16_t& hi, uint16_t& lo, bool keep = false) {
   hi = Out16<DT>::cvt(v);
+  if (keep) hi |= v != 0.f && !(hi & 0x7fffu) ? 1 : 0;
   const float rest = v - from_bits<DT>(hi);
   lo = Out16<DT>::cvt(__builtin_isfinite(rest) ? rest : 0.f);  // an infinity stays one
 }
@@ -248,7 +250,7 @@ template <class C, int DT, bool NT> struct LoraProblem {
   static constexpr int PITCH = C::TN * 32 + 16, STAGE_WAVE = 16 * PITCH;
   static constexpr int SMEM_BYTES = C::EPI_OFF + C::NWAVES * STAGE_WAVE;
   static constexpr int CHUNK = 8;  // column tiles that are taken together
-  static constexpr uint32_t EXPONENT = DT == DT_BF16 ? 0x7f80u : 0x7c00u;
+  static constexpr uint32_t EXPONENT = DT == DT_BF16 ? 0x7f80u : 0x7c00u, ONES = DT == DT_BF16 ? 0x3f803f80u : 0x3c003c00u;
 
   const LoraGemm& p;
   StreamWalk walk;
@@ -277,7 +279,8 @@ template <class C, int DT, bool NT> struct LoraProblem {
   TGG_DEV void turn() { seek(tile_at(pos + 1)); }
 
   // The adapters' part.  Rows of other adapters are zeros against an adapter, and zero times infinity or NaN is NaN: where a wave's rows do not all have the
-  // adapter, what is not finite is taken out of it, and add_infinite() adds it to the rows that it belongs to.
+  // adapter, what is not finite becomes a one of its sign (so that an infinite row stays infinite), and add_infinite() adds it to the rows that it belongs to.  The low plane of h meets ones
+  // instead of what is not finite in any case: it may be zero or of the other sign, and the high plane's product is infinite, or NaN, by itself.
   TGG_DEV void begin(int id, f32x4_t (&acc)[C::TM][C::TN], const StreamPlace<C>& at) {
     const Place tile = locate(id);
     int el = at.lane;
@@ -328,18 +331,19 @@ template <class C, int DT, bool NT> struct LoraProblem {
       for (int i = 0; i < C::TM; ++i) a[i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(hw, ids[i] == s.l && k < 2 * p.R ? ((16 * i + l16) * 2 * p.R + k) * 2 : kNowhere, 0, 0));
     };
     auto multiply = [&](const Step& s, const i32x4_t (&a)[C::TM], i32x4_t (&b)[C::TN]) __attribute__((always_inline)) {
-      if (s.mixed) {
+      if (s.mixed || s.k0 + 32 > p.R) {
+        const uint32_t replaced = s.mixed || s.k0 + 8 * lg >= p.R ? 0xffffffffu : 0u;
+        uint32_t out = 0;
 #pragma unroll
         for (int j = 0; j < C::TN; ++j) {
-          uint32_t out = 0;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const uint32_t x = (uint32_t)b[j][w], bad = ((x & EXPONENT) == EXPONENT ? 0xffffu : 0u) | ((x >> 16 & EXPONENT) == EXPONENT ? 0xffff0000u : 0u);
-            b[j][w] = (int)(x & ~bad);
+            const uint32_t x = (uint32_t)b[j][w], bad = (((x & EXPONENT) == EXPONENT ? 0xffffu : 0u) | ((x >> 16 & EXPONENT) == EXPONENT ? 0xffff0000u : 0u)) & replaced;
+            b[j][w] = (int)((x & ~bad) | (((x & 0x80008000u) | ONES) & bad));
             out |= bad;
           }
-          infinite = infinite || __ballot(out != 0) != 0;
         }
+        infinite = infinite || (s.mixed && __ballot(out != 0) != 0);
       }
       i32x4_t rest[C::TN];
       if (DT == DT_F16) {
@@ -348,10 +352,11 @@ template <class C, int DT, bool NT> struct LoraProblem {
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const float v0 = from_bits<DT_F16>((uint16_t)b[j][w]), v1 = from_bits<DT_F16>((uint16_t)((uint32_t)b[j][w] >> 16));
-            const uint32_t high = pack2<DT_BF16>(v0, v1);
-            const float r0 = v0 - from_bits<DT_BF16>((uint16_t)high), r1 = v1 - from_bits<DT_BF16>((uint16_t)(high >> 16));
-            b[j][w] = (int)high;
-            rest[j][w] = (int)pack2<DT_BF16>(__builtin_isfinite(r0) ? r0 : 0.f, __builtin_isfinite(r1) ? r1 : 0.f);
+            // the eight bits next to v on zero's side, and what is left (four bits): both have v's sign and neither is zero but for v = 0, so that they agree on an infinite h's product
+            const uint32_t u0 = __builtin_bit_cast(uint32_t, v0), u1 = __builtin_bit_cast(uint32_t, v1);
+            const uint32_t t0 = (u0 - (v0 != 0.f ? 1u : 0u)) & 0xffff0000u, t1 = (u1 - (v1 != 0.f ? 1u : 0u)) & 0xffff0000u;
+            b[j][w] = (int)(t0 >> 16 | t1);
+            rest[j][w] = (int)pack2<DT_BF16>(v0 - __builtin_bit_cast(float, t0), v1 - __builtin_bit_cast(float, t1));
           }
       }
 #pragma unroll
@@ -386,7 +391,7 @@ template <class C, int DT, bool NT> struct LoraProblem {
       }
     }
   }
-  // What begin() has taken out: an infinity or a NaN, whatever it is added to, so it may as well be added to the stored outputs.
+  // What begin() has taken out: an infinity or a NaN, whatever finite value or infinity of its sign it is added to, so it may as well be added to the stored outputs.
   TGG_DEV void add_infinite(int64_t row0, int col0, int lane) const {
     wait_vmcnt<0>();  // (the wave's own stores)
     const int col = col0 + lane;
@@ -535,6 +540,7 @@ struct OuterParams {
 template <int DT, int RC> __global__ __launch_bounds__(kOuterThreads) void lora_outer_kernel(const OuterParams p) {
   typedef Operand<kOuterCols, false> OpZ;
   constexpr int Z_BYTES = OpZ::SLAB_BYTES, PP = RC * 32 + 16, P_BYTES = kOuterRows * PP;  // a plane of the P tile: 64 rows of RC * 16 values
+  constexpr uint32_t EXPONENTS = DT == DT_BF16 ? 0x7f807f80u : 0x7c007c00u, EXPONENT_STEP = DT == DT_BF16 ? 0x00800080u : 0x04000400u;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   char* const zbuf = smem;                   // two tiles of 64 rows x 128 columns
   char* const pbuf = smem + 2 * Z_BYTES;     // high and low plane
@@ -626,7 +632,7 @@ template <int DT, int RC> __global__ __launch_bounds__(kOuterThreads) void lora_
         top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const float want = row_scale(top);
         if (top > 0.f && (unit == 0.f || want < unit)) {  // larger values than before: the sums move to their scale
-          const float by = unit == 0.f ? 0.f : want / unit;
+          const float by = unit == 0.f ? 0.f : fmaxf(want / unit, __FLT_MIN__);  // (zero would make NaN of infinite sums)
 #pragma unroll
           for (int q = 0; q < RC; ++q)
 #pragma unroll
@@ -641,7 +647,7 @@ template <int DT, int RC> __global__ __launch_bounds__(kOuterThreads) void lora_
       for (int i = 0; i < VALUES; i += 4) {
         uint16_t hi[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) split2<DT>(v[i + e] * by, hi[e], lo[e]);
+        for (int e = 0; e < 4; ++e) split2<DT>(v[i + e] * by, hi[e], lo[e], DT == DT_F16);
         *(uint2*)(pbuf + pr * PP + (pc + i) * 2) = {(uint32_t)hi[0] | (uint32_t)hi[1] << 16, (uint32_t)hi[2] | (uint32_t)hi[3] << 16};
         *(uint2*)(pbuf + P_BYTES + pr * PP + (pc + i) * 2) = {(uint32_t)lo[0] | (uint32_t)lo[1] << 16, (uint32_t)lo[2] | (uint32_t)lo[3] << 16};
       }
@@ -660,6 +666,22 @@ template <int DT, int RC> __global__ __launch_bounds__(kOuterThreads) void lora_
           const i16x4_t hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr_t)(q + 4 * OpZ::ROW_BYTES));
           zf[b] = __builtin_bit_cast(i32x4_t, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
         }
+        // Z for the low plane of P, which may be zero or of the other sign: without infinities and NaN, whose products the high plane has.  (An exponent of ones carries into the sign's place)
+        i32x4_t zl[2] = {zf[0], zf[1]};
+        uint32_t ones = 0;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) ones |= ((uint32_t)zf[b][w] & EXPONENTS) + EXPONENT_STEP;
+        if (__builtin_expect(__ballot((ones & 0x80008000u) != 0) != 0, 0)) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t at = (((uint32_t)zf[b][w] & EXPONENTS) + EXPONENT_STEP) & 0x80008000u;
+              zl[b][w] = (int)((uint32_t)zf[b][w] & ~((at >> 15) * 0xffffu));
+            }
+        }
 #pragma unroll
         for (int plane = 0; plane < 2; ++plane)
 #pragma unroll
@@ -669,7 +691,10 @@ template <int DT, int RC> __global__ __launch_bounds__(kOuterThreads) void lora_
             const i16x4_t hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr_t)(s + 4 * PP));
             const i32x4_t pf = __builtin_bit_cast(i32x4_t, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-            for (int b = 0; b < 2; ++b) acc[q][b] = is_a ? stream_mma<DT>(zf[b], pf, acc[q][b]) : stream_mma<DT>(pf, zf[b], acc[q][b]);
+            for (int b = 0; b < 2; ++b) {
+              const i32x4_t& zv = plane ? zl[b] : zf[b];
+              acc[q][b] = is_a ? stream_mma<DT>(zv, pf, acc[q][b]) : stream_mma<DT>(pf, zv, acc[q][b]);
+            }
           }
       }
     }
