@@ -267,8 +267,8 @@ int tgg_moe_router_bwd(const void* logits, int64_t row_stride, const float* prob
 
 /* Low-rank adapters of many requests beside a shared projection (dtype TGG_BF16 or TGG_F16):
  *   out[m] = W x[m] + scales[l] B_l (A_l x[m]),  l = adapters[m];  rows whose entry is outside [0, L) have no adapter
- * x [M, K], w [N, K], a [L, R, K], b [L, N, R], adapters [M] int32 or int64, scales [L] fp32 or null (1), out [M, N]; rows in any order.  One rounding, at the
- * end.  N and K multiples of 8 up to 65536, R a multiple of 8 up to 128, L up to 1024, M up to 2^27 - 16.  h [M, R] fp32 (or null) receives scales[l] A_l x[m], zeros without an
+ * x [M, K], w [N, K], a [L, R, K], b [L, N, R], adapters [M] int32 or int64, scales [L] fp32 or null (1), out [M, N]; rows in any order.  fp32 sums, one rounding at
+ * the end; beyond 128 rows and in _bwd, h (and dh) enter the second product in two bfloat16 parts, which leave out at most 2^-17 of them (in da and db two parts of dtype).  N and K multiples of 8 up to 65536, R a multiple of 8 up to 128, L up to 1024, M up to 2^27 - 16.  h [M, R] fp32 (or null) receives scales[l] A_l x[m], zeros without an
  * adapter, which the backward pass takes.
  * _bwd: dx [M, K] = W^T g + A_l^T dh, da [L, R, K] = sum of dh[m] x[m]^T, db [L, N, R] = sum of g[m] h[m]^T over each adapter's rows, with
  * dh[m] = scales[l] B_l^T g[m]; any of the three may be null (x is read for da, w for dx, h for db).  Adapters without rows get zeros.
@@ -282,7 +282,8 @@ int tgg_lora_linear_bwd(const void* grad, const void* x, const void* w, const vo
 
 /* Newton-Schulz orthogonalisation of every matrix of a stack [batch, rows, cols] (contiguous; dtype TGG_BF16, TGG_F16 or 2 = fp32):
  *   X = x / (|x|_F + eps), then `steps` times  G = X X^T, X = a X + (b G + c G^2) X   (of the transposed matrix where rows > cols: the same matrix),
- * out in x's type (out may be x).  Matrices are multiplied and carried from step to step in 22 bits with fp32 sums, whatever the type.  Values must keep |X| entries below 64 and those of the polynomial
+ * out in x's type (out may be x).  Matrices are multiplied and carried from step to step in 22 bits with fp32 sums, whatever the type
+ * (entries below 2^-13 of the norm have fewer).  The workspace has about 8 m (m + n) bytes a matrix, m the shorter side.  Values must keep |X| entries below 64 and those of the polynomial
  * below 64 (any coefficients that keep singular values near 1 do); beyond, results are not finite.
  * tgg_muon_update: the optimiser's step, in place:
  *   momentum = beta momentum + (1 - beta) grad (fp32; beta and 1 - beta are rounded from the double);  u = nesterov ? beta momentum + (1 - beta) grad : momentum;

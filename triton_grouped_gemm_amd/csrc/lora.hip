@@ -12,8 +12,6 @@
 //               values without loss.  Infinities come out as the formulas have them: no part of a value that is zero, or of the other sign, meets one.
 //   lora_outer  dA and dB: sums over an adapter's rows, which are gathered from wherever they stand.
 // and lora_few, which streams W for the few rows of a decode step.
-#include <type_traits>
-
 #include "launch.hpp"
 #include "stream_gemm.hpp"
 
@@ -231,7 +229,7 @@ __global__ __launch_bounds__(256) void lora_transpose_kernel(const TransposePara
 }
 
 // ---- the shared product with the adapters' depth added ---------------------------------------------------------------------
-// 16384 rows, 4096 x 4096, rank 16: y 392 to 408 us, dx 402 to 411 (1.35 PFLOP/s, the matrix pipe 0.73 of the cycles; torch's library product of 8192 x 8192 x 8192 reaches 1.39).  Where a tile's rows are of many
+// 16384 rows, 4096 x 4096, rank 16: y 392 to 424 us, dx 402 to 431 (1.28 to 1.40 PFLOP/s, the matrix pipe 0.73 of the cycles; torch's library product of 8192 x 8192 x 8192 reaches 1.39).  Where a tile's rows are of many
 // adapters every one of them is R more values of depth in two planes (and again two for the parts of half-precision adapters): 2047 rows of 16 adapters, rank 32, 1536 x 2048, 57 and 63 us, of which the
 // adapters' part is more than half.
 
@@ -536,7 +534,8 @@ struct OuterParams {
 };
 
 // blockIdx.x: 128 columns of K (dA), then of N (dB); y: adapter; z: part of the rows.  RC blocks of 16 of R.  Every workgroup lists its adapter's rows window by window, so that ids may stand in any
-// order, and sums them in the order of their numbers.  Bound by reading x and g once: 16384 rows of 8 adapters, 4096 + 4096 columns, 85 us for 268 MB (3.2 TB/s); 2047 rows of 16, 13.6 us.
+// order, and sums them in the order of their numbers.  Bound by reading x and g once: 16384 rows of 8 adapters, 4096 + 4096 columns, 85 to 91 us for 268 MB (3.0 TB/s); 2047 rows of 16, 14 us.
+// (Every workgroup reads all ids: 1024 adapters of 16384 rows, 65536 workgroups, 4.3 GB of them, from L2.)
 template <int DT, int RC> __global__ __launch_bounds__(kOuterThreads) void lora_outer_kernel(const OuterParams p) {
   typedef Operand<kOuterCols, false> OpZ;
   constexpr int Z_BYTES = OpZ::SLAB_BYTES, PP = RC * 32 + 16, P_BYTES = kOuterRows * PP;  // a plane of the P tile: 64 rows of RC * 16 values
@@ -783,15 +782,21 @@ template <int DT, bool NT> int launch_gemm(LoraGemm p, int tile, hipStream_t s) 
   return tile == 256 ? gemm_launch<LoraWide, DT, NT>(p, s) : gemm_launch<LoraNarrow, DT, NT>(p, s);
 }
 
-// Tiles of 256 or of 128 for M x cols outputs: as for newton_schulz.hip's products
+// Tiles of 256 or of 128 for M x cols outputs: a round of 256-row tiles, one a compute unit, takes 1.5 times one of 128-row tiles, two a compute unit.  With the kernel in front, of 8 adapters, rank 16, in runs, in tiles of 128
+// and 256: 2048 rows, 4096 x 4096, 78 and 91 us; 4096 rows 146 and 110; 6000 rows, 2568 columns x 4104, 170 and 221; 16384 rows 555 and 404; 16384 rows, 1024 x 1024, 55 and 49.  Rank 64, and 16 adapters in
+// mixed rows, have the same faster side in all these (the choice within 5 %), so the rule leaves both out.
 int tile_of(int64_t M, int cols) {
   auto tiles = [&](int b) { return (M + b - 1) / b * ((cols + b - 1) / b); };
   const int64_t cus = num_cus();
   return (tiles(256) + cus - 1) / cus * 3 <= (tiles(128) + 2 * cus - 1) / (2 * cus) * 2 ? 256 : 128;
 }
 
-// lora_few up to 128 rows.  It reads W once for 64 rows, and rows of many adapters cost it little: 4096 x 4096, every row another adapter, 64 rows 26 us (lora_gemm: 124), 128 rows 39 (128), 256 rows
-// 65 (126); 2048 x 8192, one adapter, 64 rows 29 (42), 128 rows 45 (43).
+// lora_few up to 128 rows.  It reads W once for 64 rows, and rows of many adapters cost it little; with the kernel in front, of 1, 16 and 128 adapters in mixed rows (lora_gemm in brackets), us:
+//   columns x depth, rank   64 rows               128                   129                   256                    512
+//   4096 x 4096, 16         19 20 21 (64 77 110)  31 32 33 (65 79 112)  41 42 45 (62 74 109)  57 58 61 (65 79 109)   103 108 115 (65 81 111)
+//   8192 x 2048, 16         23 24 26 (36 49 83)   40 41 43 (38 50 78)   53 55 57 (35 48 83)   75 76 80 (38 51 85)    138 145 152 (39 54 84)
+//   2048 x 1536, 32         13 14 15 (23 42 88)   14 15 16 (24 44 102)  20 21 24 (24 45 95)   23 25 29 (24 46 105)   38 45 52 (24 55 108)
+// So up to 128 rows it is the faster one or within 7 %.  Beyond, a limit that looked at N and the number of adapters would gain up to 4 times; this one does not.
 bool few_rows(int64_t M) { return M <= 128; }
 constexpr int kFewParts = 2;  // parts of the depth in lora_down for few rows: more workgroups, 64 rows of 4096 25.9 us in 2 parts, 26.7 in 1 and 26.4 in 4
 

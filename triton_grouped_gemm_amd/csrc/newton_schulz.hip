@@ -3,17 +3,17 @@
 //   X_0 = X / (|X|_F + eps);   G = X X^T,   X <- a X + (b G + c G^2) X      once a step
 //
 // X is taken as [M, N] with M <= N (a tall matrix is transposed on its way in and out: the iteration commutes with it).  X is carried as two
-// planes of half precision, high and low, 22 bits together, scaled by 2^10 so that the low plane keeps its bits: singular values
+// planes of half precision, high and low, 22 bits together (values below 2^-13 in steps of 2^-34), scaled by 2^10 so that the low plane keeps its bits: singular values
 // stay near or below 1, so entries do not overflow.
 //
 // Products add up high x high, high x low and low x high planes, three multiplies for one, whatever the result's type.  (High planes alone, 11 bits, do not do for bfloat16 results either.  What X's rounding
 // leaves out lands in weak directions too, and each of them grows by up to 3.4445 a step: in front of the last rounding, which is 1.7e-3 of the norm, emulated, 7e-4 for random matrices of 512 rows, but 8e-3 for
 // 8 x 4096 of rank 4 over 0.3 % noise, 3e-2 for exactly low-rank ones after eight steps.  Both planes of X alone: 3e-3 for 512 x 2048 of which four rows are not zero.  Both planes of everything: 3e-5 at most in
-// five steps.)
+// five steps.  What two planes leave out, and fp32 sums round, grows in a direction that is exactly zero as well, so that more steps of low-rank matrices leave more: 9e-4 after eight.)
 // G and the polynomial enter products less their mean diagonal, whose part is exact, so that the rounding of near-identity matrices is that of what is left of them:
 //   A = G - d I,   B = (b + 2 c d) A + c (A^2 - e I),   X <- (a + b d + c d^2 + c e) X + B X,   d = |X|^2 / M,   e = |A|^2 / M.
 //
-// A step of 64 matrices of 1536 x 2048 takes 1015 us for G, 843 for the polynomial and 1595 for the update; 17.5 ms in all, 1.0 PFLOP/s counting three products and half of a symmetric one.
+// A step of 64 matrices of 1536 x 2048 takes 1015 to 1044 us for G, 838 to 867 for the polynomial and 1595 to 1640 for the update; 17.5 to 18.1 ms in all, 1.0 PFLOP/s counting three products and half of a symmetric one.
 // Between tiles eight waves store results and read what they add to (25 us a tile of 256, of 1.4 us a slab of 64), and 64 x 21 triangular tiles are 5.25 rounds of the chip.  What is small is bound by
 // latency: 512 x 512, three kernels of 13.5 us a step.
 //

@@ -179,7 +179,9 @@ def lora_linear(x: Tensor, weight: Tensor, lora_a: Tensor, lora_b: Tensor, adapt
 
     ``x`` ``[M, K]``, ``weight`` ``[N, K]``, ``lora_a`` ``[L, R, K]`` and ``lora_b`` ``[L, N, R]`` in bf16 or fp16 (N and K multiples of 8 up to 65536, R one of
     8 up to 128, L up to 1024, M up to 2^27 - 16; operands that are not contiguous, or do not begin at a multiple of 16 bytes, are copied); ``adapters`` ``[M]`` int32 or int64 on the GPU, in any order: a row whose entry is outside ``[0, L)``
-    (-1, say) has no adapter; ``scales`` ``[L]`` fp32, 1 unless given.  fp32 to the one rounding at the end.  Differentiable in ``x``, ``weight``,
+    (-1, say) has no adapter; ``scales`` ``[L]`` fp32, 1 unless given.  fp32 sums and one rounding of the result.  The hidden values ``scales[l] lora_a[l] x[m]``
+    (in the gradients those of the output's gradient too) are fp32; beyond 128 rows, and in the gradients, they enter the second product in two bfloat16 parts, which leave out at most 2^-17 of each (in ``lora_a``'s and
+    ``lora_b``'s gradients two parts of the operands' type).  Differentiable in ``x``, ``weight``,
     ``lora_a`` and ``lora_b``, once and backwards (forward-mode tangents are refused); adapters without rows get zero gradients."""
     if not (_lora_linear.replaced or torch.compiler.is_compiling()):
         out = (_native._host or _native.host()).lora_linear(x, weight, lora_a, lora_b, adapters, scales, False)
